@@ -8,7 +8,7 @@
  * passes a cudaStream_t.  Reference paths are relative to the mongoose
  * checkout.
  *
- * Three groups, mirroring what the reference's cgo blocks bind:
+ * Three groups, mirroring what the reference's cgo blocks bind, and a fourth beside them:
  *   1. tw_gpu_*        device memory shim            (cuda_tensor.go:19-52)
  *   2. mongoose_*      one launch per decode op      (kernels.go:12-72, 150-226;
  *                                                     bodies kernels/mongoose.cu)
@@ -16,6 +16,7 @@
  *                      CUDAStreamInfer and CUDAGraph do behind their Go methods
  *                      (cuda_fused_infer.go, cuda_fused_infer_q4.go,
  *                       cuda_q4_0.go, cuda_fused_stream.go, cuda_graph.go)
+ *   4. mg_paged_*      several requests out of one paged KV cache (no counterpart)
  *
  * Error convention.  The reference's kernels return void and report nothing;
  * its Go methods return -1 when the object is not built.  Here mongoose_*
@@ -468,6 +469,75 @@ void       mg_stream_destroy(mg_stream* s);
 int mg_stream_forward_token(mg_stream* s, int pos, const float* embHidden, int nLayers,
                             const void* const* layerPtrs, const int32_t* layerSizes,
                             float* logitsOut);
+
+/* ------------------------------------------------------------------ */
+/* 4. Several requests out of one paged KV cache                        */
+/*    No counterpart in the reference, whose caches hold one sequence   */
+/*    (cuda_fused_infer.go:542-554); beside mongoose_kv_cache_write,    */
+/*    mongoose_rope and mongoose_decode_attention.                      */
+/* ------------------------------------------------------------------ */
+/* A layer's cache is two pools, K and V, of nPages pages of pageSize positions, [nPages, pageSize, nKVHeads * headDim], fp32
+ * (kvFormat 0) or fp16 (1; written rounded to nearest even), from tw_gpu_alloc or any hipMalloc.  Request r's position p is in
+ * page table[r * width + p / pageSize], width = mg_paged_table_width.  One table serves all layers.
+ *
+ * A step of a server:   mg_paged_tables   once a step: rows, slots and block tables from the requests' lengths
+ *                       mg_paged_plan     once a step (and once for every other window or prefix its layers use)
+ *                       mg_paged_store    each layer: rotary positions, K and V rows into the slots
+ *                       mg_paged_attention  each layer
+ * All take device pointers, launch kernels on `stream` and neither allocate, synchronise nor copy: they can be captured into a
+ * graph, and lengths may change between its replays (nReqs and rows are upper bounds then: requests of no rows and no length do
+ * nothing, rows behind the last request's are left as they were).
+ *
+ * A handle owns a plan and the workspace of the attention that reads it: calls on it run in the order of one stream (or are
+ * ordered by events), from one thread at a time -- two graphs that hold calls on one handle must not run at once.  It belongs to
+ * the device that was current at its creation; calls make that device current while they run.  It takes workspace for maxReqs
+ * requests and maxRows rows a step of at most maxLen positions.  headDim 64 or 128; nHeads a multiple of nKVHeads; pageSize a power
+ * of two up to 4096; nPages * pageSize < 2^31; maxReqs <= 4096, maxRows <= 2^20, maxLen <= 2^24.  NULL on failure.  All of this
+ * returns MG_E_ARG where an argument does not fit, with the reason in mg_last_error; nothing is launched then. */
+typedef struct mg_paged mg_paged;
+mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, int nPages, int kvFormat, int maxReqs, int maxRows,
+                          int maxLen);
+void mg_paged_destroy(mg_paged* h);
+int mg_paged_table_width(const mg_paged* h);      /* ceil(maxLen / pageSize): entries of a request's row of the block table */
+
+/* Block tables and slot maps of a step.  newLens[r]: tokens that request r adds (0: none), or -1 when it has ended.  lens[r]:
+ * its positions so far.  ring: the free pages, a ring of nPages entries; ringState = {first free entry, free pages}.
+ * Pages are taken from the ring's front in the order of the requests and, within one, of its positions, and written into its
+ * row of the table; the pages of ended requests go behind the ring's last in the same order (and are free from the next call
+ * on; their table rows stay as they are).  Written besides: lensOut[r] = lens[r] + newLens[r] (0 for an ended one), ringStateOut
+ * (these two may be lens and ringState themselves, or else do not overlap them), rowStart[nReqs + 1] = the first row of every
+ * request, slots[rows] = page * pageSize + place of each row and positions[rows] (both -1 behind the last row; a slot is -1 too
+ * where the table or the ring hold an entry that is no page), counts[4] = {rows, pages taken, pages given back, 0}.
+ * A step that does not fit changes no length, no table and no ring: rowStart is 0 throughout, slots and positions -1, counts =
+ * {0, 0, 0, why}, why a sum of 1 (more pages needed than free), 2 (more new tokens than `rows`), 4 (a length that is negative or
+ * passes maxLen, a newLens below -1), 8 (ringState that fits no ring of nPages). */
+int mg_paged_tables(mg_paged* h, const int* newLens, int nReqs, const int* lens, int* lensOut, int* table, int* ring,
+                    const int* ringState, int* ringStateOut, int rows, int* rowStart, int* slots, int* positions, int* counts,
+                    void* stream);
+
+/* mongoose_rope on the rows of q and k at positions[t] (pairs (j, j + headDim/2), table row = position, [tableRows, headDim/2])
+ * and mongoose_kv_cache_write of the turned k rows and the v rows at slots[t].  ldq, ldk, ldv, ldqOut: floats from one row to the
+ * next (multiples of 4, pointers 16-byte aligned: q, k and v may be columns of one projection); qOut may be q.  A row whose
+ * position is negative or past the tables is passed over, one whose slot is no slot of the pools is turned but not stored.
+ * The slots of a call differ from one another. */
+int mg_paged_store(mg_paged* h, const float* q, const float* k, const float* v, int ldq, int ldk, int ldv, float* qOut, int ldqOut,
+                   void* K, void* V, const int* slots, const int* positions, int rows, const float* cosTab, const float* sinTab,
+                   int tableRows, void* stream);
+
+/* Takes the lengths of the step for the attention calls that follow: rows rowStart[r] .. rowStart[r+1]-1 are the last
+ * positions of request r's lens[r] (after this step).  The arrays are copied (clamped to `rows` and maxLen).  Which positions j a
+ * token at position i sees: j <= i, and where window > 0 only j > i - window; with prefixLens also every j < prefixLens[r],
+ * before or behind i and whatever the window. */
+int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int window, const int* prefixLens, void* stream);
+
+/* out[row, head] = sum_j softmax_j(s_j) v_j over the positions that the row sees, of KV head `head / (nHeads / nKVHeads)`:
+ * s_j = scale * q.k_j (scale 0: 1 / sqrt(headDim)); with softcap > 0 then softcap * tanh(s_j / softcap); with slopes [nHeads]
+ * then minus slopes[head] * |i - j|.  Scores, their maxima and sums are fp32; products of an fp32 cache too, those of an fp16 cache
+ * are of q and the probabilities to 22 bits.  ldq, ldo: floats from one row to the next (multiples of 4, 16-byte aligned
+ * pointers).  A table entry that is no page hides its positions; a row that sees nothing is zeros; what the cache holds
+ * behind a request's length is not read into any result.  MG_E_STATE without a plan. */
+int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, const void* V, const int* table, float* out, int ldo,
+                       float scale, float softcap, const float* slopes, void* stream);
 
 /* ------------------------------------------------------------------ */
 /* Host-side helpers shared with the loaders                            */

@@ -1,0 +1,116 @@
+// paged_rules.h -- what the calls on a paged KV cache accept and which positions a token sees.  Plain C++, shared by the host
+// side, the kernels and the CPU tests.
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __HIPCC__
+#define MG_HD __host__ __device__ __forceinline__
+#else
+#define MG_HD inline
+#endif
+
+namespace mg {
+
+// Limits of a handle: the block-table kernel holds three sums a request in LDS (48 KB); a distance between positions is exact in fp32.
+constexpr int PAGED_MAX_REQS = 4096, PAGED_MAX_LEN = 1 << 24, PAGED_MAX_ROWS = 1 << 20, PAGED_MAX_PAGE = 4096, PAGED_MAX_GROUP = 128;
+
+struct PagedGeo {
+    int nHeads, nKVHeads, headDim, pageSize, nPages, kvHalf, maxReqs, maxRows, maxLen;
+    int group;        // query heads a KV head
+    int kvDim;        // elements of a position's K (or V) row
+    int pageShift;    // log2(pageSize)
+    int width;        // entries of a request's row of the block table
+};
+
+// nullptr, or why there is no such handle
+inline const char* paged_geo(PagedGeo& g, int nHeads, int nKVHeads, int headDim, int pageSize, int nPages, int kvFormat, int maxReqs,
+                             int maxRows, int maxLen) {
+    if (headDim != 64 && headDim != 128) return "headDim must be 64 or 128";
+    if (nKVHeads <= 0 || nHeads <= 0 || nHeads % nKVHeads != 0) return "nHeads must be a positive multiple of nKVHeads";
+    if (nHeads / nKVHeads > PAGED_MAX_GROUP || nHeads > 65536) return "at most 128 query heads a KV head and 65536 in all";
+    if (pageSize <= 0 || pageSize > PAGED_MAX_PAGE || (pageSize & (pageSize - 1))) return "pageSize must be a power of two up to 4096";
+    if (nPages <= 0 || (long long)nPages * pageSize > 0x7fffffffll) return "nPages must be positive and nPages * pageSize below 2^31";
+    if (kvFormat != 0 && kvFormat != 1) return "kvFormat must be 0 (fp32) or 1 (fp16)";
+    if (maxReqs <= 0 || maxReqs > PAGED_MAX_REQS) return "maxReqs must be between 1 and 4096";
+    if (maxRows <= 0 || maxRows > PAGED_MAX_ROWS) return "maxRows must be between 1 and 2^20";
+    if (maxLen <= 0 || maxLen > PAGED_MAX_LEN) return "maxLen must be between 1 and 2^24";
+    g.nHeads = nHeads; g.nKVHeads = nKVHeads; g.headDim = headDim; g.pageSize = pageSize; g.nPages = nPages; g.kvHalf = kvFormat;
+    g.maxReqs = maxReqs; g.maxRows = maxRows; g.maxLen = maxLen;
+    g.group = nHeads / nKVHeads;
+    g.kvDim = nKVHeads * headDim;
+    g.pageShift = 0;
+    while ((1 << g.pageShift) < pageSize) g.pageShift++;
+    g.width = (maxLen + pageSize - 1) / pageSize;
+    return nullptr;
+}
+
+inline bool paged_aligned(const void* p, size_t a) { return p != nullptr && ((uintptr_t)p & (a - 1)) == 0; }
+
+// The arguments of the calls: nullptr, or what is wrong with them.
+inline const char* paged_tables_refusal(const PagedGeo& g, const void* newLens, int nReqs, const void* lens, const void* lensOut,
+                                        const void* table, const void* ring, const void* ringState, const void* ringStateOut, int rows,
+                                        const void* rowStart, const void* slots, const void* positions, const void* counts) {
+    if (nReqs < 0 || nReqs > g.maxReqs) return "nReqs is negative or above the handle's maxReqs";
+    if (rows < 0 || rows > g.maxRows) return "rows is negative or above the handle's maxRows";
+    const void* always[] = {ring, ringState, ringStateOut, rowStart, counts};
+    for (const void* p : always) if (!paged_aligned(p, 4)) return "a pointer is NULL or not aligned to 4 bytes";
+    if (nReqs > 0) {
+        const void* reqs[] = {newLens, lens, lensOut, table};
+        for (const void* p : reqs) if (!paged_aligned(p, 4)) return "a pointer is NULL or not aligned to 4 bytes";
+        if (newLens == lensOut) return "newLens and lensOut are the same array";
+    }
+    if (rows > 0 && (!paged_aligned(slots, 4) || !paged_aligned(positions, 4))) return "a pointer is NULL or not aligned to 4 bytes";
+    return nullptr;
+}
+inline const char* paged_store_refusal(const PagedGeo& g, const void* q, const void* k, const void* v, int ldq, int ldk, int ldv,
+                                       const void* qOut, int ldqOut, const void* K, const void* V, const void* slots,
+                                       const void* positions, int rows, const void* cosTab, const void* sinTab, int tableRows) {
+    if (rows < 0 || rows > g.maxRows) return "rows is negative or above the handle's maxRows";
+    if (rows == 0) return nullptr;
+    const void* wide[] = {q, k, v, qOut, K, V, cosTab, sinTab};
+    for (const void* p : wide) if (!paged_aligned(p, 16)) return "a pointer is NULL or not aligned to 16 bytes";
+    if (!paged_aligned(slots, 4) || !paged_aligned(positions, 4)) return "a pointer is NULL or not aligned to 4 bytes";
+    if (ldq < g.nHeads * g.headDim || ldqOut < g.nHeads * g.headDim || ldk < g.kvDim || ldv < g.kvDim) return "a row stride is smaller than the row";
+    if ((ldq | ldk | ldv | ldqOut) & 3) return "a row stride is not a multiple of 4";
+    if (tableRows <= 0) return "the rotary tables have no rows";
+    if (K == V) return "K and V are the same array";
+    return nullptr;
+}
+inline const char* paged_plan_refusal(const PagedGeo& g, const void* rowStart, const void* lens, int nReqs, int rows, int window,
+                                      const void* prefixLens) {
+    if (nReqs < 0 || nReqs > g.maxReqs) return "nReqs is negative or above the handle's maxReqs";
+    if (rows < 0 || rows > g.maxRows) return "rows is negative or above the handle's maxRows";
+    if (window < 0) return "window is negative";
+    if (!paged_aligned(rowStart, 4) || (nReqs > 0 && !paged_aligned(lens, 4))) return "a pointer is NULL or not aligned to 4 bytes";
+    if (prefixLens && !paged_aligned(prefixLens, 4)) return "prefixLens is not aligned to 4 bytes";
+    return nullptr;
+}
+inline const char* paged_attention_refusal(const PagedGeo& g, const void* q, int ldq, const void* K, const void* V, const void* table,
+                                           const void* out, int ldo, float scale, float softcap, const void* slopes) {
+    const void* wide[] = {q, K, V, out};
+    for (const void* p : wide) if (!paged_aligned(p, 16)) return "a pointer is NULL or not aligned to 16 bytes";
+    if (!paged_aligned(table, 4) || (slopes && !paged_aligned(slopes, 4))) return "a pointer is NULL or not aligned to 4 bytes";
+    if (ldq < g.nHeads * g.headDim || ldo < g.nHeads * g.headDim) return "a row stride is smaller than the row";
+    if ((ldq | ldo) & 3) return "a row stride is not a multiple of 4";
+    if (!(scale >= 0.f && scale <= 3.0e38f)) return "scale must be finite and positive, or 0 for 1 / sqrt(headDim)";
+    if (!(softcap >= 0.f && softcap <= 3.0e38f)) return "softcap must be finite and positive, or 0 for none";
+    if (q == out) return "q and out are the same array";
+    return nullptr;
+}
+
+// Sums that stop at 2^31 - 1 instead of wrapping (still associative): an overflowing total is only ever compared with a limit.
+MG_HD unsigned sat_add(unsigned a, unsigned b) {
+    const unsigned s = a + b;            // both below 2^31
+    return s > 0x7fffffffu ? 0x7fffffffu : s;
+}
+MG_HD int paged_pages(int len, int pageShift) { return (int)(((unsigned)len + (1u << pageShift) - 1) >> pageShift); }
+// Whether the token at position i of a request of `len` positions sees position j.
+MG_HD bool paged_sees(int i, int j, int len, int window, int prefix) {
+    return j < len && ((j <= i && (window == 0 || j > i - window)) || j < prefix);
+}
+
+// Why mg_paged_tables changes nothing
+enum { PAGED_NO_PAGES = 1, PAGED_NO_ROWS = 2, PAGED_BAD_LENGTH = 4, PAGED_BAD_RING = 8 };
+
+}  // namespace mg

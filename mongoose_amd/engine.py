@@ -10,6 +10,7 @@ in for, so that tests read like the reference's:
     HIPFusedInference          CUDAFusedInference (cuda_fused_infer.go,
                                cuda_fused_infer_q4.go, cuda_fused_infer_stub.go:7-49)
     HIPStreamInfer             CUDAStreamInfer (cuda_fused_stream.go)
+    HIPPaged                   no counterpart: several requests out of one paged KV cache
 
 Everything here is a thin ctypes call into libmongoose_hip.so; there is no
 computation in Python and no CPU fallback.
@@ -750,3 +751,50 @@ def KQ8Gemm(act, w, scales, bias, out, T, N, K, accumulate, workspace, workspace
     """Multi-row form of KQ8MatvecRowScale on the matrix cores (out[T,N] (+)= act[T,K] . w[N,K]^T * scales + bias)."""
     lib.mongoose_q8_gemm(_p(act), _p(w), _p(scales), _p(bias) if bias is not None else None, _p(out), T, N, K,
                          1 if accumulate else 0, _p(workspace), workspaceBytes, None)
+
+
+class HIPPaged:
+    """Several requests out of one KV cache in pages (mg_paged_*): block tables and slot maps from the requests' lengths, rotary
+    positions with the K/V rows stored by slot, attention of the requests' new tokens over their pages.  No counterpart in the
+    reference.  Arguments are device buffers (Tensor, or an address); every method returns 0 or a negative code (last_error)."""
+
+    def __init__(self, handle):
+        self._h = handle
+
+    def Close(self):
+        if self._h:
+            lib.mg_paged_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.Close()
+        except Exception:
+            pass
+
+    def TableWidth(self):
+        """Entries of a request's row of the block table."""
+        return lib.mg_paged_table_width(self._h)
+
+    def Tables(self, newLens, nReqs, lens, lensOut, table, ring, ringState, ringStateOut, rows, rowStart, slots, positions, counts,
+               stream=None):
+        return lib.mg_paged_tables(self._h, _p(newLens), nReqs, _p(lens), _p(lensOut), _p(table), _p(ring), _p(ringState),
+                                   _p(ringStateOut), rows, _p(rowStart), _p(slots), _p(positions), _p(counts), stream)
+
+    def Store(self, q, k, v, ldq, ldk, ldv, qOut, ldqOut, K, V, slots, positions, rows, cosTab, sinTab, tableRows, stream=None):
+        return lib.mg_paged_store(self._h, _p(q), _p(k), _p(v), ldq, ldk, ldv, _p(qOut), ldqOut, _p(K), _p(V), _p(slots),
+                                  _p(positions), rows, _p(cosTab), _p(sinTab), tableRows, stream)
+
+    def Plan(self, rowStart, lens, nReqs, rows, window=0, prefixLens=None, stream=None):
+        return lib.mg_paged_plan(self._h, _p(rowStart), _p(lens), nReqs, rows, window, _p(prefixLens), stream)
+
+    def Attention(self, q, ldq, K, V, table, out, ldo, scale=0.0, softcap=0.0, slopes=None, stream=None):
+        return lib.mg_paged_attention(self._h, _p(q), ldq, _p(K), _p(V), _p(table), _p(out), ldo, scale, softcap, _p(slopes), stream)
+
+
+def NewHIPPaged(eng, nHeads, nKVHeads, headDim, pageSize, nPages, kvFormat, maxReqs, maxRows, maxLen):
+    """mg_paged_create: None on failure (last_error)."""
+    if eng is None:
+        return None
+    h = lib.mg_paged_create(nHeads, nKVHeads, headDim, pageSize, nPages, kvFormat, maxReqs, maxRows, maxLen)
+    return HIPPaged(h) if h else None

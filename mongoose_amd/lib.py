@@ -136,6 +136,15 @@ _sig("mg_stream_build", c_void_p, c_void_p)
 _sig("mg_stream_destroy", None, c_void_p)
 _sig("mg_stream_forward_token", c_int, c_void_p, c_int, _f, c_int, POINTER(c_void_p), _i, _f)
 
+# 4. several requests out of one paged KV cache
+_sig("mg_paged_create", c_void_p, *[c_int] * 9)
+_sig("mg_paged_destroy", None, c_void_p)
+_sig("mg_paged_table_width", c_int, c_void_p)
+_sig("mg_paged_tables", c_int, c_void_p, _p, c_int, _p, _p, _p, _p, _p, _p, c_int, _p, _p, _p, _p, _p)
+_sig("mg_paged_store", c_int, c_void_p, _p, _p, _p, c_int, c_int, c_int, _p, c_int, _p, _p, _p, _p, c_int, _p, _p, c_int, _p)
+_sig("mg_paged_plan", c_int, c_void_p, _p, _p, c_int, c_int, c_int, _p, _p)
+_sig("mg_paged_attention", c_int, c_void_p, _p, c_int, _p, _p, _p, _p, c_int, c_float, c_float, _p, _p)
+
 # host helpers
 _sig("mg_quantize_q8", None, _f, c_int, c_int, c_int, _i8, _f)
 _sig("mg_quantize_q4_0", None, _f, c_int, c_int, _u8)

@@ -1,0 +1,108 @@
+"""What the calls on a paged KV cache refuse, and the positions that a token sees, on the host (paged_rules.h)."""
+import os
+import subprocess
+
+import numpy as np
+import pytest
+
+from mongoose_amd import engine as E
+from mongoose_amd.lib import lib
+from tests import paged_model as P
+
+CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "mongoose_amd", "csrc")
+
+
+def _run(tmp_path, source):
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text('#include "paged_rules.h"\n#include <algorithm>\n#include <cstdio>\n#include <vector>\nusing namespace mg;\n' + source)
+    subprocess.run(["g++", "-std=c++17", "-Wall", "-Werror", "-I", CSRC, str(src), "-o", str(exe)], check=True)
+    return subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+
+
+GOOD = dict(nHeads=14, nKVHeads=2, headDim=64, pageSize=16, nPages=100, kvFormat=0, maxReqs=4, maxRows=64, maxLen=1000)
+
+
+@pytest.mark.parametrize("change,why", [
+    (dict(headDim=80), "headDim"), (dict(nHeads=15), "multiple"), (dict(nKVHeads=0), "multiple"), (dict(nHeads=-14), "multiple"),
+    (dict(nHeads=129, nKVHeads=1), "128 query heads"), (dict(pageSize=0), "power of two"), (dict(pageSize=24), "power of two"),
+    (dict(pageSize=8192), "power of two"), (dict(nPages=0), "nPages"), (dict(nPages=1 << 27), "2^31"), (dict(kvFormat=2), "kvFormat"),
+    (dict(maxReqs=0), "maxReqs"), (dict(maxReqs=4097), "maxReqs"), (dict(maxRows=0), "maxRows"), (dict(maxRows=(1 << 20) + 1), "maxRows"),
+    (dict(maxLen=0), "maxLen"), (dict(maxLen=(1 << 24) + 1), "maxLen")])
+def test_create_refuses(change, why):
+    assert lib.mg_paged_create(*{**GOOD, **change}.values()) is None
+    assert why in E.last_error(), E.last_error()
+
+
+def test_calls_without_a_handle():
+    assert lib.mg_paged_table_width(None) == 0
+    lib.mg_paged_destroy(None)
+    assert lib.mg_paged_plan(None, None, None, 0, 0, 0, None, None) == -1
+    assert lib.mg_paged_tables(None, None, 0, None, None, None, None, None, None, 0, None, None, None, None, None) == -1
+    assert lib.mg_paged_store(None, None, None, None, 0, 0, 0, None, 0, None, None, None, None, 0, None, None, 0, None) == -1
+    assert lib.mg_paged_attention(None, None, 0, None, None, None, None, 0, 0.0, 0.0, None, None) == -1
+
+
+def test_arguments_that_are_refused(tmp_path):
+    out = _run(tmp_path, r"""
+static char mem[4096] __attribute__((aligned(16)));
+static void is(const char* what, const char* why) { std::printf("%s|%s\n", what, why ? why : "-"); }
+int main() {
+    PagedGeo g{};
+    if (paged_geo(g, 14, 2, 64, 16, 100, 0, 4, 64, 1000)) return 1;
+    std::printf("%d %d %d %d\n", g.group, g.kvDim, g.pageShift, g.width);
+    char *a = mem, *b = mem + 64, *odd = mem + 2, *four = mem + 4;
+    auto T = [&](const void* nl, int n, const void* l, const void* lo, const void* ring, int rows, const void* slots) {
+        return paged_tables_refusal(g, nl, n, l, lo, a, ring, a, a, rows, a, slots, a, a); };
+    is("-", T(a, 4, b, b, a, 64, a)); is("-", T(nullptr, 0, nullptr, nullptr, a, 0, nullptr)); is("nReqs", T(a, 5, b, b, a, 64, a));
+    is("nReqs", T(a, -1, b, b, a, 64, a)); is("rows", T(a, 4, b, b, a, 65, a)); is("rows", T(a, 4, b, b, a, -1, a)); is("pointer", T(nullptr, 1, b, b, a, 1, a));
+    is("pointer", T(a, 1, odd, b, a, 1, a)); is("pointer", T(a, 1, b, b, nullptr, 1, a)); is("pointer", T(a, 1, b, b, a, 1, nullptr)); is("same array", T(a, 1, b, a, a, 1, a));
+    auto S = [&](const void* q, int ldq, int ldk, int ldv, int ldo, const void* K, const void* V, const void* slots, int rows, int tab) {
+        return paged_store_refusal(g, q, a, a, ldq, ldk, ldv, a, ldo, K, V, slots, a, rows, a, a, tab); };
+    is("-", S(a, 896, 128, 128, 896, a, b, four, 64, 1)); is("-", S(nullptr, 0, 0, 0, 0, nullptr, nullptr, nullptr, 0, 0)); is("16 bytes", S(four, 896, 128, 128, 896, a, b, a, 1, 1));
+    is("16 bytes", S(a, 896, 128, 128, 896, nullptr, b, a, 1, 1)); is("4 bytes", S(a, 896, 128, 128, 896, a, b, odd, 1, 1)); is("smaller", S(a, 895, 128, 128, 896, a, b, a, 1, 1));
+    is("smaller", S(a, 896, 124, 128, 896, a, b, a, 1, 1)); is("smaller", S(a, 896, 128, -4, 896, a, b, a, 1, 1)); is("smaller", S(a, 896, 128, 128, 892, a, b, a, 1, 1));
+    is("multiple of 4", S(a, 898, 128, 128, 896, a, b, a, 1, 1)); is("no rows", S(a, 896, 128, 128, 896, a, b, a, 1, 0)); is("same array", S(a, 896, 128, 128, 896, a, a, a, 1, 1));
+    is("rows", S(a, 896, 128, 128, 896, a, b, a, 65, 1)); is("rows", S(a, 896, 128, 128, 896, a, b, a, -1, 1));
+    is("-", paged_plan_refusal(g, a, b, 4, 64, 0, nullptr)); is("-", paged_plan_refusal(g, a, nullptr, 0, 0, 0, nullptr)); is("nReqs", paged_plan_refusal(g, a, b, 5, 64, 0, nullptr));
+    is("rows", paged_plan_refusal(g, a, b, 4, 65, 0, nullptr)); is("window", paged_plan_refusal(g, a, b, 4, 64, -1, nullptr)); is("pointer", paged_plan_refusal(g, nullptr, b, 4, 64, 0, nullptr));
+    is("pointer", paged_plan_refusal(g, a, nullptr, 1, 64, 0, nullptr)); is("prefixLens", paged_plan_refusal(g, a, b, 1, 64, 0, odd));
+    auto A = [&](const void* q, int ldq, const void* K, const void* t, const void* o, int ldo, float sc, float cap, const void* sl) { return paged_attention_refusal(g, q, ldq, K, b, t, o, ldo, sc, cap, sl); };
+    is("-", A(a, 896, a, four, b, 900, 0.f, 0.f, nullptr)); is("-", A(a, 896, a, a, b, 896, 0.1f, 50.f, four)); is("16 bytes", A(four, 896, a, a, b, 896, 0, 0, nullptr));
+    is("16 bytes", A(a, 896, a, a, nullptr, 896, 0, 0, nullptr)); is("4 bytes", A(a, 896, a, odd, b, 896, 0, 0, nullptr)); is("4 bytes", A(a, 896, a, a, b, 896, 0, 0, odd));
+    is("smaller", A(a, 892, a, a, b, 896, 0, 0, nullptr)); is("smaller", A(a, 896, a, a, b, 0, 0, 0, nullptr)); is("multiple of 4", A(a, 897, a, a, b, 896, 0, 0, nullptr));
+    is("scale", A(a, 896, a, a, b, 896, -1.f, 0, nullptr)); is("scale", A(a, 896, a, a, b, 896, __builtin_nanf(""), 0, nullptr)); is("scale", A(a, 896, a, a, b, 896, __builtin_inff(), 0, nullptr));
+    is("softcap", A(a, 896, a, a, b, 896, 0, -1.f, nullptr)); is("softcap", A(a, 896, a, a, b, 896, 0, __builtin_nanf(""), nullptr)); is("same array", A(a, 896, a, a, a, 896, 0, 0, nullptr));
+}
+""")
+    lines = out.splitlines()
+    assert lines[0] == "7 128 4 63"
+    for line in lines[1:]:
+        want, got = line.split("|")
+        assert (want in got) if want != "-" else got == "-", line
+    assert len(lines) == 49
+
+
+def test_what_a_token_sees(tmp_path):
+    out = _run(tmp_path, r"""
+int main() {
+    for (int len : {1, 7}) for (int w : {0, 1, 3, 100}) for (int pre : {0, 1, 4, 7}) for (int i = -1; i < len; i++) for (int j = 0; j < 9; j++) std::printf("%d", paged_sees(i, j, len, w, pre));
+    std::printf("\n%u %u\n", sat_add(0x7fffffffu, 0x7fffffffu), sat_add(3, 4));
+    std::printf("%d %d %d %d\n", paged_pages(0, 4), paged_pages(1, 4), paged_pages(16, 4), paged_pages(0x7fffffff, 0));
+}
+""").splitlines()
+    want = "".join(str(int(P.sees(i, np.int64(j), n, w, pre))) for n in (1, 7) for w in (0, 1, 3, 100) for pre in (0, 1, 4, 7) for i in range(-1, n) for j in range(9))
+    assert out[0] == want
+    assert out[1:] == ["2147483647 7", "0 1 1 2147483647"]
+
+
+def test_the_model_of_a_step():
+    """The block tables' plain form itself, on a step worked out by hand: pages of 4, a request that grows into a new page, one
+    that ends and one that is new."""
+    table = np.array([[5, 9], [2, 7], [9, 9]], np.int32)
+    ring = P.Ring([0, 1, 3, 4, 6, 8, -7, -7, -7, -7], 4, 2)          # free: 6, 8
+    got = P.tables(np.array([2, -1, 1], np.int32), np.array([3, 5, 0], np.int32), table, ring, 4, 8, 4)
+    assert got["table"].tolist() == [[5, 6], [2, 7], [8, 9]]
+    assert got["slots"].tolist() == [23, 24, 32, -1] and got["positions"].tolist() == [3, 4, 0, -1]
+    assert got["rowStart"].tolist() == [0, 2, 2, 3] and got["lensOut"].tolist() == [5, 0, 1]
+    assert got["ring"].tolist() == [0, 1, 3, 4, 6, 8, 2, 7, -7, -7] and got["ringState"].tolist() == [6, 2]
+    assert got["counts"].tolist() == [3, 2, 2, 0]
