@@ -492,7 +492,8 @@ int mg_stream_forward_token(mg_stream* s, int pos, const float* embHidden, int n
  * ordered by events), from one thread at a time -- two graphs that hold calls on one handle must not run at once.  It belongs to
  * the device that was current at its creation; calls make that device current while they run.  It takes workspace for maxReqs
  * requests and maxRows rows a step of at most maxLen positions.  headDim 64 or 128; nHeads a multiple of nKVHeads; pageSize a power
- * of two up to 4096; nPages * pageSize < 2^31; maxReqs <= 4096, maxRows <= 2^20, maxLen <= 2^24.  NULL on failure.  All of this
+ * of two from 8 to 4096; nPages * pageSize < 2^31; maxReqs <= 4096, maxRows <= 2^20, maxLen <= 2^24, maxRows * (nHeads / nKVHeads)
+ * * maxLen <= 2^40, maxReqs * maxLen <= 2^34.  NULL on failure.  All of this
  * returns MG_E_ARG where an argument does not fit, with the reason in mg_last_error; nothing is launched then. */
 typedef struct mg_paged mg_paged;
 mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, int nPages, int kvFormat, int maxReqs, int maxRows,

@@ -22,23 +22,37 @@ struct PagedStore {
 };
 hipError_t launch_paged_store(const PagedStore& p, hipStream_t s);
 
-// What a step's attention calls share, copied when the plan is made: the requests' rows, lengths and prefixes.
+// A worker's share [a, b) of the line, and the tile that it starts in
+struct PagedWorker { PagedTile tile; int a, b, tiles, pad[13]; };
+static_assert(sizeof(PagedTile) == 64 && sizeof(PagedWorker) == 128, "read as 16-byte words");
+
+// The plan that a step's attention calls share.
 struct PagedPlan {
     const int *rowStart, *lens, *prefixLens;      // the caller's
-    int* reqs;                                    // the handle's: 4 ints a request {first row, rows, length, prefix}
-    int nReqs, rows, window, maxLen;
+    PagedTile* tiles;                             // the handle's: maxTiles of them,
+    PagedWorker* workers;                         // and `nWorkers` of these
+    int nReqs, rows, window, maxLen, group, kvHalf, maxTiles, nWorkers;
 };
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s);
 
 struct PagedAttention {
     const float *q, *slopes;
     const void *K, *V;
-    const int *table, *reqs;
+    const int* table;
     float* out;
+    const PagedTile* tiles;
+    const PagedWorker* workers;
+    float* parts;              // partial results: two of every worker and KV head
+    unsigned* arrived;         // how many workers are done with a tile, [KV head][tile]; zeros between calls
+    const float* zeros;        // headDim zeros: what a position outside a tile's, or on a page that is gone, is read from
     float scale, softcap;
-    int ldq, ldo, rows, nReqs, window;
+    int ldq, ldo, window, maxTiles, nWorkers;
     PagedGeo g;
 };
+size_t paged_part_floats(const PagedGeo& g);
+int paged_max_tiles(const PagedGeo& g);
+int paged_workers(const PagedGeo& g, int nReqs, int rows);       // workers a KV head
+hipError_t paged_attention_setup(const PagedGeo& g);
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t s);
 
 }  // namespace mg

@@ -2,11 +2,13 @@
 // request lengths, and rotary positions with the K/V rows stored by slot.  The attention that reads the pages is in paged_attn.hip.
 #include "paged.h"
 
+#include <cmath>
 #include <new>
 #include <string>
 
 #include "../../include/mongoose_hip.h"
 #include "fused_infer.h"
+#include "kernels.h"
 
 namespace mg {
 
@@ -207,8 +209,13 @@ struct OnDevice {
 struct mg_paged {
     mg::PagedGeo g;
     int device;
-    int* reqs;             // 4 ints a request: {first row, rows, length, prefix}
-    int planReqs, planRows, planWindow;      // the last plan (planReqs < 0: none yet)
+    char* mem;             // one allocation: zeros, tiles, workers, arrival counts, partial results
+    float* zeros;
+    mg::PagedTile* tiles;
+    mg::PagedWorker* workers;
+    unsigned* arrived;
+    float* parts;
+    int planReqs, planRows, planWindow, planWorkers;      // the last plan (planReqs < 0: none yet)
 };
 
 namespace {
@@ -249,19 +256,34 @@ mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, i
     h->g = g;
     h->device = device;
     h->planReqs = -1;
-    if (hipMalloc(reinterpret_cast<void**>(&h->reqs), (size_t)g.maxReqs * 16) != hipSuccess) {
+    const size_t tiles = (size_t)mg::paged_max_tiles(g), workers = (size_t)mg::paged_workers(g, g.maxReqs, g.maxRows), heads = (size_t)g.nKVHeads;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
+    const size_t oZeros = take((size_t)g.headDim * 4), oArrived = take(heads * tiles * 4), clear = at;      // (the part that starts as zeros)
+    const size_t oTiles = take(tiles * sizeof(mg::PagedTile)), oWorkers = take(workers * sizeof(mg::PagedWorker));
+    const size_t oParts = take(heads * workers * 2 * mg::paged_part_floats(g) * 4);
+    hipError_t e = hipMalloc(reinterpret_cast<void**>(&h->mem), at);
+    if (e == hipSuccess) e = mg::launch_fill_zero(h->mem, clear, nullptr);
+    if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
+    if (e == hipSuccess) e = mg::paged_attention_setup(g);
+    if (e != hipSuccess) {
         (void)hipGetLastError();
-        mg::set_error("mg_paged_create: out of device memory");
+        mg::set_error("mg_paged_create: " + std::to_string(at) + " bytes of workspace: " + hipGetErrorString(e));
         mg_paged_destroy(h);
         return nullptr;
     }
+    h->zeros = reinterpret_cast<float*>(h->mem + oZeros);
+    h->arrived = reinterpret_cast<unsigned*>(h->mem + oArrived);
+    h->tiles = reinterpret_cast<mg::PagedTile*>(h->mem + oTiles);
+    h->workers = reinterpret_cast<mg::PagedWorker*>(h->mem + oWorkers);
+    h->parts = reinterpret_cast<float*>(h->mem + oParts);
     return h;
 }
 void mg_paged_destroy(mg_paged* h) {
     if (!h) return;
     {
         mg::OnDevice guard(h->device);
-        if (h->reqs) (void)hipFree(h->reqs);
+        if (h->mem) (void)hipFree(h->mem);
     }
     delete h;
 }
@@ -288,9 +310,11 @@ int mg_paged_store(mg_paged* h, const float* q, const float* k, const float* v, 
 int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int window, const int* prefixLens, void* stream) {
     PAGED(h, "mg_paged_plan");
     if (const char* why = mg::paged_plan_refusal(h->g, rowStart, lens, nReqs, rows, window, prefixLens)) return refuse("mg_paged_plan", why);
-    mg::PagedPlan p{rowStart, lens, prefixLens, h->reqs, nReqs, rows, window, h->g.maxLen};
+    const mg::PagedGeo& g = h->g;
+    const int workers = mg::paged_workers(g, nReqs, rows);
+    mg::PagedPlan p{rowStart, lens, prefixLens, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, mg::paged_max_tiles(g), workers};
     const int rc = launched("mg_paged_plan", mg::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
-    if (rc == MG_OK) { h->planReqs = nReqs; h->planRows = rows; h->planWindow = window; }
+    if (rc == MG_OK) { h->planReqs = nReqs; h->planRows = rows; h->planWindow = window; h->planWorkers = workers; }
     return rc;
 }
 int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, const void* V, const int* table, float* out, int ldo, float scale,
@@ -299,7 +323,9 @@ int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, cons
     if (h->planReqs < 0) { mg::set_error("mg_paged_attention: no plan yet (mg_paged_plan)"); return MG_E_STATE; }
     if (h->planReqs == 0 || h->planRows == 0) return MG_OK;
     if (const char* why = mg::paged_attention_refusal(h->g, q, ldq, K, V, table, out, ldo, scale, softcap, slopes)) return refuse("mg_paged_attention", why);
-    mg::PagedAttention p{q, slopes, K, V, table, h->reqs, out, scale, softcap, ldq, ldo, h->planRows, h->planReqs, h->planWindow, h->g};
+    const mg::PagedGeo& g = h->g;
+    mg::PagedAttention p{q, slopes, K, V, table, out, h->tiles, h->workers, h->parts, h->arrived, h->zeros,
+                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, ldq, ldo, h->planWindow, mg::paged_max_tiles(g), h->planWorkers, g};
     return launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
 }
 

@@ -12,8 +12,9 @@
 
 namespace mg {
 
-// Limits of a handle: the block-table kernel holds three sums a request in LDS (48 KB); a distance between positions is exact in fp32.
-constexpr int PAGED_MAX_REQS = 4096, PAGED_MAX_LEN = 1 << 24, PAGED_MAX_ROWS = 1 << 20, PAGED_MAX_PAGE = 4096, PAGED_MAX_GROUP = 128;
+// Limits of a handle: the block-table kernel holds three sums a request in LDS (48 KB); a distance between positions is exact in
+// fp32; a page holds whole runs of eight positions, the finest run that the attention looks up a page for.
+constexpr int PAGED_MAX_REQS = 4096, PAGED_MAX_LEN = 1 << 24, PAGED_MAX_ROWS = 1 << 20, PAGED_MIN_PAGE = 8, PAGED_MAX_PAGE = 4096, PAGED_MAX_GROUP = 128;
 
 struct PagedGeo {
     int nHeads, nKVHeads, headDim, pageSize, nPages, kvHalf, maxReqs, maxRows, maxLen;
@@ -29,12 +30,14 @@ inline const char* paged_geo(PagedGeo& g, int nHeads, int nKVHeads, int headDim,
     if (headDim != 64 && headDim != 128) return "headDim must be 64 or 128";
     if (nKVHeads <= 0 || nHeads <= 0 || nHeads % nKVHeads != 0) return "nHeads must be a positive multiple of nKVHeads";
     if (nHeads / nKVHeads > PAGED_MAX_GROUP || nHeads > 65536) return "at most 128 query heads a KV head and 65536 in all";
-    if (pageSize <= 0 || pageSize > PAGED_MAX_PAGE || (pageSize & (pageSize - 1))) return "pageSize must be a power of two up to 4096";
+    if (pageSize < PAGED_MIN_PAGE || pageSize > PAGED_MAX_PAGE || (pageSize & (pageSize - 1))) return "pageSize must be a power of two from 8 to 4096";
     if (nPages <= 0 || (long long)nPages * pageSize > 0x7fffffffll) return "nPages must be positive and nPages * pageSize below 2^31";
     if (kvFormat != 0 && kvFormat != 1) return "kvFormat must be 0 (fp32) or 1 (fp16)";
     if (maxReqs <= 0 || maxReqs > PAGED_MAX_REQS) return "maxReqs must be between 1 and 4096";
     if (maxRows <= 0 || maxRows > PAGED_MAX_ROWS) return "maxRows must be between 1 and 2^20";
     if (maxLen <= 0 || maxLen > PAGED_MAX_LEN) return "maxLen must be between 1 and 2^24";
+    if ((long long)maxRows * (nHeads / nKVHeads) > (1ll << 40) / maxLen) return "maxRows * (nHeads / nKVHeads) * maxLen must be at most 2^40";
+    if ((long long)maxReqs * maxLen > (1ll << 34)) return "maxReqs * maxLen must be at most 2^34";
     g.nHeads = nHeads; g.nKVHeads = nKVHeads; g.headDim = headDim; g.pageSize = pageSize; g.nPages = nPages; g.kvHalf = kvFormat;
     g.maxReqs = maxReqs; g.maxRows = maxRows; g.maxLen = maxLen;
     g.group = nHeads / nKVHeads;
@@ -107,7 +110,54 @@ MG_HD unsigned sat_add(unsigned a, unsigned b) {
 MG_HD int paged_pages(int len, int pageShift) { return (int)(((unsigned)len + (1u << pageShift) - 1) >> pageShift); }
 // Whether the token at position i of a request of `len` positions sees position j.
 MG_HD bool paged_sees(int i, int j, int len, int window, int prefix) {
-    return j < len && ((j <= i && (window == 0 || j > i - window)) || j < prefix);
+    return (j < len) & (((j <= i) & ((window == 0) | (j > i - window))) | (j < prefix));
+}
+
+// ---------------------------------------------------------------------------
+// The plan of an attention call.  The rows of a request under one KV head (its new tokens x the head group, token by token) are cut
+// into tiles of tileRows, the positions a tile sees into units of unitKeys.  All tiles of a batch, one behind the other, make a line
+// of cost -- PAGED_TILE_COST for a tile's own start and end, then `weight` for each of its units -- that is cut into equal shares, one
+// a worker: any mix of long, short, one and many requests keeps every CU busy to the end.  A tile whose units fall to several
+// workers is put together by the last of them to finish.  The line is the same for every KV head.
+// ---------------------------------------------------------------------------
+constexpr int PAGED_TILE_COST = 1;
+
+struct PagedTile {
+    int req, row0, rows, len, prefix;   // the request, its first row and number of rows in the batch, its length and prefix
+    int first;                          // the tile's first row among the request's rows x group
+    int cost0;                          // where the tile starts on the line
+    int unit0, units;                   // the units it sees
+    int worker0, worker1;               // the first and last worker that have some of them
+    int index;                          // its number
+    int tileRows, unitKeys, weight;     // its kind
+    int pad;
+};
+
+// The positions [begin, end) that rows first .. first + tileRows - 1 of a request see some of, and the positions of its first and last token.
+struct PagedSpan { int begin, end, pos0, pos1; };
+MG_HD PagedSpan paged_span(int rows, int len, int prefix, int window, int group, int first, int tileRows) {
+    const int all = rows * group;
+    const int last = (first + tileRows < all ? first + tileRows : all) - 1;
+    PagedSpan s;
+    s.pos0 = len - rows + first / group;
+    s.pos1 = len - rows + last / group;
+    s.end = s.pos1 + 1 > prefix ? s.pos1 + 1 : prefix;
+    s.begin = window > 0 && prefix == 0 && s.pos0 - window + 1 > 0 ? s.pos0 - window + 1 : 0;
+    return s;
+}
+MG_HD void paged_units(PagedTile& t, int window, int group) {
+    const PagedSpan s = paged_span(t.rows, t.len, t.prefix, window, group, t.first, t.tileRows);
+    t.unit0 = s.begin / t.unitKeys;
+    t.units = s.end > s.begin ? (s.end + t.unitKeys - 1) / t.unitKeys - t.unit0 : 0;
+}
+// Where worker w's share of a line of `cost` starts; workers <= cost / weight, so that each has a unit of every tile that it spans.
+MG_HD int paged_share(int cost, int workers, int w) { return (int)((long long)cost * w / workers); }
+MG_HD int paged_worker_of(int cost, int workers, int x) { return (int)((((long long)x + 1) * workers - 1) / cost); }
+// The units [u0, u1) of a tile that start within the share [a, b).
+MG_HD int paged_unit_at(const PagedTile& t, int a) {
+    const int x = a - (t.cost0 + PAGED_TILE_COST);
+    const int u = x <= 0 ? 0 : (x + t.weight - 1) / t.weight;
+    return u < t.units ? u : t.units;
 }
 
 // Why mg_paged_tables changes nothing

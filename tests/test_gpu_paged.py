@@ -134,8 +134,8 @@ def _filled(rng, lens, page, width, nPages, free, head):
 
 
 @pytest.mark.parametrize("inPlace", [True, False])
-@pytest.mark.parametrize("n,page,most,rows", [(1, 16, 1, 1), (3, 1, 5, 40), (64, 16, 1, 64), (65, 16, 1, 128), (100, 8, 40, 5000), (300, 128, 9, 1024), (300, 128, 9, 1500),
-                                             (1000, 16, 3, 3000), (1025, 32, 1, 1025), (4096, 4, 2, 8200), (2, 64, 3000, 6001)])
+@pytest.mark.parametrize("n,page,most,rows", [(1, 16, 1, 1), (3, 8, 5, 40), (64, 16, 1, 64), (65, 16, 1, 128), (100, 8, 40, 5000), (300, 128, 9, 1024), (300, 128, 9, 1500),
+                                             (1000, 16, 3, 3000), (1025, 32, 1, 1025), (4096, 8, 2, 8200), (2, 64, 3000, 6001)])
 def test_tables(hip, bufs, n, page, most, rows, inPlace):
     print(f"tables n={n} page={page} most={most} rows={rows} inPlace={inPlace}", flush=True)
     rng = np.random.default_rng(n + page)
@@ -203,11 +203,11 @@ def test_tables_that_do_not_fit_change_nothing(hip, bufs, what, why, inPlace):
 
 def test_tables_with_entries_that_are_no_page(hip, bufs):
     """A page that is gone (-1, or past the pool) leaves its rows without a slot; nothing is read or written through it."""
-    lens, new = np.array([5, 8, 0], np.int32), np.array([4, 1, 3], np.int32)
-    step = Step(hip, bufs, 4, 10, 3, 8, 16)
+    lens, new = np.array([13, 16, 0], np.int32), np.array([4, 1, 3], np.int32)
+    step = Step(hip, bufs, 8, 10, 3, 8, 32)
     table = np.array([[3, -1, -9, -9], [7, 10, -9, -9], [-9] * 4], np.int32)
     got = step.run(new, lens, table, P.Ring([1, 0x7fffffff, 2, 4, 5, 6, 8, 9, 0, 0], 0, 8), 8, False)
-    assert got["slots"].tolist() == [-1, -1, -1, 4, -1, 8, 9, 10] and got["counts"][3] == 0
+    assert got["slots"].tolist() == [-1, -1, -1, 8, -1, 16, 17, 18] and got["counts"][3] == 0
 
 
 def test_tables_of_no_requests(hip, bufs):
@@ -279,9 +279,9 @@ def test_store(hip, bufs, heads, kv, hd, half, rows, pad, inPlace):
 def test_store_overflows_to_infinity_in_fp16(hip, bufs):
     x = np.full((1, 3 * 64), 7e4, np.float32)
     z = np.zeros((1, 32), np.float32)
-    h = E.NewHIPPaged(hip, 1, 1, 64, 1, 1, 1, 1, 1, 1)
-    K = bufs.up(np.zeros(64, np.float16))
-    V = bufs.up(np.zeros(64, np.float16))
+    h = E.NewHIPPaged(hip, 1, 1, 64, 8, 1, 1, 1, 1, 1)
+    K = bufs.up(np.zeros(512, np.float16))
+    V = bufs.up(np.zeros(512, np.float16))
     d = bufs.up(x)
     one, q = bufs.up(z + 1), bufs.up(np.zeros(64, np.float32))
     p = d.DevicePtr()
@@ -371,7 +371,7 @@ class Case:
 SHAPES = [(14, 2, 64, 0), (14, 2, 64, 1), (32, 8, 128, 1), (8, 2, 128, 0), (4, 4, 64, 1), (3, 3, 128, 0), (40, 2, 128, 1), (32, 1, 64, 0), (17, 1, 128, 1)]
 
 
-@pytest.mark.parametrize("page", [1, 16, 128])
+@pytest.mark.parametrize("page", [8, 16, 128])
 @pytest.mark.parametrize("heads,kv,hd,half", SHAPES)
 def test_one_token_a_request(hip, bufs, heads, kv, hd, half, page):
     lens = [1, 2, 15, 16, 17, 31, 32, 33, 63, 64, 65, 127, 128, 129, 255, 257, 500, 1023]
@@ -386,7 +386,7 @@ def test_one_long_request(hip, bufs, heads, kv, hd, half, length):
     Case(hip, bufs, heads, kv, hd, half, 64, [1], [length], seed=length).check()
 
 
-@pytest.mark.parametrize("page", [4, 32, 4096])
+@pytest.mark.parametrize("page", [8, 32, 4096])
 @pytest.mark.parametrize("heads,kv,hd,half", SHAPES)
 def test_chunks(hip, bufs, heads, kv, hd, half, page):
     """Fresh prompts, chunks behind cached positions, drafted tokens, single tokens; odd lengths."""

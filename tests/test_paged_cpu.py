@@ -25,9 +25,11 @@ GOOD = dict(nHeads=14, nKVHeads=2, headDim=64, pageSize=16, nPages=100, kvFormat
 @pytest.mark.parametrize("change,why", [
     (dict(headDim=80), "headDim"), (dict(nHeads=15), "multiple"), (dict(nKVHeads=0), "multiple"), (dict(nHeads=-14), "multiple"),
     (dict(nHeads=129, nKVHeads=1), "128 query heads"), (dict(pageSize=0), "power of two"), (dict(pageSize=24), "power of two"),
-    (dict(pageSize=8192), "power of two"), (dict(nPages=0), "nPages"), (dict(nPages=1 << 27), "2^31"), (dict(kvFormat=2), "kvFormat"),
+    (dict(pageSize=8192), "power of two"), (dict(pageSize=4), "power of two"), (dict(nPages=0), "nPages"), (dict(nPages=1 << 27), "2^31"), (dict(kvFormat=2), "kvFormat"),
     (dict(maxReqs=0), "maxReqs"), (dict(maxReqs=4097), "maxReqs"), (dict(maxRows=0), "maxRows"), (dict(maxRows=(1 << 20) + 1), "maxRows"),
-    (dict(maxLen=0), "maxLen"), (dict(maxLen=(1 << 24) + 1), "maxLen")])
+    (dict(maxLen=0), "maxLen"), (dict(maxLen=(1 << 24) + 1), "maxLen"),
+    (dict(maxRows=1 << 20, maxLen=1 << 18), "2^40"),
+    (dict(maxReqs=4096, maxLen=1 << 23), "2^34")])
 def test_create_refuses(change, why):
     assert lib.mg_paged_create(*{**GOOD, **change}.values()) is None
     assert why in E.last_error(), E.last_error()
@@ -106,3 +108,65 @@ def test_the_model_of_a_step():
     assert got["rowStart"].tolist() == [0, 2, 2, 3] and got["lensOut"].tolist() == [5, 0, 1]
     assert got["ring"].tolist() == [0, 1, 3, 4, 6, 8, 2, 7, -7, -7] and got["ringState"].tolist() == [6, 2]
     assert got["counts"].tolist() == [3, 2, 2, 0]
+
+
+@pytest.mark.parametrize("tileRows,unitKeys,weight", [(16, 128, 1), (16, 64, 1), (128, 64, 2), (128, 64, 3)])
+def test_the_plan_gives_every_unit_to_one_worker(tmp_path, tileRows, unitKeys, weight):
+    """Random batches: every position that a token sees is in its tile's units, every unit in exactly one worker's share, the workers of
+    a tile are all of worker0 .. worker1, no two partial results share a place, and a tile without units has one worker."""
+    out = _run(tmp_path, r"""
+#include <random>
+#include <set>
+int main() {
+    std::mt19937 rng(7);
+    auto rnd = [&](int a, int b) { return a + (int)(rng() %% (unsigned)(b - a + 1)); };
+    long long split = 0, empty = 0;
+    for (int it = 0; it < 400; it++) {
+        const int group = rnd(1, 9), n = rnd(1, 12), window = rnd(0, 2) ? 0 : rnd(1, 300), most = rnd(1, 3) == 1 ? rnd(1, 3) : rnd(1, 200);
+        std::vector<PagedTile> tiles;
+        long long cost = 0;
+        for (int r = 0; r < n; r++) {
+            const int rows = rnd(0, 2) ? rnd(0, 3) : rnd(0, 60), len = rnd(0, 20) ? rnd(0, 40) + rnd(0, 1) * rnd(0, 3000) : 0, prefix = rnd(0, 3) ? 0 : rnd(0, len);
+            for (int f = 0; f < rows * group; f += %(tileRows)d) {
+                PagedTile t{};
+                t.req = r; t.rows = rows; t.len = len; t.prefix = prefix; t.first = f; t.index = (int)tiles.size();
+                t.tileRows = %(tileRows)d; t.unitKeys = %(unitKeys)d; t.weight = %(weight)d;
+                paged_units(t, window, group);
+                t.cost0 = (int)cost;
+                cost += PAGED_TILE_COST + t.units * t.weight;
+                for (int q = f; q < std::min(f + t.tileRows, rows * group); q++)
+                    for (int j = 0; j < len; j++)
+                        if (paged_sees(len - rows + q / group, j, len, window, prefix) && (j / t.unitKeys < t.unit0 || j / t.unitKeys >= t.unit0 + t.units)) { std::printf("position %%d\n", j); return 0; }
+                const PagedSpan s = paged_span(rows, len, prefix, window, group, f, t.tileRows);
+                if (s.begin < 0 || s.end > len || s.pos1 >= len) { std::printf("span\n"); return 0; }
+                tiles.push_back(t);
+            }
+        }
+        if (tiles.empty()) continue;
+        const int C = (int)cost, workers = std::max(1, std::min(most, C / %(weight)d));
+        std::set<int> places;
+        std::vector<int> seen(tiles.size(), 0), zero(tiles.size(), 0), done(tiles.size(), 0);
+        for (auto& t : tiles) if (t.units) { t.worker0 = paged_worker_of(C, workers, t.cost0 + PAGED_TILE_COST); t.worker1 = paged_worker_of(C, workers, t.cost0 + PAGED_TILE_COST + (t.units - 1) * t.weight); }
+        for (int w = 0; w < workers; w++) {
+            const int a = paged_share(C, workers, w), b = paged_share(C, workers, w + 1);
+            size_t i = tiles.size() - 1;
+            while (tiles[i].cost0 > a) i--;
+            for (; i < tiles.size() && tiles[i].cost0 < b; i++) {
+                const PagedTile& t = tiles[i];
+                const int u0 = paged_unit_at(t, a), u1 = paged_unit_at(t, b);
+                if (t.units == 0) { zero[i] += a <= t.cost0; continue; }
+                if (u0 > u1 || (u0 < u1 && u0 != seen[i])) { std::printf("order\n"); return 0; }
+                if ((u0 < u1) != (w >= t.worker0 && w <= t.worker1)) { std::printf("workers %%d %%d..%%d\n", w, t.worker0, t.worker1); return 0; }
+                if (u0 < u1) { seen[i] = u1; done[i]++; }
+                if (u0 < u1 && t.worker0 != t.worker1) { split++; if (!places.insert(w * 2 + (w == t.worker0)).second) { std::printf("place\n"); return 0; } }
+            }
+        }
+        for (size_t i = 0; i < tiles.size(); i++) {
+            if (tiles[i].units == 0 ? zero[i] != 1 : seen[i] != tiles[i].units || done[i] != tiles[i].worker1 - tiles[i].worker0 + 1) { std::printf("left out\n"); return 0; }
+            empty += tiles[i].units == 0;
+        }
+    }
+    std::printf(split > 1000 && empty > 10 ? "ok\n" : "too few %%lld %%lld\n", split, empty);
+}
+""" % dict(tileRows=tileRows, unitKeys=unitKeys, weight=weight))
+    assert out == "ok\n", out
