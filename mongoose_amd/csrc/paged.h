@@ -29,9 +29,9 @@ static_assert(sizeof(PagedTile) == 64 && sizeof(PagedWorker) == 128, "read as 16
 // The plan that a step's attention calls share.
 struct PagedPlan {
     const int *rowStart, *lens, *prefixLens;      // the caller's
-    PagedTile* tiles;                             // the handle's: maxTiles of them,
-    PagedWorker* workers;                         // and `nWorkers` of these
-    int nReqs, rows, window, maxLen, group, kvHalf, maxTiles, nWorkers;
+    PagedTile* tiles;                             // the handle's: maxTiles of them, for narrow tiles and again for wide ones,
+    PagedWorker* workers;                         // and maxWorkers of these
+    int nReqs, rows, window, maxLen, group, kvHalf, maxTiles, maxWorkers, nWorkers, narrowRows;
 };
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s);
 
@@ -40,18 +40,20 @@ struct PagedAttention {
     const void *K, *V;
     const int* table;
     float* out;
-    const PagedTile* tiles;
+    const PagedTile* tiles;    // narrow tiles' and wide ones', maxTiles and maxWorkers apart, as in the plan
     const PagedWorker* workers;
     float* parts;              // partial results: two of every worker and KV head
     unsigned* arrived;         // how many workers are done with a tile, [KV head][tile]; zeros between calls
     const float* zeros;        // headDim zeros: what a position outside a tile's, or on a page that is gone, is read from
+    size_t partStride;
     float scale, softcap;
-    int ldq, ldo, window, maxTiles, nWorkers;
+    int ldq, ldo, window, maxTiles, maxWorkers, nWorkers, wide;
     PagedGeo g;
 };
 size_t paged_part_floats(const PagedGeo& g);
 int paged_max_tiles(const PagedGeo& g);
 int paged_workers(const PagedGeo& g, int nReqs, int rows);       // workers a KV head
+int paged_narrow_rows(const PagedGeo& g, int rows);              // requests of up to so many rows a KV head have narrow tiles
 hipError_t paged_attention_setup(const PagedGeo& g);
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t s);
 

@@ -215,7 +215,8 @@ struct mg_paged {
     mg::PagedWorker* workers;
     unsigned* arrived;
     float* parts;
-    int planReqs, planRows, planWindow, planWorkers;      // the last plan (planReqs < 0: none yet)
+    int maxTiles, maxWorkers;
+    int planReqs, planRows, planWindow, planWorkers, planWide;      // the last plan (planReqs < 0: none yet)
 };
 
 namespace {
@@ -260,7 +261,7 @@ mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, i
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
     const size_t oZeros = take((size_t)g.headDim * 4), oArrived = take(heads * tiles * 4), clear = at;      // (the part that starts as zeros)
-    const size_t oTiles = take(tiles * sizeof(mg::PagedTile)), oWorkers = take(workers * sizeof(mg::PagedWorker));
+    const size_t oTiles = take(2 * tiles * sizeof(mg::PagedTile)), oWorkers = take(2 * workers * sizeof(mg::PagedWorker));
     const size_t oParts = take(heads * workers * 2 * mg::paged_part_floats(g) * 4);
     hipError_t e = hipMalloc(reinterpret_cast<void**>(&h->mem), at);
     if (e == hipSuccess) e = mg::launch_fill_zero(h->mem, clear, nullptr);
@@ -272,6 +273,8 @@ mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, i
         mg_paged_destroy(h);
         return nullptr;
     }
+    h->maxTiles = (int)tiles;
+    h->maxWorkers = (int)workers;
     h->zeros = reinterpret_cast<float*>(h->mem + oZeros);
     h->arrived = reinterpret_cast<unsigned*>(h->mem + oArrived);
     h->tiles = reinterpret_cast<mg::PagedTile*>(h->mem + oTiles);
@@ -311,10 +314,13 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
     PAGED(h, "mg_paged_plan");
     if (const char* why = mg::paged_plan_refusal(h->g, rowStart, lens, nReqs, rows, window, prefixLens)) return refuse("mg_paged_plan", why);
     const mg::PagedGeo& g = h->g;
-    const int workers = mg::paged_workers(g, nReqs, rows);
-    mg::PagedPlan p{rowStart, lens, prefixLens, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, mg::paged_max_tiles(g), workers};
+    const int workers = mg::paged_workers(g, nReqs, rows), narrow = mg::paged_narrow_rows(g, rows);
+    mg::PagedPlan p{rowStart, lens, prefixLens, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, h->maxTiles, h->maxWorkers, workers, narrow};
     const int rc = launched("mg_paged_plan", mg::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
-    if (rc == MG_OK) { h->planReqs = nReqs; h->planRows = rows; h->planWindow = window; h->planWorkers = workers; }
+    if (rc == MG_OK) {
+        h->planReqs = nReqs; h->planRows = rows; h->planWindow = window; h->planWorkers = workers;
+        h->planWide = (long long)rows * g.group > narrow;
+    }
     return rc;
 }
 int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, const void* V, const int* table, float* out, int ldo, float scale,
@@ -324,8 +330,8 @@ int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, cons
     if (h->planReqs == 0 || h->planRows == 0) return MG_OK;
     if (const char* why = mg::paged_attention_refusal(h->g, q, ldq, K, V, table, out, ldo, scale, softcap, slopes)) return refuse("mg_paged_attention", why);
     const mg::PagedGeo& g = h->g;
-    mg::PagedAttention p{q, slopes, K, V, table, out, h->tiles, h->workers, h->parts, h->arrived, h->zeros,
-                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, ldq, ldo, h->planWindow, mg::paged_max_tiles(g), h->planWorkers, g};
+    mg::PagedAttention p{q, slopes, K, V, table, out, h->tiles, h->workers, h->parts, h->arrived, h->zeros, mg::paged_part_floats(g),
+                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, ldq, ldo, h->planWindow, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWide, g};
     return launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
 }
 

@@ -16,20 +16,30 @@
 namespace mg {
 
 constexpr int PT = 1024;                  // threads of the plan
-constexpr int NARROW = 16;                // rows of a tile
+constexpr int NARROW = 16, WIDE = 128;    // rows of a tile
 constexpr int PLAN_LDS_TILES = 4096;      // tiles whose places on the line the plan holds in LDS
 constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
+typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef unsigned uint2_t __attribute__((ext_vector_type(2)));
 typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
 
-static int narrow_keys(int kvHalf) { return kvHalf ? 128 : 64; }       // positions of a unit: four waves x a step of 32 or 16
-int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / NARROW) + g.maxReqs; }
-size_t paged_part_floats(const PagedGeo& g) { return (size_t)NARROW * (g.headDim + 2); }
+// Positions of a unit: a narrow tile's four waves take 32 of an fp16 cache or 16 of an fp32 one each, a wide tile's share them.
+MG_HD int narrow_keys(int kvHalf) { return kvHalf ? 128 : 64; }
+MG_HD int wide_keys(int kvHalf) { return kvHalf ? 64 : 32; }
+
+// A request of up to 16 rows a KV head goes to the kernel that waits for memory, others to the one that waits for the matrix units.
+int paged_narrow_rows(const PagedGeo& g, int rows) {
+    return (long long)rows * g.group <= 128 ? 128 : NARROW;
+}
+int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + WIDE / NARROW; }
+size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
 // Two workgroups a CU, in turns of the KV heads; fewer where the batch cannot have that many units.
 int paged_workers(const PagedGeo& g, int nReqs, int rows) {
-    const long long tiles = (long long)rows * g.group / NARROW + nReqs, units = tiles * (g.maxLen / narrow_keys(g.kvHalf) + 2);
+    const long long tiles = (long long)rows * g.group / NARROW + nReqs, units = tiles * (g.maxLen / 32 + 2);
     const long long most = 512 / g.nKVHeads > 0 ? 512 / g.nKVHeads : 1;
     return (int)(units < 1 ? 1 : units < most ? units : most);
 }
@@ -62,7 +72,11 @@ __device__ __forceinline__ int4 plan_request(const PagedPlan& p, int r) {
     const int len = max(0, min(p.lens[r], p.maxLen));
     return make_int4(first, last - first, len, p.prefixLens ? max(0, min(p.prefixLens[r], len)) : 0);
 }
-__global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p, int unitKeys) {
+__global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
+    const bool wide = blockIdx.x != 0;
+    const int tileRows = wide ? WIDE : NARROW, unitKeys = wide ? wide_keys(p.kvHalf) : narrow_keys(p.kvHalf);
+    p.tiles += wide ? p.maxTiles : 0;
+    p.workers += wide ? p.maxWorkers : 0;
     __shared__ unsigned tile0[PAGED_MAX_REQS + 1], place[PLAN_LDS_TILES], part[PT / 64];
     const int tid = threadIdx.x;
     unsigned nTiles = 0;
@@ -70,7 +84,10 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p, int unitKey
     for (int r0 = 0; r0 < p.nReqs; r0 += PT) {
         const int r = r0 + tid;
         unsigned n = 0;
-        if (r < p.nReqs) n = (unsigned)((plan_request(p, r).y * p.group + NARROW - 1) / NARROW);
+        if (r < p.nReqs) {
+            const long long rows = (long long)plan_request(p, r).y * p.group;
+            if (wide == (rows > p.narrowRows)) n = (unsigned)((rows + tileRows - 1) / tileRows);
+        }
         n = plan_scan(n, nTiles, part);
         if (r < p.nReqs) tile0[r + 1] = n;
     }
@@ -89,9 +106,9 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p, int unitKey
             }
             const int4 rq = plan_request(p, lo);
             t.req = lo; t.row0 = rq.x; t.rows = rq.y; t.len = rq.z; t.prefix = rq.w;
-            t.first = (int)(i - tile0[lo]) * NARROW;
+            t.tileRows = tileRows; t.unitKeys = unitKeys; t.weight = 1;
+            t.first = (int)(i - tile0[lo]) * tileRows;
             t.index = (int)i;
-            t.tileRows = NARROW; t.unitKeys = unitKeys; t.weight = 1;
             paged_units(t, p.window, p.group);
             c = (unsigned)(PAGED_TILE_COST + t.units * t.weight);
         }
@@ -128,7 +145,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p, int unitKey
     }
 }
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s) {
-    hipLaunchKernelGGL(paged_plan_kernel, dim3(1), dim3(PT), 0, s, p, narrow_keys(p.kvHalf));
+    hipLaunchKernelGGL(paged_plan_kernel, dim3((long long)p.rows * p.group > p.narrowRows ? 2 : 1), dim3(PT), 0, s, p);
     return hipGetLastError();
 }
 
@@ -164,6 +181,12 @@ __device__ __forceinline__ PagedTile tile_at(const PagedTile* from) {
     for (int i = 0; i < (int)(sizeof(PagedTile) / 4); i++) x[i] = __builtin_amdgcn_readfirstlane(x[i]);
     return t;
 }
+// A value to be worked with anew where it is asked for: what is made of it (addresses, masks) is not worth registers across a loop
+__device__ __forceinline__ int anew(int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+}
+__device__ __forceinline__ int thread_anew() { return anew(threadIdx.x); }
 // What a tile's code needs of its row, on the lane's behalf
 struct PagedRow { int token, head, pos; };
 __device__ __forceinline__ PagedRow paged_row(const PagedTile& t, int group, int kvh, int row) {
@@ -178,43 +201,29 @@ __device__ __forceinline__ const char* kv_row(const char* pool, const char* zero
     return (held ? pool : zeros) + (size_t)at * rowBytes;
 }
 
-// The workgroup's result of a tile: row r at o + r * HD (LDS), maxima and sums behind; written out, or as a partial result with the
-// last worker to finish putting the tile together.
+// Where a worker leaves its share of a tile's result: rows of headDim floats, then the rows' maxima and sums.
+__device__ __forceinline__ float* part_of(const PagedAttention& p, const PagedTile& t, int kvh, int w) {
+    return p.parts + (((size_t)kvh * p.nWorkers + w) * 2 + (w == t.worker0)) * p.partStride;
+}
+// After a worker has stored its share (through to memory): the last one to come here adds the shares up and writes the rows.
 template <int HD, int ROWS>
-__device__ __forceinline__ void finish(const PagedAttention& p, const PagedTile& t, int kvh, int w, const float* o, const float* ms, const float* ls, float* scratch) {
-    const int tid = threadIdx.x, R = min(ROWS, t.rows * p.g.group - t.first);
-    if (t.worker0 == t.worker1) {
-        for (int i = tid; i < R * (HD / 4); i += WG) {
-            const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
-            const float l = ls[row];
-            const float4 v = *reinterpret_cast<const float4*>(o + row * (HD + 4) + d);
-            const PagedRow at = paged_row(t, p.g.group, kvh, row);
-            *reinterpret_cast<float4*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) =
-                l == 0.f ? v : make_float4(v.x / l, v.y / l, v.z / l, v.w / l);       // (nothing seen: zeros)
-        }
-        return;
-    }
-    constexpr size_t stride = (size_t)ROWS * (HD + 2);
-    float* parts = p.parts + (size_t)kvh * p.nWorkers * 2 * stride;
-    float* mine = parts + ((size_t)w * 2 + (w == t.worker0)) * stride;
-    for (int i = tid; i < R * (HD / 4); i += WG) {
-        const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
-        store_through(mine + row * HD + d, *reinterpret_cast<const float4_t*>(o + row * (HD + 4) + d));
-    }
-    for (int i = tid; i < R; i += WG) { st_agent(mine + ROWS * HD + i, ms[i]); st_agent(mine + ROWS * HD + ROWS + i, ls[i]); }
-    __shared__ unsigned before;
+__device__ __forceinline__ void merge(const PagedAttention& p, const PagedTile& t, int kvh, float* scratch) {
+    const int tid = thread_anew(), R = min(ROWS, t.rows * p.g.group - t.first);
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     const int segs = t.worker1 - t.worker0 + 1;
     unsigned* count = p.arrived + (size_t)kvh * p.maxTiles + t.index;
-    if (tid == 0) before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    unsigned* before = reinterpret_cast<unsigned*>(scratch);
+    if (tid == 0) *before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    if (before + 1 != (unsigned)segs) return;
+    const bool last = *before + 1 == (unsigned)segs;
+    __syncthreads();
+    if (!last) return;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
     if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     // Rows' greatest maxima and sums first, into `scratch` beside every partial result's weight; then the outputs, the workgroup's
     // threads sharing out rows, columns and, where there are few of those, partial results.
-    auto part_of = [&](int s) { return parts + ((size_t)(t.worker0 + s) * 2 + (s == 0)) * stride; };
+    auto part = [&](int s) { return part_of(p, t, kvh, t.worker0 + s); };
     float* M = scratch;                   // [ROWS]
     float* den = scratch + ROWS;          // [ROWS]
     float* wt = scratch + 2 * ROWS;       // [segs in turn][R]
@@ -223,7 +232,7 @@ __device__ __forceinline__ void finish(const PagedAttention& p, const PagedTile&
     if (tid < R) {
         float m = -INFINITY;
 #pragma unroll 8
-        for (int s = 0; s < segs; s++) m = fmaxf(m, part_of(s)[ROWS * HD + tid]);
+        for (int s = 0; s < segs; s++) m = fmaxf(m, part(s)[ROWS * HD + tid]);
         M[tid] = m == -INFINITY ? 0.f : m;
         den[tid] = 0.f;
     }
@@ -233,12 +242,12 @@ __device__ __forceinline__ void finish(const PagedAttention& p, const PagedTile&
     for (int s0 = 0; s0 < segs; s0 += perTurn) {
         const int n = min(perTurn, segs - s0);
         __syncthreads();
-        for (int i = tid; i < n * R; i += WG) wt[i] = __builtin_amdgcn_exp2f(part_of(s0 + i / R)[ROWS * HD + i % R] - M[i % R]);
+        for (int i = tid; i < n * R; i += WG) wt[i] = __builtin_amdgcn_exp2f(part(s0 + i / R)[ROWS * HD + i % R] - M[i % R]);
         __syncthreads();
         if (tid < R) {
             float d = den[tid];
 #pragma unroll 8
-            for (int s = 0; s < n; s++) d = fmaf(wt[s * R + tid], part_of(s0 + s)[ROWS * HD + ROWS + tid], d);
+            for (int s = 0; s < n; s++) d = fmaf(wt[s * R + tid], part(s0 + s)[ROWS * HD + ROWS + tid], d);
             den[tid] = d;
         }
 #pragma unroll
@@ -248,7 +257,7 @@ __device__ __forceinline__ void finish(const PagedAttention& p, const PagedTile&
             const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
 #pragma unroll 4
             for (int s = from; s < n; s += par) {
-                const float4 v = *reinterpret_cast<const float4*>(part_of(s0 + s) + row * HD + d);
+                const float4 v = *reinterpret_cast<const float4*>(part(s0 + s) + row * HD + d);
                 const float f = wt[s * R + row];
                 acc[k].x = fmaf(f, v.x, acc[k].x); acc[k].y = fmaf(f, v.y, acc[k].y); acc[k].z = fmaf(f, v.z, acc[k].z); acc[k].w = fmaf(f, v.w, acc[k].w);
             }
@@ -312,7 +321,7 @@ struct NarrowTile {
     float4_t o[EPL];
 
     __device__ __forceinline__ NarrowTile(const PagedAttention& p_, const PagedTile& t_, int kvh) : p(p_), t(t_) {
-        const int tid = threadIdx.x;
+        const int tid = thread_anew();
         lane = tid & 63; l16 = lane & 15; g = lane >> 4;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, NARROW);
@@ -533,7 +542,7 @@ struct NarrowTile {
             }
         }
     }
-    __device__ __forceinline__ void run(int u0, int u1) {
+    __device__ __forceinline__ void run(int u0, int u1, float* lds) {
         int here = page_of(u0), next = page_of(min(u0 + 1, u1 - 1));
         load_k(u0, here);
         load_v(u0, here);
@@ -545,6 +554,7 @@ struct NarrowTile {
             here = next;
             next = behind;
         }
+        join(lds);
     }
     // The four waves' results as one, at lds (rows of HD + 4 floats) with maxima and sums behind
     static constexpr int FLOATS = 4 * NARROW * (HD + 4) + 8 * NARROW;
@@ -560,7 +570,7 @@ struct NarrowTile {
             for (int e = 0; e < EPL; e += 4) *reinterpret_cast<float4_t*>(mine + i * EPL + e) = float4_t{o[e][i], o[e + 1][i], o[e + 2][i], o[e + 3][i]};
         if (g == 0) { wm[wave * NARROW + l16] = m; wl[wave * NARROW + l16] = l; }
         __syncthreads();
-        const int tid = threadIdx.x;
+        const int tid = thread_anew();
 #pragma unroll
         for (int i = tid; i < NARROW * (HD / 4); i += WG) {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
@@ -581,11 +591,383 @@ struct NarrowTile {
         if (tid < NARROW) { wm[tid] = M; wl[tid] = L; }
         __syncthreads();
     }
+    __device__ __forceinline__ void write(int kvh, int w, float* lds) const {
+        const float* ms = lds + 4 * NARROW * (HD + 4);
+        const float* ls = ms + 4 * NARROW;
+        const int tid = thread_anew(), R = min(NARROW, t.rows * p.g.group - t.first);
+        const bool whole = t.worker0 == t.worker1;
+        float* mine = part_of(p, t, kvh, w);
+        for (int i = tid; i < R * (HD / 4); i += WG) {
+            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            const float4_t v = *reinterpret_cast<const float4_t*>(lds + r * (HD + 4) + d);
+            if (!whole) { store_through(mine + r * HD + d, v); continue; }
+            const PagedRow at = paged_row(t, p.g.group, kvh, r);
+            *reinterpret_cast<float4_t*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) = ls[r] == 0.f ? v : v / ls[r];       // (nothing seen: zeros)
+        }
+        if (whole) return;
+        if (tid < R) { st_agent(mine + NARROW * HD + tid, ms[tid]); st_agent(mine + NARROW * HD + NARROW + tid, ls[tid]); }
+        merge<HD, NARROW>(p, t, kvh, lds);
+    }
 };
 
+// A tile of 128 rows: a wave takes 32 of them over all the positions, which go through LDS (two buffers, filled by loads that run a
+// unit ahead), so that a K or V row is fetched once for 128 rows.  Bound by the matrix units: 32x32 instructions, two terms a product
+// with an fp16 cache (as in NarrowTile), four K = 2 fp32 instructions a 16-byte piece with an fp32 one.
+//   K (A operand): lane l = position l%32, 16 bytes at dimensions 16 s + 8 (l/32) (fp16) or 8 s + 4 (l/32) (fp32).
+//   V (A operand): dimension l%32 of a block of 32, the positions of the lane's own probabilities -- 4 (l/32) + 0..3 of every eight --
+//     fp16 through the transposing LDS read, fp32 word by word.
+// A row's 16-byte pieces lie in LDS at piece ^ swz(row), so that neither rows of one piece nor (fp16) four rows of two meet in a bank.
 template <typename KVT, int HD, bool MOD>
-__global__ __launch_bounds__(WG, 2) void paged_attn_kernel(PagedAttention p) {
-    extern __shared__ __attribute__((aligned(16))) float lds[];
+struct WideTile {
+    static constexpr bool HALF = sizeof(KVT) == 2;
+    static constexpr int UK = HALF ? 64 : 32, NB = UK / 32, DB = HD / 32;
+    static constexpr int ROWB = HD * (int)sizeof(KVT), PR = ROWB / 16;      // bytes and 16-byte pieces of a row
+    static constexpr int RI = 64 / PR, NI = UK / RI / 4;                    // rows a load instruction brings, instructions a wave
+    static constexpr int TILEB = UK * ROWB, BUFB = 2 * TILEB;               // K, then V
+    static constexpr int QS = HALF ? HD / 16 : HD / 8;
+    static constexpr float SHIFT = HALF ? 13.f : 0.f;      // probabilities times 2^SHIFT,
+    static constexpr float LAZY = HALF ? 2.f : 8.f;        // and up to 2^LAZY more: the maximum is only moved where it grows by more
+
+    const PagedAttention& p;
+    const PagedTile& t;
+    int lane, n32, hf, wave;
+    PagedSpan span;           // the tile's
+    int pos0, pos1, begin, end;      // the wave's own rows'
+    bool active;
+    PagedRow row;
+    const int* pages;
+    const char *Kp, *Vp, *zeros;
+    size_t rowBytes;
+    static constexpr unsigned ldsBase = 0;
+    unsigned from[NI];      // the lane's offset of every load instruction from its run of eight positions
+    float c, cap, invCap, slope;
+    half8_t qh[HALF ? QS : 1], ql[HALF ? QS : 1];
+    float4_t qf[HALF ? 1 : QS];
+    float m, l;
+    float16_t o[DB];
+
+    static __device__ __forceinline__ int swz(int r) { return HALF ? ((r & 3) << 1) | ((r >> 2) & 1) : r & 7; }
+
+    __device__ __forceinline__ WideTile(const PagedAttention& p_, const PagedTile& t_, int kvh) : p(p_), t(t_) {
+        const int tid = thread_anew();
+        lane = tid & 63; n32 = lane & 31; hf = lane >> 5;
+        wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, WIDE);
+        const int mine = t.first + 32 * wave;
+        active = mine < t.rows * p.g.group;
+        const PagedSpan own = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, active ? mine : t.first, 32);
+        pos0 = own.pos0; pos1 = own.pos1; begin = own.begin; end = own.end;
+        row = paged_row(t, p.g.group, kvh, 32 * wave + n32);
+        pages = p.table + (size_t)t.req * p.g.width;
+        rowBytes = (size_t)p.g.kvDim * sizeof(KVT);
+        Kp = static_cast<const char*>(p.K) + (size_t)kvh * ROWB;
+        Vp = static_cast<const char*>(p.V) + (size_t)kvh * ROWB;
+        zeros = reinterpret_cast<const char*>(p.zeros);
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int r = (wave * NI + i) * RI + lane / PR;
+            from[i] = (unsigned)(r & 7) * (unsigned)rowBytes + (unsigned)((lane % PR) ^ swz(r)) * 16;
+        }
+        cap = p.softcap;
+        invCap = MOD && cap > 0.f ? 1.f / cap : 0.f;
+        slope = MOD && p.slopes ? p.slopes[row.head] : 0.f;
+        const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
+        c = p.scale;
+        if constexpr (HALF) {
+            float top = 0.f;
+#pragma unroll
+            for (int s = 0; s < QS; s++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float4 a = *reinterpret_cast<const float4*>(q + s * 16 + hf * 8 + 4 * j);
+                    top = fmaxf(fmaxf(top, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(a.z), fabsf(a.w)));
+                }
+            float other = top;
+            row_swap32(top, other);
+            top = fmaxf(top, other);
+            const int up = top > 0.f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+#pragma unroll
+            for (int s = 0; s < QS; s++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float4_t a = *reinterpret_cast<const float4_t*>(q + s * 16 + hf * 8 + 4 * j);
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float x = ldexpf(a[i], up);
+                        qh[s][4 * j + i] = (_Float16)x;
+                        ql[s][4 * j + i] = (_Float16)(x - (float)qh[s][4 * j + i]);
+                    }
+                }
+            c = ldexpf(c, -up);
+        } else {
+#pragma unroll
+            for (int s = 0; s < QS; s++) qf[s] = *reinterpret_cast<const float4_t*>(q + s * 8 + hf * 4);
+        }
+        if (!MOD) c *= 1.4426950408889634f;
+        m = -INFINITY;
+        l = 0.f;
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[b][i] = 0.f;
+    }
+
+    __device__ __forceinline__ int base_of(int u) const { return (t.unit0 + u) * UK; }
+    // The page of the unit's run lane % (UK / 8) of eight positions, -1 where there is none
+    __device__ __forceinline__ int page_of(int u) const {
+        const int key = min(base_of(u) + (lane & (UK / 8 - 1)) * 8, span.end - 1);
+        const int page = pages[max(key, 0) >> p.g.pageShift];
+        return page >= 0 && page < p.g.nPages ? page : -1;
+    }
+    // Loads a unit into a buffer.  A load instruction's rows are within one run of eight positions.
+    __device__ __forceinline__ void issue(int u, int mine, unsigned buf) const {
+        const int base = base_of(u);
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int r0 = (wave * NI + i) * RI, run = r0 >> 3;
+            const int page = __builtin_amdgcn_readlane(mine, run), key = base + run * 8;
+            const bool inside = page >= 0 && key >= span.begin && key + 8 <= span.end;
+            const size_t at = (size_t)(inside ? ((unsigned)page << p.g.pageShift) + ((unsigned)key & (unsigned)(p.g.pageSize - 1)) : 0u) * rowBytes;
+            const unsigned dst = ldsBase + buf * BUFB + (unsigned)r0 * ROWB;
+            if (inside) {
+                asm volatile(MG_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(from[i]), "s"(Kp + at) : "memory");
+                asm volatile(MG_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst + TILEB), "v"(from[i]), "s"(Vp + at) : "memory");
+            } else {
+                const int r = r0 + lane / PR, piece = ((lane % PR) ^ swz(r)) * 16;
+                const char* k = kv_row(Kp, zeros, rowBytes, base + r, page, span.begin, span.end, p.g.pageShift) + piece;
+                const char* v = kv_row(Vp, zeros, rowBytes, base + r, page, span.begin, span.end, p.g.pageShift) + piece;
+                asm volatile(MG_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(k) : "memory");
+                asm volatile(MG_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst + TILEB), "v"(v) : "memory");
+            }
+        }
+    }
+    static __device__ __forceinline__ uint4_t lds16(unsigned at) { return *reinterpret_cast<__attribute__((address_space(3))) const uint4_t*>(at); }
+    // S^T of a unit: element i of block b is position 32 b + 8 (i/4) + 4 hf + i%4.  mends: where a NaN comes from the second term's
+    // product with an infinite key, the first term's alone.
+    __device__ __forceinline__ void scores(unsigned K, float16_t (&S)[NB], bool mend) const {
+        const int r = anew(n32);
+        const unsigned at = K + (unsigned)r * ROWB + (unsigned)(hf ^ swz(r)) * 16;
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) S[b][i] = 0.f;
+#pragma unroll
+            for (int s = 0; s < QS; s++) {
+                if (s % 4 == 0) __builtin_amdgcn_sched_barrier(0);       // (reads for four steps at once; for all, q would not stay in registers)
+                const uint4_t k = lds16((at ^ (unsigned)(s * 32)) + b * 32 * ROWB);
+                if constexpr (HALF) {
+                    S[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, k), qh[s], S[b], 0, 0, 0);
+                    S[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, k), ql[s], S[b], 0, 0, 0);
+                } else {
+                    const float4_t kf = __builtin_bit_cast(float4_t, k);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) S[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(kf[j], qf[s][j], S[b], 0, 0, 0);
+                }
+            }
+            if constexpr (HALF)
+                if (mend) {
+                    float16_t first;
+#pragma unroll
+                    for (int i = 0; i < 16; i++) first[i] = 0.f;
+#pragma unroll
+                    for (int s = 0; s < QS; s++)
+                        first = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, lds16((at ^ (unsigned)(s * 32)) + b * 32 * ROWB)), qh[s], first, 0, 0, 0);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) S[b][i] = S[b][i] != S[b][i] ? first[i] : S[b][i];
+                }
+        }
+    }
+    // Where the lane reads V of a unit at V: position 4 hf (fp32) or 4 hf + its quad's number (fp16), dimension block 0
+    __device__ __forceinline__ unsigned v_base(unsigned V) const {
+        const int x = anew(lane), h = x >> 5;
+        if (HALF) {
+            const int i16 = x & 15, a = i16 >> 2;
+            return V + (unsigned)(4 * h + a) * ROWB + (unsigned)((2 * ((x >> 4) & 1) + ((i16 & 3) >> 1)) ^ ((a << 1) | h)) * 16 + (unsigned)(i16 & 1) * 8;
+        }
+        return V + (unsigned)(4 * h) * ROWB + (unsigned)(((x & 31) >> 2) ^ (4 * h)) * 16 + (unsigned)(x & 3) * 4;
+    }
+    // Block d of V^T P^T on top of `out`; MASKED: without the positions that a token at `pos` does not see
+    struct Weights { half8_t hi[HALF ? UK / 16 : 1], lo[HALF ? UK / 16 : 1]; };
+    template <bool MASKED>
+    __device__ __forceinline__ float16_t product(unsigned V, int d, const float16_t (&S)[NB], const Weights& w, int base, int pos, float16_t out) const {
+        if constexpr (HALF) {
+            const unsigned at = V ^ (unsigned)(d * 64);
+#pragma unroll
+            for (int kk = 0; kk < UK / 16; kk++) {
+                typedef __attribute__((address_space(3))) short4_t* lp;
+                uint2_t x = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB)));
+                uint2_t y = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB + 8 * ROWB)));
+                if (MASKED) {
+                    const int j = base + 16 * kk + 4 * hf;
+                    auto keep = [&](int k) { return (paged_sees(pos, k, t.len, p.window, t.prefix) ? 0xffffu : 0u) | (paged_sees(pos, k + 1, t.len, p.window, t.prefix) ? 0xffff0000u : 0u); };
+                    x[0] &= keep(j); x[1] &= keep(j + 2); y[0] &= keep(j + 8); y[1] &= keep(j + 10);
+                }
+                const half8_t v = __builtin_bit_cast(half8_t, uint4_t{x[0], x[1], y[0], y[1]});
+                out = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.hi[kk], out, 0, 0, 0);
+                out = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.lo[kk], out, 0, 0, 0);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                float v = *reinterpret_cast<__attribute__((address_space(3))) const float*>((V ^ (unsigned)(i % 4 * 16)) + (unsigned)(8 * (i / 4) + i % 4) * ROWB + (unsigned)d * 128);
+                if (MASKED && !paged_sees(pos, base + 8 * (i / 4) + 4 * hf + i % 4, t.len, p.window, t.prefix)) v = 0.f;
+                out = __builtin_amdgcn_mfma_f32_32x32x2f32(v, S[0][i], out, 0, 0, 0);
+            }
+        }
+        return out;
+    }
+    __device__ __forceinline__ bool values_finite(unsigned V) const {
+        bool odd = false;
+        for (int i = lane; i < UK * PR; i += 64) {
+            const uint4_t x = lds16(V + (unsigned)i * 16);
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const unsigned w = x[j];
+                if (HALF) odd |= ((w & 0x7fffu) >= 0x7c00u) | ((w & 0x7fff0000u) >= 0x7c000000u);
+                else odd |= (w & 0x7fffffffu) >= 0x7f800000u;
+            }
+        }
+        return !__any(odd);
+    }
+    // Scores to probabilities (times 2^SHIFT, over the maximum mNew); returns the lane's sum of them
+    __device__ __forceinline__ float weigh(float16_t (&S)[NB], int base, unsigned long long held, bool all, float& mNew) const {
+        const int first = base + 4 * anew(hf);            // the lane's first position
+        if constexpr (MOD) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    float x = S[b][i] * c;
+                    if (cap > 0.f) x = capped(x, cap, invCap);
+                    S[b][i] = (x - slope * (float)abs(row.pos - (first + 32 * b + 8 * (i / 4) + i % 4))) * 1.4426950408889634f;
+                }
+        }
+        if (!all) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++)
+                    if (!((held >> (4 * b + i / 4)) & 1) || !paged_sees(row.pos, first + 32 * b + 8 * (i / 4) + i % 4, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
+        }
+        float top = S[0][0];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, S[b][i]);
+        float other = top;
+        row_swap32(top, other);
+        top = fmaxf(top, other);
+        if (!MOD) top = top == -INFINITY ? top : top * c;
+        mNew = top > m + LAZY || m == -INFINITY ? fmaxf(m, top) : m;
+        const float shift = SHIFT - (mNew == -INFINITY ? 0.f : mNew);          // (a score that is a NaN stays one)
+        float ts = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                S[b][i] = __builtin_amdgcn_exp2f(MOD ? S[b][i] + shift : fmaf(S[b][i], c, shift));
+                ts += S[b][i];
+            }
+        return ts;
+    }
+    __device__ __forceinline__ void compute(int u, int mine, unsigned buf) {
+        const int base = base_of(u);
+        if (!active || base >= end || base + UK <= begin) return;
+        const unsigned K = ldsBase + buf * BUFB, V = K + TILEB;
+        const unsigned long long held = __ballot(mine >= 0);
+        constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
+        const bool all = (held & runs) == runs && (base + UK <= t.prefix || (base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window)));
+        float16_t S[NB];
+        float mNew;
+        scores(K, S, false);
+        float ts = weigh(S, base, held, all, mNew);
+        if (HALF && __any(ts != ts)) {            // (not a loop: what the masks need would be worked out ahead of it, for every unit)
+            scores(K, S, true);
+            ts = weigh(S, base, held, all, mNew);
+        }
+        if (__any(mNew != m)) {
+            const float f = mNew == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mNew);
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < DB; b++) o[b] *= f;
+            m = mNew;
+        }
+        l += ts;
+        Weights w;
+        if constexpr (HALF) {
+#pragma unroll
+            for (int kk = 0; kk < UK / 16; kk++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float x = S[kk / 2][8 * (kk % 2) + i];
+                    w.hi[kk][i] = (_Float16)x;
+                    w.lo[kk][i] = (_Float16)(x - (float)w.hi[kk][i]);
+                }
+        }
+        const unsigned Vl = v_base(V);
+        if (all || pos0 == pos1 || values_finite(V)) {
+#pragma unroll
+            for (int d = 0; d < DB; d++) o[d] = product<false>(Vl, d, S, w, base, 0, o[d]);
+            return;
+        }
+        // Values that are no numbers at positions that not every token sees: token by token (as in NarrowTile)
+#pragma unroll 1
+        for (int pos = pos0; pos <= pos1; pos++)
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                float16_t part;
+#pragma unroll
+                for (int i = 0; i < 16; i++) part[i] = 0.f;
+                part = product<true>(Vl, d, S, w, base, pos, part);
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] = row.pos == pos ? o[d][i] + part[i] : o[d][i];
+            }
+    }
+    __device__ __forceinline__ void run(int u0, int u1, float*) {
+        int here = page_of(u0), next = page_of(min(u0 + 1, u1 - 1));
+        __syncthreads();                          // (the tile before is done with the LDS)
+        issue(u0, here, 0);
+        unsigned buf = 0;
+        for (int u = u0; u < u1; u++) {
+            // this unit's rows have landed; nobody reads the other buffer any more
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (u + 1 < u1) issue(u + 1, next, buf ^ 1);
+            const int behind = page_of(min(u + 2, u1 - 1));
+            compute(u, here, buf);
+            here = next;
+            next = behind;
+            buf ^= 1;
+        }
+        float other = l;
+        row_swap32(l, other);
+        l += other;
+    }
+    __device__ __forceinline__ void write(int kvh, int w, float* lds) const {
+        const int r = 32 * wave + n32;
+        const bool mine = t.first + r < t.rows * p.g.group, whole = t.worker0 == t.worker1;
+        float* part = part_of(p, t, kvh, w);
+        float* out = p.out + (size_t)(t.row0 + row.token) * p.ldo + (size_t)row.head * HD;
+        if (mine) {
+#pragma unroll
+            for (int b = 0; b < DB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int d = 32 * b + 2 * i + 4 * hf;
+                    const float4_t v{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
+                    if (whole) *reinterpret_cast<float4_t*>(out + d) = l == 0.f ? v : v / l;
+                    else store_through(part + r * HD + d, v);
+                }
+            if (!whole && hf == 0) { st_agent(part + WIDE * HD + r, m); st_agent(part + WIDE * HD + WIDE + r, l); }
+        }
+        if (!whole) {
+            __syncthreads();                      // (all waves are done with the last unit's LDS, which the weights go over)
+            merge<HD, WIDE>(p, t, kvh, lds);
+        }
+    }
+};
+
+template <typename KVT, int HD, bool MOD, template <typename, int, bool> class Tile, int ROWS>
+__device__ __forceinline__ void attend(const PagedAttention& p, float* lds) {
     // neighbouring shares on one die, whose L2 then holds the KV head's rows that they have in common
     const int id = (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3));
     const int kvh = id / p.nWorkers, w = id % p.nWorkers;
@@ -597,12 +979,11 @@ __global__ __launch_bounds__(WG, 2) void paged_attn_kernel(PagedAttention p) {
     for (;;) {
         const int u0 = paged_unit_at(t, a), u1 = paged_unit_at(t, b);
         if (u0 < u1) {
-            NarrowTile<KVT, HD, MOD> n(p, t, kvh);
-            n.run(u0, u1);
-            n.join(lds);
-            finish<HD, NARROW>(p, t, kvh, w, lds, lds + 4 * NARROW * (HD + 4), lds + 4 * NARROW * (HD + 4) + 4 * NARROW, lds);
+            Tile<KVT, HD, MOD> n(p, t, kvh);
+            n.run(u0, u1, lds);
+            n.write(kvh, w, lds);
         } else if (t.units == 0 && a <= t.cost0 && t.cost0 < b) {
-            for (int i = threadIdx.x; i < min(NARROW, t.rows * p.g.group - t.first) * (HD / 4); i += WG) {
+            for (int i = threadIdx.x; i < min(ROWS, t.rows * p.g.group - t.first) * (HD / 4); i += WG) {
                 const PagedRow at = paged_row(t, p.g.group, kvh, i / (HD / 4));
                 *reinterpret_cast<float4*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + (i % (HD / 4)) * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
             }
@@ -612,35 +993,56 @@ __global__ __launch_bounds__(WG, 2) void paged_attn_kernel(PagedAttention p) {
         if (t.cost0 >= b) break;
     }
 }
+template <typename KVT, int HD, bool MOD>
+__global__ __launch_bounds__(WG, 2) void paged_narrow_kernel(PagedAttention p) {
+    extern __shared__ __attribute__((aligned(1024))) float lds[];      // (all the LDS there is: it starts at 0)
+    attend<KVT, HD, MOD, NarrowTile, NARROW>(p, lds);
+}
+template <typename KVT, int HD, bool MOD>
+__global__ __launch_bounds__(WG, 2) void paged_wide_kernel(PagedAttention p) {
+    extern __shared__ __attribute__((aligned(1024))) float lds[];
+    attend<KVT, HD, MOD, WideTile, WIDE>(p, lds);
+}
 
-static size_t attn_lds(int headDim) {
-    const int tile = 4 * NARROW * (headDim + 4) + 8 * NARROW, merge = 2 * NARROW + MERGE_LDS;
-    return (size_t)(tile > merge ? tile : merge) * 4;
+static size_t attn_lds(int headDim, bool wide) {
+    const size_t tile = wide ? (size_t)2 * 2 * 64 * headDim * 2 : (size_t)(4 * NARROW * (headDim + 4) + 8 * NARROW) * 4;
+    const size_t merge = (size_t)(2 * (wide ? WIDE : NARROW) + MERGE_LDS) * 4;
+    return tile > merge ? tile : merge;
 }
 template <typename F>
-static hipError_t with_kernel(const PagedGeo& g, bool mod, F f) {
+static hipError_t with_kernel(const PagedGeo& g, bool mod, bool wide, F f) {
+#define PAGED_PICK(KVT, HD, MOD) (wide ? f(paged_wide_kernel<KVT, HD, MOD>) : f(paged_narrow_kernel<KVT, HD, MOD>))
     if (g.kvHalf) {
-        if (g.headDim == 64) return mod ? f(paged_attn_kernel<_Float16, 64, true>) : f(paged_attn_kernel<_Float16, 64, false>);
-        return mod ? f(paged_attn_kernel<_Float16, 128, true>) : f(paged_attn_kernel<_Float16, 128, false>);
+        if (g.headDim == 64) return mod ? PAGED_PICK(_Float16, 64, true) : PAGED_PICK(_Float16, 64, false);
+        return mod ? PAGED_PICK(_Float16, 128, true) : PAGED_PICK(_Float16, 128, false);
     }
-    if (g.headDim == 64) return mod ? f(paged_attn_kernel<float, 64, true>) : f(paged_attn_kernel<float, 64, false>);
-    return mod ? f(paged_attn_kernel<float, 128, true>) : f(paged_attn_kernel<float, 128, false>);
+    if (g.headDim == 64) return mod ? PAGED_PICK(float, 64, true) : PAGED_PICK(float, 64, false);
+    return mod ? PAGED_PICK(float, 128, true) : PAGED_PICK(float, 128, false);
+#undef PAGED_PICK
 }
 hipError_t paged_attention_setup(const PagedGeo& g) {
-    for (bool mod : {false, true}) {
-        hipError_t e = with_kernel(g, mod, [&](auto* k) {
-            return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)attn_lds(g.headDim));
+    for (int i = 0; i < 4; i++) {
+        hipError_t e = with_kernel(g, i & 1, i >> 1, [&](auto* k) {
+            return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)attn_lds(g.headDim, i >> 1));
         });
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
 }
-hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t s) {
-    const int groups = (p.nWorkers * p.g.nKVHeads + 7) / 8 * 8;
-    return with_kernel(p.g, p.softcap > 0.f || p.slopes, [&](auto* k) {
-        hipLaunchKernelGGL(k, dim3(groups), dim3(WG), attn_lds(p.g.headDim), s, p);
-        return hipGetLastError();
-    });
+hipError_t launch_paged_attention(const PagedAttention& p0, hipStream_t s) {
+    const int groups = (p0.nWorkers * p0.g.nKVHeads + 7) / 8 * 8;
+    for (int wide = p0.wide; wide >= 0; wide--) {
+        PagedAttention p = p0;
+        p.tiles += wide ? p.maxTiles : 0;
+        p.workers += wide ? p.maxWorkers : 0;
+        const size_t lds = attn_lds(p.g.headDim, wide);
+        hipError_t e = with_kernel(p.g, p.softcap > 0.f || p.slopes, wide, [&](auto* k) {
+            hipLaunchKernelGGL(k, dim3(groups), dim3(WG), lds, s, p);
+            return hipGetLastError();
+        });
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 }  // namespace mg
