@@ -168,8 +168,14 @@ __device__ __forceinline__ float capped(float s, float cap, float invCap) {
 }
 // 16 bytes through to memory, for a workgroup of another die to read within the launch
 __device__ __forceinline__ void store_through(float* p, float4_t v) {
-    asm volatile("global_store_dwordx4 %0, %1, off sc1" : : "v"(p), "v"(v) : "memory");
+    const uint4_t w = __builtin_bit_cast(uint4_t, v);
+    unsigned long long* d = reinterpret_cast<unsigned long long*>(p);
+    __hip_atomic_store(d, w[0] | (unsigned long long)w[1] << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(d + 1, w[2] | (unsigned long long)w[3] << 32, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
+// Opens a load into LDS (as MG_SET_M0), with the five wait states that an address from a vector instruction's scalar result needs:
+// the compiler keeps no distances to what is inside a string.
+#define PAGED_SET_M0 "s_mov_b32 m0, %0\n\ts_nop 4\n\t"
 template <int J>
 __device__ __forceinline__ int quad_lane(int v) { return dpp_i<J * 0x55>(v); }      // lane J of the quad
 
@@ -205,86 +211,47 @@ __device__ __forceinline__ const char* kv_row(const char* pool, const char* zero
 __device__ __forceinline__ float* part_of(const PagedAttention& p, const PagedTile& t, int kvh, int w) {
     return p.parts + (((size_t)kvh * p.nWorkers + w) * 2 + (w == t.worker0)) * p.partStride;
 }
-// After a worker has stored its share (through to memory): the last one to come here adds the shares up and writes the rows.
-template <int HD, int ROWS>
-__device__ __forceinline__ void merge(const PagedAttention& p, const PagedTile& t, int kvh, float* scratch) {
-    const int tid = thread_anew(), R = min(ROWS, t.rows * p.g.group - t.first);
+// After a worker has stored its share (through to memory): whether it is the last one of the tile's to come here.  scratch: LDS
+// that nobody reads any more.
+__device__ __forceinline__ bool last_to_finish(const PagedAttention& p, const PagedTile& t, int kvh, float* scratch) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
-    const int segs = t.worker1 - t.worker0 + 1;
     unsigned* count = p.arrived + (size_t)kvh * p.maxTiles + t.index;
     unsigned* before = reinterpret_cast<unsigned*>(scratch);
-    if (tid == 0) *before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (threadIdx.x == 0) *before = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     __syncthreads();
-    const bool last = *before + 1 == (unsigned)segs;
+    const bool last = *before == (unsigned)(t.worker1 - t.worker0);
     __syncthreads();
-    if (!last) return;
+    if (!last) return false;
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "agent");
-    if (tid == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    // Rows' greatest maxima and sums first, into `scratch` beside every partial result's weight; then the outputs, the workgroup's
-    // threads sharing out rows, columns and, where there are few of those, partial results.
-    auto part = [&](int s) { return part_of(p, t, kvh, t.worker0 + s); };
-    float* M = scratch;                   // [ROWS]
-    float* den = scratch + ROWS;          // [ROWS]
-    float* wt = scratch + 2 * ROWS;       // [segs in turn][R]
-    const int perTurn = MERGE_LDS / ROWS;
-    const int cols = R * (HD / 4), par = max(1, WG / cols);
-    if (tid < R) {
+    if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+// The weights of shares s0 .. s0 + n - 1 in each row's result, wt[s][ROWS], and the rows' sums with them, den[ROWS]; the rows' greatest
+// maxima, M[ROWS], where s0 is 0.  Ends with the LDS written.
+template <int HD, int ROWS>
+__device__ __forceinline__ void merge_weights(const PagedAttention& p, const PagedTile& t, int kvh, int R, int s0, int n, float* M, float* den, float* wt) {
+    const int tid = thread_anew(), segs = t.worker1 - t.worker0 + 1;
+    auto at = [&](int s, int i) { return part_of(p, t, kvh, t.worker0 + s)[ROWS * HD + i]; };
+    if (s0 == 0 && tid < R) {
         float m = -INFINITY;
 #pragma unroll 8
-        for (int s = 0; s < segs; s++) m = fmaxf(m, part(s)[ROWS * HD + tid]);
+        for (int s = 0; s < segs; s++) m = fmaxf(m, at(s, tid));
         M[tid] = m == -INFINITY ? 0.f : m;
         den[tid] = 0.f;
     }
-    float4 acc[(ROWS * HD / 4 + WG - 1) / WG];
-#pragma unroll
-    for (auto& a : acc) a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s0 = 0; s0 < segs; s0 += perTurn) {
-        const int n = min(perTurn, segs - s0);
-        __syncthreads();
-        for (int i = tid; i < n * R; i += WG) wt[i] = __builtin_amdgcn_exp2f(part(s0 + i / R)[ROWS * HD + i % R] - M[i % R]);
-        __syncthreads();
-        if (tid < R) {
-            float d = den[tid];
-#pragma unroll 8
-            for (int s = 0; s < n; s++) d = fmaf(wt[s * R + tid], part(s0 + s)[ROWS * HD + ROWS + tid], d);
-            den[tid] = d;
-        }
-#pragma unroll
-        for (int k = 0; k < (int)(sizeof(acc) / sizeof(acc[0])); k++) {
-            const int i = par > 1 ? tid % cols : tid + k * WG, from = par > 1 ? tid / cols : 0;
-            if (i >= cols || from >= par || (par > 1 && k > 0)) continue;
-            const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
-#pragma unroll 4
-            for (int s = from; s < n; s += par) {
-                const float4 v = *reinterpret_cast<const float4*>(part(s0 + s) + row * HD + d);
-                const float f = wt[s * R + row];
-                acc[k].x = fmaf(f, v.x, acc[k].x); acc[k].y = fmaf(f, v.y, acc[k].y); acc[k].z = fmaf(f, v.z, acc[k].z); acc[k].w = fmaf(f, v.w, acc[k].w);
-            }
-        }
-    }
+    __syncthreads();                      // (and the weights before these are used up)
+    for (int i = tid; i < n * ROWS; i += WG)
+        if (i % ROWS < R) wt[i] = __builtin_amdgcn_exp2f(at(s0 + i / ROWS, i % ROWS) - M[i % ROWS]);
     __syncthreads();
-    if (par > 1) {                        // the shares of the same columns, in their order
-        float4* x = reinterpret_cast<float4*>(wt);
-        if (tid / cols < par) x[tid] = acc[0];
-        __syncthreads();
-        if (tid < cols)
-            for (int k = 1; k < par; k++) {
-                const float4 v = x[tid + k * cols];
-                acc[0].x += v.x; acc[0].y += v.y; acc[0].z += v.z; acc[0].w += v.w;
-            }
-    }
-#pragma unroll
-    for (int k = 0; k < (int)(sizeof(acc) / sizeof(acc[0])); k++) {
-        const int i = tid + k * WG;
-        if (i >= cols) continue;
-        const int row = i / (HD / 4), d = (i % (HD / 4)) * 4;
-        const float l = den[row];
-        const PagedRow at = paged_row(t, p.g.group, kvh, row);
-        *reinterpret_cast<float4*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) =
-            l == 0.f ? acc[k] : make_float4(acc[k].x / l, acc[k].y / l, acc[k].z / l, acc[k].w / l);
+    if (tid < R) {
+        float d = den[tid];
+#pragma unroll 8
+        for (int s = 0; s < n; s++) d = fmaf(wt[s * ROWS + tid], at(s0 + s, ROWS + tid), d);
+        den[tid] = d;
     }
 }
+__device__ __forceinline__ float4_t over(float4_t v, float l) { return l == 0.f ? v : v / l; }       // (nothing seen: zeros)
 
 // A tile of 16 rows: four waves take a step of KB positions each of every unit, each with its own running maximum, sum and output.
 // Bound by HBM: a lane loads its K and V operands from the pages straight into registers, a step ahead and the page numbers two
@@ -320,7 +287,9 @@ struct NarrowTile {
     float m, l;
     float4_t o[EPL];
 
-    __device__ __forceinline__ NarrowTile(const PagedAttention& p_, const PagedTile& t_, int kvh) : p(p_), t(t_) {
+    int here, next;                // page numbers of the step at hand and of the one behind it
+
+    __device__ __forceinline__ NarrowTile(const PagedAttention& p_, const PagedTile& t_, int kvh, int u0, int u1) : p(p_), t(t_) {
         const int tid = thread_anew();
         lane = tid & 63; l16 = lane & 15; g = lane >> 4;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -331,34 +300,38 @@ struct NarrowTile {
         Kp = static_cast<const char*>(p.K) + (size_t)kvh * HD * sizeof(KVT);
         Vp = static_cast<const char*>(p.V) + (size_t)kvh * HD * sizeof(KVT);
         zeros = reinterpret_cast<const char*>(p.zeros);
+        here = page_of(u0);
+        const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
+        float4_t x[HD / 16];                      // the row's elements as the operands want them
+#pragma unroll
+        for (int i = 0; i < HD / 16; i++) x[i] = *reinterpret_cast<const float4_t*>(q + (HALF ? i / 2 * 32 + g * 8 + i % 2 * 4 : i * 16 + g * 4));
+        next = page_of(min(u0 + 1, u1 - 1));
+        load_k(u0, here);
+        load_v(u0, here);
         cap = p.softcap;
         invCap = MOD && cap > 0.f ? 1.f / cap : 0.f;
         slope = MOD && p.slopes ? p.slopes[row.head] : 0.f;
-        const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
         c = p.scale;
         if constexpr (HALF) {
-            float x[HD / 32][8], top = 0.f;
+            float top = 0.f;
 #pragma unroll
-            for (int s = 0; s < HD / 32; s++) {
-                const float4 a = *reinterpret_cast<const float4*>(q + s * 32 + g * 8), b = *reinterpret_cast<const float4*>(q + s * 32 + g * 8 + 4);
-                x[s][0] = a.x; x[s][1] = a.y; x[s][2] = a.z; x[s][3] = a.w; x[s][4] = b.x; x[s][5] = b.y; x[s][6] = b.z; x[s][7] = b.w;
+            for (int i = 0; i < HD / 16; i++)
 #pragma unroll
-                for (int j = 0; j < 8; j++) top = fmaxf(top, fabsf(x[s][j]));
-            }
+                for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(x[i][j]));
             top = rows_max(top);
             const int up = top > 0.f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
 #pragma unroll
             for (int s = 0; s < HD / 32; s++)
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
-                    const float v = ldexpf(x[s][j], up);
-                    qh[s][j] = (_Float16)v;
-                    ql[s][j] = (_Float16)(v - (float)qh[s][j]);
+                    const float y = ldexpf(x[2 * s + j / 4][j % 4], up);
+                    qh[s][j] = (_Float16)y;
+                    ql[s][j] = (_Float16)(y - (float)qh[s][j]);
                 }
             c = ldexpf(c, -up);
         } else {
 #pragma unroll
-            for (int s = 0; s < HD / 16; s++) qf[s] = *reinterpret_cast<const float4_t*>(q + s * 16 + g * 4);
+            for (int s = 0; s < HD / 16; s++) qf[s] = x[s];
         }
         if (!MOD) c *= 1.4426950408889634f;
         m = -INFINITY;
@@ -543,9 +516,6 @@ struct NarrowTile {
         }
     }
     __device__ __forceinline__ void run(int u0, int u1, float* lds) {
-        int here = page_of(u0), next = page_of(min(u0 + 1, u1 - 1));
-        load_k(u0, here);
-        load_v(u0, here);
         for (int u = u0; u < u1; u++) {
             const int behind = page_of(min(u + 2, u1 - 1));
             const bool more = u + 1 < u1;
@@ -572,8 +542,8 @@ struct NarrowTile {
         __syncthreads();
         const int tid = thread_anew();
 #pragma unroll
-        for (int i = tid; i < NARROW * (HD / 4); i += WG) {
-            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        for (int n = 0; n < NARROW * (HD / 4) / WG; n++) {
+            const int i = tid + n * WG, r = i / (HD / 4), d = (i % (HD / 4)) * 4;
             const float M = fmaxf(fmaxf(wm[r], wm[NARROW + r]), fmaxf(wm[2 * NARROW + r], wm[3 * NARROW + r])), from = M == -INFINITY ? 0.f : M;
             float4_t a{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -602,11 +572,49 @@ struct NarrowTile {
             const float4_t v = *reinterpret_cast<const float4_t*>(lds + r * (HD + 4) + d);
             if (!whole) { store_through(mine + r * HD + d, v); continue; }
             const PagedRow at = paged_row(t, p.g.group, kvh, r);
-            *reinterpret_cast<float4_t*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) = ls[r] == 0.f ? v : v / ls[r];       // (nothing seen: zeros)
+            *reinterpret_cast<float4_t*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) = over(v, ls[r]);
         }
         if (whole) return;
         if (tid < R) { st_agent(mine + NARROW * HD + tid, ms[tid]); st_agent(mine + NARROW * HD + NARROW + tid, ls[tid]); }
-        merge<HD, NARROW>(p, t, kvh, lds);
+        if (last_to_finish(p, t, kvh, lds)) merge(kvh, R, lds);
+    }
+    // All workers' shares: threads take rows and columns and, where there are fewer of those than threads, shares in turn
+    __device__ __forceinline__ void merge(int kvh, int R, float* lds) const {
+        float *M = lds, *den = lds + NARROW, *wt = lds + 2 * NARROW;
+        constexpr int TURN = MERGE_LDS / NARROW, N = NARROW * HD / 4 / WG > 0 ? NARROW * HD / 4 / WG : 1;
+        const int tid = thread_anew(), segs = t.worker1 - t.worker0 + 1, cols = R * (HD / 4), par = max(1, WG / cols);
+        float4_t acc[N];
+#pragma unroll
+        for (int k = 0; k < N; k++) acc[k] = float4_t{0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < segs; s0 += TURN) {
+            const int n = min(TURN, segs - s0);
+            merge_weights<HD, NARROW>(p, t, kvh, R, s0, n, M, den, wt);
+#pragma unroll
+            for (int k = 0; k < N; k++) {
+                const int i = par > 1 ? tid % cols : tid + k * WG, from = par > 1 ? tid / cols : 0;
+                if (i >= cols || from >= par || (par > 1 && k > 0)) continue;
+                const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+#pragma unroll 4
+                for (int s = from; s < n; s += par)
+                    acc[k] += wt[s * NARROW + r] * *reinterpret_cast<const float4_t*>(part_of(p, t, kvh, t.worker0 + s0 + s) + r * HD + d);
+            }
+        }
+        __syncthreads();
+        if (par > 1) {                        // the shares of the same columns, in their order
+            float4_t* x = reinterpret_cast<float4_t*>(wt);
+            if (tid / cols < par) x[tid] = acc[0];
+            __syncthreads();
+            if (tid < cols)
+                for (int k = 1; k < par; k++) acc[0] += x[tid + k * cols];
+        }
+#pragma unroll
+        for (int k = 0; k < N; k++) {
+            const int i = tid + k * WG;
+            if (i >= cols) continue;
+            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+            const PagedRow at = paged_row(t, p.g.group, kvh, r);
+            *reinterpret_cast<float4_t*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) = over(acc[k], den[r]);
+        }
     }
 };
 
@@ -648,7 +656,9 @@ struct WideTile {
 
     static __device__ __forceinline__ int swz(int r) { return HALF ? ((r & 3) << 1) | ((r >> 2) & 1) : r & 7; }
 
-    __device__ __forceinline__ WideTile(const PagedAttention& p_, const PagedTile& t_, int kvh) : p(p_), t(t_) {
+    int here, next;                  // page numbers of the unit at hand and of the one behind it
+
+    __device__ __forceinline__ WideTile(const PagedAttention& p_, const PagedTile& t_, int kvh, int u0, int u1) : p(p_), t(t_) {
         const int tid = thread_anew();
         lane = tid & 63; n32 = lane & 31; hf = lane >> 5;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -668,20 +678,24 @@ struct WideTile {
             const int r = (wave * NI + i) * RI + lane / PR;
             from[i] = (unsigned)(r & 7) * (unsigned)rowBytes + (unsigned)((lane % PR) ^ swz(r)) * 16;
         }
+        here = page_of(u0);
+        const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
+        float4_t x[HD / 8];                       // the row's elements as the operands want them, all asked for at once
+#pragma unroll
+        for (int i = 0; i < HD / 8; i++) x[i] = *reinterpret_cast<const float4_t*>(q + (HALF ? i / 2 * 16 + hf * 8 + i % 2 * 4 : i * 8 + hf * 4));
+        next = page_of(min(u0 + 1, u1 - 1));
+        __syncthreads();                          // (the tile before is done with the LDS)
+        issue(u0, here, 0);
         cap = p.softcap;
         invCap = MOD && cap > 0.f ? 1.f / cap : 0.f;
         slope = MOD && p.slopes ? p.slopes[row.head] : 0.f;
-        const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
         c = p.scale;
         if constexpr (HALF) {
             float top = 0.f;
 #pragma unroll
-            for (int s = 0; s < QS; s++)
+            for (int i = 0; i < HD / 8; i++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float4 a = *reinterpret_cast<const float4*>(q + s * 16 + hf * 8 + 4 * j);
-                    top = fmaxf(fmaxf(top, fmaxf(fabsf(a.x), fabsf(a.y))), fmaxf(fabsf(a.z), fabsf(a.w)));
-                }
+                for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(x[i][j]));
             float other = top;
             row_swap32(top, other);
             top = fmaxf(top, other);
@@ -689,19 +703,15 @@ struct WideTile {
 #pragma unroll
             for (int s = 0; s < QS; s++)
 #pragma unroll
-                for (int j = 0; j < 2; j++) {
-                    const float4_t a = *reinterpret_cast<const float4_t*>(q + s * 16 + hf * 8 + 4 * j);
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const float x = ldexpf(a[i], up);
-                        qh[s][4 * j + i] = (_Float16)x;
-                        ql[s][4 * j + i] = (_Float16)(x - (float)qh[s][4 * j + i]);
-                    }
+                for (int j = 0; j < 8; j++) {
+                    const float y = ldexpf(x[2 * s + j / 4][j % 4], up);
+                    qh[s][j] = (_Float16)y;
+                    ql[s][j] = (_Float16)(y - (float)qh[s][j]);
                 }
             c = ldexpf(c, -up);
         } else {
 #pragma unroll
-            for (int s = 0; s < QS; s++) qf[s] = *reinterpret_cast<const float4_t*>(q + s * 8 + hf * 4);
+            for (int s = 0; s < QS; s++) qf[s] = x[s];
         }
         if (!MOD) c *= 1.4426950408889634f;
         m = -INFINITY;
@@ -730,14 +740,14 @@ struct WideTile {
             const size_t at = (size_t)(inside ? ((unsigned)page << p.g.pageShift) + ((unsigned)key & (unsigned)(p.g.pageSize - 1)) : 0u) * rowBytes;
             const unsigned dst = ldsBase + buf * BUFB + (unsigned)r0 * ROWB;
             if (inside) {
-                asm volatile(MG_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(from[i]), "s"(Kp + at) : "memory");
-                asm volatile(MG_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst + TILEB), "v"(from[i]), "s"(Vp + at) : "memory");
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(from[i]), "s"(Kp + at) : "memory");
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst + TILEB), "v"(from[i]), "s"(Vp + at) : "memory");
             } else {
                 const int r = r0 + lane / PR, piece = ((lane % PR) ^ swz(r)) * 16;
                 const char* k = kv_row(Kp, zeros, rowBytes, base + r, page, span.begin, span.end, p.g.pageShift) + piece;
                 const char* v = kv_row(Vp, zeros, rowBytes, base + r, page, span.begin, span.end, p.g.pageShift) + piece;
-                asm volatile(MG_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(k) : "memory");
-                asm volatile(MG_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst + TILEB), "v"(v) : "memory");
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(k) : "memory");
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst + TILEB), "v"(v) : "memory");
             }
         }
     }
@@ -770,8 +780,10 @@ struct WideTile {
 #pragma unroll
                     for (int i = 0; i < 16; i++) first[i] = 0.f;
 #pragma unroll
-                    for (int s = 0; s < QS; s++)
+                    for (int s = 0; s < QS; s++) {
+                        __builtin_amdgcn_sched_barrier(0);
                         first = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, lds16((at ^ (unsigned)(s * 32)) + b * 32 * ROWB)), qh[s], first, 0, 0, 0);
+                    }
 #pragma unroll
                     for (int i = 0; i < 16; i++) S[b][i] = S[b][i] != S[b][i] ? first[i] : S[b][i];
                 }
@@ -795,10 +807,11 @@ struct WideTile {
 #pragma unroll
             for (int kk = 0; kk < UK / 16; kk++) {
                 typedef __attribute__((address_space(3))) short4_t* lp;
+                if (MASKED) __builtin_amdgcn_sched_barrier(0);
                 uint2_t x = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB)));
                 uint2_t y = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB + 8 * ROWB)));
                 if (MASKED) {
-                    const int j = base + 16 * kk + 4 * hf;
+                    const int j = anew(base + 16 * kk + 4 * hf);
                     auto keep = [&](int k) { return (paged_sees(pos, k, t.len, p.window, t.prefix) ? 0xffffu : 0u) | (paged_sees(pos, k + 1, t.len, p.window, t.prefix) ? 0xffff0000u : 0u); };
                     x[0] &= keep(j); x[1] &= keep(j + 2); y[0] &= keep(j + 8); y[1] &= keep(j + 10);
                 }
@@ -810,7 +823,7 @@ struct WideTile {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 float v = *reinterpret_cast<__attribute__((address_space(3))) const float*>((V ^ (unsigned)(i % 4 * 16)) + (unsigned)(8 * (i / 4) + i % 4) * ROWB + (unsigned)d * 128);
-                if (MASKED && !paged_sees(pos, base + 8 * (i / 4) + 4 * hf + i % 4, t.len, p.window, t.prefix)) v = 0.f;
+                if (MASKED && !paged_sees(pos, anew(base + 8 * (i / 4) + 4 * hf + i % 4), t.len, p.window, t.prefix)) v = 0.f;
                 out = __builtin_amdgcn_mfma_f32_32x32x2f32(v, S[0][i], out, 0, 0, 0);
             }
         }
@@ -907,7 +920,10 @@ struct WideTile {
         const unsigned Vl = v_base(V);
         if (all || pos0 == pos1 || values_finite(V)) {
 #pragma unroll
-            for (int d = 0; d < DB; d++) o[d] = product<false>(Vl, d, S, w, base, 0, o[d]);
+            for (int d = 0; d < DB; d++) {
+                __builtin_amdgcn_sched_barrier(0);        // (as in scores)
+                o[d] = product<false>(Vl, d, S, w, base, 0, o[d]);
+            }
             return;
         }
         // Values that are no numbers at positions that not every token sees: token by token (as in NarrowTile)
@@ -915,6 +931,7 @@ struct WideTile {
         for (int pos = pos0; pos <= pos1; pos++)
 #pragma unroll
             for (int d = 0; d < DB; d++) {
+                __builtin_amdgcn_sched_barrier(0);
                 float16_t part;
 #pragma unroll
                 for (int i = 0; i < 16; i++) part[i] = 0.f;
@@ -924,9 +941,6 @@ struct WideTile {
             }
     }
     __device__ __forceinline__ void run(int u0, int u1, float*) {
-        int here = page_of(u0), next = page_of(min(u0 + 1, u1 - 1));
-        __syncthreads();                          // (the tile before is done with the LDS)
-        issue(u0, here, 0);
         unsigned buf = 0;
         for (int u = u0; u < u1; u++) {
             // this unit's rows have landed; nobody reads the other buffer any more
@@ -942,27 +956,55 @@ struct WideTile {
         row_swap32(l, other);
         l += other;
     }
-    __device__ __forceinline__ void write(int kvh, int w, float* lds) const {
+    // A share lies as its registers do -- a wave's block b, rows of four i / 4, then its 64 lanes -- so that stores and loads are whole lines
+    __device__ __forceinline__ void write(int kvh, int w, float* lds) {
         const int r = 32 * wave + n32;
-        const bool mine = t.first + r < t.rows * p.g.group, whole = t.worker0 == t.worker1;
-        float* part = part_of(p, t, kvh, w);
-        float* out = p.out + (size_t)(t.row0 + row.token) * p.ldo + (size_t)row.head * HD;
-        if (mine) {
+        if (t.worker0 != t.worker1) {
+            float* part = part_of(p, t, kvh, w);
+            if (active) {
+#pragma unroll
+                for (int b = 0; b < DB; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        store_through(part + ((wave * DB + b) * 4 + i) * 256 + lane * 4, float4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]});
+                if (hf == 0) { st_agent(part + WIDE * HD + r, m); st_agent(part + WIDE * HD + WIDE + r, l); }
+            }
+            __syncthreads();                      // (all waves are done with the last unit's LDS)
+            if (!last_to_finish(p, t, kvh, lds)) return;
+            float *M = lds, *den = lds + WIDE, *wt = lds + 2 * WIDE;
+            constexpr int TURN = MERGE_LDS / WIDE;
+            const int segs = t.worker1 - t.worker0 + 1, R = min(WIDE, t.rows * p.g.group - t.first);
 #pragma unroll
             for (int b = 0; b < DB; b++)
 #pragma unroll
-                for (int i = 0; i < 16; i += 4) {
-                    const int d = 32 * b + 2 * i + 4 * hf;
-                    const float4_t v{o[b][i], o[b][i + 1], o[b][i + 2], o[b][i + 3]};
-                    if (whole) *reinterpret_cast<float4_t*>(out + d) = l == 0.f ? v : v / l;
-                    else store_through(part + r * HD + d, v);
+                for (int i = 0; i < 16; i++) o[b][i] = 0.f;
+            for (int s0 = 0; s0 < segs; s0 += TURN) {
+                const int n = min(TURN, segs - s0);
+                merge_weights<HD, WIDE>(p, t, kvh, R, s0, n, M, den, wt);
+                if (!active) continue;
+                for (int s = 0; s < n; s++) {
+                    const float* from = part_of(p, t, kvh, t.worker0 + s0 + s) + wave * DB * 4 * 256 + lane * 4;
+                    const float f = wt[s * WIDE + r];
+#pragma unroll
+                    for (int b = 0; b < DB; b++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float4_t v = *reinterpret_cast<const float4_t*>(from + (b * 4 + i) * 256);
+#pragma unroll
+                            for (int j = 0; j < 4; j++) o[b][4 * i + j] = fmaf(f, v[j], o[b][4 * i + j]);
+                        }
                 }
-            if (!whole && hf == 0) { st_agent(part + WIDE * HD + r, m); st_agent(part + WIDE * HD + WIDE + r, l); }
+            }
+            __syncthreads();
+            l = den[r];
         }
-        if (!whole) {
-            __syncthreads();                      // (all waves are done with the last unit's LDS, which the weights go over)
-            merge<HD, WIDE>(p, t, kvh, lds);
-        }
+        if (t.first + r >= t.rows * p.g.group) return;
+        float* out = p.out + (size_t)(t.row0 + row.token) * p.ldo + (size_t)row.head * HD + 4 * hf;
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                *reinterpret_cast<float4_t*>(out + 32 * b + 8 * i) = over(float4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]}, l);
     }
 };
 
@@ -979,7 +1021,7 @@ __device__ __forceinline__ void attend(const PagedAttention& p, float* lds) {
     for (;;) {
         const int u0 = paged_unit_at(t, a), u1 = paged_unit_at(t, b);
         if (u0 < u1) {
-            Tile<KVT, HD, MOD> n(p, t, kvh);
+            Tile<KVT, HD, MOD> n(p, t, kvh, u0, u1);
             n.run(u0, u1, lds);
             n.write(kvh, w, lds);
         } else if (t.units == 0 && a <= t.cost0 && t.cost0 < b) {
