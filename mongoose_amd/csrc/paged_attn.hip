@@ -23,6 +23,7 @@ constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of pa
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
+typedef unsigned uint16v_t __attribute__((ext_vector_type(16)));
 typedef unsigned uint2_t __attribute__((ext_vector_type(2)));
 typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
@@ -515,7 +516,7 @@ struct NarrowTile {
             }
         }
     }
-    __device__ __forceinline__ void run(int u0, int u1, float* lds) {
+    __device__ __forceinline__ void run(int u0, int u1, int, int, float* lds) {
         for (int u = u0; u < u1; u++) {
             const int behind = page_of(min(u + 2, u1 - 1));
             const bool more = u + 1 < u1;
@@ -798,23 +799,16 @@ struct WideTile {
         }
         return V + (unsigned)(4 * h) * ROWB + (unsigned)(((x & 31) >> 2) ^ (4 * h)) * 16 + (unsigned)(x & 3) * 4;
     }
-    // Block d of V^T P^T on top of `out`; MASKED: without the positions that a token at `pos` does not see
+    // Block d of V^T P^T on top of `out`
     struct Weights { half8_t hi[HALF ? UK / 16 : 1], lo[HALF ? UK / 16 : 1]; };
-    template <bool MASKED>
-    __device__ __forceinline__ float16_t product(unsigned V, int d, const float16_t (&S)[NB], const Weights& w, int base, int pos, float16_t out) const {
+    __device__ __forceinline__ float16_t product(unsigned V, int d, const float16_t (&S)[NB], const Weights& w, float16_t out) const {
         if constexpr (HALF) {
             const unsigned at = V ^ (unsigned)(d * 64);
 #pragma unroll
             for (int kk = 0; kk < UK / 16; kk++) {
                 typedef __attribute__((address_space(3))) short4_t* lp;
-                if (MASKED) __builtin_amdgcn_sched_barrier(0);
-                uint2_t x = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB)));
-                uint2_t y = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB + 8 * ROWB)));
-                if (MASKED) {
-                    const int j = anew(base + 16 * kk + 4 * hf);
-                    auto keep = [&](int k) { return (paged_sees(pos, k, t.len, p.window, t.prefix) ? 0xffffu : 0u) | (paged_sees(pos, k + 1, t.len, p.window, t.prefix) ? 0xffff0000u : 0u); };
-                    x[0] &= keep(j); x[1] &= keep(j + 2); y[0] &= keep(j + 8); y[1] &= keep(j + 10);
-                }
+                const uint2_t x = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB)));
+                const uint2_t y = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB + 8 * ROWB)));
                 const half8_t v = __builtin_bit_cast(half8_t, uint4_t{x[0], x[1], y[0], y[1]});
                 out = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.hi[kk], out, 0, 0, 0);
                 out = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.lo[kk], out, 0, 0, 0);
@@ -822,8 +816,7 @@ struct WideTile {
         } else {
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                float v = *reinterpret_cast<__attribute__((address_space(3))) const float*>((V ^ (unsigned)(i % 4 * 16)) + (unsigned)(8 * (i / 4) + i % 4) * ROWB + (unsigned)d * 128);
-                if (MASKED && !paged_sees(pos, anew(base + 8 * (i / 4) + 4 * hf + i % 4), t.len, p.window, t.prefix)) v = 0.f;
+                const float v = *reinterpret_cast<__attribute__((address_space(3))) const float*>((V ^ (unsigned)(i % 4 * 16)) + (unsigned)(8 * (i / 4) + i % 4) * ROWB + (unsigned)d * 128);
                 out = __builtin_amdgcn_mfma_f32_32x32x2f32(v, S[0][i], out, 0, 0, 0);
             }
         }
@@ -831,7 +824,8 @@ struct WideTile {
     }
     __device__ __forceinline__ bool values_finite(unsigned V) const {
         bool odd = false;
-        for (int i = lane; i < UK * PR; i += 64) {
+#pragma unroll 2
+        for (int i = lane; i < UK * PR; i += 64) {       // (unrolled whole it would take q's registers)
             const uint4_t x = lds16(V + (unsigned)i * 16);
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -883,16 +877,22 @@ struct WideTile {
             }
         return ts;
     }
-    __device__ __forceinline__ void compute(int u, int mine, unsigned buf) {
-        const int base = base_of(u);
-        if (!active || base >= end || base + UK <= begin) return;
+    // Unit u, of page numbers `here`, in buffer `buf`; asks for the one behind it on the way
+    __device__ __forceinline__ void compute(int u, bool more, unsigned buf) {
+        const int base = base_of(u), mine = here;
+        if (!active || base >= end || base + UK <= begin) {
+            if (more) issue(u + 1, next, buf ^ 1);
+            return;
+        }
         const unsigned K = ldsBase + buf * BUFB, V = K + TILEB;
         const unsigned long long held = __ballot(mine >= 0);
         constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
-        const bool all = (held & runs) == runs && (base + UK <= t.prefix || (base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window)));
+        const bool inner = base + UK <= t.prefix || (base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
+        const bool all = inner && (held & runs) == runs;
         float16_t S[NB];
         float mNew;
         scores(K, S, false);
+        if (more) issue(u + 1, next, buf ^ 1);
         float ts = weigh(S, base, held, all, mNew);
         if (HALF && __any(ts != ts)) {            // (not a loop: what the masks need would be worked out ahead of it, for every unit)
             scores(K, S, true);
@@ -917,37 +917,81 @@ struct WideTile {
                     w.lo[kk][i] = (_Float16)(x - (float)w.hi[kk][i]);
                 }
         }
-        const unsigned Vl = v_base(V);
-        if (all || pos0 == pos1 || values_finite(V)) {
-#pragma unroll
-            for (int d = 0; d < DB; d++) {
-                __builtin_amdgcn_sched_barrier(0);        // (as in scores)
-                o[d] = product<false>(Vl, d, S, w, base, 0, o[d]);
+        if (!inner) {
+            if (!__any(ts != 0.f)) return;                // (no row has anything here: a value that is no number must not get to any)
+            if (pos0 != pos1 && !values_finite(V)) {
+                lateHi = lateHi << 20 | lateLo >> 40;
+                lateLo = (lateLo << 20 | (unsigned)u) & ((1ull << 60) - 1);
+                lates++;
+                return;
             }
-            return;
         }
-        // Values that are no numbers at positions that not every token sees: token by token (as in NarrowTile)
+        const unsigned Vl = v_base(V);
+#pragma unroll
+        for (int d = 0; d < DB; d++) {
+            __builtin_amdgcn_sched_barrier(0);            // (as in scores)
+            o[d] = product(Vl, d, S, w, o[d]);
+        }
+    }
+    // A unit with values that are no numbers at positions that not every token sees -- zero times them is no zero -- is left out of
+    // the product (its scores are in the sums).  At the end its positions are gone through row by row, each with those it sees,
+    // by way of the worker's place for a share.  There are at most five: the tokens of 32 rows end in two units, their windows begin
+    // in two, a prefix ends in one; unit numbers take 20 bits (2^24 positions, 32 a unit).
+    static constexpr int E = HD / 64;
+    unsigned long long lateLo = 0, lateHi = 0;
+    int lates = 0;
+    __device__ __forceinline__ void add_late(int kvh, int w) {
+        float* mine = part_of(p, t, kvh, w) + wave * 32 * HD;
+        const int x = anew(lane);
 #pragma unroll 1
-        for (int pos = pos0; pos <= pos1; pos++)
+        for (int r = 0; r < 32; r++) {
+            const PagedRow at = paged_row(t, p.g.group, kvh, 32 * wave + r);
+            const float* q = p.q + (size_t)(t.row0 + at.token) * p.ldq + (size_t)at.head * HD + x * E;
+            const float mr = lane_value(m, r), sl = MOD && p.slopes ? p.slopes[at.head] : 0.f;
+            float acc[E];
 #pragma unroll
-            for (int d = 0; d < DB; d++) {
-                __builtin_amdgcn_sched_barrier(0);
-                float16_t part;
+            for (int e = 0; e < E; e++) acc[e] = 0.f;
+#pragma unroll 1
+            for (int n = 0; n < lates; n++) {
+                const int u = (int)((n < 3 ? lateLo >> 20 * n : lateHi >> 20 * (n - 3)) & 0xfffff);
+#pragma unroll 1
+                for (int j = base_of(u); j < base_of(u) + UK; j++) {
+                    if (!paged_sees(at.pos, j, t.len, p.window, t.prefix)) continue;
+                    const int page = pages[j >> p.g.pageShift];
+                    if (page < 0 || page >= p.g.nPages) continue;
+                    const KVT* k = reinterpret_cast<const KVT*>(kv_row(Kp, zeros, rowBytes, j, page, span.begin, span.end, p.g.pageShift)) + x * E;
+                    const KVT* v = reinterpret_cast<const KVT*>(kv_row(Vp, zeros, rowBytes, j, page, span.begin, span.end, p.g.pageShift)) + x * E;
+                    float y = 0.f;
 #pragma unroll
-                for (int i = 0; i < 16; i++) part[i] = 0.f;
-                part = product<true>(Vl, d, S, w, base, pos, part);
+                    for (int e = 0; e < E; e++) y = fmaf(q[e], (float)k[e], y);
+                    y = wave_sum(y) * p.scale;
+                    if (MOD) y = (cap > 0.f ? capped(y, cap, invCap) : y) - sl * (float)abs(at.pos - j);
+                    y = __builtin_amdgcn_exp2f(fmaf(y, 1.4426950408889634f, SHIFT - (mr == -INFINITY ? 0.f : mr)));
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] = row.pos == pos ? o[d][i] + part[i] : o[d][i];
+                    for (int e = 0; e < E; e++) acc[e] = fmaf(y, (float)v[e], acc[e]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < E; e++) mine[r * HD + x * E + e] = acc[e];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");         // (read back by other lanes of the wave)
+        const float* from = mine + n32 * HD + 4 * hf;
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float4_t v = *reinterpret_cast<const float4_t*>(from + 32 * b + 8 * i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) o[b][4 * i + j] += v[j];
             }
     }
-    __device__ __forceinline__ void run(int u0, int u1, float*) {
+    __device__ __forceinline__ void run(int u0, int u1, int kvh, int w, float*) {
         unsigned buf = 0;
         for (int u = u0; u < u1; u++) {
             // this unit's rows have landed; nobody reads the other buffer any more
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            if (u + 1 < u1) issue(u + 1, next, buf ^ 1);
             const int behind = page_of(min(u + 2, u1 - 1));
-            compute(u, here, buf);
+            compute(u, u + 1 < u1, buf);
             here = next;
             next = behind;
             buf ^= 1;
@@ -955,6 +999,7 @@ struct WideTile {
         float other = l;
         row_swap32(l, other);
         l += other;
+        if (lates) add_late(kvh, w);
     }
     // A share lies as its registers do -- a wave's block b, rows of four i / 4, then its 64 lanes -- so that stores and loads are whole lines
     __device__ __forceinline__ void write(int kvh, int w, float* lds) {
@@ -1022,7 +1067,7 @@ __device__ __forceinline__ void attend(const PagedAttention& p, float* lds) {
         const int u0 = paged_unit_at(t, a), u1 = paged_unit_at(t, b);
         if (u0 < u1) {
             Tile<KVT, HD, MOD> n(p, t, kvh, u0, u1);
-            n.run(u0, u1, lds);
+            n.run(u0, u1, kvh, w, lds);
             n.write(kvh, w, lds);
         } else if (t.units == 0 && a <= t.cost0 && t.cost0 < b) {
             for (int i = threadIdx.x; i < min(ROWS, t.rows * p.g.group - t.first) * (HD / 4); i += WG) {
