@@ -18,6 +18,9 @@ namespace mg {
 constexpr int PT = 1024;                  // threads of the plan
 constexpr int NARROW = 16, WIDE = 128;    // rows of a tile
 constexpr int PLAN_LDS_TILES = 4096;      // tiles whose places on the line the plan holds in LDS
+// Units a worker has at least where a tile's workers are its own: a narrow unit is as short as a share can be (one request of 500
+// positions 8.8 us, with two 10.8); a wide share costs its 64 KB out and in (12 requests, some of 165 to 235 rows: 92 us, with one 95).
+constexpr int LEAST_NARROW = 1, LEAST_WIDE = 3;
 constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -34,9 +37,9 @@ MG_HD int wide_keys(int kvHalf) { return kvHalf ? 64 : 32; }
 
 // A request of up to 16 rows a KV head goes to the kernel that waits for memory, others to the one that waits for the matrix units.
 int paged_narrow_rows(const PagedGeo& g, int rows) {
-    return (long long)rows * g.group <= 128 ? 128 : NARROW;
+    return (long long)rows * g.group <= 256 ? 256 : NARROW;
 }
-int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + WIDE / NARROW; }
+int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + 256 / NARROW; }
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
 // Two workgroups a CU, in turns of the KV heads; fewer where the batch cannot have that many units.
 int paged_workers(const PagedGeo& g, int nReqs, int rows) {
@@ -73,76 +76,125 @@ __device__ __forceinline__ int4 plan_request(const PagedPlan& p, int r) {
     const int len = max(0, min(p.lens[r], p.maxLen));
     return make_int4(first, last - first, len, p.prefixLens ? max(0, min(p.prefixLens[r], len)) : 0);
 }
+__device__ __forceinline__ void put_tile(PagedTile* at, const PagedTile& t) {
+    int4* d = reinterpret_cast<int4*>(at);
+    d[0] = make_int4(t.req, t.row0, t.rows, t.len);
+    d[1] = make_int4(t.prefix, t.first, t.cost0, t.unit0);
+    d[2] = make_int4(t.units, t.worker0, t.worker1, t.index);
+    d[3] = make_int4(t.tileRows, t.unitKeys, 0, 0);
+}
+// Largest i with sums[i] <= x, of n sums
+__device__ __forceinline__ int plan_find(const unsigned* sums, int n, unsigned x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] <= x) lo = mid; else hi = mid;
+    }
+    return lo;
+}
+// One workgroup for the narrow tiles and one for the wide ones
 __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
     const bool wide = blockIdx.x != 0;
     const int tileRows = wide ? WIDE : NARROW, unitKeys = wide ? wide_keys(p.kvHalf) : narrow_keys(p.kvHalf);
     p.tiles += wide ? p.maxTiles : 0;
     p.workers += wide ? p.maxWorkers : 0;
     __shared__ unsigned tile0[PAGED_MAX_REQS + 1], place[PLAN_LDS_TILES], part[PT / 64];
+    __shared__ int4 held[PT];
     const int tid = threadIdx.x;
-    unsigned nTiles = 0;
+    unsigned sum = 0;
     if (tid == 0) tile0[0] = 0;
     for (int r0 = 0; r0 < p.nReqs; r0 += PT) {
         const int r = r0 + tid;
         unsigned n = 0;
         if (r < p.nReqs) {
-            const long long rows = (long long)plan_request(p, r).y * p.group;
+            const int4 rq = plan_request(p, r);
+            const long long rows = (long long)rq.y * p.group;
             if (wide == (rows > p.narrowRows)) n = (unsigned)((rows + tileRows - 1) / tileRows);
+            if (r < PT) held[r] = rq;
         }
-        n = plan_scan(n, nTiles, part);
+        n = plan_scan(n, sum, part);
         if (r < p.nReqs) tile0[r + 1] = n;
     }
     __syncthreads();
-    nTiles = min(nTiles, (unsigned)p.maxTiles);          // (more only where the caller's rows overlap)
+    const int nTiles = (int)min(sum, (unsigned)p.maxTiles);          // (more only where the caller's rows overlap)
+    PagedTile t;
     unsigned cost = 0;
-    for (unsigned i0 = 0; i0 < nTiles; i0 += PT) {
-        const unsigned i = i0 + tid;
-        PagedTile t{};
+    auto make = [&](int i) {
+        const int r = plan_find(tile0, p.nReqs, (unsigned)i);
+        const int4 rq = r < PT ? held[r] : plan_request(p, r);
+        t.req = r; t.row0 = rq.x; t.rows = rq.y; t.len = rq.z; t.prefix = rq.w;
+        t.tileRows = tileRows; t.unitKeys = unitKeys;
+        t.first = (i - (int)tile0[r]) * tileRows;
+        t.index = i;
+        paged_units(t, p.window, p.group);
+    };
+    for (int i0 = 0; i0 < nTiles; i0 += PT) {
+        const int i = i0 + tid;
         unsigned c = 0;
-        if (i < nTiles) {
-            int lo = 0, hi = p.nReqs;
-            while (hi - lo > 1) {
-                const int mid = (lo + hi) >> 1;
-                if (tile0[mid] <= i) lo = mid; else hi = mid;
-            }
-            const int4 rq = plan_request(p, lo);
-            t.req = lo; t.row0 = rq.x; t.rows = rq.y; t.len = rq.z; t.prefix = rq.w;
-            t.tileRows = tileRows; t.unitKeys = unitKeys; t.weight = 1;
-            t.first = (int)(i - tile0[lo]) * tileRows;
-            t.index = (int)i;
-            paged_units(t, p.window, p.group);
-            c = (unsigned)(PAGED_TILE_COST + t.units * t.weight);
-        }
+        if (i < nTiles) { make(i); c = (unsigned)paged_cost(t); }
         const unsigned end = plan_scan(c, cost, part);
         if (i < nTiles) {
             t.cost0 = (int)(end - c);
             if (i < PLAN_LDS_TILES) place[i] = end - c;
-            p.tiles[i] = t;
+            else p.tiles[i].cost0 = t.cost0;
         }
     }
     __syncthreads();
-    const int workers = max(1, min(p.nWorkers, (int)cost));
-    for (unsigned i = tid; i < nTiles; i += PT) {
-        PagedTile* t = p.tiles + i;
-        const int x = t->cost0 + PAGED_TILE_COST;
-        t->worker0 = t->units ? paged_worker_of((int)cost, workers, x) : 0;
-        t->worker1 = t->units ? paged_worker_of((int)cost, workers, x + (t->units - 1) * t->weight) : 0;
+    const bool few = paged_few(nTiles, p.nWorkers);                  // (512 tiles at most: one round)
+    int workers = max(1, min(p.nWorkers, (int)cost)), n = 0;
+    if (few) {
+        if (tid < nTiles) n = paged_workers_for(t, (int)cost, nTiles, p.nWorkers, wide ? LEAST_WIDE : LEAST_NARROW);
+        unsigned all = 0;
+        const unsigned end = plan_scan((unsigned)n, all, part);
+        workers = (int)all;
+        if (tid < nTiles) {
+            t.worker0 = (int)end - n;
+            t.worker1 = (int)end - 1;
+            tile0[tid] = end - n;                                    // (its first use is over: plan_scan has synchronised)
+            put_tile(p.tiles + tid, t);
+        }
+    } else {
+        for (int i = tid; i < nTiles; i += PT) {
+            const int cost0 = i < PLAN_LDS_TILES ? (int)place[i] : p.tiles[i].cost0;
+            if (nTiles > PT) make(i);                                // (else it is still at hand)
+            t.cost0 = cost0;
+            const int x = cost0 + PAGED_TILE_COST;
+            t.worker0 = t.units ? paged_worker_of((int)cost, workers, x) : 0;
+            t.worker1 = t.units ? paged_worker_of((int)cost, workers, x + t.units - 1) : 0;
+            put_tile(p.tiles + i, t);
+        }
     }
     __syncthreads();
     for (int w = tid; w < p.nWorkers; w += PT) {
-        PagedWorker k{};
+        int4* d = reinterpret_cast<int4*>(p.workers + w);
+        int4 range = make_int4(0, 0, 0, 0);
         if (w < workers && nTiles > 0) {
-            k.a = paged_share((int)cost, workers, w);
-            k.b = paged_share((int)cost, workers, w + 1);
-            unsigned lo = 0, hi = nTiles;
-            while (hi - lo > 1) {
-                const unsigned mid = (lo + hi) >> 1;
-                if ((mid < PLAN_LDS_TILES ? place[mid] : (unsigned)p.tiles[mid].cost0) <= (unsigned)k.a) lo = mid; else hi = mid;
+            int i, a, b;
+            if (few) {
+                i = plan_find(tile0, nTiles, (unsigned)w);
+            } else {
+                a = paged_share((int)cost, workers, w);
+                b = paged_share((int)cost, workers, w + 1);
+                int lo = 0, hi = nTiles;
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if ((mid < PLAN_LDS_TILES ? (int)place[mid] : p.tiles[mid].cost0) <= a) lo = mid; else hi = mid;
+                }
+                i = lo;
             }
-            k.tile = p.tiles[lo];
-            k.tiles = (int)nTiles;
+            const int4* from = reinterpret_cast<const int4*>(p.tiles + i);
+            const int4 x0 = from[0], x1 = from[1], x2 = from[2], x3 = from[3];
+            d[0] = x0; d[1] = x1; d[2] = x2; d[3] = x3;
+            if (few) {
+                PagedTile s;
+                s.cost0 = x1.z; s.units = x2.x;
+                const int parts = x2.z - x2.y + 1, k = w - x2.y;
+                a = paged_part(s, parts, k);
+                b = k + 1 < parts ? paged_part(s, parts, k + 1) : s.cost0 + paged_cost(s);
+            }
+            range = make_int4(a, b, nTiles, 0);
         }
-        p.workers[w] = k;
+        d[4] = range;
     }
 }
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s) {

@@ -116,9 +116,11 @@ MG_HD bool paged_sees(int i, int j, int len, int window, int prefix) {
 // ---------------------------------------------------------------------------
 // The plan of an attention call.  The rows of a request under one KV head (its new tokens x the head group, token by token) are cut
 // into tiles of tileRows, the positions a tile sees into units of unitKeys.  All tiles of a batch, one behind the other, make a line
-// of cost -- PAGED_TILE_COST for a tile's own start and end, then `weight` for each of its units -- that is cut into equal shares, one
-// a worker: any mix of long, short, one and many requests keeps every CU busy to the end.  A tile whose units fall to several
-// workers is put together by the last of them to finish.  The line is the same for every KV head.
+// of cost: PAGED_TILE_COST for a tile's own start and end, then 1 for each of its units.  Workers get shares [a, b) of the line, the same
+// for every KV head.  Where there are many tiles the shares are equal and pass over from tile to tile: any mix of long, short, one
+// and many requests keeps every CU busy to the end.  Where there are few, every tile has workers of its own, as many as its part of
+// the cost asks for, so that none has the start and the end of two tiles behind each other.  A tile with several workers
+// is put together by the last of them to finish.
 // ---------------------------------------------------------------------------
 constexpr int PAGED_TILE_COST = 1;
 
@@ -129,8 +131,8 @@ struct PagedTile {
     int unit0, units;                   // the units it sees
     int worker0, worker1;               // the first and last worker that have some of them
     int index;                          // its number
-    int tileRows, unitKeys, weight;     // its kind
-    int pad;
+    int tileRows, unitKeys;             // its kind
+    int pad[2];
 };
 
 // The positions [begin, end) that rows first .. first + tileRows - 1 of a request see some of, and the positions of its first and last token.
@@ -150,14 +152,26 @@ MG_HD void paged_units(PagedTile& t, int window, int group) {
     t.unit0 = s.begin / t.unitKeys;
     t.units = s.end > s.begin ? (s.end + t.unitKeys - 1) / t.unitKeys - t.unit0 : 0;
 }
-// Where worker w's share of a line of `cost` starts; workers <= cost / weight, so that each has a unit of every tile that it spans.
+MG_HD int paged_cost(const PagedTile& t) { return PAGED_TILE_COST + t.units; }
+// Many tiles: where worker w's share of a line of `cost` starts, and the worker whose share x is in (workers <= cost, so that no
+// share is empty).
 MG_HD int paged_share(int cost, int workers, int w) { return (int)((long long)cost * w / workers); }
 MG_HD int paged_worker_of(int cost, int workers, int x) { return (int)((((long long)x + 1) * workers - 1) / cost); }
-// The units [u0, u1) of a tile that start within the share [a, b).
+// Few tiles: how many workers a tile has -- at least one, together at most `workers`, and units of `least` and more each -- and where
+// the share of its i-th of n starts.
+MG_HD bool paged_few(int tiles, int workers) { return 2 * tiles <= workers; }
+MG_HD int paged_workers_for(const PagedTile& t, int cost, int tiles, int workers, int least) {
+    const int most = t.units / least > 1 ? t.units / least : 1;
+    const int n = 1 + (int)((long long)(workers - tiles) * paged_cost(t) / cost);
+    return n < most ? n : most;
+}
+MG_HD int paged_part(const PagedTile& t, int n, int i) {
+    return i == 0 ? t.cost0 : t.cost0 + PAGED_TILE_COST + (int)((long long)t.units * i / n);
+}
+// The first unit of a tile that starts at `a` on the line or behind.
 MG_HD int paged_unit_at(const PagedTile& t, int a) {
-    const int x = a - (t.cost0 + PAGED_TILE_COST);
-    const int u = x <= 0 ? 0 : (x + t.weight - 1) / t.weight;
-    return u < t.units ? u : t.units;
+    const int u = a - (t.cost0 + PAGED_TILE_COST);
+    return u <= 0 ? 0 : u < t.units ? u : t.units;
 }
 
 // Why mg_paged_tables changes nothing

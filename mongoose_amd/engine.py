@@ -65,6 +65,10 @@ class Tensor:
     def DevicePtr(self):
         return self._ptr
 
+    @property
+    def _as_parameter_(self):          # (what ctypes passes where an address is asked for)
+        return self._ptr
+
     def Size(self):
         n = 1
         for s in self.Shape:
@@ -778,18 +782,21 @@ class HIPPaged:
 
     def Tables(self, newLens, nReqs, lens, lensOut, table, ring, ringState, ringStateOut, rows, rowStart, slots, positions, counts,
                stream=None):
-        return lib.mg_paged_tables(self._h, _p(newLens), nReqs, _p(lens), _p(lensOut), _p(table), _p(ring), _p(ringState),
-                                   _p(ringStateOut), rows, _p(rowStart), _p(slots), _p(positions), _p(counts), stream)
+        return _paged_tables(self._h, newLens, nReqs, lens, lensOut, table, ring, ringState, ringStateOut, rows, rowStart, slots, positions,
+                             counts, stream)
 
     def Store(self, q, k, v, ldq, ldk, ldv, qOut, ldqOut, K, V, slots, positions, rows, cosTab, sinTab, tableRows, stream=None):
-        return lib.mg_paged_store(self._h, _p(q), _p(k), _p(v), ldq, ldk, ldv, _p(qOut), ldqOut, _p(K), _p(V), _p(slots),
-                                  _p(positions), rows, _p(cosTab), _p(sinTab), tableRows, stream)
+        return _paged_store(self._h, q, k, v, ldq, ldk, ldv, qOut, ldqOut, K, V, slots, positions, rows, cosTab, sinTab, tableRows, stream)
 
     def Plan(self, rowStart, lens, nReqs, rows, window=0, prefixLens=None, stream=None):
-        return lib.mg_paged_plan(self._h, _p(rowStart), _p(lens), nReqs, rows, window, _p(prefixLens), stream)
+        return _paged_plan(self._h, rowStart, lens, nReqs, rows, window, prefixLens, stream)
 
     def Attention(self, q, ldq, K, V, table, out, ldo, scale=0.0, softcap=0.0, slopes=None, stream=None):
-        return lib.mg_paged_attention(self._h, _p(q), ldq, _p(K), _p(V), _p(table), _p(out), ldo, scale, softcap, _p(slopes), stream)
+        return _paged_attention(self._h, q, ldq, K, V, table, out, ldo, scale, softcap, slopes, stream)
+
+
+# (a server makes these calls for every layer of every step: the functions are looked up once)
+_paged_tables, _paged_store, _paged_plan, _paged_attention = lib.mg_paged_tables, lib.mg_paged_store, lib.mg_paged_plan, lib.mg_paged_attention
 
 
 def NewHIPPaged(eng, nHeads, nKVHeads, headDim, pageSize, nPages, kvFormat, maxReqs, maxRows, maxLen):

@@ -110,8 +110,9 @@ def test_the_model_of_a_step():
     assert got["counts"].tolist() == [3, 2, 2, 0]
 
 
-@pytest.mark.parametrize("tileRows,unitKeys,weight", [(16, 128, 1), (16, 64, 1), (128, 64, 2), (128, 64, 3)])
-def test_the_plan_gives_every_unit_to_one_worker(tmp_path, tileRows, unitKeys, weight):
+@pytest.mark.parametrize("few", [0, 1])
+@pytest.mark.parametrize("tileRows,unitKeys,least", [(16, 128, 1), (16, 64, 2), (128, 64, 2), (128, 32, 3)])
+def test_the_plan_gives_every_unit_to_one_worker(tmp_path, tileRows, unitKeys, least, few):
     """Random batches: every position that a token sees is in its tile's units, every unit in exactly one worker's share, the workers of
     a tile are all of worker0 .. worker1, no two partial results share a place, and a tile without units has one worker."""
     out = _run(tmp_path, r"""
@@ -130,10 +131,10 @@ int main() {
             for (int f = 0; f < rows * group; f += %(tileRows)d) {
                 PagedTile t{};
                 t.req = r; t.rows = rows; t.len = len; t.prefix = prefix; t.first = f; t.index = (int)tiles.size();
-                t.tileRows = %(tileRows)d; t.unitKeys = %(unitKeys)d; t.weight = %(weight)d;
+                t.tileRows = %(tileRows)d; t.unitKeys = %(unitKeys)d;
                 paged_units(t, window, group);
                 t.cost0 = (int)cost;
-                cost += PAGED_TILE_COST + t.units * t.weight;
+                cost += paged_cost(t);
                 for (int q = f; q < std::min(f + t.tileRows, rows * group); q++)
                     for (int j = 0; j < len; j++)
                         if (paged_sees(len - rows + q / group, j, len, window, prefix) && (j / t.unitKeys < t.unit0 || j / t.unitKeys >= t.unit0 + t.units)) { std::printf("position %%d\n", j); return 0; }
@@ -143,12 +144,30 @@ int main() {
             }
         }
         if (tiles.empty()) continue;
-        const int C = (int)cost, workers = std::max(1, std::min(most, C / %(weight)d));
+        const int C = (int)cost, T = (int)tiles.size(), given = %(few)d ? 2 * T + most : most;
+        if (paged_few(T, given) != %(few)d) continue;
+        int workers = std::max(1, std::min(given, C));
         std::set<int> places;
-        std::vector<int> seen(tiles.size(), 0), zero(tiles.size(), 0), done(tiles.size(), 0);
-        for (auto& t : tiles) if (t.units) { t.worker0 = paged_worker_of(C, workers, t.cost0 + PAGED_TILE_COST); t.worker1 = paged_worker_of(C, workers, t.cost0 + PAGED_TILE_COST + (t.units - 1) * t.weight); }
+        std::vector<int> seen(T, 0), zero(T, 0), done(T, 0), owner;
+        if (%(few)d) {
+            workers = 0;
+            for (auto& t : tiles) {
+                const int n = paged_workers_for(t, C, T, given, %(least)d);
+                if (n < 1 || (n > 1 && t.units / n < %(least)d)) { std::printf("count\n"); return 0; }
+                t.worker0 = workers; t.worker1 = workers + n - 1;
+                workers += n;
+                owner.insert(owner.end(), n, t.index);
+            }
+            if (workers > given) { std::printf("too many\n"); return 0; }
+        } else for (auto& t : tiles) if (t.units) { t.worker0 = paged_worker_of(C, workers, t.cost0 + PAGED_TILE_COST); t.worker1 = paged_worker_of(C, workers, t.cost0 + PAGED_TILE_COST + t.units - 1); }
         for (int w = 0; w < workers; w++) {
-            const int a = paged_share(C, workers, w), b = paged_share(C, workers, w + 1);
+            int a = paged_share(C, workers, w), b = paged_share(C, workers, w + 1);
+            if (%(few)d) {
+                const PagedTile& t = tiles[owner[w]];
+                const int n = t.worker1 - t.worker0 + 1, k = w - t.worker0;
+                a = paged_part(t, n, k);
+                b = k + 1 < n ? paged_part(t, n, k + 1) : t.cost0 + paged_cost(t);
+            }
             size_t i = tiles.size() - 1;
             while (tiles[i].cost0 > a) i--;
             for (; i < tiles.size() && tiles[i].cost0 < b; i++) {
@@ -166,7 +185,7 @@ int main() {
             empty += tiles[i].units == 0;
         }
     }
-    std::printf(split > 1000 && empty > 10 ? "ok\n" : "too few %%lld %%lld\n", split, empty);
+    std::printf(split > 300 && empty > 10 ? "ok\n" : "too few %%lld %%lld\n", split, empty);
 }
-""" % dict(tileRows=tileRows, unitKeys=unitKeys, weight=weight))
+""" % dict(tileRows=tileRows, unitKeys=unitKeys, least=least, few=few))
     assert out == "ok\n", out
