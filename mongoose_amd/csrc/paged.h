@@ -31,7 +31,7 @@ struct PagedPlan {
     const int *rowStart, *lens, *prefixLens;      // the caller's
     PagedTile* tiles;                             // the handle's: maxTiles of them, for narrow tiles and again for wide ones,
     PagedWorker* workers;                         // and maxWorkers of these
-    int nReqs, rows, window, maxLen, group, kvHalf, maxTiles, maxWorkers, nWorkers, narrowRows;
+    int nReqs, rows, window, maxLen, group, kvHalf, maxTiles, maxWorkers, nWorkers, wideWorkers, narrowRows;      // wideWorkers 0: no wide tiles
 };
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s);
 
@@ -47,12 +47,12 @@ struct PagedAttention {
     const float* zeros;        // headDim zeros: what a position outside a tile's, or on a page that is gone, is read from
     size_t partStride;
     float scale, softcap;
-    int ldq, ldo, window, maxTiles, maxWorkers, nWorkers, wide;
+    int ldq, ldo, window, maxTiles, maxWorkers, nWorkers, wideWorkers;
     PagedGeo g;
 };
 size_t paged_part_floats(const PagedGeo& g);
 int paged_max_tiles(const PagedGeo& g);
-int paged_workers(const PagedGeo& g, int nReqs, int rows);       // workers a KV head
+int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide);       // workers a KV head
 int paged_narrow_rows(const PagedGeo& g, int rows);              // requests of up to so many rows a KV head have narrow tiles
 hipError_t paged_attention_setup(const PagedGeo& g);
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t s);

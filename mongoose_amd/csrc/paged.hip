@@ -2,6 +2,7 @@
 // request lengths, and rotary positions with the K/V rows stored by slot.  The attention that reads the pages is in paged_attn.hip.
 #include "paged.h"
 
+#include <algorithm>
 #include <cmath>
 #include <new>
 #include <string>
@@ -216,7 +217,7 @@ struct mg_paged {
     unsigned* arrived;
     float* parts;
     int maxTiles, maxWorkers;
-    int planReqs, planRows, planWindow, planWorkers, planWide;      // the last plan (planReqs < 0: none yet)
+    int planReqs, planRows, planWindow, planWorkers, planWideWorkers;      // the last plan (planReqs < 0: none yet)
 };
 
 namespace {
@@ -257,7 +258,7 @@ mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, i
     h->g = g;
     h->device = device;
     h->planReqs = -1;
-    const size_t tiles = (size_t)mg::paged_max_tiles(g), workers = (size_t)mg::paged_workers(g, g.maxReqs, g.maxRows), heads = (size_t)g.nKVHeads;
+    const size_t tiles = (size_t)mg::paged_max_tiles(g), workers = (size_t)std::max(mg::paged_workers(g, g.maxReqs, g.maxRows, false), mg::paged_workers(g, g.maxReqs, g.maxRows, true)), heads = (size_t)g.nKVHeads;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
     const size_t oZeros = take((size_t)g.headDim * 4), oArrived = take(heads * tiles * 4), clear = at;      // (the part that starts as zeros)
@@ -314,12 +315,12 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
     PAGED(h, "mg_paged_plan");
     if (const char* why = mg::paged_plan_refusal(h->g, rowStart, lens, nReqs, rows, window, prefixLens)) return refuse("mg_paged_plan", why);
     const mg::PagedGeo& g = h->g;
-    const int workers = mg::paged_workers(g, nReqs, rows), narrow = mg::paged_narrow_rows(g, rows);
-    mg::PagedPlan p{rowStart, lens, prefixLens, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, h->maxTiles, h->maxWorkers, workers, narrow};
+    const int workers = mg::paged_workers(g, nReqs, rows, false), narrow = mg::paged_narrow_rows(g, rows);
+    const int wide = (long long)rows * g.group > narrow ? mg::paged_workers(g, nReqs, rows, true) : 0;
+    mg::PagedPlan p{rowStart, lens, prefixLens, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, h->maxTiles, h->maxWorkers, workers, wide, narrow};
     const int rc = launched("mg_paged_plan", mg::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
     if (rc == MG_OK) {
-        h->planReqs = nReqs; h->planRows = rows; h->planWindow = window; h->planWorkers = workers;
-        h->planWide = (long long)rows * g.group > narrow;
+        h->planReqs = nReqs; h->planRows = rows; h->planWindow = window; h->planWorkers = workers; h->planWideWorkers = wide;
     }
     return rc;
 }
@@ -331,7 +332,7 @@ int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, cons
     if (const char* why = mg::paged_attention_refusal(h->g, q, ldq, K, V, table, out, ldo, scale, softcap, slopes)) return refuse("mg_paged_attention", why);
     const mg::PagedGeo& g = h->g;
     mg::PagedAttention p{q, slopes, K, V, table, out, h->tiles, h->workers, h->parts, h->arrived, h->zeros, mg::paged_part_floats(g),
-                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, ldq, ldo, h->planWindow, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWide, g};
+                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, ldq, ldo, h->planWindow, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
     return launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
 }
 

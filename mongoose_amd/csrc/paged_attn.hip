@@ -41,10 +41,13 @@ int paged_narrow_rows(const PagedGeo& g, int rows) {
 }
 int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + 256 / NARROW; }
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
-// Two workgroups a CU, in turns of the KV heads; fewer where the batch cannot have that many units.
-int paged_workers(const PagedGeo& g, int nReqs, int rows) {
+// Workgroups, in turns of the KV heads: two a CU for wide tiles; one a CU for narrow ones, though a CU holds two: HBM likes fewer
+// streams (8B shape, fp16: 120,001 positions 102 us, with two 122, with three 145; 48 requests 173, 182, 217).  Fewer where the batch
+// cannot have that many units.
+int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide) {
     const long long tiles = (long long)rows * g.group / NARROW + nReqs, units = tiles * (g.maxLen / 32 + 2);
-    const long long most = 512 / g.nKVHeads > 0 ? 512 / g.nKVHeads : 1;
+    const int resident = 256 * (wide ? 2 : 1);
+    const long long most = resident / g.nKVHeads > 0 ? resident / g.nKVHeads : 1;
     return (int)(units < 1 ? 1 : units < most ? units : most);
 }
 
@@ -98,6 +101,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
     const int tileRows = wide ? WIDE : NARROW, unitKeys = wide ? wide_keys(p.kvHalf) : narrow_keys(p.kvHalf);
     p.tiles += wide ? p.maxTiles : 0;
     p.workers += wide ? p.maxWorkers : 0;
+    p.nWorkers = wide ? p.wideWorkers : p.nWorkers;
     __shared__ unsigned tile0[PAGED_MAX_REQS + 1], place[PLAN_LDS_TILES], part[PT / 64];
     __shared__ int4 held[PT];
     const int tid = threadIdx.x;
@@ -198,7 +202,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
     }
 }
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s) {
-    hipLaunchKernelGGL(paged_plan_kernel, dim3((long long)p.rows * p.group > p.narrowRows ? 2 : 1), dim3(PT), 0, s, p);
+    hipLaunchKernelGGL(paged_plan_kernel, dim3(p.wideWorkers > 0 ? 2 : 1), dim3(PT), 0, s, p);
     return hipGetLastError();
 }
 
@@ -305,6 +309,53 @@ __device__ __forceinline__ void merge_weights(const PagedAttention& p, const Pag
     }
 }
 __device__ __forceinline__ float4_t over(float4_t v, float l) { return l == 0.f ? v : v / l; }       // (nothing seen: zeros)
+
+// Units with values that are no numbers at positions that not every token of a wave's rows sees: zero times them is no zero, so they
+// are left out of the product (their scores are in the sums), and at the tile's end their positions are gone through row by row, each
+// with those it sees.  There are at most five: the tokens of up to 32 rows end in two units, their windows begin in two, a
+// prefix ends in one; unit numbers take 20 bits (2^24 positions, 32 a wave's step).
+struct LateUnits {
+    unsigned long long lo = 0, hi = 0;
+    int n = 0;
+    __device__ __forceinline__ void add(int u) {
+        hi = hi << 20 | lo >> 40;
+        lo = (lo << 20 | (unsigned)u) & ((1ull << 60) - 1);
+        n++;
+    }
+    __device__ __forceinline__ int at(int i) const { return (int)((i < 3 ? lo >> 20 * i : hi >> 20 * (i - 3)) & 0xfffff); }
+};
+// acc[e] += probability x value of one row (maximum mr) over the late units' positions; lane x has elements x E .. of the rows
+template <typename KVT, int HD, bool MOD, int KEYS, typename Base>
+__device__ __forceinline__ void late_row(const PagedAttention& p, const PagedTile& t, const LateUnits& late, Base base_of, int kvh, int row, float mr, float shift, int x, float (&acc)[HD / 64]) {
+    constexpr int E = HD / 64;
+    const PagedRow at = paged_row(t, p.g.group, kvh, row);
+    const int* pages = p.table + (size_t)t.req * p.g.width;
+    const float* q = p.q + (size_t)(t.row0 + at.token) * p.ldq + (size_t)at.head * HD + x * E;
+    const float slope = MOD && p.slopes ? p.slopes[at.head] : 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) acc[e] = 0.f;
+#pragma unroll 1
+    for (int n = 0; n < late.n; n++) {
+        const int base = base_of(late.at(n));
+#pragma unroll 1
+        for (int j = base; j < base + KEYS; j++) {
+            if (!paged_sees(at.pos, j, t.len, p.window, t.prefix)) continue;
+            const int page = pages[j >> p.g.pageShift];
+            if (page < 0 || page >= p.g.nPages) continue;
+            const size_t from = (((size_t)page << p.g.pageShift) + (j & (p.g.pageSize - 1))) * p.g.kvDim + (size_t)kvh * HD + x * E;
+            const KVT* k = static_cast<const KVT*>(p.K) + from;
+            const KVT* v = static_cast<const KVT*>(p.V) + from;
+            float y = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; e++) y = fmaf(q[e], (float)k[e], y);
+            y = wave_sum(y) * p.scale;
+            if (MOD) y = (p.softcap > 0.f ? capped(y, p.softcap, 1.f / p.softcap) : y) - slope * (float)abs(at.pos - j);
+            y = __builtin_amdgcn_exp2f(fmaf(y, 1.4426950408889634f, shift - (mr == -INFINITY ? 0.f : mr)));
+#pragma unroll
+            for (int e = 0; e < E; e++) acc[e] = fmaf(y, (float)v[e], acc[e]);
+        }
+    }
+}
 
 // A tile of 16 rows: four waves take a step of KB positions each of every unit, each with its own running maximum, sum and output.
 // Bound by HBM: a lane loads its K and V operands from the pages straight into registers, a step ahead and the page numbers two
@@ -445,19 +496,20 @@ struct NarrowTile {
         }
         return w;
     }
-    // Block e of V^T P^T on top of `out`; keep: all ones for the lane's positions that count
-    template <bool MASKED>
-    __device__ __forceinline__ float4_t product(int e, const Weights& w, const unsigned (&keep)[NB * 4], float4_t out) const {
-        auto word = [&](int j, int i) { return MASKED ? v[j][i] & keep[j] : v[j][i]; };
+    // Block e of V^T P^T on top of `out`
+    __device__ __forceinline__ float4_t product(int e, const Weights& w, float4_t out) const {
         if constexpr (HALF) {
             uint4_t a;
 #pragma unroll
-            for (int j = 0; j < 4; j++) a[j] = __builtin_amdgcn_perm(word(2 * j + 1, e / 2), word(2 * j, e / 2), e & 1 ? 0x07060302u : 0x05040100u);
+            for (int j = 0; j < 4; j++) a[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
             out = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w.hi, out, 0, 0, 0);
             out = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w.lo, out, 0, 0, 0);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; i++) out = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, word(i, e)), w.x[i], out, 0, 0, 0);
+            for (int i = 0; i < 4; i++) {
+                const unsigned x = v[i][e];
+                out = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float, x), w.x[i], out, 0, 0, 0);
+            }
         }
         return out;
     }
@@ -513,7 +565,8 @@ struct NarrowTile {
                 x[j] = (x[j] - slope * (float)abs(row.pos - (base + 16 * (j / 4) + 4 * g + j % 4))) * 1.4426950408889634f;
             }
         }
-        const bool all = __all(mine >= 0) && (base + KB <= t.prefix || (base + KB - 1 <= span.pos0 && (p.window == 0 || base > span.pos1 - p.window)));
+        const bool inner = base + KB <= t.prefix || (base + KB - 1 <= span.pos0 && (p.window == 0 || base > span.pos1 - p.window));       // all rows see all of it
+        const bool all = inner && __all(mine >= 0);
         if (!all) {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
@@ -540,35 +593,41 @@ struct NarrowTile {
             x[j] = __builtin_amdgcn_exp2f(x[j] - from + SHIFT);
             l += x[j];
         }
-        bool odd = false;
-        if (!all && span.pos0 != span.pos1) {
+        if (!inner) {
+            bool some = false, odd = false;
 #pragma unroll
-            for (int j = 0; j < NB * 4; j++)
+            for (int j = 0; j < NB * 4; j++) some |= x[j] != 0.f;
+            if (!__any(some)) return;                     // (no row has anything here: a value that is no number must not get to any)
+            if (span.pos0 != span.pos1) {
 #pragma unroll
-                for (int e = 0; e < VW; e++) odd |= not_finite(v[j][e]);
-        }
-        const Weights wt = weights(x);
-        unsigned keep[NB * 4];
-        if (!__any(odd)) {
+                for (int j = 0; j < NB * 4; j++)
 #pragma unroll
-            for (int e = 0; e < EPL; e++) o[e] = product<false>(e, wt, keep, o[e]);
-            return;
-        }
-        // Values that are no numbers at positions that not every token sees, and zero times them is no zero: token by token, with
-        // the positions that it does not see taken out.
-#pragma unroll 1
-        for (int pos = span.pos0; pos <= span.pos1; pos++) {
-#pragma unroll
-            for (int j = 0; j < NB * 4; j++) keep[j] = paged_sees(pos, base + 16 * (j / 4) + 4 * g + j % 4, t.len, p.window, t.prefix) ? ~0u : 0u;
-#pragma unroll
-            for (int e = 0; e < EPL; e++) {
-                const float4_t part = product<true>(e, wt, keep, float4_t{0.f, 0.f, 0.f, 0.f});
-#pragma unroll
-                for (int i = 0; i < 4; i++) o[e][i] = row.pos == pos ? o[e][i] + part[i] : o[e][i];
+                    for (int e = 0; e < VW; e++) odd |= not_finite(v[j][e]);
+                if (__any(odd)) { late.add(u); return; }
             }
         }
+        const Weights wt = weights(x);
+#pragma unroll
+        for (int e = 0; e < EPL; e++) o[e] = product(e, wt, o[e]);
     }
-    __device__ __forceinline__ void run(int u0, int u1, int, int, float* lds) {
+    LateUnits late;
+    __device__ __forceinline__ void add_late(int kvh, float* mine) {          // by way of the wave's rows in LDS
+        const int rows = min(NARROW, t.rows * p.g.group - t.first), x = anew(lane);
+#pragma unroll 1
+        for (int r = 0; r < rows; r++) {
+            float acc[HD / 64];
+            late_row<KVT, HD, MOD, KB>(p, t, late, [&](int u) { return base_of(u); }, kvh, r, lane_value(m, r), SHIFT, x, acc);
+#pragma unroll
+            for (int e = 0; e < HD / 64; e++) mine[r * (HD + 4) + x * (HD / 64) + e] = acc[e];
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        if (l16 >= rows) return;
+#pragma unroll
+        for (int e = 0; e < EPL; e++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) o[e][i] += mine[l16 * (HD + 4) + (4 * g + i) * EPL + e];
+    }
+    __device__ __forceinline__ void run(int u0, int u1, int kvh, int, float* lds) {
         for (int u = u0; u < u1; u++) {
             const int behind = page_of(min(u + 2, u1 - 1));
             const bool more = u + 1 < u1;
@@ -577,15 +636,16 @@ struct NarrowTile {
             here = next;
             next = behind;
         }
-        join(lds);
+        join(kvh, lds);
     }
     // The four waves' results as one, at lds (rows of HD + 4 floats) with maxima and sums behind
     static constexpr int FLOATS = 4 * NARROW * (HD + 4) + 8 * NARROW;
-    __device__ __forceinline__ void join(float* lds) {
+    __device__ __forceinline__ void join(int kvh, float* lds) {
         float* wm = lds + 4 * NARROW * (HD + 4);
         float* wl = wm + 4 * NARROW;
         l = rows_sum(l);
         __syncthreads();                          // (the tile before has been written out)
+        if (late.n) add_late(kvh, lds + wave * NARROW * (HD + 4));
         float* mine = lds + (wave * NARROW + l16) * (HD + 4) + 4 * g * EPL;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -1169,9 +1229,10 @@ hipError_t paged_attention_setup(const PagedGeo& g) {
     return hipSuccess;
 }
 hipError_t launch_paged_attention(const PagedAttention& p0, hipStream_t s) {
-    const int groups = (p0.nWorkers * p0.g.nKVHeads + 7) / 8 * 8;
-    for (int wide = p0.wide; wide >= 0; wide--) {
+    for (int wide = p0.wideWorkers > 0; wide >= 0; wide--) {
         PagedAttention p = p0;
+        if (wide) p.nWorkers = p.wideWorkers;
+        const int groups = (p.nWorkers * p.g.nKVHeads + 7) / 8 * 8;
         p.tiles += wide ? p.maxTiles : 0;
         p.workers += wide ? p.maxWorkers : 0;
         const size_t lds = attn_lds(p.g.headDim, wide);
