@@ -209,19 +209,41 @@ hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s) {
 // ---------------------------------------------------------------------------
 // Attention
 // ---------------------------------------------------------------------------
-// cap * tanh(x / cap): the odd Taylor polynomial up to x^13 where |x / cap| < 0.45 (the next term is below 2^-26 of the result),
-// (1 - e^-2x) / (1 + e^-2x) beyond.
-__device__ __forceinline__ float capped(float s, float cap, float invCap) {
-    const float x = s * invCap, a = fabsf(x), x2 = x * x;
+// cap * tanh(s / cap).  Near zero the odd Taylor polynomial up to x^13, s + s x^2 P(x^2) with x = s / cap: where |x| < 0.45 the next
+// term is below 2^-26 of the result.  Beyond, (1 - e^-2x) / (1 + e^-2x).
+constexpr float CAP_NEAR = 0.45f;
+__device__ __forceinline__ float capped_near(float s, float x2) {
     float t = fmaf(x2, 21844.f / 6081075.f, -1382.f / 155925.f);
     t = fmaf(x2, t, 62.f / 2835.f);
     t = fmaf(x2, t, -17.f / 315.f);
     t = fmaf(x2, t, 2.f / 15.f);
     t = fmaf(x2, t, -1.f / 3.f);
-    t = fmaf(x * x2, t, x);
+    return fmaf(x2 * t, s, s);
+}
+__device__ __forceinline__ float capped(float s, float cap, float invCap) {
+    const float x = s * invCap, a = fabsf(x);
     const float e = __builtin_amdgcn_exp2f(a * -2.885390081777927f);
     const float far = copysignf((1.f - e) * __builtin_amdgcn_rcpf(1.f + e), x);
-    return cap * (a < 0.45f ? t : far);
+    return a < CAP_NEAR ? capped_near(s, x * x) : cap * far;
+}
+// The cap on all the scores of a lane: without the far form where no lane of the wave needs it (8B shape, four requests of 345 to
+// 467 rows over a window of 1,024, cap 50: 150 -> 118 us)
+template <typename T, int N>
+__device__ __forceinline__ void cap_all(T (&s)[N], float cap, float invCap) {
+    constexpr int M = sizeof(T) / 4;
+    auto at = [&](int i) -> float { if constexpr (M == 1) return s[i]; else return s[i / M][i % M]; };
+    float most = 0.f;
+#pragma unroll
+    for (int i = 0; i < N * M; i++) most = fmaxf(most, fabsf(at(i)));
+    auto all = [&](auto f) {
+#pragma unroll
+        for (int i = 0; i < N * M; i++) {
+            if (i % 8 == 0) __builtin_amdgcn_sched_barrier(0);       // (eight at once: for more there are no registers)
+            if constexpr (M == 1) s[i] = f(at(i)); else s[i / M][i % M] = f(at(i));
+        }
+    };
+    if (!__any(!(most * invCap < CAP_NEAR))) all([&](float y) { const float x = y * invCap; return capped_near(y, x * x); });
+    else all([&](float y) { return capped(y, cap, invCap); });
 }
 // 16 bytes through to memory, for a workgroup of another die to read within the launch
 __device__ __forceinline__ void store_through(float* p, float4_t v) {
@@ -558,12 +580,11 @@ struct NarrowTile {
         // scores in powers of two; the lane's positions are base + 16 b + 4 g + i
         float x[NB * 4];
 #pragma unroll
-        for (int j = 0; j < NB * 4; j++) {
-            x[j] = S[j / 4][j % 4] * c;
-            if (MOD) {
-                if (cap > 0.f) x[j] = capped(x[j], cap, invCap);
-                x[j] = (x[j] - slope * (float)abs(row.pos - (base + 16 * (j / 4) + 4 * g + j % 4))) * 1.4426950408889634f;
-            }
+        for (int j = 0; j < NB * 4; j++) x[j] = S[j / 4][j % 4] * c;
+        if constexpr (MOD) {
+            if (cap > 0.f) cap_all(x, cap, invCap);
+#pragma unroll
+            for (int j = 0; j < NB * 4; j++) x[j] = (x[j] - slope * (float)abs(row.pos - (base + 16 * (j / 4) + 4 * g + j % 4))) * 1.4426950408889634f;
         }
         const bool inner = base + KB <= t.prefix || (base + KB - 1 <= span.pos0 && (p.window == 0 || base > span.pos1 - p.window));       // all rows see all of it
         const bool all = inner && __all(mine >= 0);
@@ -953,14 +974,16 @@ struct WideTile {
         const int first = base + 4 * anew(hf);            // the lane's first position
         if constexpr (MOD) {
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+            for (int b = 0; b < NB; b++) S[b] *= c;
+            if (cap > 0.f) cap_all(S, cap, invCap);
+            if (p.slopes) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    float x = S[b][i] * c;
-                    if (cap > 0.f) x = capped(x, cap, invCap);
-                    S[b][i] = (x - slope * (float)abs(row.pos - (first + 32 * b + 8 * (i / 4) + i % 4))) * 1.4426950408889634f;
-                }
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) S[b][i] = fmaf(-slope, (float)abs(row.pos - (first + 32 * b + 8 * (i / 4) + i % 4)), S[b][i]);
+            }
         }
+        const float factor = MOD ? 1.4426950408889634f : c;          // scores to powers of two
         if (!all) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
@@ -976,7 +999,7 @@ struct WideTile {
         float other = top;
         row_swap32(top, other);
         top = fmaxf(top, other);
-        if (!MOD) top = top == -INFINITY ? top : top * c;
+        top = top == -INFINITY ? top : top * factor;
         mNew = top > m + LAZY || m == -INFINITY ? fmaxf(m, top) : m;
         const float shift = SHIFT - (mNew == -INFINITY ? 0.f : mNew);          // (a score that is a NaN stays one)
         float ts = 0.f;
@@ -984,7 +1007,7 @@ struct WideTile {
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                S[b][i] = __builtin_amdgcn_exp2f(MOD ? S[b][i] + shift : fmaf(S[b][i], c, shift));
+                S[b][i] = __builtin_amdgcn_exp2f(fmaf(S[b][i], factor, shift));
                 ts += S[b][i];
             }
         return ts;
