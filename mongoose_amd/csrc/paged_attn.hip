@@ -227,7 +227,7 @@ __device__ __forceinline__ float capped(float s, float cap, float invCap) {
     return a < CAP_NEAR ? capped_near(s, x * x) : cap * far;
 }
 // The cap on all the scores of a lane: without the far form where no lane of the wave needs it (8B shape, four requests of 345 to
-// 467 rows over a window of 1,024, cap 50: 150 -> 118 us)
+// 467 rows over a window of 1,024, cap 50: 150 -> 136 us)
 template <typename T, int N>
 __device__ __forceinline__ void cap_all(T (&s)[N], float cap, float invCap) {
     constexpr int M = sizeof(T) / 4;
