@@ -189,3 +189,19 @@ int main() {
 }
 """ % dict(tileRows=tileRows, unitKeys=unitKeys, least=least, few=few))
     assert out == "ok\n", out
+
+
+def test_scales_and_caps_without_a_reciprocal_are_refused(tmp_path):
+    out = _run(tmp_path, r"""
+static char mem[256] __attribute__((aligned(16)));
+int main() {
+    PagedGeo g{};
+    if (paged_geo(g, 8, 2, 64, 16, 100, 1, 4, 64, 1000)) return 1;
+    for (float x : {1e-30f, 1e30f, 1e-31f, 1e-40f, 1e31f}) {
+        const char* a = paged_attention_refusal(g, mem, 512, mem, mem, mem, mem + 64, 512, x, 0.f, nullptr);
+        const char* b = paged_attention_refusal(g, mem, 512, mem, mem, mem, mem + 64, 512, 0.f, x, nullptr);
+        std::printf("%d%d ", a != nullptr, b != nullptr);
+    }
+}
+""")
+    assert out == "00 00 11 11 11 "
