@@ -1056,7 +1056,7 @@ struct WideTile {
         }
         if (!inner) {
             if (!__any(ts != 0.f)) return;                // (no row has anything here: a value that is no number must not get to any)
-            if (pos0 != pos1 && !values_finite(V)) {
+            if (!values_finite(V)) {          // (one token or more: the tile holds what its other tokens see)
                 lateHi = lateHi << 20 | lateLo >> 40;
                 lateLo = (lateLo << 20 | (unsigned)u) & ((1ull << 60) - 1);
                 lates++;
