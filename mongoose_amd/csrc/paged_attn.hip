@@ -620,7 +620,8 @@ struct NarrowTile {
 #pragma unroll
             for (int j = 0; j < NB * 4; j++) some |= x[j] != 0.f;
             if (!__any(some)) return;                     // (no row has anything here: a value that is no number must not get to any)
-            if (span.pos0 != span.pos1) {
+            // (a single token sees all of its span but what lies between a prefix and a window)
+            if (span.pos0 != span.pos1 || (p.window > 0 && t.prefix > 0)) {
 #pragma unroll
                 for (int j = 0; j < NB * 4; j++)
 #pragma unroll

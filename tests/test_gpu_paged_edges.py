@@ -43,3 +43,17 @@ def test_hidden_values_where_a_wave_of_a_wide_tile_is_one_token(hip, bufs, heads
     for j in bad:
         c.V[c.where(0, j), j % 5::7] = value
     _check(c, window=window)
+
+
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("value", [np.nan, np.inf])
+@pytest.mark.parametrize("heads,kv,hd,n", [(4, 4, 64, 1), (8, 2, 128, 2), (40, 1, 128, 7), (32, 1, 64, 9)])
+def test_hidden_values_between_a_single_tokens_prefix_and_its_window(hip, bufs, heads, kv, hd, n, value, half):
+    """What lies behind the prefix and before the window shares units with both; groups of 32 and 40 in batches above 256 rows have wide tiles."""
+    print(f"gap {heads}/{kv}/{hd} x {n} half={half}", flush=True)
+    lens = [500 - 7 * r for r in range(n)]
+    for bad in ((10, 31), (420, 435), (200,)):
+        c = Case(hip, bufs, heads, kv, hd, half, 8, [1] * n, lens, seed=n)
+        for j in bad:
+            c.V[c.where(0, j), j % 5::7] = value
+        _check(c, window=64, prefix=[10] * n)
