@@ -332,52 +332,27 @@ __device__ __forceinline__ void merge_weights(const PagedAttention& p, const Pag
 }
 __device__ __forceinline__ float4_t over(float4_t v, float l) { return l == 0.f ? v : v / l; }       // (nothing seen: zeros)
 
-// Units with values that are no numbers at positions that not every token of a wave's rows sees: zero times them is no zero, so they
-// are left out of the product (their scores are in the sums), and at the tile's end their positions are gone through row by row, each
-// with those it sees.  There are at most five: the tokens of up to 32 rows end in two units, their windows begin in two, a
-// prefix ends in one; unit numbers take 20 bits (2^24 positions, 32 a wave's step).
-struct LateUnits {
-    unsigned long long lo = 0, hi = 0;
-    int n = 0;
-    __device__ __forceinline__ void add(int u) {
-        hi = hi << 20 | lo >> 40;
-        lo = (lo << 20 | (unsigned)u) & ((1ull << 60) - 1);
-        n++;
+// Values that are no numbers.  Zero times one is no zero, so that one reaches rows that do not see it, and its product with the second
+// term of a weight turns an infinity into a NaN.  A tile whose result has elements that are no numbers therefore goes through its
+// units three times more, with the maxima of the first time: with ones for +infinity and NaN, zeros for all else, and weights of 1 (or 0
+// where they are 0); the same for -infinity and NaN; with zeros for all three.  An element is what the last time gives, plus an
+// infinity where the first count is not 0, minus one where the second is not.  Other tiles pay for a look at their result.
+enum { PLUS_INFINITE, MINUS_INFINITE, FINITE };
+// What stands for the values of a word in a pass
+template <bool HALF>
+__device__ __forceinline__ unsigned stand_in(unsigned v, int pass) {
+    constexpr int BITS = HALF ? 16 : 32;
+    constexpr unsigned sign = 1u << (BITS - 1), inf = HALF ? 0x7c00u : 0x7f800000u, one = HALF ? 0x3c00u : 0x3f800000u;
+    unsigned out = 0;
+#pragma unroll
+    for (int at = 0; at < 32; at += BITS) {
+        const unsigned x = HALF ? (v >> at) & 0xffffu : v, size = x & (sign - 1);
+        const bool counts = size > inf || x == (pass == MINUS_INFINITE ? sign | inf : inf);
+        out |= (pass == FINITE ? (size < inf ? x : 0u) : counts ? one : 0u) << at;
     }
-    __device__ __forceinline__ int at(int i) const { return (int)((i < 3 ? lo >> 20 * i : hi >> 20 * (i - 3)) & 0xfffff); }
-};
-// acc[e] += probability x value of one row (maximum mr) over the late units' positions; lane x has elements x E .. of the rows
-template <typename KVT, int HD, bool MOD, int KEYS, typename Base>
-__device__ __forceinline__ void late_row(const PagedAttention& p, const PagedTile& t, const LateUnits& late, Base base_of, int kvh, int row, float mr, float shift, int x, float (&acc)[HD / 64]) {
-    constexpr int E = HD / 64;
-    const PagedRow at = paged_row(t, p.g.group, kvh, row);
-    const int* pages = p.table + (size_t)t.req * p.g.width;
-    const float* q = p.q + (size_t)(t.row0 + at.token) * p.ldq + (size_t)at.head * HD + x * E;
-    const float slope = MOD && p.slopes ? p.slopes[at.head] : 0.f;
-#pragma unroll
-    for (int e = 0; e < E; e++) acc[e] = 0.f;
-#pragma unroll 1
-    for (int n = 0; n < late.n; n++) {
-        const int base = base_of(late.at(n));
-#pragma unroll 1
-        for (int j = base; j < base + KEYS; j++) {
-            if (!paged_sees(at.pos, j, t.len, p.window, t.prefix)) continue;
-            const int page = pages[j >> p.g.pageShift];
-            if (page < 0 || page >= p.g.nPages) continue;
-            const size_t from = (((size_t)page << p.g.pageShift) + (j & (p.g.pageSize - 1))) * p.g.kvDim + (size_t)kvh * HD + x * E;
-            const KVT* k = static_cast<const KVT*>(p.K) + from;
-            const KVT* v = static_cast<const KVT*>(p.V) + from;
-            float y = 0.f;
-#pragma unroll
-            for (int e = 0; e < E; e++) y = fmaf(q[e], (float)k[e], y);
-            y = wave_sum(y) * p.scale;
-            if (MOD) y = (p.softcap > 0.f ? capped(y, p.softcap, 1.f / p.softcap) : y) - slope * (float)abs(at.pos - j);
-            y = __builtin_amdgcn_exp2f(fmaf(y, 1.4426950408889634f, shift - (mr == -INFINITY ? 0.f : mr)));
-#pragma unroll
-            for (int e = 0; e < E; e++) acc[e] = fmaf(y, (float)v[e], acc[e]);
-        }
-    }
+    return out;
 }
+__device__ __forceinline__ float with_infinities(float o, bool plus, bool minus) { return (plus ? o + INFINITY : o) + (minus ? -INFINITY : 0.f); }
 
 // A tile of 16 rows: four waves take a step of KB positions each of every unit, each with its own running maximum, sum and output.
 // Bound by HBM: a lane loads its K and V operands from the pages straight into registers, each where the last step's have gone into
@@ -536,12 +511,9 @@ struct NarrowTile {
         }
         return out;
     }
-    static __device__ __forceinline__ bool not_finite(unsigned v) {
-        if (HALF) return ((v & 0x7fffu) >= 0x7c00u) | ((v & 0x7fff0000u) >= 0x7c000000u);
-        return (v & 0x7fffffffu) >= 0x7f800000u;
-    }
     // Step u, on page numbers `mine`; loads the K rows of the one behind it (if any, on page numbers `next`) where it is done with its own
-    __device__ __forceinline__ void compute(int u, int mine, bool more, int next) {
+    template <bool AGAIN>
+    __device__ __forceinline__ void compute(int u, int mine, bool more, int next, int pass) {
         const int base = base_of(u);
         float4_t S[NB];
 #pragma unroll
@@ -616,48 +588,65 @@ struct NarrowTile {
             l += x[j];
         }
         if (!inner) {
-            bool some = false, odd = false;
+            bool some = false;
 #pragma unroll
             for (int j = 0; j < NB * 4; j++) some |= x[j] != 0.f;
-            if (!__any(some)) return;                     // (no row has anything here: a value that is no number must not get to any)
-            // (a single token sees all of its span but what lies between a prefix and a window)
-            if (span.pos0 != span.pos1 || (p.window > 0 && t.prefix > 0)) {
+            if (!__any(some)) return;                     // (no row has anything here)
+        }
+        if constexpr (AGAIN) {
 #pragma unroll
-                for (int j = 0; j < NB * 4; j++)
+            for (int j = 0; j < NB * 4; j++) {
+                x[j] = pass == FINITE ? x[j] : x[j] > 0.f ? 1.f : 0.f;
 #pragma unroll
-                    for (int e = 0; e < VW; e++) odd |= not_finite(v[j][e]);
-                if (__any(odd)) { late.add(u); return; }
+                for (int e = 0; e < VW; e++) v[j][e] = stand_in<HALF>(v[j][e], pass);
             }
         }
         const Weights wt = weights(x);
 #pragma unroll
         for (int e = 0; e < EPL; e++) o[e] = product(e, wt, o[e]);
     }
-    LateUnits late;
-    __device__ __forceinline__ void add_late(int kvh, float* mine) {          // by way of the wave's rows in LDS
-        const int rows = min(NARROW, t.rows * p.g.group - t.first), x = anew(lane);
-#pragma unroll 1
-        for (int r = 0; r < rows; r++) {
-            float acc[HD / 64];
-            late_row<KVT, HD, MOD, KB>(p, t, late, [&](int u) { return base_of(u); }, kvh, r, lane_value(m, r), SHIFT, x, acc);
-#pragma unroll
-            for (int e = 0; e < HD / 64; e++) mine[r * (HD + 4) + x * (HD / 64) + e] = acc[e];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        if (l16 >= rows) return;
-#pragma unroll
-        for (int e = 0; e < EPL; e++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) o[e][i] += mine[l16 * (HD + 4) + (4 * g + i) * EPL + e];
-    }
-    __device__ __forceinline__ void run(int u0, int u1, int kvh, int, float* lds) {
+    template <bool AGAIN>
+    __device__ __forceinline__ void units(int u0, int u1, int pass) {
         for (int u = u0; u < u1; u++) {
             const int behind = page_of(min(u + 2, u1 - 1));
             const bool more = u + 1 < u1;
-            compute(u, here, more, next);
+            compute<AGAIN>(u, here, more, next, pass);
             if (more) load_v(u + 1, next);
             here = next;
             next = behind;
+        }
+    }
+    __device__ __forceinline__ void run(int u0, int u1, int kvh, int, float* lds) {
+        units<false>(u0, u1, 0);
+        float odd = 0.f;
+#pragma unroll
+        for (int e = 0; e < EPL; e++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) odd = fmaf(o[e][i], 0.f, odd);
+        if (__any(odd != odd)) {
+            unsigned plus = 0, minus = 0;         // a bit an element
+#pragma unroll 1
+            for (int pass = PLUS_INFINITE; pass <= FINITE; pass++) {
+                here = page_of(u0);
+                next = page_of(min(u0 + 1, u1 - 1));
+                load_k(u0, here);
+                load_v(u0, here);
+                l = 0.f;
+#pragma unroll
+                for (int e = 0; e < EPL; e++) o[e] = float4_t{0.f, 0.f, 0.f, 0.f};
+                units<true>(u0, u1, pass);
+                unsigned counts = 0;
+#pragma unroll
+                for (int e = 0; e < EPL; e++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) counts |= (o[e][i] > 0.f ? 1u : 0u) << (4 * e + i);
+                if (pass == PLUS_INFINITE) plus = counts;
+                if (pass == MINUS_INFINITE) minus = counts;
+            }
+#pragma unroll
+            for (int e = 0; e < EPL; e++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) o[e][i] = with_infinities(o[e][i], plus >> (4 * e + i) & 1, minus >> (4 * e + i) & 1);
         }
         join(kvh, lds);
     }
@@ -668,7 +657,6 @@ struct NarrowTile {
         float* wl = wm + 4 * NARROW;
         l = rows_sum(l);
         __syncthreads();                          // (the tile before has been written out)
-        if (late.n) add_late(kvh, lds + wave * NARROW * (HD + 4));
         float* mine = lds + (wave * NARROW + l16) * (HD + 4) + 4 * g * EPL;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -769,6 +757,7 @@ struct WideTile {
     static constexpr int ROWB = HD * (int)sizeof(KVT), PR = ROWB / 16;      // bytes and 16-byte pieces of a row
     static constexpr int RI = 64 / PR, NI = UK / RI / 4;                    // rows a load instruction brings, instructions a wave
     static constexpr int TILEB = UK * ROWB, BUFB = 2 * TILEB;               // K, then V
+    static constexpr int VOTES = 2 * BUFB / 4;                              // a word of each wave's, behind the buffers
     static constexpr int QS = HALF ? HD / 16 : HD / 8;
     static constexpr float SHIFT = HALF ? 13.f : 0.f;      // probabilities times 2^SHIFT,
     static constexpr float LAZY = HALF ? 2.f : 8.f;        // and up to 2^LAZY more: the maximum is only moved where it grows by more
@@ -958,19 +947,15 @@ struct WideTile {
         }
         return out;
     }
-    __device__ __forceinline__ bool values_finite(unsigned V) const {
-        bool odd = false;
-#pragma unroll 2
-        for (int i = lane; i < UK * PR; i += 64) {       // (unrolled whole it would take q's registers)
-            const uint4_t x = lds16(V + (unsigned)i * 16);
+    // A unit's values in LDS to what stands for them in a pass (elements side by side: their order does not matter)
+    __device__ __forceinline__ void replace(unsigned V, int pass) const {
+#pragma unroll 1
+        for (int i = thread_anew(); i < TILEB / 16; i += WG) {
+            uint4_t x = lds16(V + (unsigned)i * 16);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const unsigned w = x[j];
-                if (HALF) odd |= ((w & 0x7fffu) >= 0x7c00u) | ((w & 0x7fff0000u) >= 0x7c000000u);
-                else odd |= (w & 0x7fffffffu) >= 0x7f800000u;
-            }
+            for (int j = 0; j < 4; j++) x[j] = stand_in<HALF>(x[j], pass);
+            *reinterpret_cast<__attribute__((address_space(3))) uint4_t*>(V + (unsigned)i * 16) = x;
         }
-        return !__any(odd);
     }
     // Scores to probabilities (times 2^SHIFT, over the maximum mNew); returns the lane's sum of them
     __device__ __forceinline__ float weigh(float16_t (&S)[NB], int base, unsigned long long held, bool all, float& mNew) const {
@@ -1016,7 +1001,8 @@ struct WideTile {
         return ts;
     }
     // Unit u, of page numbers `here`, in buffer `buf`; asks for the one behind it on the way
-    __device__ __forceinline__ void compute(int u, bool more, unsigned buf) {
+    template <bool AGAIN>
+    __device__ __forceinline__ void compute(int u, bool more, unsigned buf, int pass) {
         const int base = base_of(u), mine = here;
         if (!active || base >= end || base + UK <= begin) {
             if (more) issue(u + 1, next, buf ^ 1);
@@ -1044,6 +1030,13 @@ struct WideTile {
             m = mNew;
         }
         l += ts;
+        if (!inner && !__any(ts != 0.f)) return;          // (no row has anything here)
+        if (AGAIN && pass != FINITE) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) S[b][i] = S[b][i] > 0.f ? 1.f : 0.f;
+        }
         Weights w;
         if constexpr (HALF) {
 #pragma unroll
@@ -1055,15 +1048,6 @@ struct WideTile {
                     w.lo[kk][i] = (_Float16)(x - (float)w.hi[kk][i]);
                 }
         }
-        if (!inner) {
-            if (!__any(ts != 0.f)) return;                // (no row has anything here: a value that is no number must not get to any)
-            if (!values_finite(V)) {          // (one token or more: the tile holds what its other tokens see)
-                lateHi = lateHi << 20 | lateLo >> 40;
-                lateLo = (lateLo << 20 | (unsigned)u) & ((1ull << 60) - 1);
-                lates++;
-                return;
-            }
-        }
         const unsigned Vl = v_base(V);
 #pragma unroll
         for (int d = 0; d < DB; d++) {
@@ -1071,73 +1055,64 @@ struct WideTile {
             o[d] = product(Vl, d, S, w, o[d]);
         }
     }
-    // A unit with values that are no numbers at positions that not every token sees -- zero times them is no zero -- is left out of
-    // the product (its scores are in the sums).  At the end its positions are gone through row by row, each with those it sees,
-    // by way of the worker's place for a share.  There are at most five: the tokens of 32 rows end in two units, their windows begin
-    // in two, a prefix ends in one; unit numbers take 20 bits (2^24 positions, 32 a unit).
-    static constexpr int E = HD / 64;
-    unsigned long long lateLo = 0, lateHi = 0;
-    int lates = 0;
-    __device__ __forceinline__ void add_late(int kvh, int w) {
-        float* mine = part_of(p, t, kvh, w) + wave * 32 * HD;
-        const int x = anew(lane);
-#pragma unroll 1
-        for (int r = 0; r < 32; r++) {
-            const PagedRow at = paged_row(t, p.g.group, kvh, 32 * wave + r);
-            const float* q = p.q + (size_t)(t.row0 + at.token) * p.ldq + (size_t)at.head * HD + x * E;
-            const float mr = lane_value(m, r), sl = MOD && p.slopes ? p.slopes[at.head] : 0.f;
-            float acc[E];
-#pragma unroll
-            for (int e = 0; e < E; e++) acc[e] = 0.f;
-#pragma unroll 1
-            for (int n = 0; n < lates; n++) {
-                const int u = (int)((n < 3 ? lateLo >> 20 * n : lateHi >> 20 * (n - 3)) & 0xfffff);
-#pragma unroll 1
-                for (int j = base_of(u); j < base_of(u) + UK; j++) {
-                    if (!paged_sees(at.pos, j, t.len, p.window, t.prefix)) continue;
-                    const int page = pages[j >> p.g.pageShift];
-                    if (page < 0 || page >= p.g.nPages) continue;
-                    const KVT* k = reinterpret_cast<const KVT*>(kv_row(Kp, zeros, rowBytes, j, page, span.begin, span.end, p.g.pageShift)) + x * E;
-                    const KVT* v = reinterpret_cast<const KVT*>(kv_row(Vp, zeros, rowBytes, j, page, span.begin, span.end, p.g.pageShift)) + x * E;
-                    float y = 0.f;
-#pragma unroll
-                    for (int e = 0; e < E; e++) y = fmaf(q[e], (float)k[e], y);
-                    y = wave_sum(y) * p.scale;
-                    if (MOD) y = (cap > 0.f ? capped(y, cap, invCap) : y) - sl * (float)abs(at.pos - j);
-                    y = __builtin_amdgcn_exp2f(fmaf(y, 1.4426950408889634f, SHIFT - (mr == -INFINITY ? 0.f : mr)));
-#pragma unroll
-                    for (int e = 0; e < E; e++) acc[e] = fmaf(y, (float)v[e], acc[e]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < E; e++) mine[r * HD + x * E + e] = acc[e];
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup");         // (read back by other lanes of the wave)
-        const float* from = mine + n32 * HD + 4 * hf;
-#pragma unroll
-        for (int b = 0; b < DB; b++)
-#pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4_t v = *reinterpret_cast<const float4_t*>(from + 32 * b + 8 * i);
-#pragma unroll
-                for (int j = 0; j < 4; j++) o[b][4 * i + j] += v[j];
-            }
-    }
-    __device__ __forceinline__ void run(int u0, int u1, int kvh, int w, float*) {
+    template <bool AGAIN>
+    __device__ __forceinline__ void units(int u0, int u1, int pass) {
         unsigned buf = 0;
         for (int u = u0; u < u1; u++) {
             // this unit's rows have landed; nobody reads the other buffer any more
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             const int behind = page_of(min(u + 2, u1 - 1));
-            compute(u, u + 1 < u1, buf);
+            if constexpr (AGAIN) {
+                replace(ldsBase + buf * BUFB + TILEB, pass);
+                __syncthreads();
+            }
+            compute<AGAIN>(u, u + 1 < u1, buf, pass);
             here = next;
             next = behind;
             buf ^= 1;
         }
+    }
+    __device__ __forceinline__ void run(int u0, int u1, int, int, float* lds) {
+        units<false>(u0, u1, 0);
+        float odd = 0.f;
+#pragma unroll
+        for (int b = 0; b < DB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) odd = fmaf(o[b][i], 0.f, odd);
+        const bool any = __any(odd != odd);
+        unsigned* votes = reinterpret_cast<unsigned*>(lds) + VOTES;
+        if (lane == 0) votes[wave] = any;
+        __syncthreads();
+        if (__builtin_amdgcn_readfirstlane(votes[0] | votes[1] | votes[2] | votes[3])) {         // all four waves, or none
+            unsigned long long plus = 0, minus = 0;       // a bit an element
+#pragma unroll 1
+            for (int pass = PLUS_INFINITE; pass <= FINITE; pass++) {
+                here = page_of(u0);
+                next = page_of(min(u0 + 1, u1 - 1));
+                issue(u0, here, 0);
+                l = 0.f;
+#pragma unroll
+                for (int b = 0; b < DB; b++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) o[b][i] = 0.f;
+                units<true>(u0, u1, pass);
+                unsigned long long counts = 0;
+#pragma unroll
+                for (int b = 0; b < DB; b++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) counts |= (o[b][i] > 0.f ? 1ull : 0ull) << (16 * b + i);
+                if (pass == PLUS_INFINITE) plus = counts;
+                if (pass == MINUS_INFINITE) minus = counts;
+                __syncthreads();                          // (the last unit's buffer may be the first one's)
+            }
+#pragma unroll
+            for (int b = 0; b < DB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[b][i] = with_infinities(o[b][i], plus >> (16 * b + i) & 1, minus >> (16 * b + i) & 1);
+        }
         float other = l;
         row_swap32(l, other);
         l += other;
-        if (lates) add_late(kvh, w);
     }
     // A share lies as its registers do -- a wave's block b, rows of four i / 4, then its 64 lanes -- so that stores and loads are whole lines
     __device__ __forceinline__ void write(int kvh, int w, float* lds) {
@@ -1230,7 +1205,7 @@ __global__ __launch_bounds__(WG, 2) void paged_wide_kernel(PagedAttention p) {
 }
 
 static size_t attn_lds(int headDim, bool wide) {
-    const size_t tile = wide ? (size_t)2 * 2 * 64 * headDim * 2 : (size_t)(4 * NARROW * (headDim + 4) + 8 * NARROW) * 4;
+    const size_t tile = wide ? (size_t)2 * 2 * 64 * headDim * 2 + 16 : (size_t)(4 * NARROW * (headDim + 4) + 8 * NARROW) * 4;
     const size_t merge = (size_t)(2 * (wide ? WIDE : NARROW) + MERGE_LDS) * 4;
     return tile > merge ? tile : merge;
 }

@@ -1,5 +1,5 @@
 """Attention over a paged KV cache at the edges of its arguments: values that are no numbers at positions that a row does not
-see.  Against 64 bits, as test_gpu_paged."""
+see, infinities where it does.  Against 64 bits, as test_gpu_paged."""
 import numpy as np
 import pytest
 
@@ -24,6 +24,10 @@ def _check(c, **what):
     _, bound = c.want(**what)
     c.V = V
     got = c.result()
+    odd = ~np.isfinite(want)
+    g = got[:c.rows, :c.heads * c.hd][odd]
+    same = (g == want[odd]) | (np.isnan(g) & np.isnan(want[odd]))
+    assert same.all(), (np.argwhere(odd)[~same][:5].tolist(), g[~same][:5], want[odd][~same][:5])
     c.compare(got, want, bound)
     c.h.Close()
 
@@ -57,3 +61,41 @@ def test_hidden_values_between_a_single_tokens_prefix_and_its_window(hip, bufs, 
         for j in bad:
             c.V[c.where(0, j), j % 5::7] = value
         _check(c, window=64, prefix=[10] * n)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# infinite values at positions that are seen
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("heads,kv,hd,new,lens,window,prefix", [
+    (4, 4, 64, [1, 1], [200, 33], 0, None), (8, 2, 128, [1, 3], [900, 64], 0, None), (8, 2, 64, [70, 200], [70, 450], 0, None), (8, 2, 128, [130, 1, 40], [300, 129, 333], 0, None),
+    (32, 1, 64, [70, 1], [300, 90], 50, None), (8, 2, 128, [3, 100], [300, 400], 90, [20, 310]), (3, 3, 128, [1], [9001], 0, None), (8, 1, 64, [60], [12000], 0, None)])
+def test_infinite_values_that_are_seen_keep_their_sign(hip, bufs, heads, kv, hd, new, lens, window, prefix, half):
+    """Either infinity, both in one column (no number), and NaN, at first, middle and last positions."""
+    print(f"signs {heads}/{kv}/{hd} half={half} {new} of {lens}", flush=True)
+    c = Case(hip, bufs, heads, kv, hd, half, 8, new, lens, seed=lens[0])
+    for r, n in enumerate(lens):
+        for j, first, value in ((n - 1, 0, np.inf), (n // 2, 1, -np.inf), (n // 2 + 1, 2, np.inf), (n - new[r], 2, -np.inf), (0, 3, np.inf), (n - 1, 4, np.nan), (n - 1, 5, -np.inf)):
+            c.V[c.where(r, j), first::11] = value
+    _check(c, window=window, prefix=prefix)
+
+
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("heads,kv,new,lens", [(4, 4, [1, 2], [300, 80]), (8, 2, [100], [300])])
+def test_infinite_values_of_small_weight(hip, bufs, heads, kv, new, lens, half):
+    """Weights below what two fp16 terms hold, above the least fp32 number: the infinity counts all the same."""
+    c = Case(hip, bufs, heads, kv, 64, half, 8, new, lens, seed=2, peak=9.0)
+    small = 0
+    for r, n in enumerate(lens):
+        first = n - new[r]
+        c.V[c.where(r, 5), ::9] = -np.inf
+        c.V[c.where(r, first // 2), 4::9] = np.inf
+        at = [c.where(r, j) for j in range(n)]
+        for h in range(heads):
+            col = slice(h // c.group * 64, h // c.group * 64 + 64)
+            s = c.q[c.rowStart[r]:c.rowStart[r + 1], h * 64:h * 64 + 64] @ c.K[at][:first, col].astype(np.float32).T / 8
+            rel = (s[:, [5, first // 2]] - s.max(1, keepdims=True)) * 1.4426950408889634
+            assert rel.min() > -120
+            small += int((rel < -42).sum())
+    assert small > 0
+    _check(c)
