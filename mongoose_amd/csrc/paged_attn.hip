@@ -10,6 +10,8 @@
 // row is read once for all of them.  Scores are computed transposed, S^T = K Q^T, and the output O^T = V^T P^T: the MFMA result of the
 // first (a lane: one query row, several positions) is the operand of the second as it stands, and a row's maximum and sum are
 // a lane's own but for two exchanges.
+#include <float.h>
+
 #include "device_util.h"
 #include "paged.h"
 
@@ -354,6 +356,12 @@ __device__ __forceinline__ unsigned stand_in(unsigned v, int pass) {
 }
 __device__ __forceinline__ float with_infinities(float o, bool plus, bool minus) { return (plus ? o + INFINITY : o) + (minus ? -INFINITY : 0.f); }
 
+// The power of two that a row of q, |q| up to `top`, is scaled by: to 2^14 .. 2^15, or to less where the factor left for its scores would
+// fall below 2^-119 and no longer be a normal number (such scores are below 2^-80).
+__device__ __forceinline__ int power_up(float top, float scale) {
+    return top > 0.f && top < INFINITY ? min(15 - __builtin_amdgcn_frexp_expf(top), 118 + __builtin_amdgcn_frexp_expf(scale)) : 0;
+}
+
 // A tile of 16 rows: four waves take a step of KB positions each of every unit, each with its own running maximum, sum and output.
 // Bound by HBM: a lane loads its K and V operands from the pages straight into registers, each where the last step's have gone into
 // their products, the page numbers two steps ahead; nothing is shared between the waves before the end.  8B shape, fp16, 48 requests
@@ -421,7 +429,7 @@ struct NarrowTile {
 #pragma unroll
                 for (int j = 0; j < 4; j++) top = fmaxf(top, fabsf(x[i][j]));
             top = rows_max(top);
-            const int up = top > 0.f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+            const int up = power_up(top, c);
 #pragma unroll
             for (int s = 0; s < HD / 32; s++)
 #pragma unroll
@@ -436,6 +444,7 @@ struct NarrowTile {
             for (int s = 0; s < HD / 16; s++) qf[s] = x[s];
         }
         if (!MOD) c *= 1.4426950408889634f;
+        c = fminf(c, FLT_MAX);                    // (0 times it is 0)
         m = -INFINITY;
         l = 0.f;
 #pragma unroll
@@ -825,7 +834,7 @@ struct WideTile {
             float other = top;
             row_swap32(top, other);
             top = fmaxf(top, other);
-            const int up = top > 0.f && top < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(top) : 0;
+            const int up = power_up(top, c);
 #pragma unroll
             for (int s = 0; s < QS; s++)
 #pragma unroll
@@ -840,6 +849,7 @@ struct WideTile {
             for (int s = 0; s < QS; s++) qf[s] = x[s];
         }
         if (!MOD) c *= 1.4426950408889634f;
+        c = fminf(c, FLT_MAX);                    // (0 times it is 0)
         m = -INFINITY;
         l = 0.f;
 #pragma unroll

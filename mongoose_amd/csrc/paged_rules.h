@@ -96,7 +96,8 @@ inline const char* paged_attention_refusal(const PagedGeo& g, const void* q, int
     if (!paged_aligned(table, 4) || (slopes && !paged_aligned(slopes, 4))) return "a pointer is NULL or not aligned to 4 bytes";
     if (ldq < g.nHeads * g.headDim || ldo < g.nHeads * g.headDim) return "a row stride is smaller than the row";
     if ((ldq | ldo) & 3) return "a row stride is not a multiple of 4";
-    // (beyond these the scale in powers of two, or the cap's reciprocal, is no fp32 number)
+    // (beyond these the scale in powers of two, or the cap's reciprocal, is no normal fp32 number; the power of two that an fp16 cache's
+    // rows of q take besides is kept from making it one: power_up)
     if (!(scale == 0.f || (scale >= 1e-30f && scale <= 1e30f))) return "scale must be between 1e-30 and 1e30, or 0 for 1 / sqrt(headDim)";
     if (!(softcap == 0.f || (softcap >= 1e-30f && softcap <= 1e30f))) return "softcap must be between 1e-30 and 1e30, or 0 for none";
     if (q == out) return "q and out are the same array";

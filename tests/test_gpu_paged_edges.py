@@ -1,5 +1,5 @@
 """Attention over a paged KV cache at the edges of its arguments: values that are no numbers at positions that a row does not
-see, infinities where it does.  Against 64 bits, as test_gpu_paged."""
+see, infinities where it does; rows of q from tiny to huge.  Against 64 bits, as test_gpu_paged."""
 import numpy as np
 import pytest
 
@@ -99,3 +99,17 @@ def test_infinite_values_of_small_weight(hip, bufs, heads, kv, new, lens, half):
             small += int((rel < -42).sum())
     assert small > 0
     _check(c)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# scales and rows of q whose factor in powers of two is no fp32 number
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("scale,size,keys", [(1e-30, 1e-12, 1.0), (1e-30, 1e-36, 1.0), (0.0, 1e-38, 1.0), (1e30, 1e30, 0.0), (1e-30, 1e30, 1.0)])
+def test_scales_far_from_the_rows_of_q(hip, bufs, scale, size, keys, half):
+    """Scores next to nothing, ordinary ones of a small scale and a huge q, zero keys under a scale times q that is no fp32 number."""
+    for cap in (0.0, 20.0):
+        c = Case(hip, bufs, 8, 2, 64, half, 16, [1, 90, 3], [300, 300, 40], seed=5)
+        c.q = (c.q * size).astype(np.float32)
+        c.K = (c.K * keys).astype(c.kind)
+        c.check(scale=scale, cap=cap)
