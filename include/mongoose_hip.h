@@ -518,7 +518,9 @@ int mg_paged_tables(mg_paged* h, const int* newLens, int nReqs, const int* lens,
 
 /* mongoose_rope on the rows of q and k at positions[t] (pairs (j, j + headDim/2), table row = position, [tableRows, headDim/2])
  * and mongoose_kv_cache_write of the turned k rows and the v rows at slots[t].  ldq, ldk, ldv, ldqOut: floats from one row to the
- * next (multiples of 4, pointers 16-byte aligned: q, k and v may be columns of one projection); qOut may be q.  A row whose
+ * next (multiples of 4, pointers 16-byte aligned: q, k and v may be columns of one projection).  qOut may be q with
+ * ldqOut = ldq, or columns beside those that are read; otherwise what is written (qOut, K, V) overlaps neither what is read nor each
+ * other.  A row whose
  * position is negative or past the tables is passed over, one whose slot is no slot of the pools is turned but not stored.
  * The slots of a call differ from one another. */
 int mg_paged_store(mg_paged* h, const float* q, const float* k, const float* v, int ldq, int ldk, int ldv, float* qOut, int ldqOut,

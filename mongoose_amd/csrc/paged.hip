@@ -309,6 +309,7 @@ int mg_paged_store(mg_paged* h, const float* q, const float* k, const float* v, 
     PAGED(h, "mg_paged_store");
     if (const char* why = mg::paged_store_refusal(h->g, q, k, v, ldq, ldk, ldv, qOut, ldqOut, K, V, slots, positions, rows, cosTab, sinTab, tableRows))
         return refuse("mg_paged_store", why);
+    if (const char* why = mg::paged_store_overlap(h->g, q, k, v, ldq, ldk, ldv, qOut, ldqOut, K, V, rows)) return refuse("mg_paged_store", why);
     mg::PagedStore p{q, k, v, cosTab, sinTab, qOut, K, V, slots, positions, ldq, ldk, ldv, ldqOut, rows, tableRows,
                      h->g.nHeads, h->g.nKVHeads, h->g.headDim, h->g.kvHalf, h->g.nPages * h->g.pageSize};
     return launched("mg_paged_store", mg::launch_paged_store(p, static_cast<hipStream_t>(stream)));

@@ -80,6 +80,43 @@ inline const char* paged_store_refusal(const PagedGeo& g, const void* q, const v
     if (K == V) return "K and V are the same array";
     return nullptr;
 }
+// Arrays of `rows` rows of `width` floats, `ld` floats apart (a row no longer than that): whether they have a float in common.  Rows of
+// one stride may lie between each other (columns of one projection); of two strides, anything between the first and last float counts.
+inline bool paged_rows_meet(const void* a, int lda, int wa, const void* b, int ldb, int wb, int rows) {
+    const long long d = ((long long)(intptr_t)b - (long long)(intptr_t)a) / 4;        // (both are aligned to 16 bytes)
+    if (rows <= 0) return false;
+    if (lda != ldb) return d < (long long)(rows - 1) * lda + wa && -d < (long long)(rows - 1) * ldb + wb;
+    // rows k apart meet where -wb < d + k ld < wa, -rows < k < rows; of the numbers d + k ld only those within ld of 0 can
+    long long r = d % lda;                       // (as d / lda, towards 0)
+    const long long k = -(d / lda);
+    for (int i = -1; i <= 1; i++) {
+        const long long at = r + (long long)i * lda;
+        if (at < wa && -at < wb && k + i > -rows && k + i < rows) return true;
+    }
+    return false;
+}
+// Whether `bytes` at p and the floats of such rows have memory in common
+inline bool paged_pool_meets(const void* p, size_t bytes, const void* a, int ld, int width, int rows) {
+    const uintptr_t x = (uintptr_t)p, y = (uintptr_t)a;
+    return rows > 0 && x < y + ((size_t)(rows - 1) * ld + width) * 4 && y < x + bytes;
+}
+inline size_t paged_pool_bytes(const PagedGeo& g) { return (size_t)g.nPages * g.pageSize * g.kvDim * (g.kvHalf ? 2 : 4); }
+// What a call writes while others of its workgroups still read it: nullptr, or which of its arguments overlap (those that
+// paged_store_refusal has passed).
+inline const char* paged_store_overlap(const PagedGeo& g, const void* q, const void* k, const void* v, int ldq, int ldk, int ldv,
+                                       const void* qOut, int ldqOut, const void* K, const void* V, int rows) {
+    if (rows == 0) return nullptr;
+    const int qw = g.nHeads * g.headDim;
+    if (!(q == qOut && (ldq == ldqOut || rows == 1)) && paged_rows_meet(q, ldq, qw, qOut, ldqOut, qw, rows)) return "qOut overlaps q, and is not q with the same stride";
+    if (paged_rows_meet(k, ldk, g.kvDim, qOut, ldqOut, qw, rows) || paged_rows_meet(v, ldv, g.kvDim, qOut, ldqOut, qw, rows)) return "qOut overlaps k or v";
+    const size_t bytes = paged_pool_bytes(g);
+    if ((uintptr_t)K < (uintptr_t)V + bytes && (uintptr_t)V < (uintptr_t)K + bytes) return "K and V overlap";
+    const void* pools[] = {K, V};
+    for (const void* p : pools)
+        if (paged_pool_meets(p, bytes, q, ldq, qw, rows) || paged_pool_meets(p, bytes, k, ldk, g.kvDim, rows) ||
+            paged_pool_meets(p, bytes, v, ldv, g.kvDim, rows) || paged_pool_meets(p, bytes, qOut, ldqOut, qw, rows)) return "K or V overlaps the rows";
+    return nullptr;
+}
 inline const char* paged_plan_refusal(const PagedGeo& g, const void* rowStart, const void* lens, int nReqs, int rows, int window,
                                       const void* prefixLens) {
     if (nReqs < 0 || nReqs > g.maxReqs) return "nReqs is negative or above the handle's maxReqs";

@@ -113,3 +113,27 @@ def test_scales_far_from_the_rows_of_q(hip, bufs, scale, size, keys, half):
         c.q = (c.q * size).astype(np.float32)
         c.K = (c.K * keys).astype(c.kind)
         c.check(scale=scale, cap=cap)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# calls whose arguments overlap
+# ---------------------------------------------------------------------------------------------------------------------
+def test_overlapping_arguments_are_refused(hip, bufs):
+    x = np.ones((4, 24 * 64), np.float32)
+    d = bufs.up(x)
+    p = d.DevicePtr()
+    h = E.NewHIPPaged(hip, 8, 2, 64, 8, 4, 0, 2, 4, 32)
+    K, V, z = bufs.up(np.zeros((32, 128), np.float32)), bufs.up(np.zeros((32, 128), np.float32)), bufs.up(np.zeros(64, np.int32))
+    slots = bufs.up(np.arange(4, dtype=np.int32))
+    c, s = bufs.up(np.ones(32, np.float32)), bufs.up(np.zeros(32, np.float32))
+
+    def store(o, ldo):
+        return h.Store(p, p + 2048, p + 2560, 768, 768, 768, o, ldo, K, V, slots, z, 4, c, s, 1)
+
+    assert store(p, 512) == -2 and "qOut overlaps q" in E.last_error()
+    assert store(p + 1024, 768) == -2 and "qOut overlaps" in E.last_error()
+    E.KSync()
+    assert np.array_equal(bufs.down(d, x), x)
+    assert store(p, 768) == 0
+    E.KSync()
+    h.Close()

@@ -205,3 +205,44 @@ int main() {
 }
 """)
     assert out == "00 00 11 11 11 "
+
+
+def test_what_store_writes_overlaps_nothing_that_it_reads(tmp_path):
+    out = _run(tmp_path, r"""
+static float mem[400000] __attribute__((aligned(16)));
+int main() {
+    // strided rows against every float of them
+    for (int it = 0; it < 60000; it++) {
+        unsigned x = it * 2654435761u;
+        auto rnd = [&](int n) { x = x * 1664525u + 1013904223u; return (int)((x >> 8) % (unsigned)n); };
+        const int wa = 1 + rnd(5), wb = 1 + rnd(5), lda = wa + rnd(7), ldb = rnd(2) && lda >= wb ? lda : wb + rnd(7), rows = rnd(5), at = rnd(80);
+        bool meet = false, extent = false;
+        for (int i = 0; i < rows; i++) for (int j = 0; j < rows; j++) for (int s = 0; s < wa; s++) for (int t = 0; t < wb; t++) meet |= 40 + i * lda + s == at + j * ldb + t;
+        extent = rows > 0 && 40 < at + (rows - 1) * ldb + wb && at < 40 + (rows - 1) * lda + wa;
+        if (paged_rows_meet(mem + 40, lda, wa, mem + at, ldb, wb, rows) != (lda == ldb ? meet : extent)) { std::printf("%d %d %d %d rows %d at %d\n", lda, wa, ldb, wb, rows, at); return 0; }
+    }
+    PagedGeo g{};
+    if (paged_geo(g, 14, 2, 64, 16, 10, 1, 4, 64, 100)) return 1;       // rows of 896, 128 and 128; pools of 10,240 floats' bytes
+    auto S = [&](int q, int k, int v, int ld, int o, int ldo, int K, int V, int rows) { return paged_store_overlap(g, mem + q, mem + k, mem + v, ld, ld, ld, mem + o, ldo, mem + K, mem + V, rows); };
+    auto is = [](const char* want, const char* got) { std::printf("%s|%s\n", want, got ? got : "-"); };
+    const int K = 200000, V = K + 10240;
+    is("-", S(0, 896, 1024, 1152, 0, 1152, K, V, 8));              // in place
+    is("-", S(0, 896, 1024, 1152, 100000, 896, K, V, 8));
+    is("-", S(0, 896, 1024, 2048, 1152, 2048, K, V, 8));           // columns behind
+    is("-", S(0, 896, 1024, 1152, 0, 896, K, V, 1));               // one row has no stride
+    is("-", S(0, 896, 1024, 1152, 0, 896, K, K, 0));
+    is("same stride", S(0, 896, 1024, 1152, 0, 896, K, V, 8));
+    is("same stride", S(0, 896, 1024, 1152, 4, 1152, K, V, 8));
+    is("same stride", S(0, 896, 1024, 1152, 1152, 1152, K, V, 8));       // the next row
+    is("-", S(0, 896, 1024, 1152, 1152 * 8, 1152, K, V, 8));
+    is("k or v", S(0, 896, 1024, 2048, 1148, 2048, K, V, 8));
+    is("k or v", S(100000, 100896, 1024, 1152, 512, 1152, K, V, 1));
+    is("K and V", S(0, 896, 1024, 1152, 0, 1152, K, K + 10236, 8));
+    is("the rows", S(0, 896, 1024, 1152, 0, 1152, 1152 * 7 + 1148, V, 8));
+    is("the rows", S(0, 896, 1024, 1152, 100000, 896, K, 100000 + 7 * 896, 8));
+}
+""").splitlines()
+    assert len(out) == 14, out
+    for line in out:
+        want, got = line.split("|")
+        assert (want in got) if want != "-" else got == "-", line
