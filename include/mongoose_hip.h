@@ -537,7 +537,7 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
  * s_j = scale * q.k_j (scale 0: 1 / sqrt(headDim)); with softcap > 0 then softcap * tanh(s_j / softcap); with slopes [nHeads]
  * then minus slopes[head] * |i - j|.  Scores, their maxima and sums are fp32; products of an fp32 cache too, those of an fp16 cache
  * are of q and the probabilities to 22 bits.  ldq, ldo: floats from one row to the next (multiples of 4, 16-byte aligned
- * pointers).  A table entry that is no page hides its positions; a row that sees nothing is zeros; what the cache holds
+ * pointers); both have the plan's `rows` rows, and out overlaps neither q (other columns of one buffer are fine) nor K and V.  A table entry that is no page hides its positions; a row that sees nothing is zeros; what the cache holds
  * behind a request's length is not read into any result.  A value that is no number reaches the rows that see its position and no
  * others; an infinite one is an infinity of its sign in a row's result where its weight is 2^-126 of the row's greatest or more (with one
  * of the other sign, or a NaN, a NaN).  scale and softcap are 0 or between 1e-30 and 1e30.  MG_E_STATE without

@@ -333,6 +333,7 @@ int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, cons
     if (h->planReqs < 0) { mg::set_error("mg_paged_attention: no plan yet (mg_paged_plan)"); return MG_E_STATE; }
     if (h->planReqs == 0 || h->planRows == 0) return MG_OK;
     if (const char* why = mg::paged_attention_refusal(h->g, q, ldq, K, V, table, out, ldo, scale, softcap, slopes)) return refuse("mg_paged_attention", why);
+    if (const char* why = mg::paged_attention_overlap(h->g, q, ldq, K, V, out, ldo, h->planRows)) return refuse("mg_paged_attention", why);
     const mg::PagedGeo& g = h->g;
     mg::PagedAttention p{q, slopes, K, V, table, out, h->tiles, h->workers, h->parts, h->arrived, h->zeros, mg::paged_part_floats(g),
                          scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, ldq, ldo, h->planWindow, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};

@@ -141,6 +141,14 @@ inline const char* paged_attention_refusal(const PagedGeo& g, const void* q, int
     return nullptr;
 }
 
+inline const char* paged_attention_overlap(const PagedGeo& g, const void* q, int ldq, const void* K, const void* V, const void* out, int ldo, int rows) {
+    const int w = g.nHeads * g.headDim;
+    if (paged_rows_meet(q, ldq, w, out, ldo, w, rows)) return "out overlaps q";
+    const size_t bytes = paged_pool_bytes(g);
+    if (paged_pool_meets(K, bytes, out, ldo, w, rows) || paged_pool_meets(V, bytes, out, ldo, w, rows)) return "out overlaps K or V";
+    return nullptr;
+}
+
 // Sums that stop at 2^31 - 1 instead of wrapping (still associative): an overflowing total is only ever compared with a limit.
 MG_HD unsigned sat_add(unsigned a, unsigned b) {
     const unsigned s = a + b;            // both below 2^31

@@ -136,4 +136,8 @@ def test_overlapping_arguments_are_refused(hip, bufs):
     assert np.array_equal(bufs.down(d, x), x)
     assert store(p, 768) == 0
     E.KSync()
+    one = bufs.up(np.array([0, 1, 4], np.int32))
+    assert h.Plan(one, one, 2, 4) == 0
+    for out in (p, p + 256, p + 1536 * 2, K, V):
+        assert h.Attention(p, 768, K, V, z, out, 768) == -2 and "out" in E.last_error(), out
     h.Close()

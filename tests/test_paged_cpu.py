@@ -246,3 +246,29 @@ int main() {
     for line in out:
         want, got = line.split("|")
         assert (want in got) if want != "-" else got == "-", line
+
+
+def test_what_attention_writes_overlaps_nothing_that_it_reads(tmp_path):
+    out = _run(tmp_path, r"""
+static float mem[400000] __attribute__((aligned(16)));
+int main() {
+    PagedGeo g{};
+    if (paged_geo(g, 14, 2, 64, 16, 10, 0, 4, 64, 100)) return 1;       // rows of 896; pools of 20,480 floats
+    auto A = [&](int q, int ldq, int K, int V, int o, int ldo, int rows) { return paged_attention_overlap(g, mem + q, ldq, mem + K, mem + V, mem + o, ldo, rows); };
+    auto is = [](const char* want, const char* got) { std::printf("%s|%s\n", want, got ? got : "-"); };
+    is("-", A(0, 1792, 200000, 220480, 896, 1792, 64));        // other columns
+    is("-", A(0, 896, 200000, 200000, 57344, 896, 64));        // one behind the other; K may be V
+    is("overlaps q", A(0, 896, 200000, 220480, 57340, 896, 64));
+    is("overlaps q", A(0, 1792, 200000, 220480, 892, 1792, 64));
+    is("overlaps q", A(0, 1152, 200000, 220480, 1152, 1152, 2));
+    is("overlaps q", A(4, 1152, 200000, 220480, 0, 1152, 1));
+    is("-", A(0, 1152, 200000, 220480, 1152, 1152, 1));
+    is("K or V", A(0, 896, 200000, 220480, 240956, 896, 3));
+    is("K or V", A(0, 896, 200000, 220480, 199108, 896, 2));
+    is("-", A(0, 896, 200000, 220480, 240960, 896, 3));
+}
+""").splitlines()
+    assert len(out) == 10, out
+    for line in out:
+        want, got = line.split("|")
+        assert (want in got) if want != "-" else got == "-", line
