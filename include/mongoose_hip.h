@@ -506,7 +506,7 @@ int mg_paged_table_width(const mg_paged* h);      /* ceil(maxLen / pageSize): en
  * Pages are taken from the ring's front in the order of the requests and, within one, of its positions, and written into its
  * row of the table; the pages of ended requests go behind the ring's last in the same order (and are free from the next call
  * on; their table rows stay as they are).  Written besides: lensOut[r] = lens[r] + newLens[r] (0 for an ended one), ringStateOut
- * (these two may be lens and ringState themselves, or else do not overlap them), rowStart[nReqs + 1] = the first row of every
+ * (these two may be lens and ringState themselves; otherwise no array overlaps another), rowStart[nReqs + 1] = the first row of every
  * request, slots[rows] = page * pageSize + place of each row and positions[rows] (both -1 behind the last row; a slot is -1 too
  * where the table or the ring hold an entry that is no page), counts[4] = {rows, pages taken, pages given back, 0}.
  * A step that does not fit changes no length, no table and no ring: rowStart is 0 throughout, slots and positions -1, counts =

@@ -300,6 +300,8 @@ int mg_paged_tables(mg_paged* h, const int* newLens, int nReqs, const int* lens,
     PAGED(h, "mg_paged_tables");
     if (const char* why = mg::paged_tables_refusal(h->g, newLens, nReqs, lens, lensOut, table, ring, ringState, ringStateOut, rows, rowStart, slots, positions, counts))
         return refuse("mg_paged_tables", why);
+    if (const char* why = mg::paged_tables_overlap(h->g, newLens, nReqs, lens, lensOut, table, ring, ringState, ringStateOut, rows, rowStart, slots, positions, counts))
+        return refuse("mg_paged_tables", why);
     mg::PagedTables p{newLens, lens, ringState, lensOut, table, ring, ringStateOut, rowStart, slots, positions, counts,
                       nReqs, rows, h->g.nPages, h->g.pageShift, h->g.width, h->g.maxLen};
     return launched("mg_paged_tables", mg::launch_paged_tables(p, static_cast<hipStream_t>(stream)));

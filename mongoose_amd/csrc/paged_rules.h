@@ -80,6 +80,22 @@ inline const char* paged_store_refusal(const PagedGeo& g, const void* q, const v
     if (K == V) return "K and V are the same array";
     return nullptr;
 }
+// What the block-table kernel writes while others of its workgroups still read: nullptr, or that two of its arrays overlap.  The lengths
+// and the ring's state may be updated in place.
+inline const char* paged_tables_overlap(const PagedGeo& g, const int* newLens, int nReqs, const int* lens, const int* lensOut, const int* table,
+                                        const int* ring, const int* ringState, const int* ringStateOut, int rows, const int* rowStart,
+                                        const int* slots, const int* positions, const int* counts) {
+    const struct { const int* p; long long n; } a[] = {
+        {lensOut, nReqs}, {ringStateOut, 2}, {table, (long long)nReqs * g.width}, {ring, g.nPages}, {rowStart, nReqs + 1}, {slots, rows},
+        {positions, rows}, {counts, 4}, {newLens, nReqs}, {lens, nReqs}, {ringState, 2}};
+    for (int i = 0; i < 8; i++)             // (the first eight are written)
+        for (int j = i + 1; j < 11; j++) {
+            if (a[i].p == a[j].p && ((i == 0 && j == 9) || (i == 1 && j == 10))) continue;
+            if (a[i].n > 0 && a[j].n > 0 && (uintptr_t)a[i].p < (uintptr_t)(a[j].p + a[j].n) && (uintptr_t)a[j].p < (uintptr_t)(a[i].p + a[i].n))
+                return "arrays overlap (lensOut may be lens, ringStateOut ringState)";
+        }
+    return nullptr;
+}
 // Arrays of `rows` rows of `width` floats, `ld` floats apart (a row no longer than that): whether they have a float in common.  Rows of
 // one stride may lie between each other (columns of one projection); of two strides, anything between the first and last float counts.
 inline bool paged_rows_meet(const void* a, int lda, int wa, const void* b, int ldb, int wb, int rows) {

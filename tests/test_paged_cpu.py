@@ -272,3 +272,39 @@ int main() {
     for line in out:
         want, got = line.split("|")
         assert (want in got) if want != "-" else got == "-", line
+
+
+def test_arrays_of_the_tables_that_overlap(tmp_path):
+    """Eleven arrays one behind the other; each in turn moved onto the last entry of each other one."""
+    out = _run(tmp_path, r"""
+static int mem[4000];
+int main() {
+    PagedGeo g{};
+    if (paged_geo(g, 14, 2, 64, 16, 100, 0, 4, 64, 1000)) return 1;
+    const int n = 3, rows = 7, size[11] = {n, n, n, n * 63, 100, 2, 2, n + 1, rows, rows, 4};      // in the order of the arguments
+    auto call = [&](const int* at, int n, int rows) {
+        const int* p[11];
+        for (int i = 0; i < 11; i++) p[i] = mem + at[i];
+        return paged_tables_overlap(g, p[0], n, p[1], p[2], p[3], p[4], p[5], p[6], rows, p[7], p[8], p[9], p[10]) != nullptr;
+    };
+    int at[11], end = 0;
+    for (int i = 0; i < 11; i++) { at[i] = end; end += size[i]; }
+    std::printf("%d", call(at, n, rows));
+    for (int i = 0; i < 11; i++) for (int j = 0; j < 11; j++) if (i != j) {
+        int moved[11];
+        std::copy(at, at + 11, moved);
+        moved[i] = at[j] + size[j] - 1;
+        moved[i] = std::max(moved[i], 0);
+        int other = 1000;                               // (nothing else is in the way)
+        for (int k = 0; k < 11; k++) if (k != i && k != j) { moved[k] = other; other += size[k]; }
+        const bool reads = (i == 0 || i == 1 || i == 5) && (j == 0 || j == 1 || j == 5);        // newLens, lens, ringState are only read
+        if (call(moved, n, rows) == reads) { std::printf(" %d onto %d", i, j); return 0; }
+    }
+    at[2] = at[1]; at[6] = at[5];
+    std::printf("%d", call(at, n, rows));               // in place
+    int none[11] = {};
+    none[4] = 100; none[5] = none[6] = 300; none[7] = 310; none[10] = 320;
+    std::printf("%d\n", call(none, 0, 0));               // no requests, no rows: those arrays are nothing
+}
+""")
+    assert out == "000\n", out
