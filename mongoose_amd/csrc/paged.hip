@@ -320,6 +320,7 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
     PAGED(h, "mg_paged_plan");
     if (const char* why = mg::paged_plan_refusal(h->g, rowStart, lens, nReqs, rows, window, prefixLens)) return refuse("mg_paged_plan", why);
     const mg::PagedGeo& g = h->g;
+    window = mg::paged_window(window, g.maxLen);
     const int workers = mg::paged_workers(g, nReqs, rows, false), narrow = mg::paged_narrow_rows(g, rows);
     const int wide = (long long)rows * g.group > narrow ? mg::paged_workers(g, nReqs, rows, true) : 0;
     mg::PagedPlan p{rowStart, lens, prefixLens, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, h->maxTiles, h->maxWorkers, workers, wide, narrow};

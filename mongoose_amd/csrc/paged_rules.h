@@ -171,6 +171,9 @@ MG_HD unsigned sat_add(unsigned a, unsigned b) {
     return s > 0x7fffffffu ? 0x7fffffffu : s;
 }
 MG_HD int paged_pages(int len, int pageShift) { return (int)(((unsigned)len + (1u << pageShift) - 1) >> pageShift); }
+// A window as the calls below take it: none is wider than all positions (a difference from a row's position, which is negative where a
+// request has more rows than positions, stays a number).
+MG_HD int paged_window(int window, int maxLen) { return window < maxLen ? window : maxLen; }
 // Whether the token at position i of a request of `len` positions sees position j.
 MG_HD bool paged_sees(int i, int j, int len, int window, int prefix) {
     return (j < len) & (((j <= i) & ((window == 0) | (j > i - window))) | (j < prefix));

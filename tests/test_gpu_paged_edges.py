@@ -141,3 +141,22 @@ def test_overlapping_arguments_are_refused(hip, bufs):
     for out in (p, p + 256, p + 1536 * 2, K, V):
         assert h.Attention(p, 768, K, V, z, out, 768) == -2 and "out" in E.last_error(), out
     h.Close()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# windows wider than any request
+# ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("half", [0, 1])
+def test_the_largest_window_is_none(hip, bufs, half):
+    """Also for requests with more rows than positions, whose first rows see nothing."""
+    outs = []
+    for window in (0, (1 << 31) - 1):
+        c = Case(hip, bufs, 8, 2, 64, half, 8, [5, 1, 90], [60, 33, 120], seed=1)
+        c.lens[0], c.lens[2] = 3, 40
+        c.upload()
+        c.plan(window)
+        c.attend()
+        E.KSync()
+        outs.append(c.result())
+        c.h.Close()
+    assert np.array_equal(*outs) and (outs[0][:2] == 0).all() and (outs[0][2:6] != 0).any(1).all() and (outs[0][6:56] == 0).all() and (outs[0][56:] != 0).any(1).all()

@@ -308,3 +308,24 @@ int main() {
 }
 """)
     assert out == "000\n", out
+
+
+@pytest.mark.parametrize("window", [1, 3, 1 << 24, (1 << 31) - 2, (1 << 31) - 1])
+def test_windows_up_to_the_largest(tmp_path, window):
+    """Requests with more rows than positions among them: their first rows are at negative positions."""
+    out = _run(tmp_path, r"""
+int main() {
+    const int w = paged_window(%d, 1000);
+    for (int rows : {1, 5, 40}) for (int len : {0, 1, 3, 40, 1000}) for (int prefix : {0, 2}) for (int first = 0; first < rows * 3; first += 16) {
+        if (prefix > len) continue;
+        const PagedSpan s = paged_span(rows, len, prefix, w, 3, first, 16);
+        for (int q = first; q < std::min(first + 16, rows * 3); q++) for (int j = 0; j < len; j++) {
+            const int i = len - rows + q / 3;
+            const bool sees = (j <= i && (long long)j > (long long)i - %dll) || j < prefix;
+            if (sees != paged_sees(i, j, len, w, prefix) || (sees && (j < s.begin || j >= s.end))) { std::printf("%%d of %%d at %%d: %%d\n", rows, len, i, j); return 0; }
+        }
+    }
+    std::printf("ok\n");
+}
+""" % (window, window))
+    assert out == "ok\n", out
