@@ -530,7 +530,10 @@ int mg_paged_store(mg_paged* h, const float* q, const float* k, const float* v, 
 /* Takes the lengths of the step for the attention calls that follow: rows rowStart[r] .. rowStart[r+1]-1 are the last
  * positions of request r's lens[r] (after this step).  The arrays are copied (clamped to `rows` and maxLen).  Which positions j a
  * token at position i sees: j <= i, and where window > 0 only j > i - window; with prefixLens also every j < prefixLens[r],
- * before or behind i and whatever the window. */
+ * before or behind i and whatever the window.
+ * An attention call goes by the nReqs, rows and window of the last mg_paged_plan call, captured or not, before it, and by the lengths of the
+ * plan that ran last on the device.  Where that one was for other nReqs, rows or window -- a graph's replay came between, or the call was
+ * captured and has not run yet -- it does nothing and leaves out as it was. */
 int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int window, const int* prefixLens, void* stream);
 
 /* out[row, head] = sum_j softmax_j(s_j) v_j over the positions that the row sees, of KV head `head / (nHeads / nKVHeads)`:

@@ -26,10 +26,18 @@ hipError_t launch_paged_store(const PagedStore& p, hipStream_t s);
 struct PagedWorker { PagedTile tile; int a, b, tiles, pad[13]; };
 static_assert(sizeof(PagedTile) == 64 && sizeof(PagedWorker) == 128, "read as 16-byte words");
 
+// What a plan was made for.  The places and numbers of its tiles and workers follow from these: an attention call works on the plan that is
+// in the handle's memory only where they are its own (a graph's replay may have left another one there, or it was captured and has not run).
+struct PagedPlanFor {
+    int nReqs, rows, window, pad;
+    MG_HD bool is(const PagedPlanFor& o) const { return ((nReqs ^ o.nReqs) | (rows ^ o.rows) | (window ^ o.window)) == 0; }      // (no branch between the loads)
+};
+
 // The plan that a step's attention calls share.
 struct PagedPlan {
     const int *rowStart, *lens, *prefixLens;      // the caller's
-    PagedTile* tiles;                             // the handle's: maxTiles of them, for narrow tiles and again for wide ones,
+    PagedPlanFor* made;                           // the handle's
+    PagedTile* tiles;                             // maxTiles of them, for narrow tiles and again for wide ones,
     PagedWorker* workers;                         // and maxWorkers of these
     int nReqs, rows, window, maxLen, group, kvHalf, maxTiles, maxWorkers, nWorkers, wideWorkers, narrowRows;      // wideWorkers 0: no wide tiles
 };
@@ -40,6 +48,7 @@ struct PagedAttention {
     const void *K, *V;
     const int* table;
     float* out;
+    const PagedPlanFor* made;
     const PagedTile* tiles;    // narrow tiles' and wide ones', maxTiles and maxWorkers apart, as in the plan
     const PagedWorker* workers;
     float* parts;              // partial results: two of every worker and KV head
@@ -47,6 +56,7 @@ struct PagedAttention {
     const float* zeros;        // headDim zeros: what a position outside a tile's, or on a page that is gone, is read from
     size_t partStride;
     float scale, softcap;
+    PagedPlanFor plan;
     int ldq, ldo, window, maxTiles, maxWorkers, nWorkers, wideWorkers;
     PagedGeo g;
 };

@@ -212,14 +212,16 @@ struct OnDevice {
 struct mg_paged {
     mg::PagedGeo g;
     int device;
-    char* mem;             // one allocation: zeros, tiles, workers, arrival counts, partial results
+    char* mem;             // one allocation: zeros, what the plan is for, arrival counts, tiles, workers, partial results
     float* zeros;
+    mg::PagedPlanFor* made;
     mg::PagedTile* tiles;
     mg::PagedWorker* workers;
     unsigned* arrived;
     float* parts;
     int maxTiles, maxWorkers;
-    int planReqs, planRows, planWindow, planWorkers, planWideWorkers;      // the last plan (planReqs < 0: none yet)
+    mg::PagedPlanFor plan;                     // the last plan asked for (nReqs < 0: none yet)
+    int planWorkers, planWideWorkers;
 };
 
 namespace {
@@ -259,11 +261,11 @@ mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, i
     if (!h) { mg::set_error("mg_paged_create: out of host memory"); return nullptr; }
     h->g = g;
     h->device = device;
-    h->planReqs = -1;
+    h->plan.nReqs = -1;
     const size_t tiles = (size_t)mg::paged_max_tiles(g), workers = (size_t)std::max(mg::paged_workers(g, g.maxReqs, g.maxRows, false), mg::paged_workers(g, g.maxReqs, g.maxRows, true)), heads = (size_t)g.nKVHeads;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
-    const size_t oZeros = take((size_t)g.headDim * 4), oArrived = take(heads * tiles * 4), clear = at;      // (the part that starts as zeros)
+    const size_t oZeros = take((size_t)g.headDim * 4), oMade = take(sizeof(mg::PagedPlanFor)), oArrived = take(heads * tiles * 4), clear = at;      // (the part that starts as zeros)
     const size_t oTiles = take(2 * tiles * sizeof(mg::PagedTile)), oWorkers = take(2 * workers * sizeof(mg::PagedWorker));
     const size_t oParts = take(heads * workers * 2 * mg::paged_part_floats(g) * 4);
     hipError_t e = hipMalloc(reinterpret_cast<void**>(&h->mem), at);
@@ -279,6 +281,7 @@ mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, i
     h->maxTiles = (int)tiles;
     h->maxWorkers = (int)workers;
     h->zeros = reinterpret_cast<float*>(h->mem + oZeros);
+    h->made = reinterpret_cast<mg::PagedPlanFor*>(h->mem + oMade);
     h->arrived = reinterpret_cast<unsigned*>(h->mem + oArrived);
     h->tiles = reinterpret_cast<mg::PagedTile*>(h->mem + oTiles);
     h->workers = reinterpret_cast<mg::PagedWorker*>(h->mem + oWorkers);
@@ -323,23 +326,23 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
     window = mg::paged_window(window, g.maxLen);
     const int workers = mg::paged_workers(g, nReqs, rows, false), narrow = mg::paged_narrow_rows(g, rows);
     const int wide = (long long)rows * g.group > narrow ? mg::paged_workers(g, nReqs, rows, true) : 0;
-    mg::PagedPlan p{rowStart, lens, prefixLens, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, h->maxTiles, h->maxWorkers, workers, wide, narrow};
+    mg::PagedPlan p{rowStart, lens, prefixLens, h->made, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, h->maxTiles, h->maxWorkers, workers, wide, narrow};
     const int rc = launched("mg_paged_plan", mg::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
     if (rc == MG_OK) {
-        h->planReqs = nReqs; h->planRows = rows; h->planWindow = window; h->planWorkers = workers; h->planWideWorkers = wide;
+        h->plan = {nReqs, rows, window, 0}; h->planWorkers = workers; h->planWideWorkers = wide;
     }
     return rc;
 }
 int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, const void* V, const int* table, float* out, int ldo, float scale,
                        float softcap, const float* slopes, void* stream) {
     PAGED(h, "mg_paged_attention");
-    if (h->planReqs < 0) { mg::set_error("mg_paged_attention: no plan yet (mg_paged_plan)"); return MG_E_STATE; }
-    if (h->planReqs == 0 || h->planRows == 0) return MG_OK;
+    if (h->plan.nReqs < 0) { mg::set_error("mg_paged_attention: no plan yet (mg_paged_plan)"); return MG_E_STATE; }
+    if (h->plan.nReqs == 0 || h->plan.rows == 0) return MG_OK;
     if (const char* why = mg::paged_attention_refusal(h->g, q, ldq, K, V, table, out, ldo, scale, softcap, slopes)) return refuse("mg_paged_attention", why);
-    if (const char* why = mg::paged_attention_overlap(h->g, q, ldq, K, V, out, ldo, h->planRows)) return refuse("mg_paged_attention", why);
+    if (const char* why = mg::paged_attention_overlap(h->g, q, ldq, K, V, out, ldo, h->plan.rows)) return refuse("mg_paged_attention", why);
     const mg::PagedGeo& g = h->g;
-    mg::PagedAttention p{q, slopes, K, V, table, out, h->tiles, h->workers, h->parts, h->arrived, h->zeros, mg::paged_part_floats(g),
-                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, ldq, ldo, h->planWindow, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
+    mg::PagedAttention p{q, slopes, K, V, table, out, h->made, h->tiles, h->workers, h->parts, h->arrived, h->zeros, mg::paged_part_floats(g),
+                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, h->plan, ldq, ldo, h->plan.window, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
     return launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
 }
 

@@ -104,6 +104,7 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
     p.tiles += wide ? p.maxTiles : 0;
     p.workers += wide ? p.maxWorkers : 0;
     p.nWorkers = wide ? p.wideWorkers : p.nWorkers;
+    if (threadIdx.x == 0 && !wide) *p.made = {p.nReqs, p.rows, p.window, 0};
     __shared__ unsigned tile0[PAGED_MAX_REQS + 1], place[PLAN_LDS_TILES], part[PT / 64];
     __shared__ int4 held[PT];
     const int tid = threadIdx.x;
@@ -1184,8 +1185,9 @@ __device__ __forceinline__ void attend(const PagedAttention& p, float* lds) {
     if (kvh >= p.g.nKVHeads) return;
     const PagedWorker* k = p.workers + w;
     const int a = __builtin_amdgcn_readfirstlane(k->a), b = __builtin_amdgcn_readfirstlane(k->b), tiles = __builtin_amdgcn_readfirstlane(k->tiles);
-    if (a >= b) return;
+    const bool ours = p.made->is(p.plan);             // (asked for together with the share)
     PagedTile t = tile_at(&k->tile);
+    if (!ours || a >= b) return;
     for (;;) {
         const int u0 = paged_unit_at(t, a), u1 = paged_unit_at(t, b);
         if (u0 < u1) {

@@ -160,3 +160,76 @@ def test_the_largest_window_is_none(hip, bufs, half):
         outs.append(c.result())
         c.h.Close()
     assert np.array_equal(*outs) and (outs[0][:2] == 0).all() and (outs[0][2:6] != 0).any(1).all() and (outs[0][6:56] == 0).all() and (outs[0][56:] != 0).any(1).all()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# plans that did not run, or that another has written over
+# ---------------------------------------------------------------------------------------------------------------------
+def _two_batches(hip, bufs, half):
+    """(case, the arguments of its plan, those of a plan of its first request alone)"""
+    c = Case(hip, bufs, 8, 2, 64, half, 8, [3, 1, 90], [60, 33, 400], seed=2)
+    c.upload()
+    d = c.d
+    return c, (d["rowStart"], d["lens"], 3, c.rows, 0, None), (d["rowStart"], d["lens"], 1, 3, 0, None)
+
+
+def _got(c):
+    E.KSync()
+    assert E.HIPCheck() == 0
+    got = c.result()
+    c.b.put(c.d["out"], c.out0)
+    return got
+
+
+@pytest.mark.parametrize("half", [0, 1])
+def test_a_plan_that_was_captured_and_has_not_run(hip, bufs, rt, half):
+    c, whole, _ = _two_batches(hip, bufs, half)
+    want, bound = c.want()
+    stream = rt.stream()
+
+    def step():
+        assert c.h.Plan(*whole, stream) == 0
+        c.attend(stream=stream)
+
+    graph = rt.capture(stream, step)
+    c.attend()
+    assert (_got(c) == 7.25).all()
+    for _ in range(3):
+        rt.replay(graph, stream)
+        c.compare(_got(c), want, bound)
+        c.attend()                       # the plan is there now
+        c.compare(_got(c), want, bound)
+    c.h.Close()
+
+
+@pytest.mark.parametrize("half", [0, 1])
+def test_a_plan_of_another_batch_in_the_handle(hip, bufs, rt, half):
+    c, whole, first = _two_batches(hip, bufs, half)
+    want, bound = c.want()
+    stream = rt.stream()
+    assert c.h.Plan(*whole) == 0
+    alone = rt.capture(stream, lambda: c.attend(stream=stream))
+
+    def step():
+        assert c.h.Plan(*whole, stream) == 0
+        c.attend(stream=stream)
+
+    both = rt.capture(stream, step)
+    for _ in range(2):
+        assert c.h.Plan(*first) == 0
+        c.attend()
+        got = _got(c)
+        assert (np.abs(got[:3, :512] - want[:3]) <= bound[:3]).all() and (got[3:] == 7.25).all()
+        rt.replay(alone, stream)         # captured behind the plan of all three
+        assert (_got(c) == 7.25).all()
+        rt.replay(both, stream)
+        c.compare(_got(c), want, bound)
+        c.attend()                       # asked for behind the plan of one
+        assert (_got(c) == 7.25).all()
+        rt.replay(alone, stream)
+        c.compare(_got(c), want, bound)
+        assert c.h.Plan(*whole[:4], 5) == 0      # the same batch, another window
+        E.KSync()
+        rt.replay(alone, stream)
+        assert (_got(c) == 7.25).all()
+    c.h.Close()
