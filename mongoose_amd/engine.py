@@ -67,6 +67,8 @@ class Tensor:
 
     @property
     def _as_parameter_(self):          # (what ctypes passes where an address is asked for)
+        if self._ptr is None:          # (NULL would be an argument that is not asked for)
+            raise ValueError("a released tensor")
         return self._ptr
 
     def Size(self):
@@ -760,7 +762,8 @@ def KQ8Gemm(act, w, scales, bias, out, T, N, K, accumulate, workspace, workspace
 class HIPPaged:
     """Several requests out of one KV cache in pages (mg_paged_*): block tables and slot maps from the requests' lengths, rotary
     positions with the K/V rows stored by slot, attention of the requests' new tokens over their pages.  No counterpart in the
-    reference.  Arguments are device buffers (Tensor, or an address); every method returns 0 or a negative code (last_error)."""
+    reference.  Arguments are device buffers (Tensor, or an address); every method returns 0 or a negative code (last_error).
+    A Tensor that has been released is a ctypes.ArgumentError."""
 
     def __init__(self, handle):
         self._h = handle

@@ -1,4 +1,5 @@
 """What the calls on a paged KV cache refuse, and the positions that a token sees, on the host (paged_rules.h)."""
+import ctypes
 import os
 import subprocess
 
@@ -329,3 +330,14 @@ int main() {
 }
 """ % (window, window))
     assert out == "ok\n", out
+
+
+def test_a_released_tensor_is_no_missing_argument():
+    """None for slopes or prefixLens asks for another formula; a tensor that is gone must not."""
+    gone, live, h = E.Tensor(None, None, 64, [16]), E.Tensor(None, 64, 64, [16]), E.HIPPaged(None)
+    assert h.Plan(live, live, 1, 1, 0, live) == -1 and "NULL handle" in E.last_error()
+    for call in (lambda: h.Plan(live, live, 1, 1, 0, gone), lambda: h.Attention(live, 64, live, live, live, live, 64, slopes=gone),
+                 lambda: h.Store(live, live, live, 64, 64, 64, gone, 64, live, live, live, live, 1, live, live, 1),
+                 lambda: h.Tables(live, 1, live, live, live, live, live, live, 1, live, live, live, gone)):
+        with pytest.raises(ctypes.ArgumentError, match="released"):
+            call()
