@@ -23,7 +23,9 @@ constexpr int PLAN_LDS_TILES = 4096;      // tiles whose places on the line the 
 // Units a worker has at least where a tile's workers are its own: a narrow unit is as short as a share can be (one request of 500
 // positions 8.8 us, with two 10.8); a wide share costs its 64 KB out and in (12 requests, some of 165 to 235 rows: 92 us, with one 95).
 constexpr int LEAST_NARROW = 1, LEAST_WIDE = 3;
+constexpr int NARROW_WORKERS = 256;       // workgroups that narrow tiles have at most (a CU each)
 constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results
+static_assert(NARROW_WORKERS * NARROW <= MERGE_LDS, "a narrow tile's shares are weighed in one turn");
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
@@ -48,7 +50,7 @@ size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRo
 // cannot have that many units.
 int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide) {
     const long long tiles = (long long)rows * g.group / NARROW + nReqs, units = tiles * (g.maxLen / 32 + 2);
-    const int resident = 256 * (wide ? 2 : 1);
+    const int resident = NARROW_WORKERS * (wide ? 2 : 1);
     const long long most = resident / g.nKVHeads > 0 ? resident / g.nKVHeads : 1;
     return (int)(units < 1 ? 1 : units < most ? units : most);
 }
@@ -715,23 +717,20 @@ struct NarrowTile {
     // All workers' shares: threads take rows and columns and, where there are fewer of those than threads, shares in turn
     __device__ __forceinline__ void merge(int kvh, int R, float* lds) const {
         float *M = lds, *den = lds + NARROW, *wt = lds + 2 * NARROW;
-        constexpr int TURN = MERGE_LDS / NARROW, N = NARROW * HD / 4 / WG > 0 ? NARROW * HD / 4 / WG : 1;
+        constexpr int N = NARROW * HD / 4 / WG > 0 ? NARROW * HD / 4 / WG : 1;
         const int tid = thread_anew(), segs = t.worker1 - t.worker0 + 1, cols = R * (HD / 4), par = max(1, WG / cols);
         float4_t acc[N];
 #pragma unroll
         for (int k = 0; k < N; k++) acc[k] = float4_t{0.f, 0.f, 0.f, 0.f};
-        for (int s0 = 0; s0 < segs; s0 += TURN) {
-            const int n = min(TURN, segs - s0);
-            merge_weights<HD, NARROW>(p, t, kvh, R, s0, n, M, den, wt);
+        merge_weights<HD, NARROW>(p, t, kvh, R, 0, segs, M, den, wt);
 #pragma unroll
-            for (int k = 0; k < N; k++) {
-                const int i = par > 1 ? tid % cols : tid + k * WG, from = par > 1 ? tid / cols : 0;
-                if (i >= cols || from >= par || (par > 1 && k > 0)) continue;
-                const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+        for (int k = 0; k < N; k++) {
+            const int i = par > 1 ? tid % cols : tid + k * WG, from = par > 1 ? tid / cols : 0;
+            if (i >= cols || from >= par || (par > 1 && k > 0)) continue;
+            const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
 #pragma unroll 4
-                for (int s = from; s < n; s += par)
-                    acc[k] += wt[s * NARROW + r] * *reinterpret_cast<const float4_t*>(part_of(p, t, kvh, t.worker0 + s0 + s) + r * HD + d);
-            }
+            for (int s = from; s < segs; s += par)
+                acc[k] += wt[s * NARROW + r] * *reinterpret_cast<const float4_t*>(part_of(p, t, kvh, t.worker0 + s) + r * HD + d);
         }
         __syncthreads();
         if (par > 1) {                        // the shares of the same columns, in their order

@@ -233,3 +233,46 @@ def test_a_plan_of_another_batch_in_the_handle(hip, bufs, rt, half):
         rt.replay(alone, stream)
         assert (_got(c) == 7.25).all()
     c.h.Close()
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# many requests, tiles and shares
+# ---------------------------------------------------------------------------------------------------------------------
+def _check_some(c, which, **what):
+    """As Case.check for the rows of some requests."""
+    c.upload()
+    c.plan(what.get("window", 0))
+    c.attend()
+    E.KSync()
+    assert E.HIPCheck() == 0
+    got = c.result()
+    assert np.isfinite(got).all() and (got[c.rows:] == 7.25).all()
+    for r in which:
+        a, b = int(c.rowStart[r]), int(c.rowStart[r + 1])
+        want, bound = P.attention(c.q[a:b, :c.heads * c.hd], c.K, c.V, c.table[r:r + 1], np.array([0, b - a]), c.lens[r:r + 1], c.page, c.group, c.hd, **what)
+        assert (np.abs(got[a:b, :c.heads * c.hd] - want) <= bound).all(), r
+    c.h.Close()
+
+
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("heads,kv,n", [(4, 1, 1100), (2, 2, 4096), (32, 1, 1500), (8, 4, 2049)])
+def test_more_requests_than_the_plan_has_threads(hip, bufs, heads, kv, n, half):
+    """A token each, from 1 position up; groups of up to 16 are narrow tiles, 32 a wide one a request."""
+    print(f"{n} requests {heads}/{kv} half={half}", flush=True)
+    lens = np.random.default_rng(n).integers(1, 70, n)
+    lens[[0, n - 1]] = 1, 600
+    _check_some(Case(hip, bufs, heads, kv, 64, half, 16, [1] * n, lens, seed=n), range(n) if heads * n < 12000 else [*range(0, n, 7), n - 1])
+
+
+@pytest.mark.parametrize("half", [0, 1])
+def test_more_tiles_than_the_plan_has_places_for(hip, bufs, half):
+    """110 rows x 128 heads each: 4,400 wide tiles."""
+    lens = [110 + 3 * r for r in range(40)]
+    _check_some(Case(hip, bufs, 128, 1, 64, half, 16, [110] * 40, lens, seed=1), (0, 9, 10, 37, 38, 39))
+
+
+@pytest.mark.parametrize("half", [0, 1])
+@pytest.mark.parametrize("heads,hd,new,length", [(2, 64, 130, 33001), (4, 128, 65, 41000)])
+def test_tiles_of_more_shares_than_are_joined_at_once(hip, bufs, heads, hd, new, length, half):
+    print(f"shares {heads}/1/{hd} half={half} {new} of {length}", flush=True)
+    Case(hip, bufs, heads, 1, hd, half, 64, [new], [length], seed=new).check()
