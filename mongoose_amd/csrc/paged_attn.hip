@@ -21,7 +21,8 @@ constexpr int PT = 1024;                  // threads of the plan
 constexpr int NARROW = 16, WIDE = 128;    // rows of a tile
 constexpr int PLAN_LDS_TILES = 4096;      // tiles whose places on the line the plan holds in LDS
 // Units a worker has at least where a tile's workers are its own: a narrow unit is as short as a share can be (one request of 500
-// positions 8.8 us, with two 10.8); a wide share costs its 64 KB out and in (12 requests, some of 165 to 235 rows: 92 us, with one 95).
+// positions 8.8 us, with two 10.8); a wide share costs its 64 KB out and in (8B shape, one fresh prompt: 469 rows fp16 29 us, with one 38,
+// with five 33; 409 rows fp32 52, with one 73, with two 70, with five 53).
 constexpr int LEAST_NARROW = 1, LEAST_WIDE = 3;
 constexpr int NARROW_WORKERS = 256;       // workgroups that narrow tiles have at most (a CU each)
 constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results
@@ -39,14 +40,20 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 MG_HD int narrow_keys(int kvHalf) { return kvHalf ? 128 : 64; }
 MG_HD int wide_keys(int kvHalf) { return kvHalf ? 64 : 32; }
 
-// A request of up to 16 rows a KV head goes to the kernel that waits for memory, others to the one that waits for the matrix units.
+// Rows a KV head (tokens x group) up to which a request goes to the kernel that waits for memory, with longer ones to the one that waits for
+// the matrix units.  8B shape:
+//   A batch of up to 256 rows: all narrow, which reads K and V once for 16 rows, but in one launch.  One request of 8, 16, 32 and 64 tokens
+//   over 16,000 positions: fp16 33, 41, 64, 112 us, wide 83, 89, 103, 105; fp32 43, 66, 117, 220, wide 338, 380, 401, 317.
+//   Larger batches: narrow up to 16 rows.  24 requests of 5, 8, 12 tokens over 500 to 4,000 positions, fp16: 77, 78, 80 us wide, 75, 81, 99
+//   narrow, and 96 requests of 5 tokens 208 wide, 304 narrow.  With an fp32 cache narrow tiles would be better there, up to 64 rows (228,
+//   204, 385, and with 16 tokens 361 us wide; 169, 141, 249, 276 narrow): its wide tiles wait for the fp32 instructions of rows that are not there.
 int paged_narrow_rows(const PagedGeo& g, int rows) {
     return (long long)rows * g.group <= 256 ? 256 : NARROW;
 }
 int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + 256 / NARROW; }
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
 // Workgroups, in turns of the KV heads: two a CU for wide tiles; one a CU for narrow ones, though a CU holds two: HBM likes fewer
-// streams (8B shape, fp16: 120,001 positions 102 us, with two 122, with three 145; 48 requests 173, 182, 217).  Fewer where the batch
+// streams (8B shape, fp16: 120,001 positions 98 us, with two 113; 48 requests 174 and 182).  Fewer where the batch
 // cannot have that many units.
 int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide) {
     const long long tiles = (long long)rows * g.group / NARROW + nReqs, units = tiles * (g.maxLen / 32 + 2);
@@ -232,7 +239,7 @@ __device__ __forceinline__ float capped(float s, float cap, float invCap) {
     return a < CAP_NEAR ? capped_near(s, x * x) : cap * far;
 }
 // The cap on all the scores of a lane: without the far form where no lane of the wave needs it (8B shape, four requests of 345 to
-// 467 rows over a window of 1,024, cap 50: 150 -> 136 us)
+// 467 rows over a window of 1,024, cap 50: 131 us, without this 139)
 template <typename T, int N>
 __device__ __forceinline__ void cap_all(T (&s)[N], float cap, float invCap) {
     constexpr int M = sizeof(T) / 4;
@@ -752,7 +759,7 @@ struct NarrowTile {
 };
 
 // A tile of 128 rows: a wave takes 32 of them over all the positions, which go through LDS (two buffers, filled by loads that run a
-// unit ahead), so that a K or V row is fetched once for 128 rows.  8B shape, fp16, 2,048 tokens over 16,384 positions: 1,047 us, 985
+// unit ahead), so that a K or V row is fetched once for 128 rows.  8B shape, fp16, 2,048 tokens over 16,384 positions: 1,015 us, 1,015
 // TFLOP/s with both terms counted.  Bound by the matrix units: 32x32 instructions, two terms a product
 // with an fp16 cache (as in NarrowTile), four K = 2 fp32 instructions a 16-byte piece with an fp32 one.
 //   K (A operand): lane l = position l%32, 16 bytes at dimensions 16 s + 8 (l/32) (fp16) or 8 s + 4 (l/32) (fp32).
