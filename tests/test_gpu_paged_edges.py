@@ -1,5 +1,6 @@
 """Attention over a paged KV cache at the edges of its arguments: values that are no numbers at positions that a row does not
-see, infinities where it does; rows of q from tiny to huge.  Against 64 bits, as test_gpu_paged."""
+see, infinities where it does; rows of q from tiny to huge; the largest window; arguments that overlap; plans that did not run or
+were written over; more requests, tiles and shares than one round of the plan or of a join takes.  Against 64 bits, as test_gpu_paged."""
 import numpy as np
 import pytest
 
