@@ -477,13 +477,19 @@ int mg_stream_forward_token(mg_stream* s, int pos, const float* embHidden, int n
 /*    mongoose_rope and mongoose_decode_attention.                      */
 /* ------------------------------------------------------------------ */
 /* A layer's cache is two pools, K and V, of nPages pages of pageSize positions, [nPages, pageSize, nKVHeads * headDim], fp32
- * (kvFormat 0) or fp16 (1; written rounded to nearest even), from tw_gpu_alloc or any hipMalloc.  Request r's position p is in
- * page table[r * width + p / pageSize], width = mg_paged_table_width.  One table serves all layers.
+ * (kvFormat 0), fp16 (1; written rounded to nearest even) or Q8 (8), from tw_gpu_alloc or any hipMalloc of mg_paged_pool_bytes.
+ * Request r's position p is in page table[r * width + p / pageSize], width = mg_paged_table_width.  One table serves all layers.
+ *
+ * Q8: an int8 an element and an fp32 scale a KV head's row of a position, worth q * scale: scale = max |x| / 127 over the row (rounded to
+ * fp32), q = x / scale to the nearest whole number, half away from zero, decided exactly (of K: x the turned element, exact to 64 bits and
+ * then rounded to fp32).  A row with an infinity or a NaN gets a NaN for its scale.  A pool is the int8 rows [nPages, pageSize, nKVHeads *
+ * headDim], then the scales [nPages, nKVHeads, pageSize]: headDim + 4 bytes where fp16 takes 2 * headDim.
  *
  * A step of a server:   mg_paged_tables   once a step: rows, slots and block tables from the requests' lengths
  *                       mg_paged_plan     once a step (and once for every other window or prefix its layers use)
  *                       mg_paged_store    each layer: rotary positions, K and V rows into the slots
  *                       mg_paged_attention  each layer
+ *                       mg_paged_load     where rows are wanted back (to keep a request elsewhere, to look at it)
  * All take device pointers, launch kernels on `stream` and neither allocate, synchronise nor copy: they can be captured into a
  * graph, and lengths may change between its replays (nReqs and rows are upper bounds then: requests of no rows and no length do
  * nothing, rows behind the last request's are left as they were).
@@ -500,6 +506,7 @@ mg_paged* mg_paged_create(int nHeads, int nKVHeads, int headDim, int pageSize, i
                           int maxLen);
 void mg_paged_destroy(mg_paged* h);
 int mg_paged_table_width(const mg_paged* h);      /* ceil(maxLen / pageSize): entries of a request's row of the block table */
+size_t mg_paged_pool_bytes(const mg_paged* h);    /* bytes of a layer's K (or V) pool */
 
 /* Block tables and slot maps of a step.  newLens[r]: tokens that request r adds (0: none), or -1 when it has ended.  lens[r]:
  * its positions so far.  ring: the free pages, a ring of nPages entries; ringState = {first free entry, free pages}.
@@ -527,6 +534,14 @@ int mg_paged_store(mg_paged* h, const float* q, const float* k, const float* v, 
                    void* K, void* V, const int* slots, const int* positions, int rows, const float* cosTab, const float* sinTab,
                    int tableRows, void* stream);
 
+/* Rows read back as fp32, of any format: rows rowStart[r] .. rowStart[r+1]-1 are the last positions of request r's lens[r] (a step's
+ * arrays give the rows it stored; row starts that are sums of the lengths give requests whole).  kOut and vOut have `rows` rows, ldk and
+ * ldv floats apart (multiples of 4, 16-byte aligned pointers), and overlap neither each other nor what is read.  A position on a table
+ * entry that is no page, or ahead of the request's first, is zeros; rows behind the last request's are left as they were.  `rows` is not bound by
+ * maxRows. */
+int mg_paged_load(mg_paged* h, const void* K, const void* V, const int* table, const int* rowStart, const int* lens, int nReqs, int rows,
+                  float* kOut, int ldk, float* vOut, int ldv, void* stream);
+
 /* Takes the lengths of the step for the attention calls that follow: rows rowStart[r] .. rowStart[r+1]-1 are the last
  * positions of request r's lens[r] (after this step).  The arrays are copied (clamped to `rows` and maxLen).  Which positions j a
  * token at position i sees: j <= i, and where window > 0 only j > i - window; with prefixLens also every j < prefixLens[r],
@@ -538,8 +553,8 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
 
 /* out[row, head] = sum_j softmax_j(s_j) v_j over the positions that the row sees, of KV head `head / (nHeads / nKVHeads)`:
  * s_j = scale * q.k_j (scale 0: 1 / sqrt(headDim)); with softcap > 0 then softcap * tanh(s_j / softcap); with slopes [nHeads]
- * then minus slopes[head] * |i - j|.  Scores, their maxima and sums are fp32; products of an fp32 cache too, those of an fp16 cache
- * are of q and the probabilities to 22 bits.  ldq, ldo: floats from one row to the next (multiples of 4, 16-byte aligned
+ * then minus slopes[head] * |i - j|.  Scores, their maxima and sums are fp32; products of an fp32 cache too, those of an fp16 or Q8 cache
+ * are of q and the probabilities (times the V rows' scales) to 22 bits.  ldq, ldo: floats from one row to the next (multiples of 4, 16-byte aligned
  * pointers); both have the plan's `rows` rows, and out overlaps neither q (other columns of one buffer are fine) nor K and V.  A table entry that is no page hides its positions; a row that sees nothing is zeros; what the cache holds
  * behind a request's length is not read into any result.  A value that is no number reaches the rows that see its position and no
  * others; an infinite one is an infinity of its sign in a row's result where its weight is 2^-126 of the row's greatest or more (with one

@@ -18,9 +18,18 @@ struct PagedStore {
     float* qOut;
     void *K, *V;
     const int *slots, *positions;
-    int ldq, ldk, ldv, ldqOut, rows, tableRows, nHeads, nKVHeads, headDim, kvHalf, nSlots;
+    int ldq, ldk, ldv, ldqOut, rows, tableRows, nHeads, nKVHeads, headDim, kvFormat, nSlots, pageShift;
 };
 hipError_t launch_paged_store(const PagedStore& p, hipStream_t s);
+
+struct PagedLoad {
+    const void *K, *V;
+    const int *table, *rowStart, *lens;
+    float *kOut, *vOut;
+    int nReqs, rows, ldk, ldv;
+    PagedGeo g;
+};
+hipError_t launch_paged_load(const PagedLoad& p, hipStream_t s);
 
 // A worker's share [a, b) of the line, and the tile that it starts in
 struct PagedWorker { PagedTile tile; int a, b, tiles, pad[13]; };
@@ -39,7 +48,7 @@ struct PagedPlan {
     PagedPlanFor* made;                           // the handle's
     PagedTile* tiles;                             // maxTiles of them, for narrow tiles and again for wide ones,
     PagedWorker* workers;                         // and maxWorkers of these
-    int nReqs, rows, window, maxLen, group, kvHalf, maxTiles, maxWorkers, nWorkers, wideWorkers, narrowRows;      // wideWorkers 0: no wide tiles
+    int nReqs, rows, window, maxLen, group, kvFormat, maxTiles, maxWorkers, nWorkers, wideWorkers, narrowRows;      // wideWorkers 0: no wide tiles
 };
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s);
 

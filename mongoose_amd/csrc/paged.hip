@@ -1,5 +1,5 @@
 // paged.hip -- a KV cache in pages that several requests share: the handle (mg_paged_*), block tables and slot maps from
-// request lengths, and rotary positions with the K/V rows stored by slot.  The attention that reads the pages is in paged_attn.hip.
+// request lengths, rotary positions with the K/V rows stored by slot, and rows read back.  The attention that reads the pages is in paged_attn.hip.
 #include "paged.h"
 
 #include <algorithm>
@@ -189,10 +189,159 @@ __global__ __launch_bounds__(256) void paged_store_kernel(PagedStore p) {
     if (store)
         for (int i = threadIdx.x; i < kvDim / 4; i += 256) put4(Vr + 4 * i, *reinterpret_cast<const float4*>(p.v + (size_t)t * p.ldv + 4 * i));
 }
+
+// The same into a Q8 cache.  A row of a KV head is held as q d, d = max |x| / 127 (fp32) and q = x / d rounded to the nearest whole number,
+// half away from zero.  Which side of a half x / d is on is decided exactly, so that nothing but x decides q: x is the turned element to
+// 64 bits, rounded to fp32 (its two products are exact in 64), the quotient a guess that the exact rest x - q d puts right.  A row with a
+// value that is no number gets a NaN for its scale.  hd / 8 neighbouring lanes have a row, eight elements a lane.
+__device__ __forceinline__ unsigned held4(float4 v, double d, double inv) {
+    const float x[4] = {v.x, v.y, v.z, v.w};
+    unsigned out = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const double size = fabs((double)x[i]);
+        double n = floor(fma(size, inv, 0.5));
+        const double rest = fma(-n, d, size);
+        if (2.0 * rest >= d) n += 1.0;
+        else if (2.0 * rest < -d) n -= 1.0;
+        const int q = d > 0.0 ? (int)fmin(n, 127.0) : 0;
+        out |= ((unsigned)(x[i] < 0.f ? -q : q) & 0xffu) << (8 * i);
+    }
+    return out;
+}
+__device__ __forceinline__ float most4(float4 v) { return fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))); }
+__device__ __forceinline__ bool odd4(float4 v) { const float z = (v.x * 0.f + v.y * 0.f) + (v.z * 0.f + v.w * 0.f); return z != z; }
+__global__ __launch_bounds__(256) void paged_store_q8_kernel(PagedStore p) {
+    const int t = blockIdx.x, pos = p.positions[t], slot = p.slots[t];
+    if (pos < 0 || pos >= p.tableRows) return;
+    const bool store = slot >= 0 && slot < p.nSlots;
+    const int eighth = p.headDim / 8, half = p.headDim / 2, kvDim = p.nKVHeads * p.headDim;
+    const float* c = p.cosTab + (size_t)pos * half;
+    const float* s = p.sinTab + (size_t)pos * half;
+    const int nq = p.nHeads * eighth, nk = p.nKVHeads * eighth;
+    const int pageSize = 1 << p.pageShift;
+    const size_t scale0 = (size_t)(store ? slot >> p.pageShift : 0) * p.nKVHeads * pageSize + (store ? slot & (pageSize - 1) : 0);
+    for (int i = threadIdx.x; i < nq + (store ? 2 * nk : 0); i += 256) {
+        const int part = i < nq ? 0 : i < nq + nk ? 1 : 2, e = part == 0 ? i : part == 1 ? i - nq : i - nq - nk;
+        const int h = e / eighth, j = (e % eighth) * 4;
+        const float* x = (part == 0 ? p.q + (size_t)t * p.ldq : part == 1 ? p.k + (size_t)t * p.ldk : p.v + (size_t)t * p.ldv) + (size_t)h * p.headDim + j;
+        const float4 a = *reinterpret_cast<const float4*>(x), b = *reinterpret_cast<const float4*>(x + half);
+        float4 y = a, z = b;
+        if (part != 2) {
+            const float4 cc = *reinterpret_cast<const float4*>(c + j), ss = *reinterpret_cast<const float4*>(s + j);
+            if (part == 0) {
+                y = make_float4(a.x * cc.x - b.x * ss.x, a.y * cc.y - b.y * ss.y, a.z * cc.z - b.z * ss.z, a.w * cc.w - b.w * ss.w);
+                z = make_float4(a.x * ss.x + b.x * cc.x, a.y * ss.y + b.y * cc.y, a.z * ss.z + b.z * cc.z, a.w * ss.w + b.w * cc.w);
+                float* o = p.qOut + (size_t)t * p.ldqOut + (size_t)h * p.headDim + j;
+                put4(o, y);
+                put4(o + half, z);
+                continue;
+            }
+            auto less = [](float a, float c, float b, float s) { return (float)((double)a * c - (double)b * s); };
+            auto more = [](float a, float s, float b, float c) { return (float)((double)a * s + (double)b * c); };
+            y = make_float4(less(a.x, cc.x, b.x, ss.x), less(a.y, cc.y, b.y, ss.y), less(a.z, cc.z, b.z, ss.z), less(a.w, cc.w, b.w, ss.w));
+            z = make_float4(more(a.x, ss.x, b.x, cc.x), more(a.y, ss.y, b.y, cc.y), more(a.z, ss.z, b.z, cc.z), more(a.w, ss.w, b.w, cc.w));
+        }
+        float top = fmaxf(most4(y), most4(z));
+        int odd = odd4(y) || odd4(z);
+        for (int d = 1; d < eighth; d <<= 1) { top = fmaxf(top, __shfl_xor(top, d, 64)); odd |= __shfl_xor(odd, d, 64); }      // (a row's lanes are all here)
+        const float scale = odd ? __builtin_nanf("") : top / 127.f;
+        const double d = odd ? 0.0 : (double)scale, inv = d > 0.0 ? 1.0 / d : 0.0;
+        signed char* row = static_cast<signed char*>(part == 1 ? p.K : p.V) + (size_t)slot * kvDim + (size_t)h * p.headDim + j;
+        *reinterpret_cast<unsigned*>(row) = held4(y, d, inv);
+        *reinterpret_cast<unsigned*>(row + half) = held4(z, d, inv);
+        if (j == 0) {
+            float* scales = reinterpret_cast<float*>(static_cast<signed char*>(part == 1 ? p.K : p.V) + (size_t)p.nSlots * kvDim);
+            scales[scale0 + (size_t)h * pageSize] = scale;
+        }
+    }
+}
 hipError_t launch_paged_store(const PagedStore& p, hipStream_t s) {
     if (p.rows <= 0) return hipSuccess;
-    if (p.kvHalf) hipLaunchKernelGGL(paged_store_kernel<_Float16>, dim3(p.rows), dim3(256), 0, s, p);
+    if (p.kvFormat == PAGED_Q8) hipLaunchKernelGGL(paged_store_q8_kernel, dim3(p.rows), dim3(256), 0, s, p);
+    else if (p.kvFormat == PAGED_F16) hipLaunchKernelGGL(paged_store_kernel<_Float16>, dim3(p.rows), dim3(256), 0, s, p);
     else hipLaunchKernelGGL(paged_store_kernel<float>, dim3(p.rows), dim3(256), 0, s, p);
+    return hipGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// Rows read back
+//
+// Row i of the call is position len_r - end_r + i of the request r whose rows cover it, end_r the row behind its last.  A wave a row: the
+// request is found in at most two rounds (64 of the row starts at once, then those of the stretch in between), then every lane
+// takes four neighbouring elements at a time.
+// ---------------------------------------------------------------------------
+constexpr int LOAD_ROWS = 4;          // rows (waves) of a workgroup
+// How many of starts[0 .. n] are at most i, less one: the request of row i where the starts ascend (whatever they are, 0 .. n - 1 or -1)
+__device__ __forceinline__ int wave_find(const int* starts, int n, int i) {
+    const int lane = threadIdx.x & 63;
+    int first = 0;
+    for (int step = n > 64 ? (n + 63) / 64 : 1;;) {
+        const int at = first + lane * step;
+        const int below = __popcll(__ballot(at < n && starts[min(at, n)] <= i));
+        if (below == 0) return first - (first == 0);
+        first += (below - 1) * step;
+        if (step == 1) return first;
+        n = min(n, first + step);
+        step = (n - first + 63) / 64;
+    }
+}
+template <typename T> __device__ __forceinline__ float4 get4(const T* p);
+template <> __device__ __forceinline__ float4 get4<float>(const float* p) { return *reinterpret_cast<const float4*>(p); }
+template <> __device__ __forceinline__ float4 get4<_Float16>(const _Float16* p) {
+    const half4_t h = *reinterpret_cast<const half4_t*>(p);
+    return make_float4((float)h[0], (float)h[1], (float)h[2], (float)h[3]);
+}
+template <> __device__ __forceinline__ float4 get4<signed char>(const signed char* p) {
+    const int w = *reinterpret_cast<const int*>(p);
+    return make_float4((float)(signed char)w, (float)(signed char)(w >> 8), (float)(signed char)(w >> 16), (float)(w >> 24));
+}
+template <typename KVT>
+__global__ __launch_bounds__(64 * LOAD_ROWS) void paged_load_kernel(PagedLoad p) {
+    const int i = __builtin_amdgcn_readfirstlane(blockIdx.x * LOAD_ROWS + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    if (i >= p.rows) return;
+    const int r = wave_find(p.rowStart, p.nReqs, i);
+    if (r < 0) return;
+    const int start = p.rowStart[r], end = p.rowStart[r + 1];
+    if (start < 0 || i < start || i >= end) return;              // behind the last request's rows
+    const long long pos = (long long)p.lens[r] - end + i;
+    int page = -1;
+    if (pos >= 0 && pos < p.g.maxLen) page = p.table[(size_t)r * p.g.width + (pos >> p.g.pageShift)];
+    float* out[2] = {p.kOut + (size_t)i * p.ldk, p.vOut + (size_t)i * p.ldv};
+    if (page < 0 || page >= p.g.nPages) {
+        for (int e = lane * 4; e < p.g.kvDim; e += 256)
+#pragma unroll
+            for (int w = 0; w < 2; w++) put4(out[w] + e, make_float4(0.f, 0.f, 0.f, 0.f));
+        return;
+    }
+    const int place = (int)(pos & (p.g.pageSize - 1));
+    const size_t row = (((size_t)page << p.g.pageShift) + place) * p.g.kvDim;
+    const KVT* in[2] = {static_cast<const KVT*>(p.K) + row, static_cast<const KVT*>(p.V) + row};
+    const float* scales[2];
+    if constexpr (sizeof(KVT) == 1)
+#pragma unroll
+        for (int w = 0; w < 2; w++)
+            scales[w] = reinterpret_cast<const float*>(static_cast<const signed char*>(w ? p.V : p.K) + (size_t)p.g.nPages * p.g.pageSize * p.g.kvDim) +
+                        (size_t)page * p.g.nKVHeads * p.g.pageSize + place;
+    const int headShift = p.g.headDim == 128 ? 7 : 6;
+#pragma unroll 4
+    for (int e = lane * 4; e < p.g.kvDim; e += 256)
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            float4 x = get4<KVT>(in[w] + e);
+            if constexpr (sizeof(KVT) == 1) {
+                const float d = scales[w][(size_t)(e >> headShift) * p.g.pageSize];
+                x = make_float4(x.x * d, x.y * d, x.z * d, x.w * d);
+            }
+            put4(out[w] + e, x);
+        }
+}
+hipError_t launch_paged_load(const PagedLoad& p, hipStream_t s) {
+    if (p.rows <= 0 || p.nReqs <= 0) return hipSuccess;
+    const dim3 grid((p.rows + LOAD_ROWS - 1) / LOAD_ROWS), block(64 * LOAD_ROWS);
+    if (p.g.kvFormat == PAGED_Q8) hipLaunchKernelGGL(paged_load_kernel<signed char>, grid, block, 0, s, p);
+    else if (p.g.kvFormat == PAGED_F16) hipLaunchKernelGGL(paged_load_kernel<_Float16>, grid, block, 0, s, p);
+    else hipLaunchKernelGGL(paged_load_kernel<float>, grid, block, 0, s, p);
     return hipGetLastError();
 }
 
@@ -297,6 +446,7 @@ void mg_paged_destroy(mg_paged* h) {
     delete h;
 }
 int mg_paged_table_width(const mg_paged* h) { return h ? h->g.width : 0; }
+size_t mg_paged_pool_bytes(const mg_paged* h) { return h ? mg::paged_pool_bytes(h->g) : 0; }
 
 int mg_paged_tables(mg_paged* h, const int* newLens, int nReqs, const int* lens, int* lensOut, int* table, int* ring, const int* ringState,
                     int* ringStateOut, int rows, int* rowStart, int* slots, int* positions, int* counts, void* stream) {
@@ -316,8 +466,16 @@ int mg_paged_store(mg_paged* h, const float* q, const float* k, const float* v, 
         return refuse("mg_paged_store", why);
     if (const char* why = mg::paged_store_overlap(h->g, q, k, v, ldq, ldk, ldv, qOut, ldqOut, K, V, rows)) return refuse("mg_paged_store", why);
     mg::PagedStore p{q, k, v, cosTab, sinTab, qOut, K, V, slots, positions, ldq, ldk, ldv, ldqOut, rows, tableRows,
-                     h->g.nHeads, h->g.nKVHeads, h->g.headDim, h->g.kvHalf, h->g.nPages * h->g.pageSize};
+                     h->g.nHeads, h->g.nKVHeads, h->g.headDim, h->g.kvFormat, h->g.nPages * h->g.pageSize, h->g.pageShift};
     return launched("mg_paged_store", mg::launch_paged_store(p, static_cast<hipStream_t>(stream)));
+}
+int mg_paged_load(mg_paged* h, const void* K, const void* V, const int* table, const int* rowStart, const int* lens, int nReqs, int rows, float* kOut,
+                  int ldk, float* vOut, int ldv, void* stream) {
+    PAGED(h, "mg_paged_load");
+    if (const char* why = mg::paged_load_refusal(h->g, K, V, table, rowStart, lens, nReqs, rows, kOut, ldk, vOut, ldv)) return refuse("mg_paged_load", why);
+    if (const char* why = mg::paged_load_overlap(h->g, K, V, table, rowStart, lens, nReqs, rows, kOut, ldk, vOut, ldv)) return refuse("mg_paged_load", why);
+    mg::PagedLoad p{K, V, table, rowStart, lens, kOut, vOut, nReqs, rows, ldk, ldv, h->g};
+    return launched("mg_paged_load", mg::launch_paged_load(p, static_cast<hipStream_t>(stream)));
 }
 int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int window, const int* prefixLens, void* stream) {
     PAGED(h, "mg_paged_plan");
@@ -326,7 +484,7 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
     window = mg::paged_window(window, g.maxLen);
     const int workers = mg::paged_workers(g, nReqs, rows, false), narrow = mg::paged_narrow_rows(g, rows);
     const int wide = (long long)rows * g.group > narrow ? mg::paged_workers(g, nReqs, rows, true) : 0;
-    mg::PagedPlan p{rowStart, lens, prefixLens, h->made, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvHalf, h->maxTiles, h->maxWorkers, workers, wide, narrow};
+    mg::PagedPlan p{rowStart, lens, prefixLens, h->made, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvFormat, h->maxTiles, h->maxWorkers, workers, wide, narrow};
     const int rc = launched("mg_paged_plan", mg::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
     if (rc == MG_OK) {
         h->plan = {nReqs, rows, window, 0}; h->planWorkers = workers; h->planWideWorkers = wide;

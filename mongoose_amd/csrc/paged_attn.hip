@@ -29,6 +29,7 @@ constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of pa
 static_assert(NARROW_WORKERS * NARROW <= MERGE_LDS, "a narrow tile's shares are weighed in one turn");
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef unsigned uint16v_t __attribute__((ext_vector_type(16)));
@@ -36,9 +37,9 @@ typedef unsigned uint2_t __attribute__((ext_vector_type(2)));
 typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
-// Positions of a unit: a narrow tile's four waves take 32 of an fp16 cache or 16 of an fp32 one each, a wide tile's share them.
-MG_HD int narrow_keys(int kvHalf) { return kvHalf ? 128 : 64; }
-MG_HD int wide_keys(int kvHalf) { return kvHalf ? 64 : 32; }
+// Positions of a unit: a narrow tile's four waves take 64 of a Q8 cache, 32 of an fp16 one or 16 of an fp32 one each, a wide tile's share them.
+MG_HD int narrow_keys(int kvFormat) { return kvFormat == PAGED_F32 ? 64 : kvFormat == PAGED_F16 ? 128 : 256; }
+MG_HD int wide_keys(int kvFormat) { return kvFormat == PAGED_F32 ? 32 : 64; }
 
 // Rows a KV head (tokens x group) up to which a request goes to the kernel that waits for memory, with longer ones to the one that waits for
 // the matrix units.  8B shape:
@@ -48,9 +49,10 @@ MG_HD int wide_keys(int kvHalf) { return kvHalf ? 64 : 32; }
 //   narrow, and 96 requests of 5 tokens 208 wide, 304 narrow.  With an fp32 cache narrow tiles would be better there, up to 64 rows (228,
 //   204, 385, and with 16 tokens 361 us wide; 169, 141, 249, 276 narrow): its wide tiles wait for the fp32 instructions of rows that are not there.
 int paged_narrow_rows(const PagedGeo& g, int rows) {
+    if (g.kvFormat == PAGED_Q8) return PAGED_MAX_ROWS * PAGED_MAX_GROUP;
     return (long long)rows * g.group <= 256 ? 256 : NARROW;
 }
-int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + 256 / NARROW; }
+int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / (g.kvFormat == PAGED_Q8 ? NARROW : WIDE)) + g.maxReqs + 256 / NARROW; }
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
 // Workgroups, in turns of the KV heads: two a CU for wide tiles; one a CU for narrow ones, though a CU holds two: HBM likes fewer
 // streams (8B shape, fp16: 120,001 positions 98 us, with two 113; 48 requests 174 and 182).  Fewer where the batch
@@ -109,7 +111,7 @@ __device__ __forceinline__ int plan_find(const unsigned* sums, int n, unsigned x
 // One workgroup for the narrow tiles and one for the wide ones
 __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
     const bool wide = blockIdx.x != 0;
-    const int tileRows = wide ? WIDE : NARROW, unitKeys = wide ? wide_keys(p.kvHalf) : narrow_keys(p.kvHalf);
+    const int tileRows = wide ? WIDE : NARROW, unitKeys = wide ? wide_keys(p.kvFormat) : narrow_keys(p.kvFormat);
     p.tiles += wide ? p.maxTiles : 0;
     p.workers += wide ? p.maxWorkers : 0;
     p.nWorkers = wide ? p.wideWorkers : p.nWorkers;
@@ -350,6 +352,19 @@ __device__ __forceinline__ float4_t over(float4_t v, float l) { return l == 0.f 
 // where they are 0); the same for -infinity and NaN; with zeros for all three.  An element is what the last time gives, plus an
 // infinity where the first count is not 0, minus one where the second is not.  Other tiles pay for a look at their result.
 enum { PLUS_INFINITE, MINUS_INFINITE, FINITE };
+// Two bytes that were xored with 0x80, each under a byte 0x64 -- halves of 1024 + (q + 128), whose last place is 1 -- as the halves q
+__device__ __forceinline__ unsigned signed_halves(unsigned x) {
+    const half2_t bias = {(_Float16)-1152.f, (_Float16)-1152.f};
+    return __builtin_bit_cast(unsigned, __builtin_bit_cast(half2_t, x) + bias);
+}
+// Eight signed bytes as halves
+__device__ __forceinline__ half8_t eight_halves(unsigned lo, unsigned hi) {
+    lo ^= 0x80808080u;
+    hi ^= 0x80808080u;
+    const uint4_t x = {signed_halves(__builtin_amdgcn_perm(lo, 0x64646464u, 0x00050004u)), signed_halves(__builtin_amdgcn_perm(lo, 0x64646464u, 0x00070006u)),
+                       signed_halves(__builtin_amdgcn_perm(hi, 0x64646464u, 0x00050004u)), signed_halves(__builtin_amdgcn_perm(hi, 0x64646464u, 0x00070006u))};
+    return __builtin_bit_cast(half8_t, x);
+}
 // What stands for the values of a word in a pass
 template <bool HALF>
 __device__ __forceinline__ unsigned stand_in(unsigned v, int pass) {
@@ -384,12 +399,12 @@ __device__ __forceinline__ int power_up(float top, float scale) {
 // fp32 caches: fp32 matrix instructions throughout.
 template <typename KVT, int HD, bool MOD>
 struct NarrowTile {
-    static constexpr bool HALF = sizeof(KVT) == 2;
-    static constexpr int KB = HALF ? 32 : 16;              // positions of a wave's step
+    static constexpr bool Q8 = sizeof(KVT) == 1, HALF = sizeof(KVT) <= 2;       // HALF: products of fp16 operands
+    static constexpr int KB = 64 / (int)sizeof(KVT);       // positions of a wave's step
     static constexpr int NB = KB / 16, UK = 4 * KB, EPL = HD / 16;
-    static constexpr int KV4 = HALF ? HD / 32 : HD / 16;   // 16-byte pieces a lane holds of a block's K rows
-    static constexpr int VW = HALF ? EPL / 2 : EPL;        // words a lane holds of a V row
-    static constexpr float SHIFT = HALF ? 14.f : 0.f;      // probabilities are held times 2^SHIFT
+    static constexpr int KV4 = HD * (int)sizeof(KVT) / 64; // 16-byte pieces a lane holds of a block's K rows
+    static constexpr int VW = EPL * (int)sizeof(KVT) / 4;  // words a lane holds of a V row
+    static constexpr float SHIFT = Q8 ? 0.f : HALF ? 14.f : 0.f;      // probabilities are held times 2^SHIFT
 
     const PagedAttention& p;
     const PagedTile& t;
@@ -404,7 +419,10 @@ struct NarrowTile {
     float4_t qf[HALF ? 1 : HD / 16];
     uint4_t k[NB][KV4];            // the step's K and V, then the next one's
     unsigned v[NB * 4][VW];
+    float4_t ks[Q8 ? NB : 1], vs[Q8 ? NB : 1];       // Q8: the scales of the lane's positions 16 b + 4 g + 0..3
+    const char *Ksc, *Vsc;
     float m, l;
+    float ref;                     // Q8: probabilities are 2^(x - ref)
     float4_t o[EPL];
 
     int here, next;                // page numbers of the step at hand and of the one behind it
@@ -420,11 +438,17 @@ struct NarrowTile {
         Kp = static_cast<const char*>(p.K) + (size_t)kvh * HD * sizeof(KVT);
         Vp = static_cast<const char*>(p.V) + (size_t)kvh * HD * sizeof(KVT);
         zeros = reinterpret_cast<const char*>(p.zeros);
+        if constexpr (Q8) {
+            const size_t slots = (size_t)p.g.nPages * p.g.pageSize, head = (size_t)kvh * p.g.pageSize * 4;
+            Ksc = static_cast<const char*>(p.K) + slots * rowBytes + head;
+            Vsc = static_cast<const char*>(p.V) + slots * rowBytes + head;
+        }
         here = page_of(u0);
         const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
         float4_t x[HD / 16];                      // the row's elements as the operands want them
 #pragma unroll
-        for (int i = 0; i < HD / 16; i++) x[i] = *reinterpret_cast<const float4_t*>(q + (HALF ? i / 2 * 32 + g * 8 + i % 2 * 4 : i * 16 + g * 4));
+        for (int i = 0; i < HD / 16; i++)
+            x[i] = *reinterpret_cast<const float4_t*>(q + (Q8 ? i / 4 * 64 + g * 16 + i % 4 * 4 : HALF ? i / 2 * 32 + g * 8 + i % 2 * 4 : i * 16 + g * 4));
         next = page_of(min(u0 + 1, u1 - 1));
         load_k(u0, here);
         load_v(u0, here);
@@ -447,6 +471,7 @@ struct NarrowTile {
                     const float y = ldexpf(x[2 * s + j / 4][j % 4], up);
                     qh[s][j] = (_Float16)y;
                     ql[s][j] = (_Float16)(y - (float)qh[s][j]);
+                    if (Q8 && !(fabsf(y) < INFINITY)) ql[s][j] = (_Float16)0.f;      // (the first term's product is what the formula gives)
                 }
             c = ldexpf(c, -up);
         } else {
@@ -456,7 +481,7 @@ struct NarrowTile {
         if (!MOD) c *= 1.4426950408889634f;
         c = fminf(c, FLT_MAX);                    // (0 times it is 0)
         m = -INFINITY;
-        l = 0.f;
+        l = ref = 0.f;
 #pragma unroll
         for (int e = 0; e < EPL; e++) o[e] = float4_t{0.f, 0.f, 0.f, 0.f};
     }
@@ -470,6 +495,10 @@ struct NarrowTile {
     }
     // The page of the positions 16 b .. 16 b + 15 that the lane has to do with: of its upper eight or its lower
     __device__ __forceinline__ int page_in(int mine, int b, bool upper) const {
+        if constexpr (Q8) {                           // (eight runs: each one's page in a scalar register)
+            const int lo = __builtin_amdgcn_readlane(mine, 2 * b), hi = __builtin_amdgcn_readlane(mine, 2 * b + 1);
+            return upper ? hi : lo;
+        }
         const int lo = HALF && b ? quad_lane<2>(mine) : quad_lane<0>(mine), hi = HALF && b ? quad_lane<3>(mine) : quad_lane<1>(mine);
         return upper ? hi : lo;                       // (all lanes take part in both exchanges)
     }
@@ -481,6 +510,16 @@ struct NarrowTile {
 #pragma unroll
             for (int i = 0; i < KV4; i++) k[b][i] = *reinterpret_cast<const uint4_t*>(at + i * 64);
         }
+        if constexpr (Q8) load_scales(ks, Ksc, base, mine);
+    }
+    // The scales of the lane's positions, by fours (what lies behind a request's end is read and not used)
+    __device__ __forceinline__ void load_scales(float4_t (&to)[Q8 ? NB : 1], const char* from, int base, int mine) const {
+#pragma unroll
+        for (int b = 0; b < (Q8 ? NB : 1); b++) {
+            const int page = page_in(mine, b, g & 2);
+            const size_t at = page >= 0 ? (((size_t)(unsigned)page * p.g.nKVHeads << p.g.pageShift) + ((unsigned)(base + 16 * b + 4 * g) & (unsigned)(p.g.pageSize - 1))) * 4 : 0;
+            to[b] = *reinterpret_cast<const float4_t*>((page >= 0 ? from : zeros) + at);
+        }
     }
     __device__ __forceinline__ void load_v(int u, int mine) {
         const int base = base_of(u);
@@ -488,7 +527,9 @@ struct NarrowTile {
         for (int j = 0; j < NB * 4; j++) {
             const int page = page_in(mine, j / 4, g & 2);
             const char* at = kv_row(Vp, zeros, rowBytes, base + 16 * (j / 4) + 4 * g + j % 4, page, span.begin, span.end, p.g.pageShift) + l16 * (VW * 4);
-            if constexpr (VW == 2) {
+            if constexpr (VW == 1) {
+                v[j][0] = *reinterpret_cast<const unsigned*>(at);
+            } else if constexpr (VW == 2) {
                 const uint2 x = *reinterpret_cast<const uint2*>(at);
                 v[j][0] = x.x; v[j][1] = x.y;
             } else {
@@ -500,13 +541,17 @@ struct NarrowTile {
                 }
             }
         }
+        if constexpr (Q8) load_scales(vs, Vsc, base, mine);
     }
-    struct Weights { half8_t hi, lo; float x[NB * 4]; };
+    static constexpr int WS = Q8 ? NB / 2 : 1;        // products of 32 positions a step
+    struct Weights { half8_t hi[WS], lo[WS]; float x[NB * 4]; };
     static __device__ __forceinline__ Weights weights(const float (&x)[NB * 4]) {
         Weights w;
         if constexpr (HALF) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) { w.hi[j] = (_Float16)x[j]; w.lo[j] = (_Float16)(x[j] - (float)w.hi[j]); }
+            for (int s = 0; s < WS; s++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) { w.hi[s][j] = (_Float16)x[8 * s + j]; w.lo[s][j] = (_Float16)(x[8 * s + j] - (float)w.hi[s][j]); }
         } else {
 #pragma unroll
             for (int j = 0; j < NB * 4; j++) w.x[j] = x[j];
@@ -515,12 +560,23 @@ struct NarrowTile {
     }
     // Block e of V^T P^T on top of `out`
     __device__ __forceinline__ float4_t product(int e, const Weights& w, float4_t out) const {
-        if constexpr (HALF) {
+        if constexpr (Q8) {
+            // byte e % 4 of two positions' words as halves, without its sign (bit 7 the other way round), the halves 1024 + that
+            const unsigned pick = 0x0c000c04u + (unsigned)(e % 4) * 0x00010001u;
+#pragma unroll
+            for (int s = 0; s < WS; s++) {
+                uint4_t a;
+#pragma unroll
+                for (int j = 0; j < 4; j++) a[j] = signed_halves(__builtin_amdgcn_perm(v[8 * s + 2 * j][e / 4], v[8 * s + 2 * j + 1][e / 4], pick) ^ 0x64806480u);
+                out = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w.hi[s], out, 0, 0, 0);
+                out = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w.lo[s], out, 0, 0, 0);
+            }
+        } else if constexpr (HALF) {
             uint4_t a;
 #pragma unroll
             for (int j = 0; j < 4; j++) a[j] = __builtin_amdgcn_perm(v[2 * j + 1][e / 2], v[2 * j][e / 2], e & 1 ? 0x07060302u : 0x05040100u);
-            out = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w.hi, out, 0, 0, 0);
-            out = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w.lo, out, 0, 0, 0);
+            out = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w.hi[0], out, 0, 0, 0);
+            out = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, a), w.lo[0], out, 0, 0, 0);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; i++) {
@@ -538,7 +594,16 @@ struct NarrowTile {
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             S[b] = float4_t{0.f, 0.f, 0.f, 0.f};
-            if constexpr (HALF) {
+            if constexpr (Q8) {
+#pragma unroll
+                for (int i = 0; i < KV4; i++)
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+                        const half8_t a = eight_halves(k[b][i][2 * h], k[b][i][2 * h + 1]);
+                        S[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, qh[2 * i + h], S[b], 0, 0, 0);
+                        S[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, ql[2 * i + h], S[b], 0, 0, 0);
+                    }
+            } else if constexpr (HALF) {
 #pragma unroll
                 for (int i = 0; i < KV4; i++) {
                     S[b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8_t, k[b][i]), qh[i], S[b], 0, 0, 0);
@@ -551,7 +616,7 @@ struct NarrowTile {
                     for (int j = 0; j < 4; j++) S[b] = __builtin_amdgcn_mfma_f32_16x16x4f32(__builtin_bit_cast(float4_t, k[b][i])[j], qf[i][j], S[b], 0, 0, 0);
             }
         }
-        if constexpr (HALF) {
+        if constexpr (HALF && !Q8) {
             // Infinite keys: the second term's product with one may be an infinity of the other sign, or zero times it; the first
             // term's alone is what the formula gives.
             float sum = 0.f;
@@ -568,9 +633,13 @@ struct NarrowTile {
                 }
             }
         }
+        float x[NB * 4];
+        if constexpr (Q8) {
+#pragma unroll
+            for (int j = 0; j < NB * 4; j++) S[j / 4][j % 4] *= ks[j / 4][j % 4];
+        }
         if (more) load_k(u + 1, next);
         // scores in powers of two; the lane's positions are base + 16 b + 4 g + i
-        float x[NB * 4];
 #pragma unroll
         for (int j = 0; j < NB * 4; j++) x[j] = S[j / 4][j % 4] * c;
         if constexpr (MOD) {
@@ -586,7 +655,10 @@ struct NarrowTile {
                 const bool held = page_in(mine, b, g & 2) >= 0;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (!held || !paged_sees(row.pos, base + 16 * b + 4 * g + i, t.len, p.window, t.prefix)) x[4 * b + i] = -INFINITY;
+                    if (!held || !paged_sees(row.pos, base + 16 * b + 4 * g + i, t.len, p.window, t.prefix)) {
+                        x[4 * b + i] = -INFINITY;
+                        if constexpr (Q8) vs[b][i] = 0.f;       // (its scale may be anything)
+                    }
             }
         }
         float top = x[0];
@@ -594,6 +666,9 @@ struct NarrowTile {
         for (int j = 1; j < NB * 4; j++) top = fmaxf(top, x[j]);
         top = fmaxf(m, rows_max(top));
         const float from = top == -INFINITY ? 0.f : top;          // (a score that is a NaN stays one)
+        if constexpr (Q8) {
+            weigh_q8(x, top, from);
+        } else {
         if (__any(top > m)) {
             const float f = __builtin_amdgcn_exp2f(m - from);
             l *= f;
@@ -605,6 +680,7 @@ struct NarrowTile {
         for (int j = 0; j < NB * 4; j++) {
             x[j] = __builtin_amdgcn_exp2f(x[j] - from + SHIFT);
             l += x[j];
+        }
         }
         if (!inner) {
             bool some = false;
@@ -624,6 +700,47 @@ struct NarrowTile {
 #pragma unroll
         for (int e = 0; e < EPL; e++) o[e] = product(e, wt, o[e]);
     }
+    // Q8: scores to the weights of V's whole numbers, 2^(x - m) times the position's scale.  Both terms of a weight have to fit fp16 whatever
+    // the scales are, so a row's weights are held times a power of two, which puts the largest of a step at 2^12: anew
+    // where the row's maximum moves, and less where a weight passes 2^15 (rows' references: ref = m - that power's exponent).
+    __device__ __forceinline__ void weigh_q8(float (&x)[NB * 4], float top, float from) {
+        constexpr float FIT = 32768.f;
+        auto most_of = [&](auto f) {
+            float most = 0.f;
+#pragma unroll
+            for (int j = 0; j < NB * 4; j++) most = fmaxf(most, f(j));
+            return most;
+        };
+        auto exponent = [](float most) { return (float)(12 - __builtin_amdgcn_frexp_expf(fminf(most, FLT_MAX))); };
+        auto again = [&](float f) {
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < EPL; e++) o[e] *= f;
+        };
+        if (__any(top > m)) {
+            const float most = rows_max(most_of([&](int j) { return __builtin_amdgcn_exp2f(x[j] - from) * vs[j / 4][j % 4]; }));
+            const float to = top > m ? from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), 110.f)) : 0.f) : ref;
+            again(m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to));
+            ref = to;
+            m = top;
+        }
+#pragma unroll
+        for (int j = 0; j < NB * 4; j++) {
+            x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
+            l += x[j];
+            x[j] *= vs[j / 4][j % 4];
+        }
+        float most = most_of([&](int j) { return x[j]; });
+        if (__any(most > FIT)) {
+            most = rows_max(most);
+            const float down = most > FIT ? exponent(most) : 0.f;
+            const float f = __builtin_amdgcn_exp2f(down);
+            again(f);
+            ref -= down;
+#pragma unroll
+            for (int j = 0; j < NB * 4; j++) x[j] *= f;
+        }
+    }
     template <bool AGAIN>
     __device__ __forceinline__ void units(int u0, int u1, int pass) {
         for (int u = u0; u < u1; u++) {
@@ -637,6 +754,14 @@ struct NarrowTile {
     }
     __device__ __forceinline__ void run(int u0, int u1, int kvh, int, float* lds) {
         units<false>(u0, u1, 0);
+        if constexpr (Q8) {
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - m);
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < EPL; e++) o[e] *= f;
+            join(kvh, lds);
+            return;
+        }
         float odd = 0.f;
 #pragma unroll
         for (int e = 0; e < EPL; e++)
@@ -1230,7 +1355,12 @@ static size_t attn_lds(int headDim, bool wide) {
 template <typename F>
 static hipError_t with_kernel(const PagedGeo& g, bool mod, bool wide, F f) {
 #define PAGED_PICK(KVT, HD, MOD) (wide ? f(paged_wide_kernel<KVT, HD, MOD>) : f(paged_narrow_kernel<KVT, HD, MOD>))
-    if (g.kvHalf) {
+    if (g.kvFormat == PAGED_Q8) {
+        if (wide) return hipErrorInvalidValue;
+        if (g.headDim == 64) return mod ? f(paged_narrow_kernel<signed char, 64, true>) : f(paged_narrow_kernel<signed char, 64, false>);
+        return mod ? f(paged_narrow_kernel<signed char, 128, true>) : f(paged_narrow_kernel<signed char, 128, false>);
+    }
+    if (g.kvFormat == PAGED_F16) {
         if (g.headDim == 64) return mod ? PAGED_PICK(_Float16, 64, true) : PAGED_PICK(_Float16, 64, false);
         return mod ? PAGED_PICK(_Float16, 128, true) : PAGED_PICK(_Float16, 128, false);
     }
@@ -1239,7 +1369,7 @@ static hipError_t with_kernel(const PagedGeo& g, bool mod, bool wide, F f) {
 #undef PAGED_PICK
 }
 hipError_t paged_attention_setup(const PagedGeo& g) {
-    for (int i = 0; i < 4; i++) {
+    for (int i = 0; i < (g.kvFormat == PAGED_Q8 ? 2 : 4); i++) {
         hipError_t e = with_kernel(g, i & 1, i >> 1, [&](auto* k) {
             return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)attn_lds(g.headDim, i >> 1));
         });

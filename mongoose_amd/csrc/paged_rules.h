@@ -16,8 +16,13 @@ namespace mg {
 // fp32; a page holds whole runs of eight positions, the finest run that the attention looks up a page for.
 constexpr int PAGED_MAX_REQS = 4096, PAGED_MAX_LEN = 1 << 24, PAGED_MAX_ROWS = 1 << 20, PAGED_MIN_PAGE = 8, PAGED_MAX_PAGE = 4096, PAGED_MAX_GROUP = 128;
 
+// Formats of a cache: fp32, fp16, or Q8 -- an int8 an element and an fp32 scale a KV head's row (the row's greatest size / 127).  A Q8
+// pool holds its int8 rows [slots, kvDim], then the scales [pages, KV heads, pageSize]: those of a KV head's positions lie side by side,
+// as the attention reads them.
+enum { PAGED_F32 = 0, PAGED_F16 = 1, PAGED_Q8 = 8 };
+
 struct PagedGeo {
-    int nHeads, nKVHeads, headDim, pageSize, nPages, kvHalf, maxReqs, maxRows, maxLen;
+    int nHeads, nKVHeads, headDim, pageSize, nPages, kvFormat, maxReqs, maxRows, maxLen;
     int group;        // query heads a KV head
     int kvDim;        // elements of a position's K (or V) row
     int pageShift;    // log2(pageSize)
@@ -32,13 +37,13 @@ inline const char* paged_geo(PagedGeo& g, int nHeads, int nKVHeads, int headDim,
     if (nHeads / nKVHeads > PAGED_MAX_GROUP || nHeads > 65536) return "at most 128 query heads a KV head and 65536 in all";
     if (pageSize < PAGED_MIN_PAGE || pageSize > PAGED_MAX_PAGE || (pageSize & (pageSize - 1))) return "pageSize must be a power of two from 8 to 4096";
     if (nPages <= 0 || (long long)nPages * pageSize > 0x7fffffffll) return "nPages must be positive and nPages * pageSize below 2^31";
-    if (kvFormat != 0 && kvFormat != 1) return "kvFormat must be 0 (fp32) or 1 (fp16)";
+    if (kvFormat != PAGED_F32 && kvFormat != PAGED_F16 && kvFormat != PAGED_Q8) return "kvFormat must be 0 (fp32), 1 (fp16) or 8 (Q8)";
     if (maxReqs <= 0 || maxReqs > PAGED_MAX_REQS) return "maxReqs must be between 1 and 4096";
     if (maxRows <= 0 || maxRows > PAGED_MAX_ROWS) return "maxRows must be between 1 and 2^20";
     if (maxLen <= 0 || maxLen > PAGED_MAX_LEN) return "maxLen must be between 1 and 2^24";
     if ((long long)maxRows * (nHeads / nKVHeads) > (1ll << 40) / maxLen) return "maxRows * (nHeads / nKVHeads) * maxLen must be at most 2^40";
     if ((long long)maxReqs * maxLen > (1ll << 34)) return "maxReqs * maxLen must be at most 2^34";
-    g.nHeads = nHeads; g.nKVHeads = nKVHeads; g.headDim = headDim; g.pageSize = pageSize; g.nPages = nPages; g.kvHalf = kvFormat;
+    g.nHeads = nHeads; g.nKVHeads = nKVHeads; g.headDim = headDim; g.pageSize = pageSize; g.nPages = nPages; g.kvFormat = kvFormat;
     g.maxReqs = maxReqs; g.maxRows = maxRows; g.maxLen = maxLen;
     g.group = nHeads / nKVHeads;
     g.kvDim = nKVHeads * headDim;
@@ -116,7 +121,11 @@ inline bool paged_pool_meets(const void* p, size_t bytes, const void* a, int ld,
     const uintptr_t x = (uintptr_t)p, y = (uintptr_t)a;
     return rows > 0 && x < y + ((size_t)(rows - 1) * ld + width) * 4 && y < x + bytes;
 }
-inline size_t paged_pool_bytes(const PagedGeo& g) { return (size_t)g.nPages * g.pageSize * g.kvDim * (g.kvHalf ? 2 : 4); }
+inline size_t paged_element_bytes(int kvFormat) { return kvFormat == PAGED_F32 ? 4 : kvFormat == PAGED_F16 ? 2 : 1; }
+inline size_t paged_pool_bytes(const PagedGeo& g) {
+    const size_t slots = (size_t)g.nPages * g.pageSize;
+    return slots * g.kvDim * paged_element_bytes(g.kvFormat) + (g.kvFormat == PAGED_Q8 ? slots * g.nKVHeads * 4 : 0);
+}
 // What a call writes while others of its workgroups still read it: nullptr, or which of its arguments overlap (those that
 // paged_store_refusal has passed).
 inline const char* paged_store_overlap(const PagedGeo& g, const void* q, const void* k, const void* v, int ldq, int ldk, int ldv,
@@ -131,6 +140,30 @@ inline const char* paged_store_overlap(const PagedGeo& g, const void* q, const v
     for (const void* p : pools)
         if (paged_pool_meets(p, bytes, q, ldq, qw, rows) || paged_pool_meets(p, bytes, k, ldk, g.kvDim, rows) ||
             paged_pool_meets(p, bytes, v, ldv, g.kvDim, rows) || paged_pool_meets(p, bytes, qOut, ldqOut, qw, rows)) return "K or V overlaps the rows";
+    return nullptr;
+}
+inline const char* paged_load_refusal(const PagedGeo& g, const void* K, const void* V, const void* table, const void* rowStart, const void* lens,
+                                      int nReqs, int rows, const void* kOut, int ldk, const void* vOut, int ldv) {
+    if (nReqs < 0 || nReqs > g.maxReqs) return "nReqs is negative or above the handle's maxReqs";
+    if (rows < 0) return "rows is negative";
+    if (nReqs == 0 || rows == 0) return nullptr;
+    const void* wide[] = {K, V, kOut, vOut};
+    for (const void* p : wide) if (!paged_aligned(p, 16)) return "a pointer is NULL or not aligned to 16 bytes";
+    const void* ints[] = {table, rowStart, lens};
+    for (const void* p : ints) if (!paged_aligned(p, 4)) return "a pointer is NULL or not aligned to 4 bytes";
+    if (ldk < g.kvDim || ldv < g.kvDim) return "a row stride is smaller than the row";
+    if ((ldk | ldv) & 3) return "a row stride is not a multiple of 4";
+    return nullptr;
+}
+// What mg_paged_load writes while others of its workgroups still read
+inline const char* paged_load_overlap(const PagedGeo& g, const void* K, const void* V, const void* table, const void* rowStart, const void* lens, int nReqs,
+                                      int rows, const void* kOut, int ldk, const void* vOut, int ldv) {
+    if (nReqs == 0 || rows == 0) return nullptr;
+    if (paged_rows_meet(kOut, ldk, g.kvDim, vOut, ldv, g.kvDim, rows)) return "kOut overlaps vOut";
+    const size_t bytes = paged_pool_bytes(g);
+    const struct { const void* p; size_t n; } in[] = {{K, bytes}, {V, bytes}, {table, (size_t)nReqs * g.width * 4}, {rowStart, ((size_t)nReqs + 1) * 4}, {lens, (size_t)nReqs * 4}};
+    for (auto& a : in)
+        if (paged_pool_meets(a.p, a.n, kOut, ldk, g.kvDim, rows) || paged_pool_meets(a.p, a.n, vOut, ldv, g.kvDim, rows)) return "kOut or vOut overlaps what is read";
     return nullptr;
 }
 inline const char* paged_plan_refusal(const PagedGeo& g, const void* rowStart, const void* lens, int nReqs, int rows, int window,

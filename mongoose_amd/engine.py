@@ -761,7 +761,7 @@ def KQ8Gemm(act, w, scales, bias, out, T, N, K, accumulate, workspace, workspace
 
 class HIPPaged:
     """Several requests out of one KV cache in pages (mg_paged_*): block tables and slot maps from the requests' lengths, rotary
-    positions with the K/V rows stored by slot, attention of the requests' new tokens over their pages.  No counterpart in the
+    positions with the K/V rows stored by slot, attention of the requests' new tokens over their pages, rows read back.  No counterpart in the
     reference.  Arguments are device buffers (Tensor, or an address); every method returns 0 or a negative code (last_error).
     A Tensor that has been released is a ctypes.ArgumentError."""
 
@@ -783,6 +783,10 @@ class HIPPaged:
         """Entries of a request's row of the block table."""
         return lib.mg_paged_table_width(self._h)
 
+    def PoolBytes(self):
+        """Bytes of a layer's K (or V) pool."""
+        return lib.mg_paged_pool_bytes(self._h)
+
     def Tables(self, newLens, nReqs, lens, lensOut, table, ring, ringState, ringStateOut, rows, rowStart, slots, positions, counts,
                stream=None):
         return _paged_tables(self._h, newLens, nReqs, lens, lensOut, table, ring, ringState, ringStateOut, rows, rowStart, slots, positions,
@@ -790,6 +794,9 @@ class HIPPaged:
 
     def Store(self, q, k, v, ldq, ldk, ldv, qOut, ldqOut, K, V, slots, positions, rows, cosTab, sinTab, tableRows, stream=None):
         return _paged_store(self._h, q, k, v, ldq, ldk, ldv, qOut, ldqOut, K, V, slots, positions, rows, cosTab, sinTab, tableRows, stream)
+
+    def Load(self, K, V, table, rowStart, lens, nReqs, rows, kOut, ldk, vOut, ldv, stream=None):
+        return _paged_load(self._h, K, V, table, rowStart, lens, nReqs, rows, kOut, ldk, vOut, ldv, stream)
 
     def Plan(self, rowStart, lens, nReqs, rows, window=0, prefixLens=None, stream=None):
         return _paged_plan(self._h, rowStart, lens, nReqs, rows, window, prefixLens, stream)
@@ -799,7 +806,8 @@ class HIPPaged:
 
 
 # (a server makes these calls for every layer of every step: the functions are looked up once)
-_paged_tables, _paged_store, _paged_plan, _paged_attention = lib.mg_paged_tables, lib.mg_paged_store, lib.mg_paged_plan, lib.mg_paged_attention
+_paged_tables, _paged_store, _paged_load, _paged_plan, _paged_attention = (
+    lib.mg_paged_tables, lib.mg_paged_store, lib.mg_paged_load, lib.mg_paged_plan, lib.mg_paged_attention)
 
 
 def NewHIPPaged(eng, nHeads, nKVHeads, headDim, pageSize, nPages, kvFormat, maxReqs, maxRows, maxLen):

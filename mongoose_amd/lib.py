@@ -142,6 +142,8 @@ _sig("mg_paged_destroy", None, c_void_p)
 _sig("mg_paged_table_width", c_int, c_void_p)
 _sig("mg_paged_tables", c_int, c_void_p, _p, c_int, _p, _p, _p, _p, _p, _p, c_int, _p, _p, _p, _p, _p)
 _sig("mg_paged_store", c_int, c_void_p, _p, _p, _p, c_int, c_int, c_int, _p, c_int, _p, _p, _p, _p, c_int, _p, _p, c_int, _p)
+_sig("mg_paged_pool_bytes", c_size_t, c_void_p)
+_sig("mg_paged_load", c_int, c_void_p, _p, _p, _p, _p, _p, c_int, c_int, _p, c_int, _p, c_int, _p)
 _sig("mg_paged_plan", c_int, c_void_p, _p, _p, c_int, c_int, c_int, _p, _p)
 _sig("mg_paged_attention", c_int, c_void_p, _p, c_int, _p, _p, _p, _p, c_int, c_float, c_float, _p, _p)
 
