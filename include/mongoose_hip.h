@@ -546,10 +546,23 @@ int mg_paged_load(mg_paged* h, const void* K, const void* V, const int* table, c
  * positions of request r's lens[r] (after this step).  The arrays are copied (clamped to `rows` and maxLen).  Which positions j a
  * token at position i sees: j <= i, and where window > 0 only j > i - window; with prefixLens also every j < prefixLens[r],
  * before or behind i and whatever the window.
- * An attention call goes by the nReqs, rows and window of the last mg_paged_plan call, captured or not, before it, and by the lengths of the
+ * An attention call goes by the nReqs, rows and window of the last mg_paged_plan (or mg_paged_plan_shared) call, captured or not, before it, and by the lengths of the
  * plan that ran last on the device.  Where that one was for other nReqs, rows or window -- a graph's replay came between, or the call was
  * captured and has not run yet -- it does nothing and leaves out as it was. */
 int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int window, const int* prefixLens, void* stream);
+
+/* Requests that share their first positions: groupStart[g] .. groupStart[g+1]-1 are requests whose tables name the same pages for the
+ * positions below sharedLens[g] (from the first one's on: the last page that is shared may differ behind them, and the pages of
+ * the first request with rows are the ones that are read).  mg_paged_plan_shared takes the lengths as mg_paged_plan does, without a window or
+ * a prefix; the attention calls that follow compute what they would without it -- to rounding --, a group's shared positions once for all
+ * its rows.  A shared length is cut to the positions that all of its requests with rows have ahead of their new ones; requests
+ * of no group, and groups of one request with rows, share nothing.  mostNew: the most rows that a request of the step has, if the caller knows (0: any
+ * number; more of them than said cost time, not results).  nGroups <= maxReqs; all arrays are device memory and are copied.
+ * mg_paged_share allocates the workspace for it, once, before the first such plan: about maxRows * nHeads * (headDim + 2) floats
+ * (MG_E_STATE without it).  Of attention's rule on plans, nGroups is a part. */
+int mg_paged_share(mg_paged* h);
+int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int mostNew, const int* groupStart,
+                         const int* sharedLens, int nGroups, void* stream);
 
 /* out[row, head] = sum_j softmax_j(s_j) v_j over the positions that the row sees, of KV head `head / (nHeads / nKVHeads)`:
  * s_j = scale * q.k_j (scale 0: 1 / sqrt(headDim)); with softcap > 0 then softcap * tanh(s_j / softcap); with slopes [nHeads]

@@ -38,19 +38,31 @@ static_assert(sizeof(PagedTile) == 64 && sizeof(PagedWorker) == 128, "read as 16
 // What a plan was made for.  The places and numbers of its tiles and workers follow from these: an attention call works on the plan that is
 // in the handle's memory only where they are its own (a graph's replay may have left another one there, or it was captured and has not run).
 struct PagedPlanFor {
-    int nReqs, rows, window, pad;
-    MG_HD bool is(const PagedPlanFor& o) const { return ((nReqs ^ o.nReqs) | (rows ^ o.rows) | (window ^ o.window)) == 0; }      // (no branch between the loads)
+    int nReqs, rows, window, groups;
+    MG_HD bool is(const PagedPlanFor& o) const { return ((nReqs ^ o.nReqs) | (rows ^ o.rows) | (window ^ o.window) | (groups ^ o.groups)) == 0; }      // (no branch between the loads)
 };
 
 // The plan that a step's attention calls share.
 struct PagedPlan {
     const int *rowStart, *lens, *prefixLens;      // the caller's
+    const int4* given;                            // or, with shared prefixes, what paged_groups_kernel has made of them
+    bool grouped;                                 // `given` are groups
     PagedPlanFor* made;                           // the handle's
     PagedTile* tiles;                             // maxTiles of them, for narrow tiles and again for wide ones,
     PagedWorker* workers;                         // and maxWorkers of these
     int nReqs, rows, window, maxLen, group, kvFormat, maxTiles, maxWorkers, nWorkers, wideWorkers, narrowRows;      // wideWorkers 0: no wide tiles
+    PagedPlanFor plan;
 };
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s);
+
+// Groups of requests with the same first positions: what the two plans (the groups' shared positions, and every request's own) go by.
+struct PagedGroups {
+    const int *rowStart, *lens, *groupStart, *sharedLens;      // the caller's
+    int4* reqs;          // of every request: first row, rows, length, first position of its own
+    int4* groups;        // of every group: first row, rows, shared positions, the request whose pages are read
+    int nReqs, rows, nGroups, maxLen;
+};
+hipError_t launch_paged_plan_shared(const PagedGroups& g, const PagedPlan& shared, const PagedPlan& own, hipStream_t s);
 
 struct PagedAttention {
     const float *q, *slopes;
@@ -66,12 +78,19 @@ struct PagedAttention {
     size_t partStride;
     float scale, softcap;
     PagedPlanFor plan;
+    // Shared prefixes: a call's first pass leaves each row's result over its group's positions here, [row, head][headDim] with the rows' maxima
+    // and sums behind, and its second one, over the requests' own positions, takes it in.
+    float* shared;
+    const int4* reqs;
+    int pass;                  // 0: no prefix is shared; 1, 2
     int ldq, ldo, window, maxTiles, maxWorkers, nWorkers, wideWorkers;
     PagedGeo g;
 };
 size_t paged_part_floats(const PagedGeo& g);
 int paged_max_tiles(const PagedGeo& g);
+int paged_max_tiles_shared(const PagedGeo& g);
 int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide);       // workers a KV head
+int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool groups);
 int paged_narrow_rows(const PagedGeo& g, int rows);              // requests of up to so many rows a KV head have narrow tiles
 hipError_t paged_attention_setup(const PagedGeo& g);
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t s);

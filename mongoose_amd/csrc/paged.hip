@@ -371,6 +371,14 @@ struct mg_paged {
     int maxTiles, maxWorkers;
     mg::PagedPlanFor plan;                     // the last plan asked for (nReqs < 0: none yet)
     int planWorkers, planWideWorkers;
+    // mg_paged_share: another allocation, for plans of groups (0) and of their requests (1)
+    char* sharedMem;
+    int4 *reqs, *groups;
+    mg::PagedTile* sharedTiles[2];
+    mg::PagedWorker* sharedWorkers[2];
+    unsigned* sharedArrived;
+    float* sharedRows;
+    int sharedMaxTiles, sharedPlanWorkers[2], sharedPlanWide[2];
 };
 
 namespace {
@@ -442,6 +450,7 @@ void mg_paged_destroy(mg_paged* h) {
     {
         mg::OnDevice guard(h->device);
         if (h->mem) (void)hipFree(h->mem);
+        if (h->sharedMem) (void)hipFree(h->sharedMem);
     }
     delete h;
 }
@@ -484,10 +493,68 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
     window = mg::paged_window(window, g.maxLen);
     const int workers = mg::paged_workers(g, nReqs, rows, false), narrow = mg::paged_narrow_rows(g, rows);
     const int wide = (long long)rows * g.group > narrow ? mg::paged_workers(g, nReqs, rows, true) : 0;
-    mg::PagedPlan p{rowStart, lens, prefixLens, h->made, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvFormat, h->maxTiles, h->maxWorkers, workers, wide, narrow};
+    mg::PagedPlan p{rowStart, lens, prefixLens, nullptr, false, h->made, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvFormat, h->maxTiles, h->maxWorkers, workers, wide, narrow,
+                    {nReqs, rows, window, 0}};
     const int rc = launched("mg_paged_plan", mg::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
     if (rc == MG_OK) {
-        h->plan = {nReqs, rows, window, 0}; h->planWorkers = workers; h->planWideWorkers = wide;
+        h->plan = p.plan; h->planWorkers = workers; h->planWideWorkers = wide;
+    }
+    return rc;
+}
+int mg_paged_share(mg_paged* h) {
+    PAGED(h, "mg_paged_share");
+    if (h->sharedMem) return MG_OK;
+    const mg::PagedGeo& g = h->g;
+    const size_t tiles = (size_t)mg::paged_max_tiles_shared(g), rows = (size_t)g.maxRows * g.nHeads;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
+    const size_t oArrived = take(tiles * g.nKVHeads * 4), clear = at, oReqs = take((size_t)g.maxReqs * sizeof(int4)), oGroups = take((size_t)g.maxReqs * sizeof(int4));
+    size_t oTiles[2], oWorkers[2];
+    for (int i = 0; i < 2; i++) { oTiles[i] = take(2 * tiles * sizeof(mg::PagedTile)); oWorkers[i] = take(2 * (size_t)h->maxWorkers * sizeof(mg::PagedWorker)); }
+    const size_t oRows = take(rows * (g.headDim + 2) * 4);
+    char* mem = nullptr;
+    hipError_t e = hipMalloc(reinterpret_cast<void**>(&mem), at);
+    if (e == hipSuccess) {
+        e = mg::launch_fill_zero(mem, clear, nullptr);
+        if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
+        if (e != hipSuccess) (void)hipFree(mem);
+    }
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        mg::set_error("mg_paged_share: " + std::to_string(at) + " bytes of workspace: " + hipGetErrorString(e));
+        return MG_E_HIP;
+    }
+    h->sharedMem = mem;
+    h->sharedMaxTiles = (int)tiles;
+    h->sharedArrived = reinterpret_cast<unsigned*>(mem + oArrived);
+    h->reqs = reinterpret_cast<int4*>(mem + oReqs);
+    h->groups = reinterpret_cast<int4*>(mem + oGroups);
+    for (int i = 0; i < 2; i++) {
+        h->sharedTiles[i] = reinterpret_cast<mg::PagedTile*>(mem + oTiles[i]);
+        h->sharedWorkers[i] = reinterpret_cast<mg::PagedWorker*>(mem + oWorkers[i]);
+    }
+    h->sharedRows = reinterpret_cast<float*>(mem + oRows);
+    return MG_OK;
+}
+int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int mostNew, const int* groupStart, const int* sharedLens,
+                         int nGroups, void* stream) {
+    PAGED(h, "mg_paged_plan_shared");
+    if (!h->sharedMem) { mg::set_error("mg_paged_plan_shared: no workspace for shared prefixes (mg_paged_share)"); return MG_E_STATE; }
+    const mg::PagedGeo& g = h->g;
+    if (const char* why = mg::paged_plan_shared_refusal(g, rowStart, lens, nReqs, rows, mostNew, groupStart, sharedLens, nGroups)) return refuse("mg_paged_plan_shared", why);
+    if (nGroups == 0) return mg_paged_plan(h, rowStart, lens, nReqs, rows, 0, nullptr, stream);
+    const mg::PagedPlanFor made{nReqs, rows, 0, nGroups};
+    mg::PagedPlan p[2];
+    for (int i = 0; i < 2; i++) {
+        const int n = i ? nReqs : nGroups, narrow = mg::paged_narrow_rows_shared(g, rows, i ? mostNew : 0, i == 0);
+        p[i] = {nullptr, nullptr, nullptr, i ? h->reqs : h->groups, i == 0, h->made, h->sharedTiles[i], h->sharedWorkers[i], n, rows, 0, g.maxLen, g.group, g.kvFormat,
+                h->sharedMaxTiles, h->maxWorkers, mg::paged_workers(g, n, rows, false), (long long)rows * g.group > narrow ? mg::paged_workers(g, n, rows, true) : 0, narrow, made};
+    }
+    const int rc = launched("mg_paged_plan_shared", mg::launch_paged_plan_shared({rowStart, lens, groupStart, sharedLens, h->reqs, h->groups, nReqs, rows, nGroups, g.maxLen}, p[0], p[1],
+                                                                                 static_cast<hipStream_t>(stream)));
+    if (rc == MG_OK) {
+        h->plan = made;
+        for (int i = 0; i < 2; i++) { h->sharedPlanWorkers[i] = p[i].narrowRows > 0 ? p[i].nWorkers : 0; h->sharedPlanWide[i] = p[i].wideWorkers; }
     }
     return rc;
 }
@@ -500,8 +567,20 @@ int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, cons
     if (const char* why = mg::paged_attention_overlap(h->g, q, ldq, K, V, out, ldo, h->plan.rows)) return refuse("mg_paged_attention", why);
     const mg::PagedGeo& g = h->g;
     mg::PagedAttention p{q, slopes, K, V, table, out, h->made, h->tiles, h->workers, h->parts, h->arrived, h->zeros, mg::paged_part_floats(g),
-                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, h->plan, ldq, ldo, h->plan.window, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
-    return launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
+                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, h->plan, h->sharedRows, h->reqs, 0, ldq, ldo, h->plan.window, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
+    if (h->plan.groups == 0) return launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
+    p.arrived = h->sharedArrived;
+    p.maxTiles = h->sharedMaxTiles;
+    for (int i = 0; i < 2; i++) {
+        p.pass = i + 1;
+        p.tiles = h->sharedTiles[i];
+        p.workers = h->sharedWorkers[i];
+        p.nWorkers = h->sharedPlanWorkers[i];
+        p.wideWorkers = h->sharedPlanWide[i];
+        const int rc = launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
+        if (rc != MG_OK) return rc;
+    }
+    return MG_OK;
 }
 
 }  // extern "C"

@@ -52,6 +52,16 @@ int paged_narrow_rows(const PagedGeo& g, int rows) {
     if (g.kvFormat == PAGED_Q8) return PAGED_MAX_ROWS * PAGED_MAX_GROUP;
     return (long long)rows * g.group <= 256 ? 256 : NARROW;
 }
+// The same with shared prefixes, for groups (0: all groups have wide tiles) and for requests, of which the caller may know that none adds more than
+// mostNew rows.
+int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool groups) {
+    constexpr int ALL = PAGED_MAX_ROWS * PAGED_MAX_GROUP;
+    if (g.kvFormat == PAGED_Q8 || (long long)rows * g.group <= 256) return ALL;
+    if (groups) return 0;
+    return mostNew > 0 && (long long)mostNew * g.group <= NARROW ? ALL : NARROW;
+}
+// (with shared prefixes requests of any number of rows may have narrow tiles)
+int paged_max_tiles_shared(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / NARROW) + g.maxReqs; }
 int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / (g.kvFormat == PAGED_Q8 ? NARROW : WIDE)) + g.maxReqs + 256 / NARROW; }
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
 // Workgroups, in turns of the KV heads: two a CU for wide tiles; one a CU for narrow ones, though a CU holds two: HBM likes fewer
@@ -87,17 +97,23 @@ __device__ __forceinline__ unsigned plan_scan(unsigned v, unsigned& carry, unsig
     return sat_add(mine, v);
 }
 // A request as the plan takes it: rows inside the call's, a length inside the handle's.
+__device__ __forceinline__ int4 plan_request(const int* rowStart, const int* lens, int rows, int maxLen, int r) {
+    const int first = max(0, min(rowStart[r], rows)), last = max(first, min(rowStart[r + 1], rows));
+    return make_int4(first, last - first, max(0, min(lens[r], maxLen)), 0);
+}
+// Its first row, rows, length, and its prefix, or what `given` has there.
 __device__ __forceinline__ int4 plan_request(const PagedPlan& p, int r) {
-    const int first = max(0, min(p.rowStart[r], p.rows)), last = max(first, min(p.rowStart[r + 1], p.rows));
-    const int len = max(0, min(p.lens[r], p.maxLen));
-    return make_int4(first, last - first, len, p.prefixLens ? max(0, min(p.prefixLens[r], len)) : 0);
+    if (p.given) return p.given[r];
+    int4 rq = plan_request(p.rowStart, p.lens, p.rows, p.maxLen, r);
+    if (p.prefixLens) rq.w = max(0, min(p.prefixLens[r], rq.z));
+    return rq;
 }
 __device__ __forceinline__ void put_tile(PagedTile* at, const PagedTile& t) {
     int4* d = reinterpret_cast<int4*>(at);
     d[0] = make_int4(t.req, t.row0, t.rows, t.len);
     d[1] = make_int4(t.prefix, t.first, t.cost0, t.unit0);
     d[2] = make_int4(t.units, t.worker0, t.worker1, t.index);
-    d[3] = make_int4(t.tileRows, t.unitKeys, 0, 0);
+    d[3] = make_int4(t.tileRows, t.unitKeys, t.from, 0);
 }
 // Largest i with sums[i] <= x, of n sums
 __device__ __forceinline__ int plan_find(const unsigned* sums, int n, unsigned x) {
@@ -109,13 +125,12 @@ __device__ __forceinline__ int plan_find(const unsigned* sums, int n, unsigned x
     return lo;
 }
 // One workgroup for the narrow tiles and one for the wide ones
-__global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
-    const bool wide = blockIdx.x != 0;
+__device__ __forceinline__ void make_plan(PagedPlan p, bool wide) {
     const int tileRows = wide ? WIDE : NARROW, unitKeys = wide ? wide_keys(p.kvFormat) : narrow_keys(p.kvFormat);
     p.tiles += wide ? p.maxTiles : 0;
     p.workers += wide ? p.maxWorkers : 0;
     p.nWorkers = wide ? p.wideWorkers : p.nWorkers;
-    if (threadIdx.x == 0 && !wide) *p.made = {p.nReqs, p.rows, p.window, 0};
+    if (threadIdx.x == 0 && !wide && !p.grouped) *p.made = p.plan;
     __shared__ unsigned tile0[PAGED_MAX_REQS + 1], place[PLAN_LDS_TILES], part[PT / 64];
     __shared__ int4 held[PT];
     const int tid = threadIdx.x;
@@ -140,7 +155,9 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
     auto make = [&](int i) {
         const int r = plan_find(tile0, p.nReqs, (unsigned)i);
         const int4 rq = r < PT ? held[r] : plan_request(p, r);
-        t.req = r; t.row0 = rq.x; t.rows = rq.y; t.len = rq.z; t.prefix = rq.w;
+        t.req = r; t.row0 = rq.x; t.rows = rq.y; t.len = rq.z; t.prefix = rq.w; t.from = 0;
+        if (p.given) { t.prefix = 0; t.from = rq.w; }
+        if (p.grouped) { t.req = rq.w; t.prefix = rq.z; t.from = 0; }        // (all rows see all of it)
         t.tileRows = tileRows; t.unitKeys = unitKeys;
         t.first = (i - (int)tile0[r]) * tileRows;
         t.index = i;
@@ -215,8 +232,63 @@ __global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) {
         d[4] = range;
     }
 }
+__global__ __launch_bounds__(PT) void paged_plan_kernel(PagedPlan p) { make_plan(p, blockIdx.x != 0); }
 hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s) {
     hipLaunchKernelGGL(paged_plan_kernel, dim3(p.wideWorkers > 0 ? 2 : 1), dim3(PT), 0, s, p);
+    return hipGetLastError();
+}
+
+// With shared prefixes a step has two plans: one of the groups -- a group's rows are those of one request of the shared length, all of which
+// they all see -- and one of the requests, each from the group's shared length on.  This kernel cuts the shared lengths to what
+// every request with rows in the group has ahead of its first new token, so that no row's mask reaches into them; a group with one such request shares
+// nothing.  One workgroup, a thread a request.
+__global__ __launch_bounds__(PT) void paged_groups_kernel(PagedGroups p) {
+    __shared__ int least[PAGED_MAX_REQS], first[PAGED_MAX_REQS], count[PAGED_MAX_REQS];
+    for (int g = threadIdx.x; g < p.nGroups; g += PT) { least[g] = p.maxLen; first[g] = p.nReqs; count[g] = 0; }
+    __syncthreads();
+    auto group_of = [&](int r) {          // -1: none
+        int lo = 0, hi = p.nGroups;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.groupStart[mid] <= r) lo = mid; else hi = mid;
+        }
+        return p.groupStart[lo] <= r && r < p.groupStart[lo + 1] ? lo : -1;
+    };
+    for (int r = threadIdx.x; r < p.nReqs; r += PT) {
+        const int4 rq = plan_request(p.rowStart, p.lens, p.rows, p.maxLen, r);
+        const int g = rq.y > 0 ? group_of(r) : -1;
+        if (g < 0) continue;
+        atomicMin(&least[g], rq.z - rq.y);
+        atomicMin(&first[g], r);
+        atomicAdd(&count[g], 1);
+    }
+    __syncthreads();
+    for (int g = threadIdx.x; g < p.nGroups; g += PT) {
+        const int len = count[g] > 1 ? max(0, min(p.sharedLens[g], least[g])) : 0;
+        least[g] = len;
+        int4 at = make_int4(0, 0, 0, 0);
+        if (len > 0) {
+            const int a = max(0, min(p.groupStart[g], p.nReqs)), b = max(a, min(p.groupStart[g + 1], p.nReqs));
+            const int row0 = max(0, min(p.rowStart[a], p.rows)), row1 = max(row0, min(p.rowStart[b], p.rows));
+            at = make_int4(row0, row1 - row0, len, first[g]);
+        }
+        p.groups[g] = at;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < p.nReqs; r += PT) {
+        int4 rq = plan_request(p.rowStart, p.lens, p.rows, p.maxLen, r);
+        const int g = rq.y > 0 ? group_of(r) : -1;
+        rq.w = g < 0 ? 0 : least[g];
+        p.reqs[r] = rq;
+    }
+}
+__global__ __launch_bounds__(PT) void paged_plan_shared_kernel(PagedPlan shared, PagedPlan own) {
+    if (blockIdx.x >> 1) { if (shared.wideWorkers > 0 || !(blockIdx.x & 1)) make_plan(shared, blockIdx.x & 1); }
+    else if (own.wideWorkers > 0 || !(blockIdx.x & 1)) make_plan(own, blockIdx.x & 1);
+}
+hipError_t launch_paged_plan_shared(const PagedGroups& g, const PagedPlan& shared, const PagedPlan& own, hipStream_t s) {
+    hipLaunchKernelGGL(paged_groups_kernel, dim3(1), dim3(PT), 0, s, g);
+    hipLaunchKernelGGL(paged_plan_shared_kernel, dim3(4), dim3(PT), 0, s, shared, own);
     return hipGetLastError();
 }
 
@@ -345,6 +417,36 @@ __device__ __forceinline__ void merge_weights(const PagedAttention& p, const Pag
     }
 }
 __device__ __forceinline__ float4_t over(float4_t v, float l) { return l == 0.f ? v : v / l; }       // (nothing seen: zeros)
+// Four elements from d on of a row's result: v, with sum l over the reference m (the greatest score where SHIFT is 0).  Where the positions are
+// a shared prefix they are kept as they are for the requests' own pass, which joins the two.
+__device__ __forceinline__ void put_result(const PagedAttention& p, const PagedTile& t, const PagedRow& at, int d, float4_t v, float l, float m) {
+    const size_t row = (size_t)(t.row0 + at.token), i = row * p.g.nHeads + at.head;
+    const size_t all = (size_t)p.plan.rows * p.g.nHeads;
+    float* rows = p.shared;
+    float* ml = p.shared + all * p.g.headDim;
+    if (p.pass == 1) {
+        *reinterpret_cast<float4_t*>(rows + i * p.g.headDim + d) = v;
+        if (d == 0) { ml[i] = l == 0.f ? -INFINITY : m; ml[all + i] = l; }
+        return;
+    }
+    if (p.pass == 2 && t.from > 0) {
+        const float ms = ml[i], ls = ml[all + i], mine = l == 0.f ? -INFINITY : m, M = fmaxf(mine, ms), to = M == -INFINITY ? 0.f : M;
+        const float a = __builtin_amdgcn_exp2f(mine - to), b = __builtin_amdgcn_exp2f(ms - to);
+        v = v * a + *reinterpret_cast<const float4_t*>(rows + i * p.g.headDim + d) * b;
+        l = fmaf(l, a, ls * b);
+    }
+    *reinterpret_cast<float4_t*>(p.out + row * p.ldo + (size_t)at.head * p.g.headDim + d) = over(v, l);
+}
+// The position of a row of a group: of the request that it is a row of
+__device__ __forceinline__ int shared_pos(const PagedAttention& p, int row) {
+    int lo = 0, hi = p.plan.nReqs;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (p.reqs[mid].x <= row) lo = mid; else hi = mid;
+    }
+    const int4 rq = p.reqs[lo];
+    return rq.z - rq.y + row - rq.x;
+}
 
 // Values that are no numbers.  Zero times one is no zero, so that one reaches rows that do not see it, and its product with the second
 // term of a weight turns an infinity into a NaN.  A tile whose result has elements that are no numbers therefore goes through its
@@ -431,8 +533,9 @@ struct NarrowTile {
         const int tid = thread_anew();
         lane = tid & 63; l16 = lane & 15; g = lane >> 4;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, NARROW);
+        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, NARROW, t.from);
         row = paged_row(t, p.g.group, kvh, l16);
+        if (MOD && p.pass == 1 && p.slopes) row.pos = shared_pos(p, t.row0 + row.token);
         pages = p.table + (size_t)t.req * p.g.width;
         rowBytes = (size_t)p.g.kvDim * sizeof(KVT);
         Kp = static_cast<const char*>(p.K) + (size_t)kvh * HD * sizeof(KVT);
@@ -647,7 +750,7 @@ struct NarrowTile {
 #pragma unroll
             for (int j = 0; j < NB * 4; j++) x[j] = (x[j] - slope * (float)abs(row.pos - (base + 16 * (j / 4) + 4 * g + j % 4))) * 1.4426950408889634f;
         }
-        const bool inner = base + KB <= t.prefix || (base + KB - 1 <= span.pos0 && (p.window == 0 || base > span.pos1 - p.window));       // all rows see all of it
+        const bool inner = base + KB <= t.prefix || (base >= t.from && base + KB - 1 <= span.pos0 && (p.window == 0 || base > span.pos1 - p.window));       // all rows see all of it
         const bool all = inner && __all(mine >= 0);
         if (!all) {
 #pragma unroll
@@ -655,7 +758,7 @@ struct NarrowTile {
                 const bool held = page_in(mine, b, g & 2) >= 0;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (!held || !paged_sees(row.pos, base + 16 * b + 4 * g + i, t.len, p.window, t.prefix)) {
+                    if (!held || base + 16 * b + 4 * g + i < t.from || !paged_sees(row.pos, base + 16 * b + 4 * g + i, t.len, p.window, t.prefix)) {
                         x[4 * b + i] = -INFINITY;
                         if constexpr (Q8) vs[b][i] = 0.f;       // (its scale may be anything)
                     }
@@ -839,8 +942,7 @@ struct NarrowTile {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
             const float4_t v = *reinterpret_cast<const float4_t*>(lds + r * (HD + 4) + d);
             if (!whole) { store_through(mine + r * HD + d, v); continue; }
-            const PagedRow at = paged_row(t, p.g.group, kvh, r);
-            *reinterpret_cast<float4_t*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) = over(v, ls[r]);
+            put_result(p, t, paged_row(t, p.g.group, kvh, r), d, v, ls[r], ms[r] - SHIFT);
         }
         if (whole) return;
         if (tid < R) { st_agent(mine + NARROW * HD + tid, ms[tid]); st_agent(mine + NARROW * HD + NARROW + tid, ls[tid]); }
@@ -877,8 +979,7 @@ struct NarrowTile {
             const int i = tid + k * WG;
             if (i >= cols) continue;
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-            const PagedRow at = paged_row(t, p.g.group, kvh, r);
-            *reinterpret_cast<float4_t*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) = over(acc[k], den[r]);
+            put_result(p, t, paged_row(t, p.g.group, kvh, r), d, acc[k], den[r], M[r] - SHIFT);
         }
     }
 };
@@ -929,12 +1030,13 @@ struct WideTile {
         const int tid = thread_anew();
         lane = tid & 63; n32 = lane & 31; hf = lane >> 5;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, WIDE);
+        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, WIDE, t.from);
         const int mine = t.first + 32 * wave;
         active = mine < t.rows * p.g.group;
-        const PagedSpan own = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, active ? mine : t.first, 32);
+        const PagedSpan own = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, active ? mine : t.first, 32, t.from);
         pos0 = own.pos0; pos1 = own.pos1; begin = own.begin; end = own.end;
         row = paged_row(t, p.g.group, kvh, 32 * wave + n32);
+        if (MOD && p.pass == 1 && p.slopes) row.pos = shared_pos(p, t.row0 + row.token);
         pages = p.table + (size_t)t.req * p.g.width;
         rowBytes = (size_t)p.g.kvDim * sizeof(KVT);
         Kp = static_cast<const char*>(p.K) + (size_t)kvh * ROWB;
@@ -1119,7 +1221,7 @@ struct WideTile {
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++)
-                    if (!((held >> (4 * b + i / 4)) & 1) || !paged_sees(row.pos, first + 32 * b + 8 * (i / 4) + i % 4, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
+                    if (!((held >> (4 * b + i / 4)) & 1) || first + 32 * b + 8 * (i / 4) + i % 4 < t.from || !paged_sees(row.pos, first + 32 * b + 8 * (i / 4) + i % 4, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
         }
         float top = S[0][0];
 #pragma unroll
@@ -1153,7 +1255,7 @@ struct WideTile {
         const unsigned K = ldsBase + buf * BUFB, V = K + TILEB;
         const unsigned long long held = __ballot(mine >= 0);
         constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
-        const bool inner = base + UK <= t.prefix || (base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
+        const bool inner = base + UK <= t.prefix || (base >= t.from && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
         const bool all = inner && (held & runs) == runs;
         float16_t S[NB];
         float mNew;
@@ -1297,14 +1399,15 @@ struct WideTile {
             }
             __syncthreads();
             l = den[r];
+            m = M[r];
         }
         if (t.first + r >= t.rows * p.g.group) return;
-        float* out = p.out + (size_t)(t.row0 + row.token) * p.ldo + (size_t)row.head * HD + 4 * hf;
+        const PagedRow at = paged_row(t, p.g.group, kvh, r);
 #pragma unroll
         for (int b = 0; b < DB; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                *reinterpret_cast<float4_t*>(out + 32 * b + 8 * i) = over(float4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]}, l);
+                put_result(p, t, at, 32 * b + 8 * i + 4 * hf, float4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]}, l, m - SHIFT);
     }
 };
 
@@ -1380,6 +1483,7 @@ hipError_t paged_attention_setup(const PagedGeo& g) {
 hipError_t launch_paged_attention(const PagedAttention& p0, hipStream_t s) {
     for (int wide = p0.wideWorkers > 0; wide >= 0; wide--) {
         PagedAttention p = p0;
+        if (!wide && p.nWorkers == 0) continue;           // (no narrow tiles)
         if (wide) p.nWorkers = p.wideWorkers;
         const int groups = (p.nWorkers * p.g.nKVHeads + 7) / 8 * 8;
         p.tiles += wide ? p.maxTiles : 0;

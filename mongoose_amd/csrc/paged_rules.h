@@ -175,6 +175,14 @@ inline const char* paged_plan_refusal(const PagedGeo& g, const void* rowStart, c
     if (prefixLens && !paged_aligned(prefixLens, 4)) return "prefixLens is not aligned to 4 bytes";
     return nullptr;
 }
+inline const char* paged_plan_shared_refusal(const PagedGeo& g, const void* rowStart, const void* lens, int nReqs, int rows, int mostNew,
+                                             const void* groupStart, const void* sharedLens, int nGroups) {
+    if (const char* why = paged_plan_refusal(g, rowStart, lens, nReqs, rows, 0, nullptr)) return why;
+    if (mostNew < 0) return "mostNew is negative";
+    if (nGroups < 0 || nGroups > g.maxReqs) return "nGroups is negative or above the handle's maxReqs";
+    if (nGroups > 0 && (!paged_aligned(groupStart, 4) || !paged_aligned(sharedLens, 4))) return "a pointer is NULL or not aligned to 4 bytes";
+    return nullptr;
+}
 inline const char* paged_attention_refusal(const PagedGeo& g, const void* q, int ldq, const void* K, const void* V, const void* table,
                                            const void* out, int ldo, float scale, float softcap, const void* slopes) {
     const void* wide[] = {q, K, V, out};
@@ -231,12 +239,13 @@ struct PagedTile {
     int worker0, worker1;               // the first and last worker that have some of them
     int index;                          // its number
     int tileRows, unitKeys;             // its kind
-    int pad[2];
+    int from;                           // the first position that is its own: those before are another tile's (a shared prefix)
+    int pad[1];
 };
 
 // The positions [begin, end) that rows first .. first + tileRows - 1 of a request see some of, and the positions of its first and last token.
 struct PagedSpan { int begin, end, pos0, pos1; };
-MG_HD PagedSpan paged_span(int rows, int len, int prefix, int window, int group, int first, int tileRows) {
+MG_HD PagedSpan paged_span(int rows, int len, int prefix, int window, int group, int first, int tileRows, int from = 0) {
     const int all = rows * group;
     const int last = (first + tileRows < all ? first + tileRows : all) - 1;
     PagedSpan s;
@@ -244,10 +253,11 @@ MG_HD PagedSpan paged_span(int rows, int len, int prefix, int window, int group,
     s.pos1 = len - rows + last / group;
     s.end = s.pos1 + 1 > prefix ? s.pos1 + 1 : prefix;
     s.begin = window > 0 && prefix == 0 && s.pos0 - window + 1 > 0 ? s.pos0 - window + 1 : 0;
+    if (s.begin < from) s.begin = from;
     return s;
 }
 MG_HD void paged_units(PagedTile& t, int window, int group) {
-    const PagedSpan s = paged_span(t.rows, t.len, t.prefix, window, group, t.first, t.tileRows);
+    const PagedSpan s = paged_span(t.rows, t.len, t.prefix, window, group, t.first, t.tileRows, t.from);
     t.unit0 = s.begin / t.unitKeys;
     t.units = s.end > s.begin ? (s.end + t.unitKeys - 1) / t.unitKeys - t.unit0 : 0;
 }

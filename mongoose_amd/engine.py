@@ -801,13 +801,20 @@ class HIPPaged:
     def Plan(self, rowStart, lens, nReqs, rows, window=0, prefixLens=None, stream=None):
         return _paged_plan(self._h, rowStart, lens, nReqs, rows, window, prefixLens, stream)
 
+    def Share(self):
+        """Workspace for plans of requests that share prefixes; once, before the first PlanShared."""
+        return lib.mg_paged_share(self._h)
+
+    def PlanShared(self, rowStart, lens, nReqs, rows, mostNew, groupStart, sharedLens, nGroups, stream=None):
+        return _paged_plan_shared(self._h, rowStart, lens, nReqs, rows, mostNew, groupStart, sharedLens, nGroups, stream)
+
     def Attention(self, q, ldq, K, V, table, out, ldo, scale=0.0, softcap=0.0, slopes=None, stream=None):
         return _paged_attention(self._h, q, ldq, K, V, table, out, ldo, scale, softcap, slopes, stream)
 
 
 # (a server makes these calls for every layer of every step: the functions are looked up once)
-_paged_tables, _paged_store, _paged_load, _paged_plan, _paged_attention = (
-    lib.mg_paged_tables, lib.mg_paged_store, lib.mg_paged_load, lib.mg_paged_plan, lib.mg_paged_attention)
+_paged_tables, _paged_store, _paged_load, _paged_plan, _paged_plan_shared, _paged_attention = (
+    lib.mg_paged_tables, lib.mg_paged_store, lib.mg_paged_load, lib.mg_paged_plan, lib.mg_paged_plan_shared, lib.mg_paged_attention)
 
 
 def NewHIPPaged(eng, nHeads, nKVHeads, headDim, pageSize, nPages, kvFormat, maxReqs, maxRows, maxLen):

@@ -145,6 +145,8 @@ _sig("mg_paged_store", c_int, c_void_p, _p, _p, _p, c_int, c_int, c_int, _p, c_i
 _sig("mg_paged_pool_bytes", c_size_t, c_void_p)
 _sig("mg_paged_load", c_int, c_void_p, _p, _p, _p, _p, _p, c_int, c_int, _p, c_int, _p, c_int, _p)
 _sig("mg_paged_plan", c_int, c_void_p, _p, _p, c_int, c_int, c_int, _p, _p)
+_sig("mg_paged_share", c_int, c_void_p)
+_sig("mg_paged_plan_shared", c_int, c_void_p, _p, _p, c_int, c_int, c_int, _p, _p, c_int, _p)
 _sig("mg_paged_attention", c_int, c_void_p, _p, c_int, _p, _p, _p, _p, c_int, c_float, c_float, _p, _p)
 
 # host helpers
