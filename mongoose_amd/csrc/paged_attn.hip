@@ -49,20 +49,19 @@ MG_HD int wide_keys(int kvFormat) { return kvFormat == PAGED_F32 ? 32 : 64; }
 //   narrow, and 96 requests of 5 tokens 208 wide, 304 narrow.  With an fp32 cache narrow tiles would be better there, up to 64 rows (228,
 //   204, 385, and with 16 tokens 361 us wide; 169, 141, 249, 276 narrow): its wide tiles wait for the fp32 instructions of rows that are not there.
 int paged_narrow_rows(const PagedGeo& g, int rows) {
-    if (g.kvFormat == PAGED_Q8) return PAGED_MAX_ROWS * PAGED_MAX_GROUP;
     return (long long)rows * g.group <= 256 ? 256 : NARROW;
 }
 // The same with shared prefixes, for groups (0: all groups have wide tiles) and for requests, of which the caller may know that none adds more than
 // mostNew rows.
 int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool groups) {
     constexpr int ALL = PAGED_MAX_ROWS * PAGED_MAX_GROUP;
-    if (g.kvFormat == PAGED_Q8 || (long long)rows * g.group <= 256) return ALL;
+    if ((long long)rows * g.group <= 256) return ALL;
     if (groups) return 0;
     return mostNew > 0 && (long long)mostNew * g.group <= NARROW ? ALL : NARROW;
 }
 // (with shared prefixes requests of any number of rows may have narrow tiles)
 int paged_max_tiles_shared(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / NARROW) + g.maxReqs; }
-int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / (g.kvFormat == PAGED_Q8 ? NARROW : WIDE)) + g.maxReqs + 256 / NARROW; }
+int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + 256 / NARROW; }
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
 // Workgroups, in turns of the KV heads: two a CU for wide tiles; one a CU for narrow ones, though a CU holds two: HBM likes fewer
 // streams (8B shape, fp16: 120,001 positions 98 us, with two 113; 48 requests 174 and 182).  Fewer where the batch
@@ -994,14 +993,16 @@ struct NarrowTile {
 // A row's 16-byte pieces lie in LDS at piece ^ swz(row), so that neither rows of one piece nor (fp16) four rows of two meet in a bank.
 template <typename KVT, int HD, bool MOD>
 struct WideTile {
-    static constexpr bool HALF = sizeof(KVT) == 2;
+    static constexpr bool Q8 = sizeof(KVT) == 1, HALF = sizeof(KVT) <= 2;   // HALF: products of fp16 operands
     static constexpr int UK = HALF ? 64 : 32, NB = UK / 32, DB = HD / 32;
-    static constexpr int ROWB = HD * (int)sizeof(KVT), PR = ROWB / 16;      // bytes and 16-byte pieces of a row
+    static constexpr int ROWB = HD * (HALF ? 2 : 4);                        // bytes of a row of operands
+    static constexpr int PR = HD * (int)sizeof(KVT) / 16;                   // 16-byte pieces of a row of the cache
     static constexpr int RI = 64 / PR, NI = UK / RI / 4;                    // rows a load instruction brings, instructions a wave
     static constexpr int TILEB = UK * ROWB, BUFB = 2 * TILEB;               // K, then V
+    static constexpr int RAWB = UK * HD, SCALEB = UK * 4;                   // Q8: behind one such buffer two of K and V rows as they come, then two of scales
     static constexpr int VOTES = 2 * BUFB / 4;                              // a word of each wave's, behind the buffers
     static constexpr int QS = HALF ? HD / 16 : HD / 8;
-    static constexpr float SHIFT = HALF ? 13.f : 0.f;      // probabilities times 2^SHIFT,
+    static constexpr float SHIFT = Q8 ? 0.f : HALF ? 13.f : 0.f;      // probabilities times 2^SHIFT,
     static constexpr float LAZY = HALF ? 2.f : 8.f;        // and up to 2^LAZY more: the maximum is only moved where it grows by more
 
     const PagedAttention& p;
@@ -1013,6 +1014,7 @@ struct WideTile {
     PagedRow row;
     const int* pages;
     const char *Kp, *Vp, *zeros;
+    const char *Ksc, *Vsc;
     size_t rowBytes;
     static constexpr unsigned ldsBase = 0;
     unsigned from[NI];      // the lane's offset of every load instruction from its run of eight positions
@@ -1020,6 +1022,7 @@ struct WideTile {
     half8_t qh[HALF ? QS : 1], ql[HALF ? QS : 1];
     float4_t qf[HALF ? 1 : QS];
     float m, l;
+    float ref;                       // Q8: probabilities are 2^(x - ref)
     float16_t o[DB];
 
     static __device__ __forceinline__ int swz(int r) { return HALF ? ((r & 3) << 1) | ((r >> 2) & 1) : r & 7; }
@@ -1039,13 +1042,18 @@ struct WideTile {
         if (MOD && p.pass == 1 && p.slopes) row.pos = shared_pos(p, t.row0 + row.token);
         pages = p.table + (size_t)t.req * p.g.width;
         rowBytes = (size_t)p.g.kvDim * sizeof(KVT);
-        Kp = static_cast<const char*>(p.K) + (size_t)kvh * ROWB;
-        Vp = static_cast<const char*>(p.V) + (size_t)kvh * ROWB;
+        Kp = static_cast<const char*>(p.K) + (size_t)kvh * HD * sizeof(KVT);
+        Vp = static_cast<const char*>(p.V) + (size_t)kvh * HD * sizeof(KVT);
         zeros = reinterpret_cast<const char*>(p.zeros);
+        if constexpr (Q8) {
+            const size_t slots = (size_t)p.g.nPages * p.g.pageSize, head = (size_t)kvh * p.g.pageSize * 4;
+            Ksc = static_cast<const char*>(p.K) + slots * rowBytes + head;
+            Vsc = static_cast<const char*>(p.V) + slots * rowBytes + head;
+        }
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const int r = (wave * NI + i) * RI + lane / PR;
-            from[i] = (unsigned)(r & 7) * (unsigned)rowBytes + (unsigned)((lane % PR) ^ swz(r)) * 16;
+            from[i] = (unsigned)(r & 7) * (unsigned)rowBytes + (unsigned)((lane % PR) ^ (Q8 ? 0 : swz(r))) * 16;
         }
         here = page_of(u0);
         const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
@@ -1054,7 +1062,7 @@ struct WideTile {
         for (int i = 0; i < HD / 8; i++) x[i] = *reinterpret_cast<const float4_t*>(q + (HALF ? i / 2 * 16 + hf * 8 + i % 2 * 4 : i * 8 + hf * 4));
         next = page_of(min(u0 + 1, u1 - 1));
         __syncthreads();                          // (the tile before is done with the LDS)
-        issue(u0, here, 0);
+        if constexpr (Q8) issue_q8(u0, here, 0); else issue(u0, here, 0);
         cap = p.softcap;
         invCap = MOD && cap > 0.f ? 1.f / cap : 0.f;
         slope = MOD && p.slopes ? p.slopes[row.head] : 0.f;
@@ -1076,6 +1084,7 @@ struct WideTile {
                     const float y = ldexpf(x[2 * s + j / 4][j % 4], up);
                     qh[s][j] = (_Float16)y;
                     ql[s][j] = (_Float16)(y - (float)qh[s][j]);
+                    if (Q8 && !(fabsf(y) < INFINITY)) ql[s][j] = (_Float16)0.f;      // (as in NarrowTile)
                 }
             c = ldexpf(c, -up);
         } else {
@@ -1085,7 +1094,7 @@ struct WideTile {
         if (!MOD) c *= 1.4426950408889634f;
         c = fminf(c, FLT_MAX);                    // (0 times it is 0)
         m = -INFINITY;
-        l = 0.f;
+        l = ref = 0.f;
 #pragma unroll
         for (int b = 0; b < DB; b++)
 #pragma unroll
@@ -1119,6 +1128,48 @@ struct WideTile {
                 asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(k) : "memory");
                 asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst + TILEB), "v"(v) : "memory");
             }
+        }
+    }
+    // Q8: a unit's rows as they are, into raw buffer `buf`, and (a wave each) the scales of K and V
+    __device__ __forceinline__ void issue_q8(int u, int mine, unsigned buf) const {
+        const int base = base_of(u);
+        const unsigned raw = ldsBase + BUFB + buf * 2 * RAWB;
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const int r0 = (wave * NI + i) * RI, r = r0 + lane / PR, run = r0 >> 3;
+            const unsigned dst = raw + (unsigned)r0 * HD;
+            const int page = __builtin_amdgcn_readlane(mine, run), key = base + run * 8;
+            if (RI == 8 && page >= 0 && key >= span.begin && key + 8 <= span.end) {
+                const size_t at = (size_t)(((unsigned)page << p.g.pageShift) + ((unsigned)key & (unsigned)(p.g.pageSize - 1))) * rowBytes;
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(from[i]), "s"(Kp + at) : "memory");
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst + RAWB), "v"(from[i]), "s"(Vp + at) : "memory");
+            } else {
+                const int second = RI == 16 ? __builtin_amdgcn_readlane(mine, run + 1) : page;
+                const int pg = RI == 16 && (r & 8) ? second : page, piece = (lane % PR) * 16;
+                const char* k = kv_row(Kp, zeros, rowBytes, base + r, pg, span.begin, span.end, p.g.pageShift) + piece;
+                const char* v = kv_row(Vp, zeros, rowBytes, base + r, pg, span.begin, span.end, p.g.pageShift) + piece;
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(k) : "memory");
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst + RAWB), "v"(v) : "memory");
+            }
+        }
+        if (wave < 2) {
+            const int page = __shfl(mine, lane >> 3, 64);         // (of the lane's position; what lies behind a request's end is read and not used)
+            const size_t at = page >= 0 ? (((size_t)(unsigned)page * p.g.nKVHeads << p.g.pageShift) + ((unsigned)(base + lane) & (unsigned)(p.g.pageSize - 1))) * 4 : 0;
+            const char* s = (page >= 0 ? wave ? Vsc : Ksc : zeros) + at;
+            asm volatile(PAGED_SET_M0 "global_load_lds_dword %1, off" : : "s"(ldsBase + BUFB + 4 * RAWB + (buf * 2 + (unsigned)wave) * SCALEB), "v"(s) : "memory");
+        }
+    }
+    // Raw buffer `buf` as operands: a thread's 16 bytes of a row are two pieces of halves
+    __device__ __forceinline__ void convert(unsigned buf) const {
+        const unsigned raw = ldsBase + BUFB + buf * 2 * RAWB, tid = (unsigned)thread_anew();
+        typedef __attribute__((address_space(3))) uint4_t* lp;
+#pragma unroll
+        for (int n = 0; n < 2 * RAWB / 16 / WG; n++) {
+            const unsigned i = tid + n * WG, r = i / PR, piece = 2 * (i % PR);       // (V's rows behind K's)
+            const uint4_t x = lds16(raw + i * 16);
+            const unsigned row = ldsBase + r * ROWB, s = (unsigned)swz((int)r);
+            *reinterpret_cast<lp>(row + (piece ^ s) * 16) = __builtin_bit_cast(uint4_t, eight_halves(x[0], x[1]));
+            *reinterpret_cast<lp>(row + ((piece + 1) ^ s) * 16) = __builtin_bit_cast(uint4_t, eight_halves(x[2], x[3]));
         }
     }
     static __device__ __forceinline__ uint4_t lds16(unsigned at) { return *reinterpret_cast<__attribute__((address_space(3))) const uint4_t*>(at); }
@@ -1244,15 +1295,110 @@ struct WideTile {
             }
         return ts;
     }
-    // Unit u, of page numbers `here`, in buffer `buf`; asks for the one behind it on the way
+    // Q8: scores to weights of V's whole numbers, as NarrowTile::weigh_q8; returns the lane's sum of the probabilities (times 2^(m - ref))
+    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, unsigned buf) {
+        constexpr float FIT = 32768.f;
+        const int h4 = 4 * anew(hf), first = base + h4;
+        const unsigned scales = ldsBase + BUFB + 4 * RAWB + buf * 2 * SCALEB + (unsigned)h4 * 4;
+        auto scale4 = [&](int which, int b, int i) { return __builtin_bit_cast(float4_t, lds16(scales + which * SCALEB + (32 * b + 8 * i) * 4)); };
+        auto exponent = [](float most) { return (float)(12 - __builtin_amdgcn_frexp_expf(fminf(most, FLT_MAX))); };
+        auto both = [](float x) { float other = x; row_swap32(x, other); return fmaxf(x, other); };
+        auto again = [&](float f) {
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < DB; b++) o[b] *= f;
+        };
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);       // (as in scores)
+                const float4_t d = scale4(0, b, i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) S[b][4 * i + j] *= d[j];
+            }
+        if constexpr (MOD) {
+#pragma unroll
+            for (int b = 0; b < NB; b++) S[b] *= c;
+            if (cap > 0.f) cap_all(S, cap, invCap);
+            if (p.slopes) {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+#pragma unroll
+                    for (int i = 0; i < 16; i++) S[b][i] = fmaf(-slope, (float)abs(row.pos - (first + 32 * b + 8 * (i / 4) + i % 4)), S[b][i]);
+            }
+        }
+        const float factor = MOD ? 1.4426950408889634f : c;
+        if (!all) {
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int key = first + 32 * b + 8 * (i / 4) + i % 4;
+                    if (!((held >> (4 * b + i / 4)) & 1) || key < t.from || !paged_sees(row.pos, key, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
+                }
+        }
+        float top = S[0][0];
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) top = fmaxf(top, S[b][i]);
+        top = both(top);
+        top = top == -INFINITY ? top : top * factor;
+        const float mNew = top > m + LAZY || m == -INFINITY ? fmaxf(m, top) : m;
+        if (__any(mNew != m)) {
+            const float from = mNew == -INFINITY ? 0.f : mNew;
+            float most = 0.f;
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+                    const float4_t d = scale4(1, b, i);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) most = fmaxf(most, __builtin_amdgcn_exp2f(fmaf(S[b][4 * i + j], factor, -from)) * d[j]);
+                }
+            most = both(most);
+            const float to = mNew != m ? from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), 110.f)) : 0.f) : ref;
+            again(m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to));
+            ref = to;
+            m = mNew;
+        }
+        float ts = 0.f, most = 0.f;
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
+                const float4_t d = scale4(1, b, i);
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(S[b][4 * i + j], factor, -ref));
+                    ts += x;
+                    S[b][4 * i + j] = all ? x * d[j] : x == 0.f ? 0.f : x * d[j];        // (a hidden position's scale may be anything)
+                    most = fmaxf(most, S[b][4 * i + j]);
+                }
+            }
+        if (__any(most > FIT)) {
+            most = both(most);
+            const float down = most > FIT ? exponent(most) : 0.f, f = __builtin_amdgcn_exp2f(down);
+            again(f);
+            ts *= f;
+            ref -= down;
+#pragma unroll
+            for (int b = 0; b < NB; b++) S[b] *= f;
+        }
+        return ts;
+    }
+    // Unit u, of page numbers `here`, in buffer `buf`; asks for the one behind it on the way (Q8: its raw rows were in buffer `buf`)
     template <bool AGAIN>
     __device__ __forceinline__ void compute(int u, bool more, unsigned buf, int pass) {
         const int base = base_of(u), mine = here;
         if (!active || base >= end || base + UK <= begin) {
-            if (more) issue(u + 1, next, buf ^ 1);
+            if (!Q8 && more) issue(u + 1, next, buf ^ 1);
             return;
         }
-        const unsigned K = ldsBase + buf * BUFB, V = K + TILEB;
+        const unsigned K = ldsBase + (Q8 ? 0 : buf * BUFB), V = K + TILEB;
         const unsigned long long held = __ballot(mine >= 0);
         constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
         const bool inner = base + UK <= t.prefix || (base >= t.from && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
@@ -1260,6 +1406,11 @@ struct WideTile {
         float16_t S[NB];
         float mNew;
         scores(K, S, false);
+        if constexpr (Q8) {
+            const float ts = weigh_q8(S, base, held, all, buf);
+            l += ts;
+            if (!inner && !__any(ts != 0.f)) return;
+        } else {
         if (more) issue(u + 1, next, buf ^ 1);
         float ts = weigh(S, base, held, all, mNew);
         if (HALF && __any(ts != ts)) {            // (not a loop: what the masks need would be worked out ahead of it, for every unit)
@@ -1275,6 +1426,7 @@ struct WideTile {
         }
         l += ts;
         if (!inner && !__any(ts != 0.f)) return;          // (no row has anything here)
+        }
         if (AGAIN && pass != FINITE) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
@@ -1306,6 +1458,11 @@ struct WideTile {
             // this unit's rows have landed; nobody reads the other buffer any more
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             const int behind = page_of(min(u + 2, u1 - 1));
+            if constexpr (Q8) {
+                if (u + 1 < u1) issue_q8(u + 1, next, buf ^ 1);
+                convert(buf);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            }
             if constexpr (AGAIN) {
                 replace(ldsBase + buf * BUFB + TILEB, pass);
                 __syncthreads();
@@ -1318,6 +1475,16 @@ struct WideTile {
     }
     __device__ __forceinline__ void run(int u0, int u1, int, int, float* lds) {
         units<false>(u0, u1, 0);
+        if constexpr (Q8) {
+            const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - m);
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < DB; b++) o[b] *= f;
+            float other = l;
+            row_swap32(l, other);
+            l += other;
+            return;
+        }
         float odd = 0.f;
 #pragma unroll
         for (int b = 0; b < DB; b++)
@@ -1450,8 +1617,8 @@ __global__ __launch_bounds__(WG, 2) void paged_wide_kernel(PagedAttention p) {
     attend<KVT, HD, MOD, WideTile, WIDE>(p, lds);
 }
 
-static size_t attn_lds(int headDim, bool wide) {
-    const size_t tile = wide ? (size_t)2 * 2 * 64 * headDim * 2 + 16 : (size_t)(4 * NARROW * (headDim + 4) + 8 * NARROW) * 4;
+static size_t attn_lds(int headDim, bool wide) {           // (wide, Q8: one buffer of halves, two of bytes, 1 KB of scales)
+    const size_t tile = wide ? (size_t)2 * 2 * 64 * headDim * 2 + 1024 : (size_t)(4 * NARROW * (headDim + 4) + 8 * NARROW) * 4;
     const size_t merge = (size_t)(2 * (wide ? WIDE : NARROW) + MERGE_LDS) * 4;
     return tile > merge ? tile : merge;
 }
@@ -1459,9 +1626,8 @@ template <typename F>
 static hipError_t with_kernel(const PagedGeo& g, bool mod, bool wide, F f) {
 #define PAGED_PICK(KVT, HD, MOD) (wide ? f(paged_wide_kernel<KVT, HD, MOD>) : f(paged_narrow_kernel<KVT, HD, MOD>))
     if (g.kvFormat == PAGED_Q8) {
-        if (wide) return hipErrorInvalidValue;
-        if (g.headDim == 64) return mod ? f(paged_narrow_kernel<signed char, 64, true>) : f(paged_narrow_kernel<signed char, 64, false>);
-        return mod ? f(paged_narrow_kernel<signed char, 128, true>) : f(paged_narrow_kernel<signed char, 128, false>);
+        if (g.headDim == 64) return mod ? PAGED_PICK(signed char, 64, true) : PAGED_PICK(signed char, 64, false);
+        return mod ? PAGED_PICK(signed char, 128, true) : PAGED_PICK(signed char, 128, false);
     }
     if (g.kvFormat == PAGED_F16) {
         if (g.headDim == 64) return mod ? PAGED_PICK(_Float16, 64, true) : PAGED_PICK(_Float16, 64, false);
@@ -1472,7 +1638,7 @@ static hipError_t with_kernel(const PagedGeo& g, bool mod, bool wide, F f) {
 #undef PAGED_PICK
 }
 hipError_t paged_attention_setup(const PagedGeo& g) {
-    for (int i = 0; i < (g.kvFormat == PAGED_Q8 ? 2 : 4); i++) {
+    for (int i = 0; i < 4; i++) {
         hipError_t e = with_kernel(g, i & 1, i >> 1, [&](auto* k) {
             return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)attn_lds(g.headDim, i >> 1));
         });
