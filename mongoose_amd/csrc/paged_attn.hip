@@ -39,7 +39,7 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 
 // Positions of a unit: a narrow tile's four waves take 64 of a Q8 cache, 32 of an fp16 one or 16 of an fp32 one each, a wide tile's share them.
 MG_HD int narrow_keys(int kvFormat) { return kvFormat == PAGED_F32 ? 64 : kvFormat == PAGED_F16 ? 128 : 256; }
-MG_HD int wide_keys(int kvFormat) { return kvFormat == PAGED_F32 ? 32 : 64; }
+MG_HD int wide_keys(int kvFormat) { return kvFormat == PAGED_F16 ? 64 : 32; }
 
 // Rows a KV head (tokens x group) up to which a request goes to the kernel that waits for memory, with longer ones to the one that waits for
 // the matrix units.  8B shape:
@@ -994,12 +994,13 @@ struct NarrowTile {
 template <typename KVT, int HD, bool MOD>
 struct WideTile {
     static constexpr bool Q8 = sizeof(KVT) == 1, HALF = sizeof(KVT) <= 2;   // HALF: products of fp16 operands
-    static constexpr int UK = HALF ? 64 : 32, NB = UK / 32, DB = HD / 32;
+    static constexpr int UK = HALF && !Q8 ? 64 : 32, NB = UK / 32, DB = HD / 32;
     static constexpr int ROWB = HD * (HALF ? 2 : 4);                        // bytes of a row of operands
     static constexpr int PR = HD * (int)sizeof(KVT) / 16;                   // 16-byte pieces of a row of the cache
-    static constexpr int RI = 64 / PR, NI = UK / RI / 4;                    // rows a load instruction brings, instructions a wave
+    static constexpr int RI = 64 / PR, NI = Q8 ? 1 : UK / RI / 4;           // rows a load instruction brings, instructions a wave (for K)
     static constexpr int TILEB = UK * ROWB, BUFB = 2 * TILEB;               // K, then V
-    static constexpr int RAWB = UK * HD, SCALEB = UK * 4;                   // Q8: behind one such buffer two of K and V rows as they come, then two of scales
+    static constexpr int RAWB = UK * HD, SCALEB = UK * 4;                   // Q8: behind the two buffers two of K and V rows as they come, then the scales of
+    static constexpr int RAW = 2 * BUFB, SCALES = RAW + 4 * RAWB;           // four units
     static constexpr int VOTES = 2 * BUFB / 4;                              // a word of each wave's, behind the buffers
     static constexpr int QS = HALF ? HD / 16 : HD / 8;
     static constexpr float SHIFT = Q8 ? 0.f : HALF ? 13.f : 0.f;      // probabilities times 2^SHIFT,
@@ -1062,7 +1063,7 @@ struct WideTile {
         for (int i = 0; i < HD / 8; i++) x[i] = *reinterpret_cast<const float4_t*>(q + (HALF ? i / 2 * 16 + hf * 8 + i % 2 * 4 : i * 8 + hf * 4));
         next = page_of(min(u0 + 1, u1 - 1));
         __syncthreads();                          // (the tile before is done with the LDS)
-        if constexpr (Q8) issue_q8(u0, here, 0); else issue(u0, here, 0);
+        if constexpr (Q8) issue_q8(u0, here, 0, u0 & 3); else issue(u0, here, 0);
         cap = p.softcap;
         invCap = MOD && cap > 0.f ? 1.f / cap : 0.f;
         slope = MOD && p.slopes ? p.slopes[row.head] : 0.f;
@@ -1130,44 +1131,42 @@ struct WideTile {
             }
         }
     }
-    // Q8: a unit's rows as they are, into raw buffer `buf`, and (a wave each) the scales of K and V
-    __device__ __forceinline__ void issue_q8(int u, int mine, unsigned buf) const {
+    // Q8: a unit's rows as they are, into raw buffer `raw`, its scales into place `slot`: of the 2 UK / RI instructions for K and then V every wave
+    // has its share, the first wave the scales besides (a lane a scale).
+    __device__ __forceinline__ void issue_q8(int u, int mine, unsigned raw, unsigned slot) const {
         const int base = base_of(u);
-        const unsigned raw = ldsBase + BUFB + buf * 2 * RAWB;
+        const unsigned to = ldsBase + RAW + raw * 2 * RAWB;
 #pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const int r0 = (wave * NI + i) * RI, r = r0 + lane / PR, run = r0 >> 3;
-            const unsigned dst = raw + (unsigned)r0 * HD;
+        for (int i = 0; i < 2 * UK / RI / 4; i++) {
+            const int n = wave * (2 * UK / RI / 4) + i, r0 = n % (UK / RI) * RI, r = r0 + lane / PR, run = r0 >> 3;
+            const unsigned dst = to + (unsigned)n * (RI * HD);
+            const char* pool = n < UK / RI ? Kp : Vp;
             const int page = __builtin_amdgcn_readlane(mine, run), key = base + run * 8;
             if (RI == 8 && page >= 0 && key >= span.begin && key + 8 <= span.end) {
                 const size_t at = (size_t)(((unsigned)page << p.g.pageShift) + ((unsigned)key & (unsigned)(p.g.pageSize - 1))) * rowBytes;
-                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(from[i]), "s"(Kp + at) : "memory");
-                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst + RAWB), "v"(from[i]), "s"(Vp + at) : "memory");
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, %2" : : "s"(dst), "v"(from[0]), "s"(pool + at) : "memory");
             } else {
                 const int second = RI == 16 ? __builtin_amdgcn_readlane(mine, run + 1) : page;
-                const int pg = RI == 16 && (r & 8) ? second : page, piece = (lane % PR) * 16;
-                const char* k = kv_row(Kp, zeros, rowBytes, base + r, pg, span.begin, span.end, p.g.pageShift) + piece;
-                const char* v = kv_row(Vp, zeros, rowBytes, base + r, pg, span.begin, span.end, p.g.pageShift) + piece;
-                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(k) : "memory");
-                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst + RAWB), "v"(v) : "memory");
+                const char* x = kv_row(pool, zeros, rowBytes, base + r, RI == 16 && (r & 8) ? second : page, span.begin, span.end, p.g.pageShift) + (lane % PR) * 16;
+                asm volatile(PAGED_SET_M0 "global_load_lds_dwordx4 %1, off" : : "s"(dst), "v"(x) : "memory");
             }
         }
-        if (wave < 2) {
-            const int page = __shfl(mine, lane >> 3, 64);         // (of the lane's position; what lies behind a request's end is read and not used)
-            const size_t at = page >= 0 ? (((size_t)(unsigned)page * p.g.nKVHeads << p.g.pageShift) + ((unsigned)(base + lane) & (unsigned)(p.g.pageSize - 1))) * 4 : 0;
-            const char* s = (page >= 0 ? wave ? Vsc : Ksc : zeros) + at;
-            asm volatile(PAGED_SET_M0 "global_load_lds_dword %1, off" : : "s"(ldsBase + BUFB + 4 * RAWB + (buf * 2 + (unsigned)wave) * SCALEB), "v"(s) : "memory");
+        if (wave == 0) {
+            const int page = __shfl(mine, (lane & 31) >> 3, 64);         // (of the lane's position; what lies behind a request's end is read and not used)
+            const size_t at = page >= 0 ? (((size_t)(unsigned)page * p.g.nKVHeads << p.g.pageShift) + ((unsigned)(base + (lane & 31)) & (unsigned)(p.g.pageSize - 1))) * 4 : 0;
+            const char* x = (page >= 0 ? hf ? Vsc : Ksc : zeros) + at;
+            asm volatile(PAGED_SET_M0 "global_load_lds_dword %1, off" : : "s"(ldsBase + SCALES + slot * 2 * SCALEB), "v"(x) : "memory");
         }
     }
-    // Raw buffer `buf` as operands: a thread's 16 bytes of a row are two pieces of halves
-    __device__ __forceinline__ void convert(unsigned buf) const {
-        const unsigned raw = ldsBase + BUFB + buf * 2 * RAWB, tid = (unsigned)thread_anew();
+    // Raw buffer `raw` as operands in buffer `buf`: a thread's 16 bytes of a row are two pieces of halves
+    __device__ __forceinline__ void convert(unsigned raw, unsigned buf) const {
+        const unsigned tid = (unsigned)thread_anew(), in = ldsBase + RAW + raw * 2 * RAWB + tid * 16;
         typedef __attribute__((address_space(3))) uint4_t* lp;
 #pragma unroll
         for (int n = 0; n < 2 * RAWB / 16 / WG; n++) {
             const unsigned i = tid + n * WG, r = i / PR, piece = 2 * (i % PR);       // (V's rows behind K's)
-            const uint4_t x = lds16(raw + i * 16);
-            const unsigned row = ldsBase + r * ROWB, s = (unsigned)swz((int)r);
+            const uint4_t x = lds16(in + n * WG * 16);
+            const unsigned row = ldsBase + buf * BUFB + r * ROWB, s = (unsigned)swz((int)r);
             *reinterpret_cast<lp>(row + (piece ^ s) * 16) = __builtin_bit_cast(uint4_t, eight_halves(x[0], x[1]));
             *reinterpret_cast<lp>(row + ((piece + 1) ^ s) * 16) = __builtin_bit_cast(uint4_t, eight_halves(x[2], x[3]));
         }
@@ -1296,10 +1295,10 @@ struct WideTile {
         return ts;
     }
     // Q8: scores to weights of V's whole numbers, as NarrowTile::weigh_q8; returns the lane's sum of the probabilities (times 2^(m - ref))
-    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, unsigned buf) {
+    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, unsigned slot) {
         constexpr float FIT = 32768.f;
         const int h4 = 4 * anew(hf), first = base + h4;
-        const unsigned scales = ldsBase + BUFB + 4 * RAWB + buf * 2 * SCALEB + (unsigned)h4 * 4;
+        const unsigned scales = ldsBase + SCALES + slot * 2 * SCALEB + (unsigned)h4 * 4;
         auto scale4 = [&](int which, int b, int i) { return __builtin_bit_cast(float4_t, lds16(scales + which * SCALEB + (32 * b + 8 * i) * 4)); };
         auto exponent = [](float most) { return (float)(12 - __builtin_amdgcn_frexp_expf(fminf(most, FLT_MAX))); };
         auto both = [](float x) { float other = x; row_swap32(x, other); return fmaxf(x, other); };
@@ -1390,7 +1389,7 @@ struct WideTile {
         }
         return ts;
     }
-    // Unit u, of page numbers `here`, in buffer `buf`; asks for the one behind it on the way (Q8: its raw rows were in buffer `buf`)
+    // Unit u, of page numbers `here`, in buffer `buf`; asks for the one behind it on the way
     template <bool AGAIN>
     __device__ __forceinline__ void compute(int u, bool more, unsigned buf, int pass) {
         const int base = base_of(u), mine = here;
@@ -1398,7 +1397,7 @@ struct WideTile {
             if (!Q8 && more) issue(u + 1, next, buf ^ 1);
             return;
         }
-        const unsigned K = ldsBase + (Q8 ? 0 : buf * BUFB), V = K + TILEB;
+        const unsigned K = ldsBase + buf * BUFB, V = K + TILEB;
         const unsigned long long held = __ballot(mine >= 0);
         constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
         const bool inner = base + UK <= t.prefix || (base >= t.from && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
@@ -1407,7 +1406,7 @@ struct WideTile {
         float mNew;
         scores(K, S, false);
         if constexpr (Q8) {
-            const float ts = weigh_q8(S, base, held, all, buf);
+            const float ts = weigh_q8(S, base, held, all, u & 3);
             l += ts;
             if (!inner && !__any(ts != 0.f)) return;
         } else {
@@ -1458,11 +1457,6 @@ struct WideTile {
             // this unit's rows have landed; nobody reads the other buffer any more
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             const int behind = page_of(min(u + 2, u1 - 1));
-            if constexpr (Q8) {
-                if (u + 1 < u1) issue_q8(u + 1, next, buf ^ 1);
-                convert(buf);
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-            }
             if constexpr (AGAIN) {
                 replace(ldsBase + buf * BUFB + TILEB, pass);
                 __syncthreads();
@@ -1473,9 +1467,29 @@ struct WideTile {
             buf ^= 1;
         }
     }
+    // Q8: a unit's raw rows come two units ahead and become operands one ahead
+    __device__ __forceinline__ void units_q8(int u0, int u1) {
+        if (u0 + 1 < u1) issue_q8(u0 + 1, next, 1, (u0 + 1) & 3);
+        int third = page_of(min(u0 + 2, u1 - 1));
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        convert(0, 0);
+        unsigned buf = 0;
+        for (int u = u0; u < u1; u++) {
+            // the next unit's raw rows have landed, this one's operands are written; nobody reads the raw rows or the operands before them any more
+            asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            const int fourth = page_of(min(u + 3, u1 - 1));
+            if (u + 2 < u1) issue_q8(u + 2, third, buf, (u + 2) & 3);
+            if (u + 1 < u1) convert(buf ^ 1, buf ^ 1);
+            compute<false>(u, false, buf, 0);
+            here = next;
+            next = third;
+            third = fourth;
+            buf ^= 1;
+        }
+    }
     __device__ __forceinline__ void run(int u0, int u1, int, int, float* lds) {
-        units<false>(u0, u1, 0);
         if constexpr (Q8) {
+            units_q8(u0, u1);
             const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - m);
             l *= f;
 #pragma unroll
@@ -1485,6 +1499,7 @@ struct WideTile {
             l += other;
             return;
         }
+        units<false>(u0, u1, 0);
         float odd = 0.f;
 #pragma unroll
         for (int b = 0; b < DB; b++)
