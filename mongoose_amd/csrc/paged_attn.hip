@@ -807,6 +807,7 @@ struct NarrowTile {
     // where the row's maximum moves, and less where a weight passes 2^15 (rows' references: ref = m - that power's exponent).
     __device__ __forceinline__ void weigh_q8(float (&x)[NB * 4], float top, float from) {
         constexpr float FIT = 32768.f;
+        float f = 1.f, ts = 0.f;
         auto most_of = [&](auto f) {
             float most = 0.f;
 #pragma unroll
@@ -814,34 +815,35 @@ struct NarrowTile {
             return most;
         };
         auto exponent = [](float most) { return (float)(12 - __builtin_amdgcn_frexp_expf(fminf(most, FLT_MAX))); };
-        auto again = [&](float f) {
-            l *= f;
-#pragma unroll
-            for (int e = 0; e < EPL; e++) o[e] *= f;
-        };
         if (__any(top > m)) {
             const float most = rows_max(most_of([&](int j) { return __builtin_amdgcn_exp2f(x[j] - from) * vs[j / 4][j % 4]; }));
             const float to = top > m ? from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), 110.f)) : 0.f) : ref;
-            again(m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to));
+            f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to);
             ref = to;
             m = top;
         }
 #pragma unroll
         for (int j = 0; j < NB * 4; j++) {
             x[j] = __builtin_amdgcn_exp2f(x[j] - ref);
-            l += x[j];
+            ts += x[j];
             x[j] *= vs[j / 4][j % 4];
         }
         float most = most_of([&](int j) { return x[j]; });
         if (__any(most > FIT)) {
             most = rows_max(most);
-            const float down = most > FIT ? exponent(most) : 0.f;
-            const float f = __builtin_amdgcn_exp2f(down);
-            again(f);
+            const float down = most > FIT ? exponent(most) : 0.f, less = __builtin_amdgcn_exp2f(down);
+            f *= less;
+            ts *= less;
             ref -= down;
 #pragma unroll
-            for (int j = 0; j < NB * 4; j++) x[j] *= f;
+            for (int j = 0; j < NB * 4; j++) x[j] *= less;
         }
+        if (__any(f != 1.f)) {            // (in one place: where a loop changes o in several, the compiler keeps it twice and moves it)
+            l *= f;
+#pragma unroll
+            for (int e = 0; e < EPL; e++) o[e] *= f;
+        }
+        l += ts;
     }
     template <bool AGAIN>
     __device__ __forceinline__ void units(int u0, int u1, int pass) {
@@ -1159,13 +1161,19 @@ struct WideTile {
         }
     }
     // Raw buffer `raw` as operands in buffer `buf`: a thread's 16 bytes of a row are two pieces of halves
-    __device__ __forceinline__ void convert(unsigned raw, unsigned buf) const {
-        const unsigned tid = (unsigned)thread_anew(), in = ldsBase + RAW + raw * 2 * RAWB + tid * 16;
+    static constexpr int CN = Q8 ? 2 * RAWB / 16 / WG : 1;
+    __device__ __forceinline__ void raw_rows(unsigned raw, uint4_t (&x)[CN]) const {
+        const unsigned in = ldsBase + RAW + raw * 2 * RAWB + (unsigned)thread_anew() * 16;
+#pragma unroll
+        for (int n = 0; n < CN; n++) x[n] = lds16(in + n * WG * 16);
+    }
+    __device__ __forceinline__ void convert(const uint4_t (&rows)[CN], unsigned buf) const {
+        const unsigned tid = (unsigned)thread_anew();
         typedef __attribute__((address_space(3))) uint4_t* lp;
 #pragma unroll
-        for (int n = 0; n < 2 * RAWB / 16 / WG; n++) {
+        for (int n = 0; n < CN; n++) {
             const unsigned i = tid + n * WG, r = i / PR, piece = 2 * (i % PR);       // (V's rows behind K's)
-            const uint4_t x = lds16(in + n * WG * 16);
+            const uint4_t x = rows[n];
             const unsigned row = ldsBase + buf * BUFB + r * ROWB, s = (unsigned)swz((int)r);
             *reinterpret_cast<lp>(row + (piece ^ s) * 16) = __builtin_bit_cast(uint4_t, eight_halves(x[0], x[1]));
             *reinterpret_cast<lp>(row + ((piece + 1) ^ s) * 16) = __builtin_bit_cast(uint4_t, eight_halves(x[2], x[3]));
@@ -1220,15 +1228,33 @@ struct WideTile {
     }
     // Block d of V^T P^T on top of `out`
     struct Weights { half8_t hi[HALF ? UK / 16 : 1], lo[HALF ? UK / 16 : 1]; };
+    static __device__ __forceinline__ Weights weights(const float16_t (&S)[NB]) {
+        Weights w;
+        if constexpr (HALF) {
+#pragma unroll
+            for (int kk = 0; kk < UK / 16; kk++)
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float x = S[kk / 2][8 * (kk % 2) + i];
+                    w.hi[kk][i] = (_Float16)x;
+                    w.lo[kk][i] = (_Float16)(x - (float)w.hi[kk][i]);
+                }
+        }
+        return w;
+    }
+    // The operand of positions 16 kk .. 16 kk + 15 of a block of V at `at`
+    static __device__ __forceinline__ half8_t v_piece(unsigned at, int kk) {
+        typedef __attribute__((address_space(3))) short4_t* lp;
+        const uint2_t x = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB)));
+        const uint2_t y = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB + 8 * ROWB)));
+        return __builtin_bit_cast(half8_t, uint4_t{x[0], x[1], y[0], y[1]});
+    }
     __device__ __forceinline__ float16_t product(unsigned V, int d, const float16_t (&S)[NB], const Weights& w, float16_t out) const {
         if constexpr (HALF) {
             const unsigned at = V ^ (unsigned)(d * 64);
 #pragma unroll
             for (int kk = 0; kk < UK / 16; kk++) {
-                typedef __attribute__((address_space(3))) short4_t* lp;
-                const uint2_t x = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB)));
-                const uint2_t y = __builtin_bit_cast(uint2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(reinterpret_cast<lp>(at + kk * 16 * ROWB + 8 * ROWB)));
-                const half8_t v = __builtin_bit_cast(half8_t, uint4_t{x[0], x[1], y[0], y[1]});
+                const half8_t v = v_piece(at, kk);
                 out = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.hi[kk], out, 0, 0, 0);
                 out = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, w.lo[kk], out, 0, 0, 0);
             }
@@ -1294,24 +1320,20 @@ struct WideTile {
             }
         return ts;
     }
-    // Q8: scores to weights of V's whole numbers, as NarrowTile::weigh_q8; returns the lane's sum of the probabilities (times 2^(m - ref))
-    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, unsigned slot) {
+    // Q8: scores to weights of V's whole numbers, as NarrowTile::weigh_q8; returns the lane's sum of the probabilities (times 2^(m - ref)).  f: what
+    // l and o are multiplied by first (in one place, once: where a loop changes o in several, the compiler keeps it twice and moves it).
+    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, unsigned slot, float& f) {
         constexpr float FIT = 32768.f;
+        f = 1.f;
         const int h4 = 4 * anew(hf), first = base + h4;
         const unsigned scales = ldsBase + SCALES + slot * 2 * SCALEB + (unsigned)h4 * 4;
         auto scale4 = [&](int which, int b, int i) { return __builtin_bit_cast(float4_t, lds16(scales + which * SCALEB + (32 * b + 8 * i) * 4)); };
         auto exponent = [](float most) { return (float)(12 - __builtin_amdgcn_frexp_expf(fminf(most, FLT_MAX))); };
         auto both = [](float x) { float other = x; row_swap32(x, other); return fmaxf(x, other); };
-        auto again = [&](float f) {
-            l *= f;
-#pragma unroll
-            for (int b = 0; b < DB; b++) o[b] *= f;
-        };
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);       // (as in scores)
                 const float4_t d = scale4(0, b, i);
 #pragma unroll
                 for (int j = 0; j < 4; j++) S[b][4 * i + j] *= d[j];
@@ -1352,40 +1374,42 @@ struct WideTile {
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
                     const float4_t d = scale4(1, b, i);
 #pragma unroll
                     for (int j = 0; j < 4; j++) most = fmaxf(most, __builtin_amdgcn_exp2f(fmaf(S[b][4 * i + j], factor, -from)) * d[j]);
                 }
             most = both(most);
             const float to = mNew != m ? from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), 110.f)) : 0.f) : ref;
-            again(m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to));
+            f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to);
             ref = to;
             m = mNew;
         }
         float ts = 0.f, most = 0.f;
+        auto weights = [&](auto product) {
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+            for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                if (i % 2 == 0) __builtin_amdgcn_sched_barrier(0);
-                const float4_t d = scale4(1, b, i);
+                for (int i = 0; i < 4; i++) {
+                    const float4_t d = scale4(1, b, i);
 #pragma unroll
-                for (int j = 0; j < 4; j++) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(S[b][4 * i + j], factor, -ref));
-                    ts += x;
-                    S[b][4 * i + j] = all ? x * d[j] : x == 0.f ? 0.f : x * d[j];        // (a hidden position's scale may be anything)
-                    most = fmaxf(most, S[b][4 * i + j]);
+                    for (int j = 0; j < 4; j++) {
+                        const float x = __builtin_amdgcn_exp2f(fmaf(S[b][4 * i + j], factor, -ref));
+                        ts += x;
+                        S[b][4 * i + j] = product(x, d[j]);
+                        most = fmaxf(most, S[b][4 * i + j]);
+                    }
                 }
-            }
+        };
+        if (all) weights([](float x, float d) { return x * d; });
+        else weights([](float x, float d) { return x == 0.f ? 0.f : x * d; });        // (a hidden position's scale may be anything)
         if (__any(most > FIT)) {
             most = both(most);
-            const float down = most > FIT ? exponent(most) : 0.f, f = __builtin_amdgcn_exp2f(down);
-            again(f);
-            ts *= f;
+            const float down = most > FIT ? exponent(most) : 0.f, less = __builtin_amdgcn_exp2f(down);
+            f *= less;
+            ts *= less;
             ref -= down;
 #pragma unroll
-            for (int b = 0; b < NB; b++) S[b] *= f;
+            for (int b = 0; b < NB; b++) S[b] *= less;
         }
         return ts;
     }
@@ -1394,7 +1418,7 @@ struct WideTile {
     __device__ __forceinline__ void compute(int u, bool more, unsigned buf, int pass) {
         const int base = base_of(u), mine = here;
         if (!active || base >= end || base + UK <= begin) {
-            if (!Q8 && more) issue(u + 1, next, buf ^ 1);
+            if (more) issue(u + 1, next, buf ^ 1);
             return;
         }
         const unsigned K = ldsBase + buf * BUFB, V = K + TILEB;
@@ -1405,11 +1429,6 @@ struct WideTile {
         float16_t S[NB];
         float mNew;
         scores(K, S, false);
-        if constexpr (Q8) {
-            const float ts = weigh_q8(S, base, held, all, u & 3);
-            l += ts;
-            if (!inner && !__any(ts != 0.f)) return;
-        } else {
         if (more) issue(u + 1, next, buf ^ 1);
         float ts = weigh(S, base, held, all, mNew);
         if (HALF && __any(ts != ts)) {            // (not a loop: what the masks need would be worked out ahead of it, for every unit)
@@ -1425,24 +1444,13 @@ struct WideTile {
         }
         l += ts;
         if (!inner && !__any(ts != 0.f)) return;          // (no row has anything here)
-        }
         if (AGAIN && pass != FINITE) {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) S[b][i] = S[b][i] > 0.f ? 1.f : 0.f;
         }
-        Weights w;
-        if constexpr (HALF) {
-#pragma unroll
-            for (int kk = 0; kk < UK / 16; kk++)
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float x = S[kk / 2][8 * (kk % 2) + i];
-                    w.hi[kk][i] = (_Float16)x;
-                    w.lo[kk][i] = (_Float16)(x - (float)w.hi[kk][i]);
-                }
-        }
+        const Weights w = weights(S);
         const unsigned Vl = v_base(V);
 #pragma unroll
         for (int d = 0; d < DB; d++) {
@@ -1467,20 +1475,83 @@ struct WideTile {
             buf ^= 1;
         }
     }
-    // Q8: a unit's raw rows come two units ahead and become operands one ahead
+    // Q8: unit u, of page numbers `here`, in buffer `buf`; the raw rows of the one behind it become operands on the way, between the matrix
+    // instructions of the scores.  LDS reads run ahead of what waits for them: all of K, then all of V before the weights are worked out.
+    __device__ __forceinline__ void compute_q8(int u, unsigned buf) {
+        const int base = base_of(u), mine = here;
+        uint4_t rows[CN];
+        raw_rows(buf ^ 1, rows);
+        if (!active || base >= end || base + UK <= begin) {
+            convert(rows, buf ^ 1);
+            return;
+        }
+        const unsigned K = ldsBase + buf * BUFB, Vl = v_base(K + TILEB);
+        const unsigned long long held = __ballot(mine >= 0);
+        constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
+        const bool inner = base + UK <= t.prefix || (base >= t.from && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
+        const bool all = inner && (held & runs) == runs;
+        float16_t S[NB];
+        uint4_t k[QS];
+        const int r = anew(n32);
+        const unsigned at = K + (unsigned)r * ROWB + (unsigned)(hf ^ swz(r)) * 16;
+#pragma unroll
+        for (int s = 0; s < QS; s++) k[s] = lds16(at ^ (unsigned)(s * 32));
+#pragma unroll
+        for (int i = 0; i < 16; i++) S[0][i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < QS; s++) {
+            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, k[s]), qh[s], S[0], 0, 0, 0);
+            S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, k[s]), ql[s], S[0], 0, 0, 0);
+        }
+        convert(rows, buf ^ 1);
+        __builtin_amdgcn_sched_group_barrier(0x100, CN + QS, 0);         // LDS reads, then by turns a matrix instruction and a few others
+#pragma unroll
+        for (int i = 0; i < 2 * QS; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        half8_t v[DB][UK / 16];
+#pragma unroll
+        for (int d = 0; d < DB; d++)
+#pragma unroll
+            for (int kk = 0; kk < UK / 16; kk++) v[d][kk] = v_piece(Vl ^ (unsigned)(d * 64), kk);
+        __builtin_amdgcn_sched_barrier(0);
+        float f;
+        const float ts = weigh_q8(S, base, held, all, u & 3, f);
+        if (__any(f != 1.f)) {
+            l *= f;
+#pragma unroll
+            for (int b = 0; b < DB; b++) o[b] *= f;
+        }
+        l += ts;
+        if (!inner && !__any(ts != 0.f)) return;          // (no row has anything here)
+        const Weights w = weights(S);
+#pragma unroll
+        for (int kk = 0; kk < UK / 16; kk++)
+#pragma unroll
+            for (int d = 0; d < DB; d++) {
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d][kk], w.hi[kk], o[d], 0, 0, 0);
+                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d][kk], w.lo[kk], o[d], 0, 0, 0);
+            }
+    }
+    // A unit's raw rows come two units ahead and become operands one ahead
     __device__ __forceinline__ void units_q8(int u0, int u1) {
         if (u0 + 1 < u1) issue_q8(u0 + 1, next, 1, (u0 + 1) & 3);
         int third = page_of(min(u0 + 2, u1 - 1));
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        convert(0, 0);
+        {
+            uint4_t rows[CN];
+            raw_rows(0, rows);
+            convert(rows, 0);
+        }
         unsigned buf = 0;
         for (int u = u0; u < u1; u++) {
             // the next unit's raw rows have landed, this one's operands are written; nobody reads the raw rows or the operands before them any more
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             const int fourth = page_of(min(u + 3, u1 - 1));
             if (u + 2 < u1) issue_q8(u + 2, third, buf, (u + 2) & 3);
-            if (u + 1 < u1) convert(buf ^ 1, buf ^ 1);
-            compute<false>(u, false, buf, 0);
+            compute_q8(u, buf);           // (behind the last unit it converts rows that nobody takes)
             here = next;
             next = third;
             third = fourth;
