@@ -30,6 +30,7 @@ static_assert(NARROW_WORKERS * NARROW <= MERGE_LDS, "a narrow tile's shares are 
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
+typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef float float4_t __attribute__((ext_vector_type(4)));
 typedef float float16_t __attribute__((ext_vector_type(16)));
 typedef unsigned uint16v_t __attribute__((ext_vector_type(16)));
@@ -453,18 +454,29 @@ __device__ __forceinline__ int shared_pos(const PagedAttention& p, int row) {
 // where they are 0); the same for -infinity and NaN; with zeros for all three.  An element is what the last time gives, plus an
 // infinity where the first count is not 0, minus one where the second is not.  Other tiles pay for a look at their result.
 enum { PLUS_INFINITE, MINUS_INFINITE, FINITE };
+// Two weights as elements i and i + 1 of both terms: rounded to fp16, and what that leaves.  The latter in one instruction that takes halves
+// and floats: x + minus1 * hi, where the compiler would make a subtraction, with a conversion ahead of it, of x - hi.
+__device__ __forceinline__ void two_terms(float x, float y, int i, half8_t& hi, half8_t& lo, float minus1) {
+    const half2_t h = __builtin_convertvector(float2_t{x, y}, half2_t);
+    hi[i] = h[0];
+    hi[i + 1] = h[1];
+    const half2_t l = __builtin_convertvector(float2_t{fmaf((float)h[0], minus1, x), fmaf((float)h[1], minus1, y)}, half2_t);
+    lo[i] = l[0];
+    lo[i + 1] = l[1];
+}
 // Two bytes that were xored with 0x80, each under a byte 0x64 -- halves of 1024 + (q + 128), whose last place is 1 -- as the halves q
 __device__ __forceinline__ unsigned signed_halves(unsigned x) {
     const half2_t bias = {(_Float16)-1152.f, (_Float16)-1152.f};
     return __builtin_bit_cast(unsigned, __builtin_bit_cast(half2_t, x) + bias);
 }
-// Eight signed bytes as halves
+// Signed bytes as halves
+__device__ __forceinline__ uint2_t four_halves(unsigned x) {
+    x ^= 0x80808080u;
+    return uint2_t{signed_halves(__builtin_amdgcn_perm(x, 0x64646464u, 0x00050004u)), signed_halves(__builtin_amdgcn_perm(x, 0x64646464u, 0x00070006u))};
+}
 __device__ __forceinline__ half8_t eight_halves(unsigned lo, unsigned hi) {
-    lo ^= 0x80808080u;
-    hi ^= 0x80808080u;
-    const uint4_t x = {signed_halves(__builtin_amdgcn_perm(lo, 0x64646464u, 0x00050004u)), signed_halves(__builtin_amdgcn_perm(lo, 0x64646464u, 0x00070006u)),
-                       signed_halves(__builtin_amdgcn_perm(hi, 0x64646464u, 0x00050004u)), signed_halves(__builtin_amdgcn_perm(hi, 0x64646464u, 0x00070006u))};
-    return __builtin_bit_cast(half8_t, x);
+    const uint2_t x = four_halves(lo), y = four_halves(hi);
+    return __builtin_bit_cast(half8_t, uint4_t{x[0], x[1], y[0], y[1]});
 }
 // What stands for the values of a word in a pass
 template <bool HALF>
@@ -1026,6 +1038,7 @@ struct WideTile {
     float4_t qf[HALF ? 1 : QS];
     float m, l;
     float ref;                       // Q8: probabilities are 2^(x - ref)
+    float minus1;                    // -1, in a register (two_terms)
     float16_t o[DB];
 
     static __device__ __forceinline__ int swz(int r) { return HALF ? ((r & 3) << 1) | ((r >> 2) & 1) : r & 7; }
@@ -1163,21 +1176,30 @@ struct WideTile {
     // Raw buffer `raw` as operands in buffer `buf`: a thread's 16 bytes of a row are two pieces of halves
     static constexpr int CN = Q8 ? 2 * RAWB / 16 / WG : 1;
     __device__ __forceinline__ void raw_rows(unsigned raw, uint4_t (&x)[CN]) const {
-        const unsigned in = ldsBase + RAW + raw * 2 * RAWB + (unsigned)thread_anew() * 16;
+        const unsigned in = ldsBase + RAW + raw * 2 * RAWB + (unsigned)(64 * wave + lane) * 16;
 #pragma unroll
         for (int n = 0; n < CN; n++) x[n] = lds16(in + n * WG * 16);
     }
-    __device__ __forceinline__ void convert(const uint4_t (&rows)[CN], unsigned buf) const {
-        const unsigned tid = (unsigned)thread_anew();
+    // Where the thread's first piece goes in buffer 0; the second is 16 bytes off (either way), the next 16 bytes' are V's (two rows sets of 32
+    // apart, HD = 128) or none
+    __device__ __forceinline__ unsigned first_piece() const {
+        const int i = 64 * wave + lane, r = i / PR;
+        return ldsBase + (unsigned)r * ROWB + (unsigned)((2 * (i % PR)) ^ swz(r)) * 16;
+    }
+    // Word s of the thread's 4 CN; every other one completes a piece
+    struct Halves { unsigned x[4]; };
+    static __device__ __forceinline__ void convert(const uint4_t (&rows)[CN], unsigned to, int s, Halves& h) {
+        const uint2_t x = four_halves(rows[s / 4][s % 4]);
+        h.x[s % 2 * 2] = x[0];
+        h.x[s % 2 * 2 + 1] = x[1];
+        if (s % 2 == 0) return;
         typedef __attribute__((address_space(3))) uint4_t* lp;
+        *reinterpret_cast<lp>((s % 4 == 1 ? to : to ^ 16u) + (unsigned)(s / 4) * (WG / PR * ROWB)) = uint4_t{h.x[0], h.x[1], h.x[2], h.x[3]};
+    }
+    static __device__ __forceinline__ void convert(const uint4_t (&rows)[CN], unsigned to) {
+        Halves h;
 #pragma unroll
-        for (int n = 0; n < CN; n++) {
-            const unsigned i = tid + n * WG, r = i / PR, piece = 2 * (i % PR);       // (V's rows behind K's)
-            const uint4_t x = rows[n];
-            const unsigned row = ldsBase + buf * BUFB + r * ROWB, s = (unsigned)swz((int)r);
-            *reinterpret_cast<lp>(row + (piece ^ s) * 16) = __builtin_bit_cast(uint4_t, eight_halves(x[0], x[1]));
-            *reinterpret_cast<lp>(row + ((piece + 1) ^ s) * 16) = __builtin_bit_cast(uint4_t, eight_halves(x[2], x[3]));
-        }
+        for (int s = 0; s < 4 * CN; s++) convert(rows, to, s, h);
     }
     static __device__ __forceinline__ uint4_t lds16(unsigned at) { return *reinterpret_cast<__attribute__((address_space(3))) const uint4_t*>(at); }
     // S^T of a unit: element i of block b is position 32 b + 8 (i/4) + 4 hf + i%4.  mends: where a NaN comes from the second term's
@@ -1322,22 +1344,17 @@ struct WideTile {
     }
     // Q8: scores to weights of V's whole numbers, as NarrowTile::weigh_q8; returns the lane's sum of the probabilities (times 2^(m - ref)).  f: what
     // l and o are multiplied by first (in one place, once: where a loop changes o in several, the compiler keeps it twice and moves it).
-    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, unsigned slot, float& f) {
+    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, const float4_t (&ks)[4], const float4_t (&vs)[4], float& f) {
         constexpr float FIT = 32768.f;
+        static_assert(!Q8 || NB == 1, "16 positions a lane");
         f = 1.f;
-        const int h4 = 4 * anew(hf), first = base + h4;
-        const unsigned scales = ldsBase + SCALES + slot * 2 * SCALEB + (unsigned)h4 * 4;
-        auto scale4 = [&](int which, int b, int i) { return __builtin_bit_cast(float4_t, lds16(scales + which * SCALEB + (32 * b + 8 * i) * 4)); };
+        const int first = base + 4 * anew(hf);
         auto exponent = [](float most) { return (float)(12 - __builtin_amdgcn_frexp_expf(fminf(most, FLT_MAX))); };
         auto both = [](float x) { float other = x; row_swap32(x, other); return fmaxf(x, other); };
 #pragma unroll
         for (int b = 0; b < NB; b++)
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const float4_t d = scale4(0, b, i);
-#pragma unroll
-                for (int j = 0; j < 4; j++) S[b][4 * i + j] *= d[j];
-            }
+            for (int i = 0; i < 16; i++) S[b][i] *= ks[i / 4][i % 4];
         if constexpr (MOD) {
 #pragma unroll
             for (int b = 0; b < NB; b++) S[b] *= c;
@@ -1373,11 +1390,7 @@ struct WideTile {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4_t d = scale4(1, b, i);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) most = fmaxf(most, __builtin_amdgcn_exp2f(fmaf(S[b][4 * i + j], factor, -from)) * d[j]);
-                }
+                for (int i = 0; i < 16; i++) most = fmaxf(most, __builtin_amdgcn_exp2f(fmaf(S[b][i], factor, -from)) * vs[i / 4][i % 4]);
             most = both(most);
             const float to = mNew != m ? from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), 110.f)) : 0.f) : ref;
             f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to);
@@ -1389,15 +1402,11 @@ struct WideTile {
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float4_t d = scale4(1, b, i);
-#pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const float x = __builtin_amdgcn_exp2f(fmaf(S[b][4 * i + j], factor, -ref));
-                        ts += x;
-                        S[b][4 * i + j] = product(x, d[j]);
-                        most = fmaxf(most, S[b][4 * i + j]);
-                    }
+                for (int i = 0; i < 16; i++) {
+                    const float x = __builtin_amdgcn_exp2f(fmaf(S[b][i], factor, -ref));
+                    ts += x;
+                    S[b][i] = product(x, vs[i / 4][i % 4]);
+                    most = fmaxf(most, S[b][i]);
                 }
         };
         if (all) weights([](float x, float d) { return x * d; });
@@ -1477,48 +1486,51 @@ struct WideTile {
     }
     // Q8: unit u, of page numbers `here`, in buffer `buf`; the raw rows of the one behind it become operands on the way, between the matrix
     // instructions of the scores.  LDS reads run ahead of what waits for them: all of K, then all of V before the weights are worked out.
-    __device__ __forceinline__ void compute_q8(int u, unsigned buf) {
+    __device__ __forceinline__ void compute_q8(int u, unsigned buf, unsigned piece, unsigned kAt, unsigned vAt) {
         const int base = base_of(u), mine = here;
+        const unsigned to = piece + (buf ^ 1) * BUFB;
         uint4_t rows[CN];
         raw_rows(buf ^ 1, rows);
         if (!active || base >= end || base + UK <= begin) {
-            convert(rows, buf ^ 1);
+            convert(rows, to);
             return;
         }
-        const unsigned K = ldsBase + buf * BUFB, Vl = v_base(K + TILEB);
+        const unsigned K = kAt + buf * BUFB, V = vAt + buf * BUFB;
         const unsigned long long held = __ballot(mine >= 0);
         constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
         const bool inner = base + UK <= t.prefix || (base >= t.from && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
         const bool all = inner && (held & runs) == runs;
         float16_t S[NB];
         uint4_t k[QS];
-        const int r = anew(n32);
-        const unsigned at = K + (unsigned)r * ROWB + (unsigned)(hf ^ swz(r)) * 16;
+        // (a row's offset from its first piece's: bits 5 and 6 are among those that the piece is turned about by, bit 7 is not)
 #pragma unroll
-        for (int s = 0; s < QS; s++) k[s] = lds16(at ^ (unsigned)(s * 32));
+        for (int s = 0; s < QS; s++) k[s] = lds16((K ^ (unsigned)(s % 4 * 32)) + s / 4 * 128);
 #pragma unroll
         for (int i = 0; i < 16; i++) S[0][i] = 0.f;
+        const unsigned scales = ldsBase + SCALES + (u & 3) * 2 * SCALEB + (unsigned)hf * 16;
+        float4_t ks[4], vs[4];
+        static_assert(!Q8 || QS == 4 * CN, "a word a step");
+        Halves h;
 #pragma unroll
         for (int s = 0; s < QS; s++) {
+            __builtin_amdgcn_sched_barrier(0);
             S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, k[s]), qh[s], S[0], 0, 0, 0);
             S[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8_t, k[s]), ql[s], S[0], 0, 0, 0);
-        }
-        convert(rows, buf ^ 1);
-        __builtin_amdgcn_sched_group_barrier(0x100, CN + QS, 0);         // LDS reads, then by turns a matrix instruction and a few others
-#pragma unroll
-        for (int i = 0; i < 2 * QS; i++) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+            convert(rows, to, s, h);
         }
         __builtin_amdgcn_sched_barrier(0);
         half8_t v[DB][UK / 16];
 #pragma unroll
+        for (int i = 0; i < 4; i++) ks[i] = __builtin_bit_cast(float4_t, lds16(scales + i * 32));
+#pragma unroll
+        for (int i = 0; i < 4; i++) vs[i] = __builtin_bit_cast(float4_t, lds16(scales + SCALEB + i * 32));
+#pragma unroll
         for (int d = 0; d < DB; d++)
 #pragma unroll
-            for (int kk = 0; kk < UK / 16; kk++) v[d][kk] = v_piece(Vl ^ (unsigned)(d * 64), kk);
+            for (int kk = 0; kk < UK / 16; kk++) v[d][kk] = v_piece(V ^ (unsigned)(d * 64), kk);
         __builtin_amdgcn_sched_barrier(0);
         float f;
-        const float ts = weigh_q8(S, base, held, all, u & 3, f);
+        const float ts = weigh_q8(S, base, held, all, ks, vs, f);
         if (__any(f != 1.f)) {
             l *= f;
 #pragma unroll
@@ -1526,13 +1538,21 @@ struct WideTile {
         }
         l += ts;
         if (!inner && !__any(ts != 0.f)) return;          // (no row has anything here)
-        const Weights w = weights(S);
+        Weights w;
+        auto halve = [&](int i) { two_terms(S[0][i], S[0][i + 1], i % 8, w.hi[i / 8], w.lo[i / 8], minus1); };
+#pragma unroll
+        for (int i = 0; i < 8; i += 2) halve(i);
 #pragma unroll
         for (int kk = 0; kk < UK / 16; kk++)
 #pragma unroll
             for (int d = 0; d < DB; d++) {
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d][kk], w.hi[kk], o[d], 0, 0, 0);
                 o[d] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v[d][kk], w.lo[kk], o[d], 0, 0, 0);
+                if (kk == 0) {
+#pragma unroll
+                    for (int i = 8 + d * (8 / DB); i < 8 + (d + 1) * (8 / DB); i += 2) halve(i);
+                }
+                __builtin_amdgcn_sched_barrier(0);
             }
     }
     // A unit's raw rows come two units ahead and become operands one ahead
@@ -1540,18 +1560,21 @@ struct WideTile {
         if (u0 + 1 < u1) issue_q8(u0 + 1, next, 1, (u0 + 1) & 3);
         int third = page_of(min(u0 + 2, u1 - 1));
         asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+        const unsigned piece = first_piece(), kAt = ldsBase + (unsigned)n32 * ROWB + (unsigned)(hf ^ swz(n32)) * 16, vAt = v_base(ldsBase + TILEB);
         {
             uint4_t rows[CN];
             raw_rows(0, rows);
-            convert(rows, 0);
+            convert(rows, piece);
         }
+        minus1 = -1.f;
+        asm volatile("" : "+v"(minus1));
         unsigned buf = 0;
         for (int u = u0; u < u1; u++) {
             // the next unit's raw rows have landed, this one's operands are written; nobody reads the raw rows or the operands before them any more
             asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
             const int fourth = page_of(min(u + 3, u1 - 1));
             if (u + 2 < u1) issue_q8(u + 2, third, buf, (u + 2) & 3);
-            compute_q8(u, buf);           // (behind the last unit it converts rows that nobody takes)
+            compute_q8(u, buf, piece, kAt, vAt);           // (behind the last unit it converts rows that nobody takes)
             here = next;
             next = third;
             third = fourth;
