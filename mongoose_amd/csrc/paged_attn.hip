@@ -24,9 +24,12 @@ constexpr int PLAN_LDS_TILES = 4096;      // tiles whose places on the line the 
 // positions 8.8 us, with two 10.8); a wide share costs its 64 KB out and in (8B shape, one fresh prompt: 469 rows fp16 29 us, with one 38,
 // with five 33; 409 rows fp32 52, with one 73, with two 70, with five 53).
 constexpr int LEAST_NARROW = 1, LEAST_WIDE = 3;
-constexpr int NARROW_WORKERS = 256;       // workgroups that narrow tiles have at most (a CU each)
+// Workgroups that narrow tiles have at most: one a CU, though a CU holds two, as HBM likes fewer streams (8B shape, fp16: 120,001 positions 98 us,
+// with two 113; 48 requests 174 and 182); two for a Q8 cache, whose vector instructions take as long as its bytes (48 requests 157 us with
+// one, 123 with two; 120,001 positions 79, 76).
+constexpr int NARROW_WORKERS = 256, NARROW_WORKERS_Q8 = 512;
 constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results
-static_assert(NARROW_WORKERS * NARROW <= MERGE_LDS, "a narrow tile's shares are weighed in one turn");
+static_assert(NARROW_WORKERS_Q8 * NARROW <= MERGE_LDS, "a narrow tile's shares are weighed in one turn");
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
@@ -38,8 +41,8 @@ typedef unsigned uint2_t __attribute__((ext_vector_type(2)));
 typedef unsigned uint4_t __attribute__((ext_vector_type(4)));
 typedef short short4_t __attribute__((ext_vector_type(4)));
 
-// Positions of a unit: a narrow tile's four waves take 64 of a Q8 cache, 32 of an fp16 one or 16 of an fp32 one each, a wide tile's share them.
-MG_HD int narrow_keys(int kvFormat) { return kvFormat == PAGED_F32 ? 64 : kvFormat == PAGED_F16 ? 128 : 256; }
+// Positions of a unit: a narrow tile's four waves take 32 of an fp16 or Q8 cache or 16 of an fp32 one each, a wide tile's share them.
+MG_HD int narrow_keys(int kvFormat) { return kvFormat == PAGED_F32 ? 64 : 128; }
 MG_HD int wide_keys(int kvFormat) { return kvFormat == PAGED_F16 ? 64 : 32; }
 
 // Rows a KV head (tokens x group) up to which a request goes to the kernel that waits for memory, with longer ones to the one that waits for
@@ -64,12 +67,10 @@ int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool grou
 int paged_max_tiles_shared(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / NARROW) + g.maxReqs; }
 int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + 256 / NARROW; }
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
-// Workgroups, in turns of the KV heads: two a CU for wide tiles; one a CU for narrow ones, though a CU holds two: HBM likes fewer
-// streams (8B shape, fp16: 120,001 positions 98 us, with two 113; 48 requests 174 and 182).  Fewer where the batch
-// cannot have that many units.
+// Workgroups, in turns of the KV heads: two a CU for wide tiles, as above for narrow ones.  Fewer where the batch cannot have that many units.
 int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide) {
     const long long tiles = (long long)rows * g.group / NARROW + nReqs, units = tiles * (g.maxLen / 32 + 2);
-    const int resident = NARROW_WORKERS * (wide ? 2 : 1);
+    const int resident = wide ? 2 * 256 : g.kvFormat == PAGED_Q8 ? NARROW_WORKERS_Q8 : NARROW_WORKERS;
     const long long most = resident / g.nKVHeads > 0 ? resident / g.nKVHeads : 1;
     return (int)(units < 1 ? 1 : units < most ? units : most);
 }
@@ -513,7 +514,7 @@ __device__ __forceinline__ int power_up(float top, float scale) {
 template <typename KVT, int HD, bool MOD>
 struct NarrowTile {
     static constexpr bool Q8 = sizeof(KVT) == 1, HALF = sizeof(KVT) <= 2;       // HALF: products of fp16 operands
-    static constexpr int KB = 64 / (int)sizeof(KVT);       // positions of a wave's step
+    static constexpr int KB = HALF ? 32 : 16;              // positions of a wave's step
     static constexpr int NB = KB / 16, UK = 4 * KB, EPL = HD / 16;
     static constexpr int KV4 = HD * (int)sizeof(KVT) / 64; // 16-byte pieces a lane holds of a block's K rows
     static constexpr int VW = EPL * (int)sizeof(KVT) / 4;  // words a lane holds of a V row
@@ -534,8 +535,10 @@ struct NarrowTile {
     unsigned v[NB * 4][VW];
     float4_t ks[Q8 ? NB : 1], vs[Q8 ? NB : 1];       // Q8: the scales of the lane's positions 16 b + 4 g + 0..3
     const char *Ksc, *Vsc;
+    unsigned kOff, vOff;           // Q8: where the lane's part of a block of 16 positions' rows starts
     float m, l;
     float ref;                     // Q8: probabilities are 2^(x - ref)
+    float minus1;                  // Q8: -1, in a register (two_terms)
     float4_t o[EPL];
 
     int here, next;                // page numbers of the step at hand and of the one behind it
@@ -556,6 +559,10 @@ struct NarrowTile {
             const size_t slots = (size_t)p.g.nPages * p.g.pageSize, head = (size_t)kvh * p.g.pageSize * 4;
             Ksc = static_cast<const char*>(p.K) + slots * rowBytes + head;
             Vsc = static_cast<const char*>(p.V) + slots * rowBytes + head;
+            kOff = (unsigned)l16 * (unsigned)rowBytes + (unsigned)g * 16;
+            vOff = (unsigned)(4 * g) * (unsigned)rowBytes + (unsigned)l16 * (VW * 4);
+            minus1 = -1.f;
+            asm volatile("" : "+v"(minus1));
         }
         here = page_of(u0);
         const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
@@ -609,15 +616,41 @@ struct NarrowTile {
     }
     // The page of the positions 16 b .. 16 b + 15 that the lane has to do with: of its upper eight or its lower
     __device__ __forceinline__ int page_in(int mine, int b, bool upper) const {
-        if constexpr (Q8) {                           // (eight runs: each one's page in a scalar register)
+        if constexpr (Q8) {                           // (in scalar registers)
             const int lo = __builtin_amdgcn_readlane(mine, 2 * b), hi = __builtin_amdgcn_readlane(mine, 2 * b + 1);
             return upper ? hi : lo;
         }
         const int lo = HALF && b ? quad_lane<2>(mine) : quad_lane<0>(mine), hi = HALF && b ? quad_lane<3>(mine) : quad_lane<1>(mine);
         return upper ? hi : lo;                       // (all lanes take part in both exchanges)
     }
+    // Q8: whether a step's positions are all there, in pages of whole blocks of 16: the rows and scales of a block then start at scalar addresses
+    // (8B shape, 120,001 positions: 60 us, with an address worked out for every row 67)
+    __device__ __forceinline__ bool whole(int u, int mine) const {
+        const int base = base_of(u);
+        return p.g.pageShift >= 4 && base >= span.begin && base + KB <= span.end && (__ballot(mine >= 0) & ((1u << (KB / 8)) - 1)) == (1u << (KB / 8)) - 1;
+    }
+    __device__ __forceinline__ const char* block_rows(const char* pool, int base, int mine, int b) const {
+        const int page = __builtin_amdgcn_readlane(mine, 2 * b);
+        return pool + (size_t)(((unsigned)page << p.g.pageShift) + ((unsigned)(base + 16 * b) & (unsigned)(p.g.pageSize - 1))) * rowBytes;
+    }
+    __device__ __forceinline__ const char* block_scales(const char* scales, int base, int mine, int b) const {
+        const int page = __builtin_amdgcn_readlane(mine, 2 * b);
+        return scales + (((size_t)(unsigned)page * p.g.nKVHeads << p.g.pageShift) + ((unsigned)(base + 16 * b) & (unsigned)(p.g.pageSize - 1))) * 4;
+    }
     __device__ __forceinline__ void load_k(int u, int mine) {
         const int base = base_of(u);
+        if constexpr (Q8) {
+            if (whole(u, mine)) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const char* at = block_rows(Kp, base, mine, b);
+#pragma unroll
+                    for (int i = 0; i < KV4; i++) k[b][i] = *reinterpret_cast<const uint4_t*>(at + (kOff + i * 64));
+                    ks[b] = *reinterpret_cast<const float4_t*>(block_scales(Ksc, base, mine, b) + (unsigned)(g * 16));
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             const char* at = kv_row(Kp, zeros, rowBytes, base + 16 * b + l16, page_in(mine, b, l16 & 8), span.begin, span.end, p.g.pageShift) + g * 16;
@@ -637,6 +670,25 @@ struct NarrowTile {
     }
     __device__ __forceinline__ void load_v(int u, int mine) {
         const int base = base_of(u);
+        if constexpr (Q8) {
+            if (whole(u, mine)) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) {
+                    const char* at = block_rows(Vp, base, mine, b);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const char* row = at + (vOff + (unsigned)j * (unsigned)rowBytes);
+                        if constexpr (VW == 1) v[4 * b + j][0] = *reinterpret_cast<const unsigned*>(row);
+                        else {
+                            const uint2 x = *reinterpret_cast<const uint2*>(row);
+                            v[4 * b + j][0] = x.x; v[4 * b + j][1] = x.y;
+                        }
+                    }
+                    vs[b] = *reinterpret_cast<const float4_t*>(block_scales(Vsc, base, mine, b) + (unsigned)(g * 16));
+                }
+                return;
+            }
+        }
 #pragma unroll
         for (int j = 0; j < NB * 4; j++) {
             const int page = page_in(mine, j / 4, g & 2);
@@ -657,11 +709,14 @@ struct NarrowTile {
         }
         if constexpr (Q8) load_scales(vs, Vsc, base, mine);
     }
-    static constexpr int WS = Q8 ? NB / 2 : 1;        // products of 32 positions a step
+    static constexpr int WS = HALF ? NB / 2 : 1;      // products of 32 positions a step
     struct Weights { half8_t hi[WS], lo[WS]; float x[NB * 4]; };
-    static __device__ __forceinline__ Weights weights(const float (&x)[NB * 4]) {
+    __device__ __forceinline__ Weights weights(const float (&x)[NB * 4]) const {
         Weights w;
-        if constexpr (HALF) {
+        if constexpr (Q8) {
+#pragma unroll
+            for (int j = 0; j < NB * 4; j += 2) two_terms(x[j], x[j + 1], j % 8, w.hi[j / 8], w.lo[j / 8], minus1);
+        } else if constexpr (HALF) {
 #pragma unroll
             for (int s = 0; s < WS; s++)
 #pragma unroll
