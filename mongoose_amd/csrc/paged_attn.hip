@@ -623,33 +623,32 @@ struct NarrowTile {
         const int lo = HALF && b ? quad_lane<2>(mine) : quad_lane<0>(mine), hi = HALF && b ? quad_lane<3>(mine) : quad_lane<1>(mine);
         return upper ? hi : lo;                       // (all lanes take part in both exchanges)
     }
-    // Q8: whether a step's positions are all there, in pages of whole blocks of 16: the rows and scales of a block then start at scalar addresses
-    // (8B shape, 120,001 positions: 60 us, with an address worked out for every row 67)
-    __device__ __forceinline__ bool whole(int u, int mine) const {
-        const int base = base_of(u);
-        return p.g.pageShift >= 4 && base >= span.begin && base + KB <= span.end && (__ballot(mine >= 0) & ((1u << (KB / 8)) - 1)) == (1u << (KB / 8)) - 1;
-    }
-    __device__ __forceinline__ const char* block_rows(const char* pool, int base, int mine, int b) const {
-        const int page = __builtin_amdgcn_readlane(mine, 2 * b);
-        return pool + (size_t)(((unsigned)page << p.g.pageShift) + ((unsigned)(base + 16 * b) & (unsigned)(p.g.pageSize - 1))) * rowBytes;
+    // Q8: where the lane's part of a block of 16 positions starts, rows and scales, given the lane's offset from the block's start.  Pages of whole
+    // blocks have scalar addresses.  Rows that are not the tile's (in front of its first or behind its last position) are read all
+    // the same, and those of a page that is gone from page 0: whole numbers are always numbers, and their weights are zeros.
+    __device__ __forceinline__ const char* block_rows(const char* pool, int base, int mine, int b, unsigned off, bool upper) const {
+        const unsigned lo = (unsigned)max(__builtin_amdgcn_readlane(mine, 2 * b), 0), place = (unsigned)(base + 16 * b) & (unsigned)(p.g.pageSize - 1);
+        if (p.g.pageShift >= 4) return pool + (size_t)((lo << p.g.pageShift) + place) * rowBytes + off;
+        const unsigned hi = (unsigned)max(__builtin_amdgcn_readlane(mine, 2 * b + 1), 0);
+        return pool + (long long)(upper ? (int)hi - 1 : (int)lo) * 8 * (long long)rowBytes + off;          // (the offset is from the block's start)
     }
     __device__ __forceinline__ const char* block_scales(const char* scales, int base, int mine, int b) const {
-        const int page = __builtin_amdgcn_readlane(mine, 2 * b);
-        return scales + (((size_t)(unsigned)page * p.g.nKVHeads << p.g.pageShift) + ((unsigned)(base + 16 * b) & (unsigned)(p.g.pageSize - 1))) * 4;
+        const unsigned lo = (unsigned)max(__builtin_amdgcn_readlane(mine, 2 * b), 0), place = (unsigned)(base + 16 * b) & (unsigned)(p.g.pageSize - 1);
+        if (p.g.pageShift >= 4) return scales + (((size_t)lo * p.g.nKVHeads << p.g.pageShift) + place) * 4 + (unsigned)(g * 16);
+        const unsigned hi = (unsigned)max(__builtin_amdgcn_readlane(mine, 2 * b + 1), 0);
+        return scales + (size_t)(g & 2 ? hi : lo) * p.g.nKVHeads * 32 + (unsigned)(g & 1) * 16;
     }
     __device__ __forceinline__ void load_k(int u, int mine) {
         const int base = base_of(u);
         if constexpr (Q8) {
-            if (whole(u, mine)) {
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const char* at = block_rows(Kp, base, mine, b);
+            for (int b = 0; b < NB; b++) {
+                const char* at = block_rows(Kp, base, mine, b, kOff, l16 & 8);
 #pragma unroll
-                    for (int i = 0; i < KV4; i++) k[b][i] = *reinterpret_cast<const uint4_t*>(at + (kOff + i * 64));
-                    ks[b] = *reinterpret_cast<const float4_t*>(block_scales(Ksc, base, mine, b) + (unsigned)(g * 16));
-                }
-                return;
+                for (int i = 0; i < KV4; i++) k[b][i] = *reinterpret_cast<const uint4_t*>(at + i * 64);
+                ks[b] = *reinterpret_cast<const float4_t*>(block_scales(Ksc, base, mine, b));
             }
+            return;
         }
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -657,45 +656,30 @@ struct NarrowTile {
 #pragma unroll
             for (int i = 0; i < KV4; i++) k[b][i] = *reinterpret_cast<const uint4_t*>(at + i * 64);
         }
-        if constexpr (Q8) load_scales(ks, Ksc, base, mine);
-    }
-    // The scales of the lane's positions, by fours (what lies behind a request's end is read and not used)
-    __device__ __forceinline__ void load_scales(float4_t (&to)[Q8 ? NB : 1], const char* from, int base, int mine) const {
-#pragma unroll
-        for (int b = 0; b < (Q8 ? NB : 1); b++) {
-            const int page = page_in(mine, b, g & 2);
-            const size_t at = page >= 0 ? (((size_t)(unsigned)page * p.g.nKVHeads << p.g.pageShift) + ((unsigned)(base + 16 * b + 4 * g) & (unsigned)(p.g.pageSize - 1))) * 4 : 0;
-            to[b] = *reinterpret_cast<const float4_t*>((page >= 0 ? from : zeros) + at);
-        }
     }
     __device__ __forceinline__ void load_v(int u, int mine) {
         const int base = base_of(u);
         if constexpr (Q8) {
-            if (whole(u, mine)) {
 #pragma unroll
-                for (int b = 0; b < NB; b++) {
-                    const char* at = block_rows(Vp, base, mine, b);
+            for (int b = 0; b < NB; b++) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        const char* row = at + (vOff + (unsigned)j * (unsigned)rowBytes);
-                        if constexpr (VW == 1) v[4 * b + j][0] = *reinterpret_cast<const unsigned*>(row);
-                        else {
-                            const uint2 x = *reinterpret_cast<const uint2*>(row);
-                            v[4 * b + j][0] = x.x; v[4 * b + j][1] = x.y;
-                        }
+                for (int j = 0; j < 4; j++) {
+                    const char* at = block_rows(Vp, base, mine, b, vOff + (unsigned)j * (unsigned)rowBytes, g & 2);
+                    if constexpr (VW == 1) v[4 * b + j][0] = *reinterpret_cast<const unsigned*>(at);
+                    else {
+                        const uint2 x = *reinterpret_cast<const uint2*>(at);
+                        v[4 * b + j][0] = x.x; v[4 * b + j][1] = x.y;
                     }
-                    vs[b] = *reinterpret_cast<const float4_t*>(block_scales(Vsc, base, mine, b) + (unsigned)(g * 16));
                 }
-                return;
+                vs[b] = *reinterpret_cast<const float4_t*>(block_scales(Vsc, base, mine, b));
             }
+            return;
         }
 #pragma unroll
         for (int j = 0; j < NB * 4; j++) {
             const int page = page_in(mine, j / 4, g & 2);
             const char* at = kv_row(Vp, zeros, rowBytes, base + 16 * (j / 4) + 4 * g + j % 4, page, span.begin, span.end, p.g.pageShift) + l16 * (VW * 4);
-            if constexpr (VW == 1) {
-                v[j][0] = *reinterpret_cast<const unsigned*>(at);
-            } else if constexpr (VW == 2) {
+            if constexpr (VW == 2) {
                 const uint2 x = *reinterpret_cast<const uint2*>(at);
                 v[j][0] = x.x; v[j][1] = x.y;
             } else {
@@ -707,7 +691,6 @@ struct NarrowTile {
                 }
             }
         }
-        if constexpr (Q8) load_scales(vs, Vsc, base, mine);
     }
     static constexpr int WS = HALF ? NB / 2 : 1;      // products of 32 positions a step
     struct Weights { half8_t hi[WS], lo[WS]; float x[NB * 4]; };
@@ -914,6 +897,18 @@ struct NarrowTile {
     }
     template <bool AGAIN>
     __device__ __forceinline__ void units(int u0, int u1, int pass) {
+        if constexpr (Q8) {
+            // (the last step by itself: where a step may ask for nothing, the wait for what it has itself would be one for all that is under way)
+            for (int u = u0; u + 1 < u1; u++) {
+                const int behind = page_of(min(u + 2, u1 - 1));
+                compute<AGAIN>(u, here, true, next, pass);
+                load_v(u + 1, next);
+                here = next;
+                next = behind;
+            }
+            compute<AGAIN>(u1 - 1, here, false, next, pass);
+            return;
+        }
         for (int u = u0; u < u1; u++) {
             const int behind = page_of(min(u + 2, u1 - 1));
             const bool more = u + 1 < u1;
