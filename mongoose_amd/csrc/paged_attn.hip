@@ -28,7 +28,7 @@ constexpr int LEAST_NARROW = 1, LEAST_WIDE = 3;
 // with two 113; 48 requests 174 and 182); two for a Q8 cache, whose vector instructions take as long as its bytes (48 requests 157 us with
 // one, 123 with two; 120,001 positions 79, 76).
 constexpr int NARROW_WORKERS = 256, NARROW_WORKERS_Q8 = 512;
-constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results
+constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results, and as many for their sums
 static_assert(NARROW_WORKERS_Q8 * NARROW <= MERGE_LDS, "a narrow tile's shares are weighed in one turn");
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
@@ -399,6 +399,38 @@ template <int HD, int ROWS>
 __device__ __forceinline__ void merge_weights(const PagedAttention& p, const PagedTile& t, int kvh, int R, int s0, int n, float* M, float* den, float* wt) {
     const int tid = thread_anew(), segs = t.worker1 - t.worker0 + 1;
     auto at = [&](int s, int i) { return part_of(p, t, kvh, t.worker0 + s)[ROWS * HD + i]; };
+    if constexpr (ROWS == NARROW) {
+        // One turn, a row's shares fetched by 16 threads: what it costs is the round trips to memory (8B shape, fp16, 5,000 positions in 40
+        // shares: 17 us a call, with one thread a row as below 23)
+        float* sums = wt + MERGE_LDS;
+        const int r = tid % ROWS;
+        float m = -INFINITY;
+#pragma unroll 4
+        for (int s = tid / ROWS; s < n; s += WG / ROWS) {          // (rows past the last: anything)
+            const float x = at(s, r);
+            sums[s * ROWS + r] = at(s, ROWS + r);
+            wt[s * ROWS + r] = x;
+            m = fmaxf(m, x);
+        }
+        M[tid] = m;
+        __syncthreads();
+        if (tid < ROWS) {
+#pragma unroll
+            for (int i = 1; i < WG / ROWS; i++) m = fmaxf(m, M[tid + i * ROWS]);
+        }
+        __syncthreads();
+        if (tid < ROWS) M[tid] = m == -INFINITY ? 0.f : m;
+        __syncthreads();
+        for (int i = tid; i < n * ROWS; i += WG) wt[i] = __builtin_amdgcn_exp2f(wt[i] - M[r]);
+        __syncthreads();
+        if (tid < R) {
+            float d = 0.f;
+#pragma unroll 8
+            for (int s = 0; s < n; s++) d = fmaf(wt[s * ROWS + tid], sums[s * ROWS + tid], d);
+            den[tid] = d;
+        }
+        return;
+    }
     if (s0 == 0 && tid < R) {
         float m = -INFINITY;
 #pragma unroll 8
@@ -1013,7 +1045,7 @@ struct NarrowTile {
     }
     // All workers' shares: threads take rows and columns and, where there are fewer of those than threads, shares in turn
     __device__ __forceinline__ void merge(int kvh, int R, float* lds) const {
-        float *M = lds, *den = lds + NARROW, *wt = lds + 2 * NARROW;
+        float *M = lds, *den = lds + WG, *wt = den + NARROW;         // (M: a word a thread on the way)
         constexpr int N = NARROW * HD / 4 / WG > 0 ? NARROW * HD / 4 / WG : 1;
         const int tid = thread_anew(), segs = t.worker1 - t.worker0 + 1, cols = R * (HD / 4), par = max(1, WG / cols);
         float4_t acc[N];
@@ -1025,7 +1057,7 @@ struct NarrowTile {
             const int i = par > 1 ? tid % cols : tid + k * WG, from = par > 1 ? tid / cols : 0;
             if (i >= cols || from >= par || (par > 1 && k > 0)) continue;
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-#pragma unroll 4
+#pragma unroll 16
             for (int s = from; s < segs; s += par)
                 acc[k] += wt[s * NARROW + r] * *reinterpret_cast<const float4_t*>(part_of(p, t, kvh, t.worker0 + s) + r * HD + d);
         }
@@ -1778,7 +1810,7 @@ __global__ __launch_bounds__(WG, 2) void paged_wide_kernel(PagedAttention p) {
 
 static size_t attn_lds(int headDim, bool wide) {           // (wide, Q8: one buffer of halves, two of bytes, 1 KB of scales)
     const size_t tile = wide ? (size_t)2 * 2 * 64 * headDim * 2 + 1024 : (size_t)(4 * NARROW * (headDim + 4) + 8 * NARROW) * 4;
-    const size_t merge = (size_t)(2 * (wide ? WIDE : NARROW) + MERGE_LDS) * 4;
+    const size_t merge = (size_t)(wide ? 2 * WIDE + MERGE_LDS : WG + NARROW + 2 * MERGE_LDS) * 4;
     return tile > merge ? tile : merge;
 }
 template <typename F>
