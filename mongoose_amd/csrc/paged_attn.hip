@@ -52,8 +52,14 @@ MG_HD int wide_keys(int kvFormat) { return kvFormat == PAGED_F16 ? 64 : 32; }
 //   Larger batches: narrow up to 16 rows.  24 requests of 5, 8, 12 tokens over 500 to 4,000 positions, fp16: 77, 78, 80 us wide, 75, 81, 99
 //   narrow, and 96 requests of 5 tokens 208 wide, 304 narrow.  With an fp32 cache narrow tiles would be better there, up to 64 rows (228,
 //   204, 385, and with 16 tokens 361 us wide; 169, 141, 249, 276 narrow): its wide tiles wait for the fp32 instructions of rows that are not there.
+//   Q8: a wide tile also has its rows turned to halves for rows that are not there, so narrow ones go further: 24 requests of 5, 8, 12, 16 tokens
+//   as above 98, 90, 104, 113 us wide, 59, 55, 69, 90 narrow; 1.1B shape, 5 tokens 62 and 41.  With many requests, whose wide tiles fill the
+//   CUs, up to 32 rows: 96 requests of 5, 8, 16 tokens 233, 231, 299 and 203, 209, 405; 1.1B shape, 8 tokens 115 and 138.
+constexpr int NARROW_Q8_FEW = 64, NARROW_Q8 = 32, Q8_FEW_ROWS = 4096;
 int paged_narrow_rows(const PagedGeo& g, int rows) {
-    return (long long)rows * g.group <= 256 ? 256 : NARROW;
+    const long long all = (long long)rows * g.group;
+    if (all <= 256) return 256;
+    return g.kvFormat != PAGED_Q8 ? NARROW : all <= Q8_FEW_ROWS ? NARROW_Q8_FEW : NARROW_Q8;
 }
 // The same with shared prefixes, for groups (0: all groups have wide tiles) and for requests, of which the caller may know that none adds more than
 // mostNew rows.
@@ -61,11 +67,14 @@ int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool grou
     constexpr int ALL = PAGED_MAX_ROWS * PAGED_MAX_GROUP;
     if ((long long)rows * g.group <= 256) return ALL;
     if (groups) return 0;
-    return mostNew > 0 && (long long)mostNew * g.group <= NARROW ? ALL : NARROW;
+    const int narrow = paged_narrow_rows(g, rows);
+    return mostNew > 0 && (long long)mostNew * g.group <= narrow ? ALL : narrow;
 }
 // (with shared prefixes requests of any number of rows may have narrow tiles)
 int paged_max_tiles_shared(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / NARROW) + g.maxReqs; }
-int paged_max_tiles(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs + 256 / NARROW; }
+int paged_max_tiles(const PagedGeo& g) {
+    return (int)((long long)g.maxRows * g.group / WIDE) + g.maxReqs * (g.kvFormat == PAGED_Q8 ? NARROW_Q8_FEW / NARROW : 1) + 256 / NARROW;
+}
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
 // Workgroups, in turns of the KV heads: two a CU for wide tiles, as above for narrow ones.  Fewer where the batch cannot have that many units.
 int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide) {
