@@ -46,7 +46,8 @@ struct PagedPlanFor {
 struct PagedPlan {
     const int *rowStart, *lens, *prefixLens;      // the caller's
     const int4* given;                            // or, with shared prefixes, what paged_groups_kernel has made of them
-    bool grouped;                                 // `given` are groups
+    const int* groupOf;                           // ... and the requests' groups,
+    int* groupTile;                               // or, where `given` are groups: takes each one's first tile, and behind the last how many there are
     PagedPlanFor* made;                           // the handle's
     PagedTile* tiles;                             // maxTiles of them, for narrow tiles and again for wide ones,
     PagedWorker* workers;                         // and maxWorkers of these
@@ -59,6 +60,7 @@ hipError_t launch_paged_plan(const PagedPlan& p, hipStream_t s);
 struct PagedGroups {
     const int *rowStart, *lens, *groupStart, *sharedLens;      // the caller's
     int4* reqs;          // of every request: first row, rows, length, first position of its own
+    int* groupOf;        // its group
     int4* groups;        // of every group: first row, rows, shared positions, the request whose pages are read
     int nReqs, rows, nGroups, maxLen;
 };
@@ -78,11 +80,14 @@ struct PagedAttention {
     size_t partStride;
     float scale, softcap;
     PagedPlanFor plan;
-    // Shared prefixes: a call's first pass leaves each row's result over its group's positions here, [row, head][headDim] with the rows' maxima
-    // and sums behind, and its second one, over the requests' own positions, takes it in.
-    float* shared;
-    const int4* reqs;
+    // Shared prefixes: a call's first pass leaves its workers' shares of the groups' tiles as they are, and its second one, over the requests' own
+    // positions, takes those of its rows in.
     int pass;                  // 0: no prefix is shared; 1, 2
+    const int4 *reqs, *groups; // as in PagedGroups
+    const int* groupTile;
+    const PagedTile* sharedTiles;
+    const float* sharedParts;
+    int sharedWorkers, sharedRows;       // of the first pass: workers a KV head, rows of a tile
     int ldq, ldo, window, maxTiles, maxWorkers, nWorkers, wideWorkers;
     PagedGeo g;
 };

@@ -374,10 +374,11 @@ struct mg_paged {
     // mg_paged_share: another allocation, for plans of groups (0) and of their requests (1)
     char* sharedMem;
     int4 *reqs, *groups;
+    int *groupOf, *groupTile;
     mg::PagedTile* sharedTiles[2];
     mg::PagedWorker* sharedWorkers[2];
     unsigned* sharedArrived;
-    float* sharedRows;
+    float* sharedParts;                        // what the first pass leaves for the second
     int sharedMaxTiles, sharedPlanWorkers[2], sharedPlanWide[2];
 };
 
@@ -493,7 +494,7 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
     window = mg::paged_window(window, g.maxLen);
     const int workers = mg::paged_workers(g, nReqs, rows, false), narrow = mg::paged_narrow_rows(g, rows);
     const int wide = (long long)rows * g.group > narrow ? mg::paged_workers(g, nReqs, rows, true) : 0;
-    mg::PagedPlan p{rowStart, lens, prefixLens, nullptr, false, h->made, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvFormat, h->maxTiles, h->maxWorkers, workers, wide, narrow,
+    mg::PagedPlan p{rowStart, lens, prefixLens, nullptr, nullptr, nullptr, h->made, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvFormat, h->maxTiles, h->maxWorkers, workers, wide, narrow,
                     {nReqs, rows, window, 0}};
     const int rc = launched("mg_paged_plan", mg::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
     if (rc == MG_OK) {
@@ -505,13 +506,14 @@ int mg_paged_share(mg_paged* h) {
     PAGED(h, "mg_paged_share");
     if (h->sharedMem) return MG_OK;
     const mg::PagedGeo& g = h->g;
-    const size_t tiles = (size_t)mg::paged_max_tiles_shared(g), rows = (size_t)g.maxRows * g.nHeads;
+    const size_t tiles = (size_t)mg::paged_max_tiles_shared(g);
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
-    const size_t oArrived = take(tiles * g.nKVHeads * 4), clear = at, oReqs = take((size_t)g.maxReqs * sizeof(int4)), oGroups = take((size_t)g.maxReqs * sizeof(int4));
+    const size_t oArrived = take(tiles * g.nKVHeads * 4), clear = at, oReqs = take((size_t)g.maxReqs * sizeof(int4)), oGroups = take((size_t)g.maxReqs * sizeof(int4)),
+                 oGroupOf = take((size_t)g.maxReqs * 4), oGroupTile = take(((size_t)g.maxReqs + 1) * 4);
     size_t oTiles[2], oWorkers[2];
     for (int i = 0; i < 2; i++) { oTiles[i] = take(2 * tiles * sizeof(mg::PagedTile)); oWorkers[i] = take(2 * (size_t)h->maxWorkers * sizeof(mg::PagedWorker)); }
-    const size_t oRows = take(rows * (g.headDim + 2) * 4);
+    const size_t oParts = take((size_t)g.nKVHeads * h->maxWorkers * 2 * mg::paged_part_floats(g) * 4);
     char* mem = nullptr;
     hipError_t e = hipMalloc(reinterpret_cast<void**>(&mem), at);
     if (e == hipSuccess) {
@@ -533,7 +535,9 @@ int mg_paged_share(mg_paged* h) {
         h->sharedTiles[i] = reinterpret_cast<mg::PagedTile*>(mem + oTiles[i]);
         h->sharedWorkers[i] = reinterpret_cast<mg::PagedWorker*>(mem + oWorkers[i]);
     }
-    h->sharedRows = reinterpret_cast<float*>(mem + oRows);
+    h->groupOf = reinterpret_cast<int*>(mem + oGroupOf);
+    h->groupTile = reinterpret_cast<int*>(mem + oGroupTile);
+    h->sharedParts = reinterpret_cast<float*>(mem + oParts);
     return MG_OK;
 }
 int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int mostNew, const int* groupStart, const int* sharedLens,
@@ -547,10 +551,10 @@ int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int 
     mg::PagedPlan p[2];
     for (int i = 0; i < 2; i++) {
         const int n = i ? nReqs : nGroups, narrow = mg::paged_narrow_rows_shared(g, rows, i ? mostNew : 0, i == 0);
-        p[i] = {nullptr, nullptr, nullptr, i ? h->reqs : h->groups, i == 0, h->made, h->sharedTiles[i], h->sharedWorkers[i], n, rows, 0, g.maxLen, g.group, g.kvFormat,
+        p[i] = {nullptr, nullptr, nullptr, i ? h->reqs : h->groups, i ? h->groupOf : nullptr, i ? nullptr : h->groupTile, h->made, h->sharedTiles[i], h->sharedWorkers[i], n, rows, 0, g.maxLen, g.group, g.kvFormat,
                 h->sharedMaxTiles, h->maxWorkers, mg::paged_workers(g, n, rows, false), (long long)rows * g.group > narrow ? mg::paged_workers(g, n, rows, true) : 0, narrow, made};
     }
-    const int rc = launched("mg_paged_plan_shared", mg::launch_paged_plan_shared({rowStart, lens, groupStart, sharedLens, h->reqs, h->groups, nReqs, rows, nGroups, g.maxLen}, p[0], p[1],
+    const int rc = launched("mg_paged_plan_shared", mg::launch_paged_plan_shared({rowStart, lens, groupStart, sharedLens, h->reqs, h->groupOf, h->groups, nReqs, rows, nGroups, g.maxLen}, p[0], p[1],
                                                                                  static_cast<hipStream_t>(stream)));
     if (rc == MG_OK) {
         h->plan = made;
@@ -567,12 +571,19 @@ int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, cons
     if (const char* why = mg::paged_attention_overlap(h->g, q, ldq, K, V, out, ldo, h->plan.rows)) return refuse("mg_paged_attention", why);
     const mg::PagedGeo& g = h->g;
     mg::PagedAttention p{q, slopes, K, V, table, out, h->made, h->tiles, h->workers, h->parts, h->arrived, h->zeros, mg::paged_part_floats(g),
-                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, h->plan, h->sharedRows, h->reqs, 0, ldq, ldo, h->plan.window, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
+                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, h->plan, 0, h->reqs, h->groups, h->groupTile, h->sharedTiles[0], h->sharedParts, h->sharedPlanWorkers[0], 0, ldq, ldo, h->plan.window, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
     if (h->plan.groups == 0) return launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
     p.arrived = h->sharedArrived;
     p.maxTiles = h->sharedMaxTiles;
+    const bool wide = h->sharedPlanWorkers[0] == 0;          // (the groups' tiles)
+    p.sharedRows = wide ? mg::PAGED_WIDE : mg::PAGED_NARROW;
+    if (wide) {
+        p.sharedWorkers = h->sharedPlanWide[0];
+        p.sharedTiles += h->sharedMaxTiles;
+    }
     for (int i = 0; i < 2; i++) {
         p.pass = i + 1;
+        p.parts = i ? h->parts : h->sharedParts;
         p.tiles = h->sharedTiles[i];
         p.workers = h->sharedWorkers[i];
         p.nWorkers = h->sharedPlanWorkers[i];

@@ -18,7 +18,7 @@
 namespace mg {
 
 constexpr int PT = 1024;                  // threads of the plan
-constexpr int NARROW = 16, WIDE = 128;    // rows of a tile
+constexpr int NARROW = PAGED_NARROW, WIDE = PAGED_WIDE;    // rows of a tile
 constexpr int PLAN_LDS_TILES = 4096;      // tiles whose places on the line the plan holds in LDS
 // Units a worker has at least where a tile's workers are its own: a narrow unit is as short as a share can be (one request of 500
 // positions 8.8 us, with two 10.8); a wide share costs its 64 KB out and in (8B shape, one fresh prompt: 469 rows fp16 29 us, with one 38,
@@ -123,7 +123,7 @@ __device__ __forceinline__ void put_tile(PagedTile* at, const PagedTile& t) {
     d[0] = make_int4(t.req, t.row0, t.rows, t.len);
     d[1] = make_int4(t.prefix, t.first, t.cost0, t.unit0);
     d[2] = make_int4(t.units, t.worker0, t.worker1, t.index);
-    d[3] = make_int4(t.tileRows, t.unitKeys, t.from, 0);
+    d[3] = make_int4(t.tileRows, t.unitKeys, t.from, t.group);
 }
 // Largest i with sums[i] <= x, of n sums
 __device__ __forceinline__ int plan_find(const unsigned* sums, int n, unsigned x) {
@@ -140,7 +140,7 @@ __device__ __forceinline__ void make_plan(PagedPlan p, bool wide) {
     p.tiles += wide ? p.maxTiles : 0;
     p.workers += wide ? p.maxWorkers : 0;
     p.nWorkers = wide ? p.wideWorkers : p.nWorkers;
-    if (threadIdx.x == 0 && !wide && !p.grouped) *p.made = p.plan;
+    if (threadIdx.x == 0 && !wide && !p.groupTile) *p.made = p.plan;
     __shared__ unsigned tile0[PAGED_MAX_REQS + 1], place[PLAN_LDS_TILES], part[PT / 64];
     __shared__ int4 held[PT];
     const int tid = threadIdx.x;
@@ -160,14 +160,18 @@ __device__ __forceinline__ void make_plan(PagedPlan p, bool wide) {
     }
     __syncthreads();
     const int nTiles = (int)min(sum, (unsigned)p.maxTiles);          // (more only where the caller's rows overlap)
+    if (p.groupTile && wide == (p.narrowRows == 0)) {                // (groups' tiles are all of one kind)
+        for (int g = tid; g < p.nReqs; g += PT) p.groupTile[g] = (int)tile0[g];
+        if (tid == 0) p.groupTile[p.nReqs] = nTiles;
+    }
     PagedTile t;
     unsigned cost = 0;
     auto make = [&](int i) {
         const int r = plan_find(tile0, p.nReqs, (unsigned)i);
         const int4 rq = r < PT ? held[r] : plan_request(p, r);
-        t.req = r; t.row0 = rq.x; t.rows = rq.y; t.len = rq.z; t.prefix = rq.w; t.from = 0;
-        if (p.given) { t.prefix = 0; t.from = rq.w; }
-        if (p.grouped) { t.req = rq.w; t.prefix = rq.z; t.from = 0; }        // (all rows see all of it)
+        t.req = r; t.row0 = rq.x; t.rows = rq.y; t.len = rq.z; t.prefix = rq.w; t.from = t.group = 0;
+        if (p.groupOf) { t.prefix = 0; t.from = rq.w; t.group = p.groupOf[r]; }
+        if (p.groupTile) { t.req = rq.w; t.prefix = rq.z; }                  // (all rows see all of it)
         t.tileRows = tileRows; t.unitKeys = unitKeys;
         t.first = (i - (int)tile0[r]) * tileRows;
         t.index = i;
@@ -290,6 +294,7 @@ __global__ __launch_bounds__(PT) void paged_groups_kernel(PagedGroups p) {
         const int g = rq.y > 0 ? group_of(r) : -1;
         rq.w = g < 0 ? 0 : least[g];
         p.reqs[r] = rq;
+        p.groupOf[r] = g < 0 ? 0 : g;
     }
 }
 __global__ __launch_bounds__(PT) void paged_plan_shared_kernel(PagedPlan shared, PagedPlan own) {
@@ -459,25 +464,50 @@ __device__ __forceinline__ void merge_weights(const PagedAttention& p, const Pag
     }
 }
 __device__ __forceinline__ float4_t over(float4_t v, float l) { return l == 0.f ? v : v / l; }       // (nothing seen: zeros)
-// Four elements from d on of a row's result: v, with sum l over the reference m (the greatest score where SHIFT is 0).  Where the positions are
-// a shared prefix they are kept as they are for the requests' own pass, which joins the two.
-__device__ __forceinline__ void put_result(const PagedAttention& p, const PagedTile& t, const PagedRow& at, int d, float4_t v, float l, float m) {
-    const size_t row = (size_t)(t.row0 + at.token), i = row * p.g.nHeads + at.head;
-    const size_t all = (size_t)p.plan.rows * p.g.nHeads;
-    float* rows = p.shared;
-    float* ml = p.shared + all * p.g.headDim;
-    if (p.pass == 1) {
-        *reinterpret_cast<float4_t*>(rows + i * p.g.headDim + d) = v;
-        if (d == 0) { ml[i] = l == 0.f ? -INFINITY : m; ml[all + i] = l; }
-        return;
-    }
+// A row's result over its group's positions: the shares that the first pass's workers have left of it, tiles of ROWS rows as they write them
+// (NarrowTile, WideTile).  They are put together here, by every row's own tile: many workgroups, where the last to finish of a group's tile would be one.
+struct PagedShares { const float* first; int n, row; };
+__device__ __forceinline__ PagedShares shares_of(const PagedAttention& p, const PagedTile& t, const PagedRow& at, int kvh) {
+    const int4 g = p.groups[t.group];
+    const int r = (t.row0 + at.token - g.x) * p.g.group + at.head - kvh * p.g.group, i = p.groupTile[t.group] + r / p.sharedRows;
+    // (outside of the group or behind the last tile only where the caller's rows overlap)
+    if (r < 0 || r >= g.y * p.g.group || i >= p.groupTile[p.plan.groups]) return {nullptr, 0, 0};
+    const int w0 = p.sharedTiles[i].worker0, w1 = p.sharedTiles[i].worker1;
+    return {p.sharedParts + (((size_t)kvh * p.sharedWorkers + w0) * 2 + 1) * p.partStride, w1 - w0 + 1, r % p.sharedRows};
+}
+__device__ __forceinline__ const float* share_at(const PagedAttention& p, const PagedShares& x, int s) { return x.first + (size_t)(s > 0 ? 2 * s - 1 : 0) * p.partStride; }       // (as part_of)
+template <int HD>
+__device__ __forceinline__ float4_t share4(const PagedAttention& p, const float* share, int row, int d) {
+    const int i = p.sharedRows == NARROW ? row * HD + d : ((row / 32 * (HD / 32) + d / 32) * 4 + d % 32 / 8) * 256 + (d % 8 / 4 * 32 + row % 32) * 4;
+    return *reinterpret_cast<const float4_t*>(share + i);
+}
+// The rows' maxima in shares are greater by this than what their sums are taken over
+template <typename KVT>
+__device__ __forceinline__ float shared_shift(const PagedAttention& p) { return sizeof(KVT) != 2 ? 0.f : p.sharedRows == NARROW ? 14.f : 13.f; }
+// Four elements from d on of a row's result: v, with sum l over the reference m (the greatest score where a tile's SHIFT is 0), and what the row's
+// group shares.
+template <typename KVT, int HD>
+__device__ __forceinline__ void put_result(const PagedAttention& p, const PagedTile& t, int kvh, const PagedRow& at, int d, float4_t v, float l, float m) {
     if (p.pass == 2 && t.from > 0) {
-        const float ms = ml[i], ls = ml[all + i], mine = l == 0.f ? -INFINITY : m, M = fmaxf(mine, ms), to = M == -INFINITY ? 0.f : M;
-        const float a = __builtin_amdgcn_exp2f(mine - to), b = __builtin_amdgcn_exp2f(ms - to);
-        v = v * a + *reinterpret_cast<const float4_t*>(rows + i * p.g.headDim + d) * b;
-        l = fmaf(l, a, ls * b);
+        const PagedShares x = shares_of(p, t, at, kvh);
+        const int mAt = p.sharedRows * HD + x.row;
+        const float shift = shared_shift<KVT>(p), mine = l == 0.f ? -INFINITY : m;
+        float M = mine;
+#pragma unroll 8
+        for (int s = 0; s < x.n; s++) M = fmaxf(M, share_at(p, x, s)[mAt] - shift);
+        M = M == -INFINITY ? 0.f : M;
+        const float own = __builtin_amdgcn_exp2f(mine - M);
+        v *= own;
+        l *= own;
+#pragma unroll 8
+        for (int s = 0; s < x.n; s++) {
+            const float* share = share_at(p, x, s);
+            const float f = __builtin_amdgcn_exp2f(share[mAt] - shift - M);
+            l = fmaf(f, share[mAt + p.sharedRows], l);
+            v += f * share4<HD>(p, share, x.row, d);
+        }
     }
-    *reinterpret_cast<float4_t*>(p.out + row * p.ldo + (size_t)at.head * p.g.headDim + d) = over(v, l);
+    *reinterpret_cast<float4_t*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) = over(v, l);
 }
 // The position of a row of a group: of the request that it is a row of
 __device__ __forceinline__ int shared_pos(const PagedAttention& p, int row) {
@@ -1040,16 +1070,17 @@ struct NarrowTile {
         const float* ms = lds + 4 * NARROW * (HD + 4);
         const float* ls = ms + 4 * NARROW;
         const int tid = thread_anew(), R = min(NARROW, t.rows * p.g.group - t.first);
-        const bool whole = t.worker0 == t.worker1;
+        const bool whole = t.worker0 == t.worker1 && p.pass != 1;
         float* mine = part_of(p, t, kvh, w);
         for (int i = tid; i < R * (HD / 4); i += WG) {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
             const float4_t v = *reinterpret_cast<const float4_t*>(lds + r * (HD + 4) + d);
             if (!whole) { store_through(mine + r * HD + d, v); continue; }
-            put_result(p, t, paged_row(t, p.g.group, kvh, r), d, v, ls[r], ms[r] - SHIFT);
+            put_result<KVT, HD>(p, t, kvh, paged_row(t, p.g.group, kvh, r), d, v, ls[r], ms[r] - SHIFT);
         }
         if (whole) return;
         if (tid < R) { st_agent(mine + NARROW * HD + tid, ms[tid]); st_agent(mine + NARROW * HD + NARROW + tid, ls[tid]); }
+        if (p.pass == 1) return;
         if (last_to_finish(p, t, kvh, lds)) merge(kvh, R, lds);
     }
     // All workers' shares: threads take rows and columns and, where there are fewer of those than threads, shares in turn
@@ -1083,7 +1114,7 @@ struct NarrowTile {
             const int i = tid + k * WG;
             if (i >= cols) continue;
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-            put_result(p, t, paged_row(t, p.g.group, kvh, r), d, acc[k], den[r], M[r] - SHIFT);
+            put_result<KVT, HD>(p, t, kvh, paged_row(t, p.g.group, kvh, r), d, acc[k], den[r], M[r] - SHIFT);
         }
     }
 };
@@ -1728,7 +1759,7 @@ struct WideTile {
     // A share lies as its registers do -- a wave's block b, rows of four i / 4, then its 64 lanes -- so that stores and loads are whole lines
     __device__ __forceinline__ void write(int kvh, int w, float* lds) {
         const int r = 32 * wave + n32;
-        if (t.worker0 != t.worker1) {
+        if (t.worker0 != t.worker1 || p.pass == 1) {
             float* part = part_of(p, t, kvh, w);
             if (active) {
 #pragma unroll
@@ -1738,6 +1769,7 @@ struct WideTile {
                         store_through(part + ((wave * DB + b) * 4 + i) * 256 + lane * 4, float4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]});
                 if (hf == 0) { st_agent(part + WIDE * HD + r, m); st_agent(part + WIDE * HD + WIDE + r, l); }
             }
+            if (p.pass == 1) return;
             __syncthreads();                      // (all waves are done with the last unit's LDS)
             if (!last_to_finish(p, t, kvh, lds)) return;
             float *M = lds, *den = lds + WIDE, *wt = lds + 2 * WIDE;
@@ -1766,15 +1798,42 @@ struct WideTile {
             }
             __syncthreads();
             l = den[r];
-            m = M[r];
+            m = M[r];                             // (0 where nothing is seen, and l with it)
         }
         if (t.first + r >= t.rows * p.g.group) return;
         const PagedRow at = paged_row(t, p.g.group, kvh, r);
+        if (p.pass == 2 && t.from > 0) {          // (as put_result, for all of the lane's elements)
+            const PagedShares x = shares_of(p, t, at, kvh);
+            const int mAt = p.sharedRows * HD + x.row;
+            const float shift = shared_shift<KVT>(p), mine = l == 0.f ? -INFINITY : m - SHIFT;
+            float M = mine;
+#pragma unroll 8
+            for (int s = 0; s < x.n; s++) M = fmaxf(M, share_at(p, x, s)[mAt] - shift);
+            M = M == -INFINITY ? 0.f : M;
+            const float own = __builtin_amdgcn_exp2f(mine - M);
+            l *= own;
+#pragma unroll
+            for (int b = 0; b < DB; b++) o[b] *= own;
+            for (int s = 0; s < x.n; s++) {
+                const float* share = share_at(p, x, s);
+                const float f = __builtin_amdgcn_exp2f(share[mAt] - shift - M);
+                l = fmaf(f, share[mAt + p.sharedRows], l);
+#pragma unroll
+                for (int b = 0; b < DB; b++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float4_t v = share4<HD>(p, share, x.row, 32 * b + 8 * i + 4 * hf);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) o[b][4 * i + j] = fmaf(f, v[j], o[b][4 * i + j]);
+                    }
+            }
+        }
+        float* out = p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + 4 * hf;
 #pragma unroll
         for (int b = 0; b < DB; b++)
 #pragma unroll
             for (int i = 0; i < 4; i++)
-                put_result(p, t, at, 32 * b + 8 * i + 4 * hf, float4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]}, l, m - SHIFT);
+                *reinterpret_cast<float4_t*>(out + 32 * b + 8 * i) = over(float4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]}, l);
     }
 };
 

@@ -230,6 +230,7 @@ MG_HD bool paged_sees(int i, int j, int len, int window, int prefix) {
 // is put together by the last of them to finish.
 // ---------------------------------------------------------------------------
 constexpr int PAGED_TILE_COST = 1;
+constexpr int PAGED_NARROW = 16, PAGED_WIDE = 128;        // rows of a tile
 
 struct PagedTile {
     int req, row0, rows, len, prefix;   // the request, its first row and number of rows in the batch, its length and prefix
@@ -239,8 +240,7 @@ struct PagedTile {
     int worker0, worker1;               // the first and last worker that have some of them
     int index;                          // its number
     int tileRows, unitKeys;             // its kind
-    int from;                           // the first position that is its own: those before are another tile's (a shared prefix)
-    int pad[1];
+    int from, group;                    // the first position that is its own -- those before are shared --, and the group that shares them
 };
 
 // The positions [begin, end) that rows first .. first + tileRows - 1 of a request see some of, and the positions of its first and last token.
