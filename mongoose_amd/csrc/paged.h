@@ -94,7 +94,8 @@ struct PagedAttention {
 size_t paged_part_floats(const PagedGeo& g);
 int paged_max_tiles(const PagedGeo& g);
 int paged_max_tiles_shared(const PagedGeo& g);
-int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide);       // workers a KV head
+bool paged_shared_twice(const PagedGeo& g, int nReqs, int rows, bool groups);
+int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide, bool twice = false);       // workers a KV head
 int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool groups);
 int paged_narrow_rows(const PagedGeo& g, int rows);              // requests of up to so many rows a KV head have narrow tiles
 hipError_t paged_attention_setup(const PagedGeo& g);

@@ -552,7 +552,7 @@ int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int 
     for (int i = 0; i < 2; i++) {
         const int n = i ? nReqs : nGroups, narrow = mg::paged_narrow_rows_shared(g, rows, i ? mostNew : 0, i == 0);
         p[i] = {nullptr, nullptr, nullptr, i ? h->reqs : h->groups, i ? h->groupOf : nullptr, i ? nullptr : h->groupTile, h->made, h->sharedTiles[i], h->sharedWorkers[i], n, rows, 0, g.maxLen, g.group, g.kvFormat,
-                h->sharedMaxTiles, h->maxWorkers, mg::paged_workers(g, n, rows, false), (long long)rows * g.group > narrow ? mg::paged_workers(g, n, rows, true) : 0, narrow, made};
+                h->sharedMaxTiles, h->maxWorkers, mg::paged_workers(g, n, rows, false, mg::paged_shared_twice(g, n, rows, i == 0)), (long long)rows * g.group > narrow ? mg::paged_workers(g, n, rows, true) : 0, narrow, made};
     }
     const int rc = launched("mg_paged_plan_shared", mg::launch_paged_plan_shared({rowStart, lens, groupStart, sharedLens, h->reqs, h->groupOf, h->groups, nReqs, rows, nGroups, g.maxLen}, p[0], p[1],
                                                                                  static_cast<hipStream_t>(stream)));

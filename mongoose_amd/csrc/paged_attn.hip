@@ -70,6 +70,14 @@ int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool grou
     const int narrow = paged_narrow_rows(g, rows);
     return mostNew > 0 && (long long)mostNew * g.group <= narrow ? ALL : narrow;
 }
+// Whether with shared prefixes narrow tiles of groups, or of requests, have two workgroups a CU.  Groups: where many tiles read the same positions, out
+// of the L2s, but for an fp32 cache (8B shape, prefix of 8,001; 16, 32, 64 requests of a token fp16 42, 63, 100 us a call, with two
+// 44, 62, 93; 32 fp32 97 and 106; 4 behind 40,000 positions fp16 59 and 80).  Requests: where there are more tiles than that, short ones all
+// (the same 44, 62, 93 with one, 48, 55, 86 with two; 32 fp32 106 and 103).
+bool paged_shared_twice(const PagedGeo& g, int nReqs, int rows, bool groups) {
+    if (!groups) return (long long)nReqs * g.nKVHeads >= 256;
+    return g.kvFormat != PAGED_F32 && (long long)rows * g.nHeads >= 64 * NARROW;
+}
 // (with shared prefixes requests of any number of rows may have narrow tiles)
 int paged_max_tiles_shared(const PagedGeo& g) { return (int)((long long)g.maxRows * g.group / NARROW) + g.maxReqs; }
 int paged_max_tiles(const PagedGeo& g) {
@@ -77,9 +85,9 @@ int paged_max_tiles(const PagedGeo& g) {
 }
 size_t paged_part_floats(const PagedGeo& g) { return (size_t)((long long)g.maxRows * g.group <= NARROW ? NARROW : WIDE) * (g.headDim + 2); }
 // Workgroups, in turns of the KV heads: two a CU for wide tiles, as above for narrow ones.  Fewer where the batch cannot have that many units.
-int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide) {
+int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide, bool twice) {
     const long long tiles = (long long)rows * g.group / NARROW + nReqs, units = tiles * (g.maxLen / 32 + 2);
-    const int resident = wide ? 2 * 256 : g.kvFormat == PAGED_Q8 ? NARROW_WORKERS_Q8 : NARROW_WORKERS;
+    const int resident = wide || twice ? 2 * 256 : g.kvFormat == PAGED_Q8 ? NARROW_WORKERS_Q8 : NARROW_WORKERS;
     const long long most = resident / g.nKVHeads > 0 ? resident / g.nKVHeads : 1;
     return (int)(units < 1 ? 1 : units < most ? units : most);
 }
