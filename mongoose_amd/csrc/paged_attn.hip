@@ -61,13 +61,15 @@ int paged_narrow_rows(const PagedGeo& g, int rows) {
     if (all <= 256) return 256;
     return g.kvFormat != PAGED_Q8 ? NARROW : all <= Q8_FEW_ROWS ? NARROW_Q8_FEW : NARROW_Q8;
 }
-// The same with shared prefixes, for groups (0: all groups have wide tiles) and for requests, of which the caller may know that none adds more than
-// mostNew rows.
+// The same with shared prefixes, for groups (0: all groups have wide tiles; up to 256 rows, as above: 64 requests behind 8,001 positions 98 us, with
+// wide ones 133) and for requests, of which the caller may know that none adds more than mostNew rows.  What requests have of their own is short, so
+// narrow tiles go further while the wide ones would not fill the CUs (80 requests, 378 rows in all, up to 40 each, Q8: 210 us a call, so 163; 32 of
+// 40 rows each, more rows than that: 219 and 235).
 int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool groups) {
     constexpr int ALL = PAGED_MAX_ROWS * PAGED_MAX_GROUP;
     if ((long long)rows * g.group <= 256) return ALL;
     if (groups) return 0;
-    const int narrow = paged_narrow_rows(g, rows);
+    const int narrow = (long long)rows * g.group <= 4096 ? 256 : paged_narrow_rows(g, rows);
     return mostNew > 0 && (long long)mostNew * g.group <= narrow ? ALL : narrow;
 }
 // Whether with shared prefixes narrow tiles of groups, or of requests, have two workgroups a CU.  Groups: where many tiles read the same positions, out
