@@ -28,8 +28,7 @@ constexpr int LEAST_NARROW = 1, LEAST_WIDE = 3;
 // with two 113; 48 requests 174 and 182); two for a Q8 cache, whose vector instructions take as long as its bytes (48 requests 157 us with
 // one, 123 with two; 120,001 positions 79, 76).
 constexpr int NARROW_WORKERS = 256, NARROW_WORKERS_Q8 = 512;
-constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results, and as many for their sums
-static_assert(NARROW_WORKERS_Q8 * NARROW <= MERGE_LDS, "a narrow tile's shares are weighed in one turn");
+constexpr int MERGE_LDS = 8192;           // floats of LDS for the weights of partial results (a wide tile's, in turns)
 
 typedef _Float16 half8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 half2_t __attribute__((ext_vector_type(2)));
@@ -426,7 +425,7 @@ __device__ __forceinline__ void merge_weights(const PagedAttention& p, const Pag
     if constexpr (ROWS == NARROW) {
         // One turn, a row's shares fetched by 16 threads: what it costs is the round trips to memory (8B shape, fp16, 5,000 positions in 40
         // shares: 17 us a call, with one thread a row as below 23)
-        float* sums = wt + MERGE_LDS;
+        float* sums = wt + p.nWorkers * NARROW;
         const int r = tid % ROWS;
         float m = -INFINITY;
 #pragma unroll 4
@@ -436,16 +435,13 @@ __device__ __forceinline__ void merge_weights(const PagedAttention& p, const Pag
             wt[s * ROWS + r] = x;
             m = fmaxf(m, x);
         }
-        M[tid] = m;
+        m = rows_max(m);
+        if ((tid & 63) < ROWS) M[ROWS * (1 + tid / 64) + r] = m;
         __syncthreads();
-        if (tid < ROWS) {
-#pragma unroll
-            for (int i = 1; i < WG / ROWS; i++) m = fmaxf(m, M[tid + i * ROWS]);
-        }
-        __syncthreads();
-        if (tid < ROWS) M[tid] = m == -INFINITY ? 0.f : m;
-        __syncthreads();
-        for (int i = tid; i < n * ROWS; i += WG) wt[i] = __builtin_amdgcn_exp2f(wt[i] - M[r]);
+        m = fmaxf(fmaxf(M[ROWS + r], M[2 * ROWS + r]), fmaxf(M[3 * ROWS + r], M[4 * ROWS + r]));
+        m = m == -INFINITY ? 0.f : m;
+        if (tid < ROWS) M[r] = m;
+        for (int s = tid / ROWS; s < n; s += WG / ROWS) wt[s * ROWS + r] = __builtin_amdgcn_exp2f(wt[s * ROWS + r] - m);       // (its own)
         __syncthreads();
         if (tid < R) {
             float d = 0.f;
@@ -496,9 +492,9 @@ template <typename KVT>
 __device__ __forceinline__ float shared_shift(const PagedAttention& p) { return sizeof(KVT) != 2 ? 0.f : p.sharedRows == NARROW ? 14.f : 13.f; }
 // Four elements from d on of a row's result: v, with sum l over the reference m (the greatest score where a tile's SHIFT is 0), and what the row's
 // group shares.
-template <typename KVT, int HD>
+template <typename KVT, int HD, bool SHARED>
 __device__ __forceinline__ void put_result(const PagedAttention& p, const PagedTile& t, int kvh, const PagedRow& at, int d, float4_t v, float l, float m) {
-    if (p.pass == 2 && t.from > 0) {
+    if (SHARED && p.pass == 2 && t.from > 0) {
         const PagedShares x = shares_of(p, t, at, kvh);
         const int mAt = p.sharedRows * HD + x.row;
         const float shift = shared_shift<KVT>(p), mine = l == 0.f ? -INFINITY : m;
@@ -592,7 +588,7 @@ __device__ __forceinline__ int power_up(float top, float scale) {
 // fp16 caches: q, scaled by a power of two to 2^14 .. 2^15, and the probabilities, times 2^14, each as two fp16 terms (22 bits;
 // what is below 2^-29 of the row's largest |q| or 2^-38 of the largest probability is lost); K and V as they are.
 // fp32 caches: fp32 matrix instructions throughout.
-template <typename KVT, int HD, bool MOD>
+template <typename KVT, int HD, bool MOD, bool SHARED>
 struct NarrowTile {
     static constexpr bool Q8 = sizeof(KVT) == 1, HALF = sizeof(KVT) <= 2;       // HALF: products of fp16 operands
     static constexpr int KB = HALF ? 32 : 16;              // positions of a wave's step
@@ -628,9 +624,9 @@ struct NarrowTile {
         const int tid = thread_anew();
         lane = tid & 63; l16 = lane & 15; g = lane >> 4;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, NARROW, t.from);
+        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, NARROW, SHARED ? t.from : 0);
         row = paged_row(t, p.g.group, kvh, l16);
-        if (MOD && p.pass == 1 && p.slopes) row.pos = shared_pos(p, t.row0 + row.token);
+        if (SHARED && MOD && p.pass == 1 && p.slopes) row.pos = shared_pos(p, t.row0 + row.token);
         pages = p.table + (size_t)t.req * p.g.width;
         rowBytes = (size_t)p.g.kvDim * sizeof(KVT);
         Kp = static_cast<const char*>(p.K) + (size_t)kvh * HD * sizeof(KVT);
@@ -880,7 +876,7 @@ struct NarrowTile {
 #pragma unroll
             for (int j = 0; j < NB * 4; j++) x[j] = (x[j] - slope * (float)abs(row.pos - (base + 16 * (j / 4) + 4 * g + j % 4))) * 1.4426950408889634f;
         }
-        const bool inner = base + KB <= t.prefix || (base >= t.from && base + KB - 1 <= span.pos0 && (p.window == 0 || base > span.pos1 - p.window));       // all rows see all of it
+        const bool inner = base + KB <= t.prefix || ((!SHARED || base >= t.from) && base + KB - 1 <= span.pos0 && (p.window == 0 || base > span.pos1 - p.window));       // all rows see all of it
         const bool all = inner && __all(mine >= 0);
         if (!all) {
 #pragma unroll
@@ -888,7 +884,7 @@ struct NarrowTile {
                 const bool held = page_in(mine, b, g & 2) >= 0;
 #pragma unroll
                 for (int i = 0; i < 4; i++)
-                    if (!held || base + 16 * b + 4 * g + i < t.from || !paged_sees(row.pos, base + 16 * b + 4 * g + i, t.len, p.window, t.prefix)) {
+                    if (!held || (SHARED && base + 16 * b + 4 * g + i < t.from) || !paged_sees(row.pos, base + 16 * b + 4 * g + i, t.len, p.window, t.prefix)) {
                         x[4 * b + i] = -INFINITY;
                         if constexpr (Q8) vs[b][i] = 0.f;       // (its scale may be anything)
                     }
@@ -1080,22 +1076,22 @@ struct NarrowTile {
         const float* ms = lds + 4 * NARROW * (HD + 4);
         const float* ls = ms + 4 * NARROW;
         const int tid = thread_anew(), R = min(NARROW, t.rows * p.g.group - t.first);
-        const bool whole = t.worker0 == t.worker1 && p.pass != 1;
+        const bool whole = t.worker0 == t.worker1 && !(SHARED && p.pass == 1);
         float* mine = part_of(p, t, kvh, w);
         for (int i = tid; i < R * (HD / 4); i += WG) {
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
             const float4_t v = *reinterpret_cast<const float4_t*>(lds + r * (HD + 4) + d);
             if (!whole) { store_through(mine + r * HD + d, v); continue; }
-            put_result<KVT, HD>(p, t, kvh, paged_row(t, p.g.group, kvh, r), d, v, ls[r], ms[r] - SHIFT);
+            put_result<KVT, HD, SHARED>(p, t, kvh, paged_row(t, p.g.group, kvh, r), d, v, ls[r], ms[r] - SHIFT);
         }
         if (whole) return;
         if (tid < R) { st_agent(mine + NARROW * HD + tid, ms[tid]); st_agent(mine + NARROW * HD + NARROW + tid, ls[tid]); }
-        if (p.pass == 1) return;
+        if (SHARED && p.pass == 1) return;
         if (last_to_finish(p, t, kvh, lds)) merge(kvh, R, lds);
     }
     // All workers' shares: threads take rows and columns and, where there are fewer of those than threads, shares in turn
     __device__ __forceinline__ void merge(int kvh, int R, float* lds) const {
-        float *M = lds, *den = lds + WG, *wt = den + NARROW;         // (M: a word a thread on the way)
+        float *M = lds, *den = lds + 5 * NARROW, *wt = den + NARROW;         // (M, and each wave's behind it)
         constexpr int N = NARROW * HD / 4 / WG > 0 ? NARROW * HD / 4 / WG : 1;
         const int tid = thread_anew(), segs = t.worker1 - t.worker0 + 1, cols = R * (HD / 4), par = max(1, WG / cols);
         float4_t acc[N];
@@ -1124,7 +1120,7 @@ struct NarrowTile {
             const int i = tid + k * WG;
             if (i >= cols) continue;
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-            put_result<KVT, HD>(p, t, kvh, paged_row(t, p.g.group, kvh, r), d, acc[k], den[r], M[r] - SHIFT);
+            put_result<KVT, HD, SHARED>(p, t, kvh, paged_row(t, p.g.group, kvh, r), d, acc[k], den[r], M[r] - SHIFT);
         }
     }
 };
@@ -1137,7 +1133,7 @@ struct NarrowTile {
 //   V (A operand): dimension l%32 of a block of 32, the positions of the lane's own probabilities -- 4 (l/32) + 0..3 of every eight --
 //     fp16 through the transposing LDS read, fp32 word by word.
 // A row's 16-byte pieces lie in LDS at piece ^ swz(row), so that neither rows of one piece nor (fp16) four rows of two meet in a bank.
-template <typename KVT, int HD, bool MOD>
+template <typename KVT, int HD, bool MOD, bool SHARED>
 struct WideTile {
     static constexpr bool Q8 = sizeof(KVT) == 1, HALF = sizeof(KVT) <= 2;   // HALF: products of fp16 operands
     static constexpr int UK = HALF && !Q8 ? 64 : 32, NB = UK / 32, DB = HD / 32;
@@ -1181,13 +1177,13 @@ struct WideTile {
         const int tid = thread_anew();
         lane = tid & 63; n32 = lane & 31; hf = lane >> 5;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, WIDE, t.from);
+        span = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, t.first, WIDE, SHARED ? t.from : 0);
         const int mine = t.first + 32 * wave;
         active = mine < t.rows * p.g.group;
-        const PagedSpan own = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, active ? mine : t.first, 32, t.from);
+        const PagedSpan own = paged_span(t.rows, t.len, t.prefix, p.window, p.g.group, active ? mine : t.first, 32, SHARED ? t.from : 0);
         pos0 = own.pos0; pos1 = own.pos1; begin = own.begin; end = own.end;
         row = paged_row(t, p.g.group, kvh, 32 * wave + n32);
-        if (MOD && p.pass == 1 && p.slopes) row.pos = shared_pos(p, t.row0 + row.token);
+        if (SHARED && MOD && p.pass == 1 && p.slopes) row.pos = shared_pos(p, t.row0 + row.token);
         pages = p.table + (size_t)t.req * p.g.width;
         rowBytes = (size_t)p.g.kvDim * sizeof(KVT);
         Kp = static_cast<const char*>(p.K) + (size_t)kvh * HD * sizeof(KVT);
@@ -1451,7 +1447,7 @@ struct WideTile {
             for (int b = 0; b < NB; b++)
 #pragma unroll
                 for (int i = 0; i < 16; i++)
-                    if (!((held >> (4 * b + i / 4)) & 1) || first + 32 * b + 8 * (i / 4) + i % 4 < t.from || !paged_sees(row.pos, first + 32 * b + 8 * (i / 4) + i % 4, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
+                    if (!((held >> (4 * b + i / 4)) & 1) || (SHARED && first + 32 * b + 8 * (i / 4) + i % 4 < t.from) || !paged_sees(row.pos, first + 32 * b + 8 * (i / 4) + i % 4, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
         }
         float top = S[0][0];
 #pragma unroll
@@ -1505,7 +1501,7 @@ struct WideTile {
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int key = first + 32 * b + 8 * (i / 4) + i % 4;
-                    if (!((held >> (4 * b + i / 4)) & 1) || key < t.from || !paged_sees(row.pos, key, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
+                    if (!((held >> (4 * b + i / 4)) & 1) || (SHARED && key < t.from) || !paged_sees(row.pos, key, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
                 }
         }
         float top = S[0][0];
@@ -1565,7 +1561,7 @@ struct WideTile {
         const unsigned K = ldsBase + buf * BUFB, V = K + TILEB;
         const unsigned long long held = __ballot(mine >= 0);
         constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
-        const bool inner = base + UK <= t.prefix || (base >= t.from && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
+        const bool inner = base + UK <= t.prefix || ((!SHARED || base >= t.from) && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
         const bool all = inner && (held & runs) == runs;
         float16_t S[NB];
         float mNew;
@@ -1630,7 +1626,7 @@ struct WideTile {
         const unsigned K = kAt + buf * BUFB, V = vAt + buf * BUFB;
         const unsigned long long held = __ballot(mine >= 0);
         constexpr unsigned long long runs = (1ull << (UK / 8)) - 1;
-        const bool inner = base + UK <= t.prefix || (base >= t.from && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
+        const bool inner = base + UK <= t.prefix || ((!SHARED || base >= t.from) && base + UK - 1 <= pos0 && (p.window == 0 || base > pos1 - p.window));        // all rows see all of it
         const bool all = inner && (held & runs) == runs;
         float16_t S[NB];
         uint4_t k[QS];
@@ -1769,7 +1765,7 @@ struct WideTile {
     // A share lies as its registers do -- a wave's block b, rows of four i / 4, then its 64 lanes -- so that stores and loads are whole lines
     __device__ __forceinline__ void write(int kvh, int w, float* lds) {
         const int r = 32 * wave + n32;
-        if (t.worker0 != t.worker1 || p.pass == 1) {
+        if (t.worker0 != t.worker1 || (SHARED && p.pass == 1)) {
             float* part = part_of(p, t, kvh, w);
             if (active) {
 #pragma unroll
@@ -1779,7 +1775,7 @@ struct WideTile {
                         store_through(part + ((wave * DB + b) * 4 + i) * 256 + lane * 4, float4_t{o[b][4 * i], o[b][4 * i + 1], o[b][4 * i + 2], o[b][4 * i + 3]});
                 if (hf == 0) { st_agent(part + WIDE * HD + r, m); st_agent(part + WIDE * HD + WIDE + r, l); }
             }
-            if (p.pass == 1) return;
+            if (SHARED && p.pass == 1) return;
             __syncthreads();                      // (all waves are done with the last unit's LDS)
             if (!last_to_finish(p, t, kvh, lds)) return;
             float *M = lds, *den = lds + WIDE, *wt = lds + 2 * WIDE;
@@ -1812,7 +1808,7 @@ struct WideTile {
         }
         if (t.first + r >= t.rows * p.g.group) return;
         const PagedRow at = paged_row(t, p.g.group, kvh, r);
-        if (p.pass == 2 && t.from > 0) {          // (as put_result, for all of the lane's elements)
+        if (SHARED && p.pass == 2 && t.from > 0) {          // (as put_result, for all of the lane's elements)
             const PagedShares x = shares_of(p, t, at, kvh);
             const int mAt = p.sharedRows * HD + x.row;
             const float shift = shared_shift<KVT>(p), mine = l == 0.f ? -INFINITY : m - SHIFT;
@@ -1847,7 +1843,7 @@ struct WideTile {
     }
 };
 
-template <typename KVT, int HD, bool MOD, template <typename, int, bool> class Tile, int ROWS>
+template <typename KVT, int HD, bool MOD, bool SHARED, template <typename, int, bool, bool> class Tile, int ROWS>
 __device__ __forceinline__ void attend(const PagedAttention& p, float* lds) {
     // neighbouring shares on one die, whose L2 then holds the KV head's rows that they have in common
     const int id = (int)((blockIdx.x & 7) * (gridDim.x >> 3) + (blockIdx.x >> 3));
@@ -1861,7 +1857,7 @@ __device__ __forceinline__ void attend(const PagedAttention& p, float* lds) {
     for (;;) {
         const int u0 = paged_unit_at(t, a), u1 = paged_unit_at(t, b);
         if (u0 < u1) {
-            Tile<KVT, HD, MOD> n(p, t, kvh, u0, u1);
+            Tile<KVT, HD, MOD, SHARED> n(p, t, kvh, u0, u1);
             n.run(u0, u1, kvh, w, lds);
             n.write(kvh, w, lds);
         } else if (t.units == 0 && a <= t.cost0 && t.cost0 < b) {
@@ -1875,41 +1871,40 @@ __device__ __forceinline__ void attend(const PagedAttention& p, float* lds) {
         if (t.cost0 >= b) break;
     }
 }
-template <typename KVT, int HD, bool MOD>
+template <typename KVT, int HD, bool MOD, bool SHARED>
 __global__ __launch_bounds__(WG, 2) void paged_narrow_kernel(PagedAttention p) {
     extern __shared__ __attribute__((aligned(1024))) float lds[];      // (all the LDS there is: it starts at 0)
-    attend<KVT, HD, MOD, NarrowTile, NARROW>(p, lds);
+    attend<KVT, HD, MOD, SHARED, NarrowTile, NARROW>(p, lds);
 }
-template <typename KVT, int HD, bool MOD>
+template <typename KVT, int HD, bool MOD, bool SHARED>
 __global__ __launch_bounds__(WG, 2) void paged_wide_kernel(PagedAttention p) {
     extern __shared__ __attribute__((aligned(1024))) float lds[];
-    attend<KVT, HD, MOD, WideTile, WIDE>(p, lds);
+    attend<KVT, HD, MOD, SHARED, WideTile, WIDE>(p, lds);
 }
 
-static size_t attn_lds(int headDim, bool wide) {           // (wide, Q8: one buffer of halves, two of bytes, 1 KB of scales)
+static size_t attn_lds(int headDim, bool wide, int workers) {       // (wide, Q8: one buffer of halves, two of bytes, 1 KB of scales)
     const size_t tile = wide ? (size_t)2 * 2 * 64 * headDim * 2 + 1024 : (size_t)(4 * NARROW * (headDim + 4) + 8 * NARROW) * 4;
-    const size_t merge = (size_t)(wide ? 2 * WIDE + MERGE_LDS : WG + NARROW + 2 * MERGE_LDS) * 4;
+    const size_t merge = (size_t)(wide ? 2 * WIDE + MERGE_LDS : 6 * NARROW + 2 * NARROW * workers) * 4;
     return tile > merge ? tile : merge;
 }
-template <typename F>
-static hipError_t with_kernel(const PagedGeo& g, bool mod, bool wide, F f) {
-#define PAGED_PICK(KVT, HD, MOD) (wide ? f(paged_wide_kernel<KVT, HD, MOD>) : f(paged_narrow_kernel<KVT, HD, MOD>))
-    if (g.kvFormat == PAGED_Q8) {
-        if (g.headDim == 64) return mod ? PAGED_PICK(signed char, 64, true) : PAGED_PICK(signed char, 64, false);
-        return mod ? PAGED_PICK(signed char, 128, true) : PAGED_PICK(signed char, 128, false);
-    }
-    if (g.kvFormat == PAGED_F16) {
-        if (g.headDim == 64) return mod ? PAGED_PICK(_Float16, 64, true) : PAGED_PICK(_Float16, 64, false);
-        return mod ? PAGED_PICK(_Float16, 128, true) : PAGED_PICK(_Float16, 128, false);
-    }
-    if (g.headDim == 64) return mod ? PAGED_PICK(float, 64, true) : PAGED_PICK(float, 64, false);
-    return mod ? PAGED_PICK(float, 128, true) : PAGED_PICK(float, 128, false);
+template <typename KVT, int HD, typename F>
+static hipError_t with_kernel_of(bool mod, bool wide, bool shared, F f) {
+#define PAGED_PICK(MOD, SHARED) (wide ? f(paged_wide_kernel<KVT, HD, MOD, SHARED>) : f(paged_narrow_kernel<KVT, HD, MOD, SHARED>))
+    if (shared) return mod ? PAGED_PICK(true, true) : PAGED_PICK(false, true);
+    return mod ? PAGED_PICK(true, false) : PAGED_PICK(false, false);
 #undef PAGED_PICK
 }
+template <typename F>
+static hipError_t with_kernel(const PagedGeo& g, bool mod, bool wide, bool shared, F f) {
+    const bool small = g.headDim == 64;
+    if (g.kvFormat == PAGED_Q8) return small ? with_kernel_of<signed char, 64>(mod, wide, shared, f) : with_kernel_of<signed char, 128>(mod, wide, shared, f);
+    if (g.kvFormat == PAGED_F16) return small ? with_kernel_of<_Float16, 64>(mod, wide, shared, f) : with_kernel_of<_Float16, 128>(mod, wide, shared, f);
+    return small ? with_kernel_of<float, 64>(mod, wide, shared, f) : with_kernel_of<float, 128>(mod, wide, shared, f);
+}
 hipError_t paged_attention_setup(const PagedGeo& g) {
-    for (int i = 0; i < 4; i++) {
-        hipError_t e = with_kernel(g, i & 1, i >> 1, [&](auto* k) {
-            return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)attn_lds(g.headDim, i >> 1));
+    for (int i = 0; i < 8; i++) {
+        hipError_t e = with_kernel(g, i & 1, i >> 1 & 1, i >> 2, [&](auto* k) {
+            return hipFuncSetAttribute(reinterpret_cast<const void*>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)attn_lds(g.headDim, i >> 1 & 1, 2 * 256));
         });
         if (e != hipSuccess) return e;
     }
@@ -1923,8 +1918,8 @@ hipError_t launch_paged_attention(const PagedAttention& p0, hipStream_t s) {
         const int groups = (p.nWorkers * p.g.nKVHeads + 7) / 8 * 8;
         p.tiles += wide ? p.maxTiles : 0;
         p.workers += wide ? p.maxWorkers : 0;
-        const size_t lds = attn_lds(p.g.headDim, wide);
-        hipError_t e = with_kernel(p.g, p.softcap > 0.f || p.slopes, wide, [&](auto* k) {
+        const size_t lds = attn_lds(p.g.headDim, wide, p.nWorkers);
+        hipError_t e = with_kernel(p.g, p.softcap > 0.f || p.slopes, wide, p.pass != 0, [&](auto* k) {
             hipLaunchKernelGGL(k, dim3(groups), dim3(WG), lds, s, p);
             return hipGetLastError();
         });
