@@ -493,36 +493,51 @@ __device__ __forceinline__ float shared_shift(const PagedAttention& p) { return 
 // Four elements from d on of a row's result: v, with sum l over the reference m (the greatest score where a tile's SHIFT is 0), and what the row's
 // group shares.
 template <typename KVT, int HD, bool SHARED>
-__device__ __forceinline__ void put_result(const PagedAttention& p, const PagedTile& t, int kvh, const PagedRow& at, int d, float4_t v, float l, float m) {
-    if (SHARED && p.pass == 2 && t.from > 0) {
-        const PagedShares x = shares_of(p, t, at, kvh);
+__device__ __forceinline__ void put_result(const PagedAttention& p, const PagedTile& t, const PagedShares& x, const PagedRow& at, int d, float4_t v, float l, float m) {
+    if (SHARED && x.n > 0) {
         const int mAt = p.sharedRows * HD + x.row;
-        const float shift = shared_shift<KVT>(p), mine = l == 0.f ? -INFINITY : m;
-        float M = mine;
-#pragma unroll 8
-        for (int s = 0; s < x.n; s++) M = fmaxf(M, share_at(p, x, s)[mAt] - shift);
-        M = M == -INFINITY ? 0.f : M;
-        const float own = __builtin_amdgcn_exp2f(mine - M);
-        v *= own;
-        l *= own;
-#pragma unroll 8
-        for (int s = 0; s < x.n; s++) {
-            const float* share = share_at(p, x, s);
-            const float f = __builtin_amdgcn_exp2f(share[mAt] - shift - M);
-            l = fmaf(f, share[mAt + p.sharedRows], l);
-            v += f * share4<HD>(p, share, x.row, d);
+        const float shift = shared_shift<KVT>(p);
+        float M = l == 0.f ? -INFINITY : m;
+        constexpr int N = 4;               // shares fetched at once
+        for (int s0 = 0; s0 < x.n; s0 += N) {
+            float ms[N], ls[N], most = M;
+            float4_t vs[N];
+#pragma unroll
+            for (int s = 0; s < N; s++) {
+                const float* share = share_at(p, x, min(s0 + s, x.n - 1));
+                ms[s] = share[mAt];
+                ls[s] = share[mAt + p.sharedRows];
+                vs[s] = share4<HD>(p, share, x.row, d);
+            }
+#pragma unroll
+            for (int s = 0; s < N; s++) {
+                ms[s] = s0 + s < x.n ? ms[s] - shift : -INFINITY;
+                most = fmaxf(most, ms[s]);
+            }
+            const float to = most == -INFINITY ? 0.f : most, own = __builtin_amdgcn_exp2f(M - to);
+            v *= own;
+            l *= own;
+#pragma unroll
+            for (int s = 0; s < N; s++) {
+                const float f = __builtin_amdgcn_exp2f(ms[s] - to);
+                if (s0 + s < x.n) { l = fmaf(f, ls[s], l); v += f * vs[s]; }
+            }
+            M = most;
         }
     }
     *reinterpret_cast<float4_t*>(p.out + (size_t)(t.row0 + at.token) * p.ldo + (size_t)at.head * HD + d) = over(v, l);
 }
 // The position of a row of a group: of the request that it is a row of
 __device__ __forceinline__ int shared_pos(const PagedAttention& p, int row) {
-    int lo = 0, hi = p.plan.nReqs;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (p.reqs[mid].x <= row) lo = mid; else hi = mid;
+    int4 rq = p.reqs[min(row, p.plan.nReqs - 1)];              // (where every request has one row it is the row's)
+    if (row < rq.x || row >= rq.x + rq.y) {
+        int lo = 0, hi = p.plan.nReqs;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (p.reqs[mid].x <= row) lo = mid; else hi = mid;
+        }
+        rq = p.reqs[lo];
     }
-    const int4 rq = p.reqs[lo];
     return rq.z - rq.y + row - rq.x;
 }
 
@@ -617,6 +632,8 @@ struct NarrowTile {
     float ref;                     // Q8: probabilities are 2^(x - ref)
     float minus1;                  // Q8: -1, in a register (two_terms)
     float4_t o[EPL];
+    static constexpr int NP = NARROW * HD / 4 / WG;        // pieces of the result that a thread writes at the end
+    PagedShares shares[NP];        // of their rows; asked for at the start
 
     int here, next;                // page numbers of the step at hand and of the one behind it
 
@@ -650,6 +667,13 @@ struct NarrowTile {
         next = page_of(min(u0 + 1, u1 - 1));
         load_k(u0, here);
         load_v(u0, here);
+        if constexpr (SHARED) {
+#pragma unroll
+            for (int i = 0; i < NP; i++) {
+                const int r = min((tid + i * WG) / (HD / 4), t.rows * p.g.group - t.first - 1);
+                shares[i] = p.pass == 2 && t.from > 0 ? shares_of(p, t, paged_row(t, p.g.group, kvh, r), kvh) : PagedShares{nullptr, 0, 0};
+            }
+        }
         cap = p.softcap;
         invCap = MOD && cap > 0.f ? 1.f / cap : 0.f;
         slope = MOD && p.slopes ? p.slopes[row.head] : 0.f;
@@ -1078,11 +1102,14 @@ struct NarrowTile {
         const int tid = thread_anew(), R = min(NARROW, t.rows * p.g.group - t.first);
         const bool whole = t.worker0 == t.worker1 && !(SHARED && p.pass == 1);
         float* mine = part_of(p, t, kvh, w);
-        for (int i = tid; i < R * (HD / 4); i += WG) {
+#pragma unroll
+        for (int k = 0; k < NP; k++) {
+            const int i = tid + k * WG;
+            if (i >= R * (HD / 4)) break;
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
             const float4_t v = *reinterpret_cast<const float4_t*>(lds + r * (HD + 4) + d);
             if (!whole) { store_through(mine + r * HD + d, v); continue; }
-            put_result<KVT, HD, SHARED>(p, t, kvh, paged_row(t, p.g.group, kvh, r), d, v, ls[r], ms[r] - SHIFT);
+            put_result<KVT, HD, SHARED>(p, t, shares[k], paged_row(t, p.g.group, kvh, r), d, v, ls[r], ms[r] - SHIFT);
         }
         if (whole) return;
         if (tid < R) { st_agent(mine + NARROW * HD + tid, ms[tid]); st_agent(mine + NARROW * HD + NARROW + tid, ls[tid]); }
@@ -1092,7 +1119,7 @@ struct NarrowTile {
     // All workers' shares: threads take rows and columns and, where there are fewer of those than threads, shares in turn
     __device__ __forceinline__ void merge(int kvh, int R, float* lds) const {
         float *M = lds, *den = lds + 5 * NARROW, *wt = den + NARROW;         // (M, and each wave's behind it)
-        constexpr int N = NARROW * HD / 4 / WG > 0 ? NARROW * HD / 4 / WG : 1;
+        constexpr int N = NP;
         const int tid = thread_anew(), segs = t.worker1 - t.worker0 + 1, cols = R * (HD / 4), par = max(1, WG / cols);
         float4_t acc[N];
 #pragma unroll
@@ -1120,7 +1147,7 @@ struct NarrowTile {
             const int i = tid + k * WG;
             if (i >= cols) continue;
             const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-            put_result<KVT, HD, SHARED>(p, t, kvh, paged_row(t, p.g.group, kvh, r), d, acc[k], den[r], M[r] - SHIFT);
+            put_result<KVT, HD, SHARED>(p, t, shares[k], paged_row(t, p.g.group, kvh, r), d, acc[k], den[r], M[r] - SHIFT);
         }
     }
 };
