@@ -143,6 +143,12 @@ __device__ __forceinline__ int plan_find(const unsigned* sums, int n, unsigned x
     }
     return lo;
 }
+// Of the workers that a narrow tile of its own would have, those that pay for what joining their shares costs: one for up to three units (8B shape,
+// four requests of 70, 130, 250, 300 positions fp16 8.0, 10.2, 10.6, 10.5 us with one a unit, so 7.1, 8.5, 9.0, 10.2); with a Q8 cache, whose tiles have
+// twice the workers, beyond 64 of them the square root of the units four times (0.5B shape, one request of 20,000 positions 38 us, so 26; of 60,000 56 and 35).
+__device__ __forceinline__ int narrow_workers(int n, int units, int kvFormat) {
+    return units < 4 ? 1 : kvFormat == PAGED_Q8 ? min(n, max(64, (int)(4.f * sqrtf((float)units)))) : n;
+}
 // One workgroup for the narrow tiles and one for the wide ones
 __device__ __forceinline__ void make_plan(PagedPlan p, bool wide) {
     const int tileRows = wide ? WIDE : NARROW, unitKeys = wide ? wide_keys(p.kvFormat) : narrow_keys(p.kvFormat);
@@ -201,7 +207,10 @@ __device__ __forceinline__ void make_plan(PagedPlan p, bool wide) {
     const bool few = paged_few(nTiles, p.nWorkers);                  // (512 tiles at most: one round)
     int workers = max(1, min(p.nWorkers, (int)cost)), n = 0;
     if (few) {
-        if (tid < nTiles) n = paged_workers_for(t, (int)cost, nTiles, p.nWorkers, wide ? LEAST_WIDE : LEAST_NARROW);
+        if (tid < nTiles) {
+            n = paged_workers_for(t, (int)cost, nTiles, p.nWorkers, wide ? LEAST_WIDE : LEAST_NARROW);
+            if (!wide) n = narrow_workers(n, t.units, p.kvFormat);
+        }
         unsigned all = 0;
         const unsigned end = plan_scan((unsigned)n, all, part);
         workers = (int)all;
