@@ -612,6 +612,9 @@ __device__ __forceinline__ int power_up(float top, float scale) {
 // fp16 caches: q, scaled by a power of two to 2^14 .. 2^15, and the probabilities, times 2^14, each as two fp16 terms (22 bits;
 // what is below 2^-29 of the row's largest |q| or 2^-38 of the largest probability is lost); K and V as they are.
 // fp32 caches: fp32 matrix instructions throughout.
+// Q8 caches: whole numbers as halves (four_halves), the scales of a lane's four positions of a block 16 bytes each for K and V; scores are multiplied by
+// K's where they leave the matrix instructions, probabilities by V's where they become weights (weigh_q8).  Two workgroups a CU; 8B shape, the same 48
+// requests 115 us, 4.3 TB/s: HBM, and vector instructions half of the time.
 template <typename KVT, int HD, bool MOD, bool SHARED>
 struct NarrowTile {
     static constexpr bool Q8 = sizeof(KVT) == 1, HALF = sizeof(KVT) <= 2;       // HALF: products of fp16 operands
@@ -1169,6 +1172,9 @@ struct NarrowTile {
 //   V (A operand): dimension l%32 of a block of 32, the positions of the lane's own probabilities -- 4 (l/32) + 0..3 of every eight --
 //     fp16 through the transposing LDS read, fp32 word by word.
 // A row's 16-byte pieces lie in LDS at piece ^ swz(row), so that neither rows of one piece nor (fp16) four rows of two meet in a bank.
+// Q8 caches: as fp16 ones, in units of 32 positions.  Rows come into LDS as they are, two units ahead, and are turned to halves there for all
+// four waves, one ahead, between the scores' matrix instructions.  8B shape, 2,048 tokens over 9,700 positions: 820 us, 880 TFLOP/s with both terms
+// counted.  Bound by the matrix units and, as much, by the vector instructions beside them (270 a unit and wave, 16 + 16 matrix instructions).
 template <typename KVT, int HD, bool MOD, bool SHARED>
 struct WideTile {
     static constexpr bool Q8 = sizeof(KVT) == 1, HALF = sizeof(KVT) <= 2;   // HALF: products of fp16 operands
@@ -1344,8 +1350,7 @@ struct WideTile {
 #pragma unroll
         for (int n = 0; n < CN; n++) x[n] = lds16(in + n * WG * 16);
     }
-    // Where the thread's first piece goes in buffer 0; the second is 16 bytes off (either way), the next 16 bytes' are V's (two rows sets of 32
-    // apart, HD = 128) or none
+    // Where the thread's first piece goes in buffer 0.  Its second is the other one of 32 bytes; what a thread takes next is V's, 32 rows behind.
     __device__ __forceinline__ unsigned first_piece() const {
         const int i = 64 * wave + lane, r = i / PR;
         return ldsBase + (unsigned)r * ROWB + (unsigned)((2 * (i % PR)) ^ swz(r)) * 16;
@@ -1508,7 +1513,7 @@ struct WideTile {
     }
     // Q8: scores to weights of V's whole numbers, as NarrowTile::weigh_q8; returns the lane's sum of the probabilities (times 2^(m - ref)).  f: what
     // l and o are multiplied by first (in one place, once: where a loop changes o in several, the compiler keeps it twice and moves it).
-    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, const float4_t (&ks)[4], const float4_t (&vs)[4], float& f) {
+    __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, const float4_t (&ks)[4], float4_t (&vs)[4], float& f) {
         constexpr float FIT = 32768.f;
         static_assert(!Q8 || NB == 1, "16 positions a lane");
         f = 1.f;
@@ -1537,7 +1542,10 @@ struct WideTile {
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int key = first + 32 * b + 8 * (i / 4) + i % 4;
-                    if (!((held >> (4 * b + i / 4)) & 1) || (SHARED && key < t.from) || !paged_sees(row.pos, key, t.len, p.window, t.prefix)) S[b][i] = -INFINITY;
+                    if (!((held >> (4 * b + i / 4)) & 1) || (SHARED && key < t.from) || !paged_sees(row.pos, key, t.len, p.window, t.prefix)) {
+                        S[b][i] = -INFINITY;
+                        vs[i / 4][i % 4] = 0.f;           // (its scale may be anything)
+                    }
                 }
         }
         float top = S[0][0];
@@ -1562,19 +1570,15 @@ struct WideTile {
             m = mNew;
         }
         float ts = 0.f, most = 0.f;
-        auto weights = [&](auto product) {
 #pragma unroll
-            for (int b = 0; b < NB; b++)
+        for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    const float x = __builtin_amdgcn_exp2f(fmaf(S[b][i], factor, -ref));
-                    ts += x;
-                    S[b][i] = product(x, vs[i / 4][i % 4]);
-                    most = fmaxf(most, S[b][i]);
-                }
-        };
-        if (all) weights([](float x, float d) { return x * d; });
-        else weights([](float x, float d) { return x == 0.f ? 0.f : x * d; });        // (a hidden position's scale may be anything)
+            for (int i = 0; i < 16; i++) {
+                const float x = __builtin_amdgcn_exp2f(fmaf(S[b][i], factor, -ref));
+                ts += x;
+                S[b][i] = x * vs[i / 4][i % 4];
+                most = fmaxf(most, S[b][i]);
+            }
         if (__any(most > FIT)) {
             most = both(most);
             const float down = most > FIT ? exponent(most) : 0.f, less = __builtin_amdgcn_exp2f(down);
