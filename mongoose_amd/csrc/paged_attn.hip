@@ -1705,7 +1705,6 @@ struct WideTile {
             for (int b = 0; b < DB; b++) o[b] *= f;
         }
         l += ts;
-        if (!inner && !__any(ts != 0.f)) return;          // (no row has anything here)
         Weights w;
         auto halve = [&](int i) { two_terms(S[0][i], S[0][i + 1], i % 8, w.hi[i / 8], w.lo[i / 8], minus1); };
 #pragma unroll

@@ -312,13 +312,15 @@ def test_rows_that_are_no_numbers_count_where_they_are_seen(hip, bufs, heads, kv
         c.h.Close()
 
 
+@pytest.mark.parametrize("around", [1, 32])
 @pytest.mark.parametrize("new,length,bad", [(1, 300, 299), (1, 300, 40), (3, 90, 88), (70, 70, 41), (70, 200, 160), (70, 200, 3)])
-def test_a_row_that_is_no_number_under_no_weight(hip, bufs, new, length, bad):
+def test_a_row_that_is_no_number_under_no_weight(hip, bufs, new, length, bad, around):
     """A probability that fp32 holds as 0, times a scale that is a NaN: the rows that see the position have it, the others have not."""
     c = Case8(hip, bufs, 8, 2, 64, 8, [new, 70], [length, 75], seed=bad)
     c.q[:] = 1.0
     x = np.float32(c.K)
-    x[c.where(0, bad)] = -100.0                      # a score of -800, the others' within 10 of 0
+    for pos in range(bad // around * around, min(bad // around * around + around, length)):
+        x[c.where(0, pos)] = -100.0                  # a score of -800, the others' within 10 of 0
     c.set_rows("K", x)
     x = np.float32(c.V)
     x[c.where(0, bad)] = np.nan
