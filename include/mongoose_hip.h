@@ -481,8 +481,8 @@ int mg_stream_forward_token(mg_stream* s, int pos, const float* embHidden, int n
  * Request r's position p is in page table[r * width + p / pageSize], width = mg_paged_table_width.  One table serves all layers.
  *
  * Q8: an int8 an element and an fp32 scale a KV head's row of a position, worth q * scale: scale = max |x| / 127 over the row (rounded to
- * fp32), q = x / scale to the nearest whole number, half away from zero, decided exactly (of K: x the turned element, exact to 64 bits and
- * then rounded to fp32).  A row with an infinity or a NaN gets a NaN for its scale.  A pool is the int8 rows [nPages, pageSize, nKVHeads *
+ * fp32), q = x / scale to the nearest whole number, half away from zero, decided exactly, and 127 at most (of K: x the turned element, exact
+ * to 64 bits and then rounded to fp32).  A row with an infinity or a NaN gets a NaN for its scale.  A pool is the int8 rows [nPages, pageSize, nKVHeads *
  * headDim], then the scales [nPages, nKVHeads, pageSize]: headDim + 4 bytes where fp16 takes 2 * headDim.
  *
  * A step of a server:   mg_paged_tables   once a step: rows, slots and block tables from the requests' lengths
