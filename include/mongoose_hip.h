@@ -558,8 +558,10 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
  * its rows.  A shared length is cut to the positions that all of its requests with rows have ahead of their new ones; requests
  * of no group, and groups of one request with rows, share nothing.  mostNew: the most rows that a request of the step has, if the caller knows (0: any
  * number; more of them than said cost time, not results).  nGroups <= maxReqs; all arrays are device memory and are copied.
- * mg_paged_share allocates the workspace for it, once, before the first such plan: a share of a tile (128 rows of headDim + 2 floats) for each of 1,024 workgroups
- * (MG_E_STATE without it).  Of attention's rule on plans, nGroups is a part. */
+ * mg_paged_share allocates the workspace for it, once, before the first such plan (MG_E_STATE without it): for every KV head a share of a tile
+ * (128 rows of headDim + 2 floats) for each of the tiles that groups may have, maxRows * (nHeads / nKVHeads) / 128 + 16 + maxReqs / 2, and for
+ * each of the head's workgroups, 512 / nKVHeads -- 94 MB for 64 requests of 2,048 rows in all, 32 heads on 8 of 128 --, and 128 bytes for each
+ * of maxRows * (nHeads / nKVHeads) / 16 + maxReqs tiles.  Of attention's rule on plans, nGroups is a part. */
 int mg_paged_share(mg_paged* h);
 int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int mostNew, const int* groupStart,
                          const int* sharedLens, int nGroups, void* stream);

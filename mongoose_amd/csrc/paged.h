@@ -86,8 +86,8 @@ struct PagedAttention {
     const int4 *reqs, *groups; // as in PagedGroups
     const int* groupTile;
     const PagedTile* sharedTiles;
-    const float* sharedParts;
-    int sharedWorkers, sharedRows;       // of the first pass: workers a KV head, rows of a tile
+    float* sharedParts;
+    int sharedPlaces, sharedRows;        // of the first pass: shares a KV head (paged_place), rows of a tile
     int ldq, ldo, window, maxTiles, maxWorkers, nWorkers, wideWorkers;
     PagedGeo g;
 };

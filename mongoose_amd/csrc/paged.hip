@@ -380,7 +380,7 @@ struct mg_paged {
     mg::PagedWorker* sharedWorkers[2];
     unsigned* sharedArrived;
     float* sharedParts;                        // what the first pass leaves for the second
-    int sharedMaxTiles, sharedPlanWorkers[2], sharedPlanWide[2];
+    int sharedMaxTiles[2], sharedPlaces, sharedPlanWorkers[2], sharedPlanWide[2];
 };
 
 namespace {
@@ -507,14 +507,14 @@ int mg_paged_share(mg_paged* h) {
     PAGED(h, "mg_paged_share");
     if (h->sharedMem) return MG_OK;
     const mg::PagedGeo& g = h->g;
-    const size_t tiles = (size_t)mg::paged_max_tiles_shared(g);
+    const size_t tiles[2] = {(size_t)mg::paged_group_tiles(g), (size_t)mg::paged_max_tiles_shared(g)}, places = tiles[0] + h->maxWorkers;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t here = at; at += (bytes + 255) & ~(size_t)255; return here; };
-    const size_t oArrived = take(tiles * g.nKVHeads * 4), clear = at, oReqs = take((size_t)g.maxReqs * sizeof(int4)), oGroups = take((size_t)g.maxReqs * sizeof(int4)),
+    const size_t oArrived = take(tiles[1] * g.nKVHeads * 4), clear = at, oReqs = take((size_t)g.maxReqs * sizeof(int4)), oGroups = take((size_t)g.maxReqs * sizeof(int4)),
                  oGroupOf = take((size_t)g.maxReqs * 4), oGroupTile = take(((size_t)g.maxReqs + 1) * 4);
     size_t oTiles[2], oWorkers[2];
-    for (int i = 0; i < 2; i++) { oTiles[i] = take(2 * tiles * sizeof(mg::PagedTile)); oWorkers[i] = take(2 * (size_t)h->maxWorkers * sizeof(mg::PagedWorker)); }
-    const size_t oParts = take((size_t)g.nKVHeads * h->maxWorkers * 2 * mg::paged_part_floats(g) * 4);
+    for (int i = 0; i < 2; i++) { oTiles[i] = take(2 * tiles[i] * sizeof(mg::PagedTile)); oWorkers[i] = take(2 * (size_t)h->maxWorkers * sizeof(mg::PagedWorker)); }
+    const size_t oParts = take((size_t)g.nKVHeads * places * mg::paged_part_floats(g) * 4);
     char* mem = nullptr;
     hipError_t e = hipMalloc(reinterpret_cast<void**>(&mem), at);
     if (e == hipSuccess) {
@@ -528,11 +528,12 @@ int mg_paged_share(mg_paged* h) {
         return MG_E_HIP;
     }
     h->sharedMem = mem;
-    h->sharedMaxTiles = (int)tiles;
+    h->sharedPlaces = (int)places;
     h->sharedArrived = reinterpret_cast<unsigned*>(mem + oArrived);
     h->reqs = reinterpret_cast<int4*>(mem + oReqs);
     h->groups = reinterpret_cast<int4*>(mem + oGroups);
     for (int i = 0; i < 2; i++) {
+        h->sharedMaxTiles[i] = (int)tiles[i];
         h->sharedTiles[i] = reinterpret_cast<mg::PagedTile*>(mem + oTiles[i]);
         h->sharedWorkers[i] = reinterpret_cast<mg::PagedWorker*>(mem + oWorkers[i]);
     }
@@ -553,7 +554,7 @@ int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int 
     for (int i = 0; i < 2; i++) {
         const int n = i ? nReqs : nGroups, narrow = mg::paged_narrow_rows_shared(g, rows, i ? mostNew : 0, i == 0);
         p[i] = {nullptr, nullptr, nullptr, i ? h->reqs : h->groups, i ? h->groupOf : nullptr, i ? nullptr : h->groupTile, h->made, h->sharedTiles[i], h->sharedWorkers[i], n, rows, 0, g.maxLen, g.group, g.kvFormat,
-                h->sharedMaxTiles, h->maxWorkers, mg::paged_workers(g, n, rows, false, mg::paged_shared_twice(g, n, rows, i == 0)), (long long)rows * g.group > narrow ? mg::paged_workers(g, n, rows, true) : 0, narrow, made};
+                h->sharedMaxTiles[i], h->maxWorkers, mg::paged_workers(g, n, rows, false, mg::paged_shared_twice(g, n, rows, i == 0)), (long long)rows * g.group > narrow ? mg::paged_workers(g, n, rows, true) : 0, narrow, made};
     }
     const int rc = launched("mg_paged_plan_shared", mg::launch_paged_plan_shared({rowStart, lens, groupStart, sharedLens, h->reqs, h->groupOf, h->groups, nReqs, rows, nGroups, g.maxLen}, p[0], p[1],
                                                                                  static_cast<hipStream_t>(stream)));
@@ -572,19 +573,15 @@ int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, cons
     if (const char* why = mg::paged_attention_overlap(h->g, q, ldq, K, V, out, ldo, h->plan.rows)) return refuse("mg_paged_attention", why);
     const mg::PagedGeo& g = h->g;
     mg::PagedAttention p{q, slopes, K, V, table, out, h->made, h->tiles, h->workers, h->parts, h->arrived, h->zeros, mg::paged_part_floats(g),
-                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, h->plan, 0, h->reqs, h->groups, h->groupTile, h->sharedTiles[0], h->sharedParts, h->sharedPlanWorkers[0], 0, ldq, ldo, h->plan.window, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
+                         scale == 0.f ? 1.0f / std::sqrt((float)g.headDim) : scale, softcap, h->plan, 0, h->reqs, h->groups, h->groupTile, h->sharedTiles[0], h->sharedParts, h->sharedPlaces, 0, ldq, ldo, h->plan.window, h->maxTiles, h->maxWorkers, h->planWorkers, h->planWideWorkers, g};
     if (h->plan.groups == 0) return launched("mg_paged_attention", mg::launch_paged_attention(p, static_cast<hipStream_t>(stream)));
     p.arrived = h->sharedArrived;
-    p.maxTiles = h->sharedMaxTiles;
     const bool wide = h->sharedPlanWorkers[0] == 0;          // (the groups' tiles)
     p.sharedRows = wide ? mg::PAGED_WIDE : mg::PAGED_NARROW;
-    if (wide) {
-        p.sharedWorkers = h->sharedPlanWide[0];
-        p.sharedTiles += h->sharedMaxTiles;
-    }
+    if (wide) p.sharedTiles += h->sharedMaxTiles[0];
     for (int i = 0; i < 2; i++) {
         p.pass = i + 1;
-        p.parts = i ? h->parts : h->sharedParts;
+        p.maxTiles = h->sharedMaxTiles[i];
         p.tiles = h->sharedTiles[i];
         p.workers = h->sharedWorkers[i];
         p.nWorkers = h->sharedPlanWorkers[i];

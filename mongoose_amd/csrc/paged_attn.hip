@@ -176,7 +176,7 @@ __device__ __forceinline__ void make_plan(PagedPlan p, bool wide) {
     __syncthreads();
     const int nTiles = (int)min(sum, (unsigned)p.maxTiles);          // (more only where the caller's rows overlap)
     if (p.groupTile && wide == (p.narrowRows == 0)) {                // (groups' tiles are all of one kind)
-        for (int g = tid; g < p.nReqs; g += PT) p.groupTile[g] = (int)tile0[g];
+        for (int g = tid; g < p.nReqs; g += PT) p.groupTile[g] = min((int)tile0[g], nTiles);
         if (tid == 0) p.groupTile[p.nReqs] = nTiles;
     }
     PagedTile t;
@@ -409,6 +409,10 @@ __device__ __forceinline__ const char* kv_row(const char* pool, const char* zero
 __device__ __forceinline__ float* part_of(const PagedAttention& p, const PagedTile& t, int kvh, int w) {
     return p.parts + (((size_t)kvh * p.nWorkers + w) * 2 + (w == t.worker0)) * p.partStride;
 }
+// The same in the first pass of shared prefixes, where tiles of one worker leave a share too
+__device__ __forceinline__ float* shared_part(const PagedAttention& p, int kvh, int tile, int w) {
+    return p.sharedParts + ((size_t)kvh * p.sharedPlaces + paged_place(tile, w)) * p.partStride;
+}
 // After a worker has stored its share (through to memory): whether it is the last one of the tile's to come here.  scratch: LDS
 // that nobody reads any more.
 __device__ __forceinline__ bool last_to_finish(const PagedAttention& p, const PagedTile& t, int kvh, float* scratch) {
@@ -488,9 +492,9 @@ __device__ __forceinline__ PagedShares shares_of(const PagedAttention& p, const 
     // (outside of the group or behind the last tile only where the caller's rows overlap)
     if (r < 0 || r >= g.y * p.g.group || i >= p.groupTile[p.plan.groups]) return {nullptr, 0, 0};
     const int w0 = p.sharedTiles[i].worker0, w1 = p.sharedTiles[i].worker1;
-    return {p.sharedParts + (((size_t)kvh * p.sharedWorkers + w0) * 2 + 1) * p.partStride, w1 - w0 + 1, r % p.sharedRows};
+    return {shared_part(p, kvh, i, w0), w1 - w0 + 1, r % p.sharedRows};
 }
-__device__ __forceinline__ const float* share_at(const PagedAttention& p, const PagedShares& x, int s) { return x.first + (size_t)(s > 0 ? 2 * s - 1 : 0) * p.partStride; }       // (as part_of)
+__device__ __forceinline__ const float* share_at(const PagedAttention& p, const PagedShares& x, int s) { return x.first + (size_t)s * p.partStride; }
 template <int HD>
 __device__ __forceinline__ float4_t share4(const PagedAttention& p, const float* share, int row, int d) {
     const int i = p.sharedRows == NARROW ? row * HD + d : ((row / 32 * (HD / 32) + d / 32) * 4 + d % 32 / 8) * 256 + (d % 8 / 4 * 32 + row % 32) * 4;
@@ -1113,7 +1117,7 @@ struct NarrowTile {
         const float* ls = ms + 4 * NARROW;
         const int tid = thread_anew(), R = min(NARROW, t.rows * p.g.group - t.first);
         const bool whole = t.worker0 == t.worker1 && !(SHARED && p.pass == 1);
-        float* mine = part_of(p, t, kvh, w);
+        float* mine = SHARED && p.pass == 1 ? shared_part(p, kvh, t.index, w) : part_of(p, t, kvh, w);
 #pragma unroll
         for (int k = 0; k < NP; k++) {
             const int i = tid + k * WG;
@@ -1805,7 +1809,7 @@ struct WideTile {
     __device__ __forceinline__ void write(int kvh, int w, float* lds) {
         const int r = 32 * wave + n32;
         if (t.worker0 != t.worker1 || (SHARED && p.pass == 1)) {
-            float* part = part_of(p, t, kvh, w);
+            float* part = SHARED && p.pass == 1 ? shared_part(p, kvh, t.index, w) : part_of(p, t, kvh, w);
             if (active) {
 #pragma unroll
                 for (int b = 0; b < DB; b++)

@@ -280,6 +280,16 @@ MG_HD int paged_workers_for(const PagedTile& t, int cost, int tiles, int workers
 MG_HD int paged_part(const PagedTile& t, int n, int i) {
     return i == 0 ? t.cost0 : t.cost0 + PAGED_TILE_COST + (int)((long long)t.units * i / n);
 }
+// The share that worker w leaves of a group's tile i, of those that a KV head has.  With shared prefixes every worker leaves one of every tile
+// that it has part of, the only one of a tile as well, so that there may be any number of a worker's.  Along the line either the tile or the
+// worker steps on from a share to the next, so no two have the same sum of their numbers.
+MG_HD int paged_place(int tile, int worker) { return tile + worker; }
+// The tiles that groups' rows may have (wide: one a group more than there are whole ones; narrow: for up to 256 rows): a group that shares
+// anything has two requests with rows.
+inline int paged_group_tiles(const PagedGeo& g) {
+    const int requests = g.maxReqs < g.maxRows ? g.maxReqs : g.maxRows;
+    return (int)((long long)g.maxRows * g.group / PAGED_WIDE) + 256 / PAGED_NARROW + requests / 2;
+}
 // The first unit of a tile that starts at `a` on the line or behind.
 MG_HD int paged_unit_at(const PagedTile& t, int a) {
     const int u = a - (t.cost0 + PAGED_TILE_COST);

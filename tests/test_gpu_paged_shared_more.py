@@ -1,0 +1,84 @@
+"""More of attention behind shared prefixes (HIPPaged.PlanShared): groups whose tiles are many for the workers that there are, so that a worker has
+several of them and leaves a share of each.  Bounds as in test_gpu_paged_shared."""
+import copy
+
+import numpy as np
+import pytest
+
+from tests.test_gpu_paged import _synced, bufs, rt  # noqa: F401  (fixtures)
+from tests.test_gpu_paged_shared import FORMATS, make, plan
+
+pytestmark = pytest.mark.gpu
+
+
+def want_of(c, reqs, **what):
+    """What the model gives for some of the requests, and their rows."""
+    s = copy.copy(c)
+    s.new, s.lens, s.table = c.new[reqs], c.lens[reqs], c.table[reqs]
+    rows = np.concatenate([np.arange(c.rowStart[r], c.rowStart[r + 1]) for r in reqs])
+    s.q, s.rowStart = c.q[rows], np.concatenate(([0], np.cumsum(s.new))).astype(np.int32)
+    return (rows, *s.want(**what))
+
+
+def check_some(c, reqs, mostNew=0, **what):
+    c.upload()
+    plan(c, mostNew)
+    c.attend(**what)
+    _synced()
+    got = c.result()
+    assert np.isfinite(got).all()
+    rows, want, bound = want_of(c, reqs, **what)
+    off = np.abs(got[rows][:, :c.heads * c.hd] - want) / bound
+    print(f"  worst {off.max():.3f} of the bound", flush=True)
+    assert off.max() <= 1.0, np.unique(rows[np.nonzero((off > 1).any(1))[0]])[:10].tolist()
+    c.h.Close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,hd,n,new,length,groups", [(16, 8, 64, 16, 400, 300, 1), (16, 8, 64, 16, 400, 300, 2), (6, 6, 128, 5, 1500, 333, 2), (32, 8, 128, 4, 1024, 1000, 1)])
+def test_prompts_that_arrive_together(hip, bufs, fmt, heads, kv, hd, n, new, length, groups):
+    """Tiles from half the workers up: a worker has the end of one and all of the next."""
+    print(f"shared prompts fmt={fmt} {heads}/{kv}/{hd} {n} of {new} behind {length}, {groups} groups", flush=True)
+    own = [new + (r % 3) * (groups - 1) for r in range(n)]
+    starts = [0, n] if groups == 1 else [0, n // 2, n]
+    c = make(fmt, hip, bufs, heads, kv, hd, 32, own, [length + x for x in own], starts, [length, length // 3][:groups], seed=n)
+    check_some(c, [0, n // 2, n - 1] if heads < 32 else [2], new + 2)
+
+
+@pytest.mark.parametrize("fmt,mostNew", [(0, 0), (1, 40), (8, 40)])
+def test_many_requests_of_some_rows(hip, bufs, fmt, mostNew):
+    """64 requests of 40 rows behind 8,001 positions: 80 tiles for 64 workers."""
+    print(f"shared 64 x 40 behind 8001 fmt={fmt} mostNew={mostNew}", flush=True)
+    c = make(fmt, hip, bufs, 32, 8, 128, 64, [40] * 64, [8041 + r % 7 for r in range(64)], [0, 64], [8001], seed=1)
+    check_some(c, [0, 21, 63], mostNew)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("heads,kv,hd,size,new", [(32, 8, 128, 2, 1), (8, 8, 64, 2, 1), (14, 2, 64, 3, 3), (8, 8, 64, 2, 9)])
+def test_many_groups_of_any_length(hip, bufs, fmt, heads, kv, hd, size, new):
+    """Groups of two or three requests behind 50 to 3,000 positions: a worker has many short tiles, or a part of a long one; narrow and wide."""
+    print(f"shared groups fmt={fmt} {heads}/{kv}/{hd} size={size} new={new}", flush=True)
+    n = 100 if new == 1 else 70
+    rng = np.random.default_rng(n + size)
+    shared = np.exp(rng.uniform(np.log(50), np.log(3000), n)).astype(int)
+    own = [new + int(rng.integers(0, 30)) for _ in range(n * size)]
+    lens = [int(shared[r // size]) + own[r] for r in range(n * size)]
+    c = make(fmt, hip, bufs, heads, kv, hd, 16, [new] * (n * size), lens, list(range(0, n * size + 1, size)), shared, seed=n)
+    check_some(c, list(range(n * size)), new)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_few_rows_in_many_groups(hip, bufs, fmt):
+    """Narrow tiles, more than workers: 60 groups of two requests, one query head a KV head, 16 KV heads."""
+    rng = np.random.default_rng(4)
+    shared = rng.integers(20, 900, 60)
+    lens = [int(shared[r // 2]) + int(rng.integers(1, 40)) for r in range(120)]
+    c = make(fmt, hip, bufs, 16, 16, 64, 8, [1] * 120, lens, list(range(0, 121, 2)), shared, seed=8)
+    check_some(c, list(range(120)), 1)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_scores_changed_by_distance_in_many_tiles(hip, bufs, fmt):
+    slopes = np.exp2(-np.arange(1, 9)).astype(np.float32)
+    c = make(fmt, hip, bufs, 8, 8, 64, 16, [150] * 40, [370 + r for r in range(40)], list(range(0, 41, 4)), [200, 60, 199, 3, 120, 210, 64, 65, 180, 1], seed=5)
+    check_some(c, [0, 5, 11, 22, 39], 150, cap=30.0, slopes=slopes)
