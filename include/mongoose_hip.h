@@ -561,7 +561,9 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
  * mg_paged_share allocates the workspace for it, once, before the first such plan (MG_E_STATE without it): for every KV head a share of a tile
  * (128 rows of headDim + 2 floats) for each of the tiles that groups may have, maxRows * (nHeads / nKVHeads) / 128 + 16 + maxReqs / 2, and for
  * each of the head's workgroups, 512 / nKVHeads -- 94 MB for 64 requests of 2,048 rows in all, 32 heads on 8 of 128 --, and 128 bytes for each
- * of maxRows * (nHeads / nKVHeads) / 16 + maxReqs tiles.  Of attention's rule on plans, nGroups is a part. */
+ * of maxRows * (nHeads / nKVHeads) / 16 + maxReqs tiles.  nGroups and mostNew
+ * are parts of attention's rule on plans: where the plan on the device was made with a mostNew that divides the requests otherwise, a call
+ * does nothing. */
 int mg_paged_share(mg_paged* h);
 int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int mostNew, const int* groupStart,
                          const int* sharedLens, int nGroups, void* stream);

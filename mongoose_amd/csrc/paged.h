@@ -35,13 +35,6 @@ hipError_t launch_paged_load(const PagedLoad& p, hipStream_t s);
 struct PagedWorker { PagedTile tile; int a, b, tiles, pad[13]; };
 static_assert(sizeof(PagedTile) == 64 && sizeof(PagedWorker) == 128, "read as 16-byte words");
 
-// What a plan was made for.  The places and numbers of its tiles and workers follow from these: an attention call works on the plan that is
-// in the handle's memory only where they are its own (a graph's replay may have left another one there, or it was captured and has not run).
-struct PagedPlanFor {
-    int nReqs, rows, window, groups;
-    MG_HD bool is(const PagedPlanFor& o) const { return ((nReqs ^ o.nReqs) | (rows ^ o.rows) | (window ^ o.window) | (groups ^ o.groups)) == 0; }      // (no branch between the loads)
-};
-
 // The plan that a step's attention calls share.
 struct PagedPlan {
     const int *rowStart, *lens, *prefixLens;      // the caller's
@@ -96,8 +89,6 @@ int paged_max_tiles(const PagedGeo& g);
 int paged_max_tiles_shared(const PagedGeo& g);
 bool paged_shared_twice(const PagedGeo& g, int nReqs, int rows, bool groups);
 int paged_workers(const PagedGeo& g, int nReqs, int rows, bool wide, bool twice = false);       // workers a KV head
-int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool groups);
-int paged_narrow_rows(const PagedGeo& g, int rows);              // requests of up to so many rows a KV head have narrow tiles
 hipError_t paged_attention_setup(const PagedGeo& g);
 hipError_t launch_paged_attention(const PagedAttention& p, hipStream_t s);
 

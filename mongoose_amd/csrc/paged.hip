@@ -496,7 +496,7 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
     const int workers = mg::paged_workers(g, nReqs, rows, false), narrow = mg::paged_narrow_rows(g, rows);
     const int wide = (long long)rows * g.group > narrow ? mg::paged_workers(g, nReqs, rows, true) : 0;
     mg::PagedPlan p{rowStart, lens, prefixLens, nullptr, nullptr, nullptr, h->made, h->tiles, h->workers, nReqs, rows, window, g.maxLen, g.group, g.kvFormat, h->maxTiles, h->maxWorkers, workers, wide, narrow,
-                    {nReqs, rows, window, 0}};
+                    {nReqs, rows, window, 0, narrow}};
     const int rc = launched("mg_paged_plan", mg::launch_paged_plan(p, static_cast<hipStream_t>(stream)));
     if (rc == MG_OK) {
         h->plan = p.plan; h->planWorkers = workers; h->planWideWorkers = wide;
@@ -549,10 +549,10 @@ int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int 
     const mg::PagedGeo& g = h->g;
     if (const char* why = mg::paged_plan_shared_refusal(g, rowStart, lens, nReqs, rows, mostNew, groupStart, sharedLens, nGroups)) return refuse("mg_paged_plan_shared", why);
     if (nGroups == 0) return mg_paged_plan(h, rowStart, lens, nReqs, rows, 0, nullptr, stream);
-    const mg::PagedPlanFor made{nReqs, rows, 0, nGroups};
+    const mg::PagedPlanFor made{nReqs, rows, 0, nGroups, mg::paged_narrow_rows_shared(g, rows, mostNew, false)};
     mg::PagedPlan p[2];
     for (int i = 0; i < 2; i++) {
-        const int n = i ? nReqs : nGroups, narrow = mg::paged_narrow_rows_shared(g, rows, i ? mostNew : 0, i == 0);
+        const int n = i ? nReqs : nGroups, narrow = i ? made.narrowRows : mg::paged_narrow_rows_shared(g, rows, 0, true);
         p[i] = {nullptr, nullptr, nullptr, i ? h->reqs : h->groups, i ? h->groupOf : nullptr, i ? nullptr : h->groupTile, h->made, h->sharedTiles[i], h->sharedWorkers[i], n, rows, 0, g.maxLen, g.group, g.kvFormat,
                 h->sharedMaxTiles[i], h->maxWorkers, mg::paged_workers(g, n, rows, false, mg::paged_shared_twice(g, n, rows, i == 0)), (long long)rows * g.group > narrow ? mg::paged_workers(g, n, rows, true) : 0, narrow, made};
     }

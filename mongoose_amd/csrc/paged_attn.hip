@@ -44,33 +44,6 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 MG_HD int narrow_keys(int kvFormat) { return kvFormat == PAGED_F32 ? 64 : 128; }
 MG_HD int wide_keys(int kvFormat) { return kvFormat == PAGED_F16 ? 64 : 32; }
 
-// Rows a KV head (tokens x group) up to which a request goes to the kernel that waits for memory, with longer ones to the one that waits for
-// the matrix units.  8B shape:
-//   A batch of up to 256 rows: all narrow, which reads K and V once for 16 rows, but in one launch.  One request of 8, 16, 32 and 64 tokens
-//   over 16,000 positions: fp16 33, 41, 64, 112 us, wide 83, 89, 103, 105; fp32 43, 66, 117, 220, wide 338, 380, 401, 317.
-//   Larger batches: narrow up to 16 rows.  24 requests of 5, 8, 12 tokens over 500 to 4,000 positions, fp16: 77, 78, 80 us wide, 75, 81, 99
-//   narrow, and 96 requests of 5 tokens 208 wide, 304 narrow.  With an fp32 cache narrow tiles would be better there, up to 64 rows (228,
-//   204, 385, and with 16 tokens 361 us wide; 169, 141, 249, 276 narrow): its wide tiles wait for the fp32 instructions of rows that are not there.
-//   Q8: a wide tile also has its rows turned to halves for rows that are not there, so narrow ones go further: 24 requests of 5, 8, 12, 16 tokens
-//   as above 98, 90, 104, 113 us wide, 59, 55, 69, 90 narrow; 1.1B shape, 5 tokens 62 and 41.  With many requests, whose wide tiles fill the
-//   CUs, up to 32 rows: 96 requests of 5, 8, 16 tokens 233, 231, 299 and 203, 209, 405; 1.1B shape, 8 tokens 115 and 138.
-constexpr int NARROW_Q8_FEW = 64, NARROW_Q8 = 32, Q8_FEW_ROWS = 4096;
-int paged_narrow_rows(const PagedGeo& g, int rows) {
-    const long long all = (long long)rows * g.group;
-    if (all <= 256) return 256;
-    return g.kvFormat != PAGED_Q8 ? NARROW : all <= Q8_FEW_ROWS ? NARROW_Q8_FEW : NARROW_Q8;
-}
-// The same with shared prefixes, for groups (0: all groups have wide tiles; up to 256 rows, as above: 64 requests behind 8,001 positions 98 us, with
-// wide ones 133) and for requests, of which the caller may know that none adds more than mostNew rows.  What requests have of their own is short, so
-// narrow tiles go further while the wide ones would not fill the CUs (80 requests, 378 rows in all, up to 40 each, Q8: 210 us a call, so 163; 32 of
-// 40 rows each, more rows than that: 219 and 235).
-int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool groups) {
-    constexpr int ALL = PAGED_MAX_ROWS * PAGED_MAX_GROUP;
-    if ((long long)rows * g.group <= 256) return ALL;
-    if (groups) return 0;
-    const int narrow = (long long)rows * g.group <= 4096 ? 256 : paged_narrow_rows(g, rows);
-    return mostNew > 0 && (long long)mostNew * g.group <= narrow ? ALL : narrow;
-}
 // Whether with shared prefixes narrow tiles of groups, or of requests, have two workgroups a CU.  Groups: where many tiles read the same positions, out
 // of the L2s, but for an fp32 cache (8B shape, prefix of 8,001; 16, 32, 64 requests of a token fp16 42, 63, 100 us a call, with two
 // 44, 62, 93; 32 fp32 97 and 106; 4 behind 40,000 positions fp16 59 and 80).  Requests: where there are more tiles than that, short ones all

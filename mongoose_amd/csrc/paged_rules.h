@@ -296,6 +296,43 @@ MG_HD int paged_unit_at(const PagedTile& t, int a) {
     return u <= 0 ? 0 : u < t.units ? u : t.units;
 }
 
+// Rows a KV head (tokens x group) up to which a request goes to the kernel that waits for memory, with longer ones to the one that waits for
+// the matrix units.  8B shape:
+//   A batch of up to 256 rows: all narrow, which reads K and V once for 16 rows, but in one launch.  One request of 8, 16, 32 and 64 tokens
+//   over 16,000 positions: fp16 33, 41, 64, 112 us, wide 83, 89, 103, 105; fp32 43, 66, 117, 220, wide 338, 380, 401, 317.
+//   Larger batches: narrow up to 16 rows.  24 requests of 5, 8, 12 tokens over 500 to 4,000 positions, fp16: 77, 78, 80 us wide, 75, 81, 99
+//   narrow, and 96 requests of 5 tokens 208 wide, 304 narrow.  With an fp32 cache narrow tiles would be better there, up to 64 rows (228,
+//   204, 385, and with 16 tokens 361 us wide; 169, 141, 249, 276 narrow): its wide tiles wait for the fp32 instructions of rows that are not there.
+//   Q8: a wide tile also has its rows turned to halves for rows that are not there, so narrow ones go further: 24 requests of 5, 8, 12, 16 tokens
+//   as above 98, 90, 104, 113 us wide, 59, 55, 69, 90 narrow; 1.1B shape, 5 tokens 62 and 41.  With many requests, whose wide tiles fill the
+//   CUs, up to 32 rows: 96 requests of 5, 8, 16 tokens 233, 231, 299 and 203, 209, 405; 1.1B shape, 8 tokens 115 and 138.
+constexpr int NARROW_Q8_FEW = 64, NARROW_Q8 = 32, Q8_FEW_ROWS = 4096;
+inline int paged_narrow_rows(const PagedGeo& g, int rows) {
+    const long long all = (long long)rows * g.group;
+    if (all <= 256) return 256;
+    return g.kvFormat != PAGED_Q8 ? PAGED_NARROW : all <= Q8_FEW_ROWS ? NARROW_Q8_FEW : NARROW_Q8;
+}
+// The same with shared prefixes, for groups (0: all groups have wide tiles; up to 256 rows, as above: 64 requests behind 8,001 positions 98 us, with
+// wide ones 133) and for requests, of which the caller may know that none adds more than mostNew rows.  What requests have of their own is short, so
+// narrow tiles go further while the wide ones would not fill the CUs (80 requests, 378 rows in all, up to 40 each, Q8: 210 us a call, so 163; 32 of
+// 40 rows each, more rows than that: 219 and 235).
+inline int paged_narrow_rows_shared(const PagedGeo& g, int rows, int mostNew, bool groups) {
+    constexpr int ALL = PAGED_MAX_ROWS * PAGED_MAX_GROUP;
+    if ((long long)rows * g.group <= 256) return ALL;
+    if (groups) return 0;
+    const int narrow = (long long)rows * g.group <= 4096 ? 256 : paged_narrow_rows(g, rows);
+    return mostNew > 0 && (long long)mostNew * g.group <= narrow ? ALL : narrow;
+}
+// What a plan was made for.  The places, numbers and kinds of its tiles and workers follow from these: an attention call works on the plan that is
+// in the handle's memory only where they are its own (a graph's replay may have left another one there, or it was captured and has not run).
+struct PagedPlanFor {
+    int nReqs, rows, window, groups;
+    int narrowRows;        // requests of up to so many rows a KV head have narrow tiles: what the caller knows of the rows is in it
+    MG_HD bool is(const PagedPlanFor& o) const {
+        return ((nReqs ^ o.nReqs) | (rows ^ o.rows) | (window ^ o.window) | (groups ^ o.groups) | (narrowRows ^ o.narrowRows)) == 0;      // (no branch between the loads)
+    }
+};
+
 // Why mg_paged_tables changes nothing
 enum { PAGED_NO_PAGES = 1, PAGED_NO_ROWS = 2, PAGED_BAD_LENGTH = 4, PAGED_BAD_RING = 8 };
 

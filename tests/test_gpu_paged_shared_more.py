@@ -1,11 +1,12 @@
 """More of attention behind shared prefixes (HIPPaged.PlanShared): groups whose tiles are many for the workers that there are, so that a worker has
-several of them and leaves a share of each.  Bounds as in test_gpu_paged_shared."""
+several of them and leaves a share of each; plans that differ in the most rows that a request has.  Bounds as in test_gpu_paged_shared."""
 import copy
 
 import numpy as np
 import pytest
 
-from tests.test_gpu_paged import _synced, bufs, rt  # noqa: F401  (fixtures)
+from mongoose_amd import engine as E
+from tests.test_gpu_paged import _ok, _synced, bufs, rt  # noqa: F401  (fixtures)
 from tests.test_gpu_paged_shared import FORMATS, make, plan
 
 pytestmark = pytest.mark.gpu
@@ -82,3 +83,68 @@ def test_scores_changed_by_distance_in_many_tiles(hip, bufs, fmt):
     slopes = np.exp2(-np.arange(1, 9)).astype(np.float32)
     c = make(fmt, hip, bufs, 8, 8, 64, 16, [150] * 40, [370 + r for r in range(40)], list(range(0, 41, 4)), [200, 60, 199, 3, 120, 210, 64, 65, 180, 1], seed=5)
     check_some(c, [0, 5, 11, 22, 39], 150, cap=30.0, slopes=slopes)
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("most", [(1, 0), (0, 1)])
+def test_plans_for_other_numbers_of_rows_in_turn(hip, bufs, rt, fmt, most):
+    """Plans of one step that differ in mostNew alone have other kinds of tiles.  Attention captured behind one does nothing on the other, and is right
+    again on its own; so is an eager call behind a plan that was captured and has not run."""
+    c = make(fmt, hip, bufs, 8, 2, 64, 8, [3, 1, 70, 1], [260, 233, 400, 50], [0, 3], [200], seed=2)
+    c.upload()
+    want, stream = c.want(), rt.stream()
+    c.d["groups"], c.d["shared"] = c.b.up(c.groups), c.b.up(c.shared)
+
+    def made(m, stream=None):
+        _ok(c.h.PlanShared(c.d["rowStart"], c.d["lens"], 4, c.bound, m, c.d["groups"], c.d["shared"], 1, stream))
+
+    def got():
+        _synced()
+        x = c.result()
+        c.b.put(c.d["out"], c.out0)
+        E.KSync()
+        return x
+
+    made(most[0])
+    alone = rt.capture(stream, lambda: c.attend(stream=stream))
+    E.KSync()
+    rt.replay(alone, stream)
+    c.compare(got(), *want)
+    for _ in range(2):
+        made(most[1])
+        E.KSync()
+        rt.replay(alone, stream)
+        assert (got() == 7.25).all()
+        c.attend()
+        c.compare(got(), *want)
+        made(most[0])
+        E.KSync()
+        rt.replay(alone, stream)
+        c.compare(got(), *want)
+    later = rt.capture(stream, lambda: made(most[1], stream))
+    c.attend()
+    assert (got() == 7.25).all()
+    rt.replay(later, stream)
+    c.attend()
+    c.compare(got(), *want)
+    c.h.Close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_a_plan_of_wide_tiles_that_has_never_run(hip, bufs, rt, fmt):
+    """The first plan of a handle has no wide tiles for requests, the second has and is only captured: an eager call leaves out as it was."""
+    c = make(fmt, hip, bufs, 8, 2, 64, 8, [1, 1, 80, 1], [260, 233, 400, 50], [0, 3], [200], seed=3)
+    c.upload()
+    want, stream = c.want(), rt.stream()
+    plan(c, 1)
+    E.KSync()
+    d = c.d
+    later = rt.capture(stream, lambda: _ok(c.h.PlanShared(d["rowStart"], d["lens"], 4, c.bound, 0, d["groups"], d["shared"], 1, stream)))
+    c.attend()
+    _synced()
+    assert (c.result() == 7.25).all()
+    rt.replay(later, stream)
+    c.attend()
+    _synced()
+    c.compare(c.result(), *want)
+    c.h.Close()

@@ -1,4 +1,5 @@
-"""Where the workers of a plan of groups leave their shares, and how many there may be, on the host (paged_rules.h)."""
+"""Where the workers of a plan of groups leave their shares, and how many there may be, and which plans an attention call takes for its own, on the
+host (paged_rules.h)."""
 from tests.test_paged_cpu import _run
 
 # The workers of every tile as the plan has them: `units` of each tile, `workers` a KV head
@@ -91,3 +92,25 @@ int main() {
 }
 """)
     assert out == "ok\n", out
+
+
+def test_plans_of_other_kinds_of_tiles_are_other_plans(tmp_path):
+    """Two plans are one where all that their tiles follow from is: also what mostNew says of the requests, where their tiles go by it."""
+    out = _run(tmp_path, r"""
+int main() {
+    const PagedPlanFor a{4, 75, 0, 1, 256};
+    for (PagedPlanFor b : {PagedPlanFor{5, 75, 0, 1, 256}, {4, 76, 0, 1, 256}, {4, 75, 9, 1, 256}, {4, 75, 0, 2, 256}, {4, 75, 0, 1, 1 << 27}}) std::printf("%d%d ", a.is(b), b.is(a));
+    std::printf("%d\n", a.is(a));
+    for (int format : {0, 1, 8}) {
+        PagedGeo g{};
+        if (paged_geo(g, 8, 2, 64, 8, 100, format, 4, 5000, 1000)) return 1;
+        auto made = [&](int rows, int most) { return PagedPlanFor{4, rows, 0, 1, paged_narrow_rows_shared(g, rows, most, false)}; };
+        std::printf("%d %d %d %d %d\n", made(75, 0).is(made(75, 1)), made(75, 0).is(made(75, 70)), made(75, 1).is(made(75, 64)), made(64, 0).is(made(64, 1)), made(5000, 5).is(made(5000, 0)));
+        // two plans that are one agree on which requests have narrow tiles
+        for (int rows : {1, 64, 65, 1024, 1025, 5000}) for (int x : {0, 1, 4, 5, 8, 9, 64, 65, 5000}) for (int y : {0, 1, 4, 5, 8, 9, 64, 65, 5000})
+            if (made(rows, x).is(made(rows, y)) != (paged_narrow_rows_shared(g, rows, x, false) == paged_narrow_rows_shared(g, rows, y, false))) std::printf("%d %d %d\n", rows, x, y);
+    }
+}
+""").splitlines()
+    # (75 rows: 300 of a KV head; up to 256 all are narrow; 5,000: 5 tokens are 20, past the line of 16 and not that of 32)
+    assert out == ["00 00 00 00 00 1", "0 1 1 1 1", "0 1 1 1 1", "0 1 1 1 0"], out
