@@ -79,7 +79,7 @@ struct PagedAttention {
     const int4 *reqs, *groups; // as in PagedGroups
     const int* groupTile;
     const PagedTile* sharedTiles;
-    float* sharedParts;
+    const float* sharedParts;
     int sharedPlaces, sharedRows;        // of the first pass: shares a KV head (paged_place), rows of a tile
     int ldq, ldo, window, maxTiles, maxWorkers, nWorkers, wideWorkers;
     PagedGeo g;

@@ -581,6 +581,7 @@ int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, cons
     if (wide) p.sharedTiles += h->sharedMaxTiles[0];
     for (int i = 0; i < 2; i++) {
         p.pass = i + 1;
+        p.parts = i ? h->parts : h->sharedParts;
         p.maxTiles = h->sharedMaxTiles[i];
         p.tiles = h->sharedTiles[i];
         p.workers = h->sharedWorkers[i];

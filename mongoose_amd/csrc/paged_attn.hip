@@ -379,12 +379,10 @@ __device__ __forceinline__ const char* kv_row(const char* pool, const char* zero
 }
 
 // Where a worker leaves its share of a tile's result: rows of headDim floats, then the rows' maxima and sums.
-__device__ __forceinline__ float* part_of(const PagedAttention& p, const PagedTile& t, int kvh, int w) {
-    return p.parts + (((size_t)kvh * p.nWorkers + w) * 2 + (w == t.worker0)) * p.partStride;
-}
-// The same in the first pass of shared prefixes, where tiles of one worker leave a share too
-__device__ __forceinline__ float* shared_part(const PagedAttention& p, int kvh, int tile, int w) {
-    return p.sharedParts + ((size_t)kvh * p.sharedPlaces + paged_place(tile, w)) * p.partStride;
+// groups: in the first pass of shared prefixes, where tiles of one worker leave a share too.
+__device__ __forceinline__ float* part_of(const PagedAttention& p, const PagedTile& t, int kvh, int w, bool groups = false) {
+    const size_t place = groups ? (size_t)kvh * p.sharedPlaces + paged_place(t.index, w) : ((size_t)kvh * p.nWorkers + w) * 2 + (w == t.worker0);
+    return p.parts + place * p.partStride;
 }
 // After a worker has stored its share (through to memory): whether it is the last one of the tile's to come here.  scratch: LDS
 // that nobody reads any more.
@@ -465,7 +463,7 @@ __device__ __forceinline__ PagedShares shares_of(const PagedAttention& p, const 
     // (outside of the group or behind the last tile only where the caller's rows overlap)
     if (r < 0 || r >= g.y * p.g.group || i >= p.groupTile[p.plan.groups]) return {nullptr, 0, 0};
     const int w0 = p.sharedTiles[i].worker0, w1 = p.sharedTiles[i].worker1;
-    return {shared_part(p, kvh, i, w0), w1 - w0 + 1, r % p.sharedRows};
+    return {p.sharedParts + ((size_t)kvh * p.sharedPlaces + paged_place(i, w0)) * p.partStride, w1 - w0 + 1, r % p.sharedRows};
 }
 __device__ __forceinline__ const float* share_at(const PagedAttention& p, const PagedShares& x, int s) { return x.first + (size_t)s * p.partStride; }
 template <int HD>
@@ -1090,7 +1088,7 @@ struct NarrowTile {
         const float* ls = ms + 4 * NARROW;
         const int tid = thread_anew(), R = min(NARROW, t.rows * p.g.group - t.first);
         const bool whole = t.worker0 == t.worker1 && !(SHARED && p.pass == 1);
-        float* mine = SHARED && p.pass == 1 ? shared_part(p, kvh, t.index, w) : part_of(p, t, kvh, w);
+        float* mine = part_of(p, t, kvh, w, SHARED && p.pass == 1);
 #pragma unroll
         for (int k = 0; k < NP; k++) {
             const int i = tid + k * WG;
@@ -1782,7 +1780,7 @@ struct WideTile {
     __device__ __forceinline__ void write(int kvh, int w, float* lds) {
         const int r = 32 * wave + n32;
         if (t.worker0 != t.worker1 || (SHARED && p.pass == 1)) {
-            float* part = SHARED && p.pass == 1 ? shared_part(p, kvh, t.index, w) : part_of(p, t, kvh, w);
+            float* part = part_of(p, t, kvh, w, SHARED && p.pass == 1);
             if (active) {
 #pragma unroll
                 for (int b = 0; b < DB; b++)
