@@ -571,7 +571,7 @@ int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int 
 /* out[row, head] = sum_j softmax_j(s_j) v_j over the positions that the row sees, of KV head `head / (nHeads / nKVHeads)`:
  * s_j = scale * q.k_j (scale 0: 1 / sqrt(headDim)); with softcap > 0 then softcap * tanh(s_j / softcap); with slopes [nHeads]
  * then minus slopes[head] * |i - j|.  Scores, their maxima and sums are fp32; products of an fp32 cache too, those of an fp16 or Q8 cache
- * are of q and the probabilities (times the V rows' scales) to 22 bits.  ldq, ldo: floats from one row to the next (multiples of 4, 16-byte aligned
+ * are of q and the probabilities (times the V rows' scales, of any sizes where the greatest of a row is 2^-100 or more) to 22 bits.  ldq, ldo: floats from one row to the next (multiples of 4, 16-byte aligned
  * pointers); both have the plan's `rows` rows, and out overlaps neither q (other columns of one buffer are fine) nor K and V.  A table entry that is no page hides its positions; a row that sees nothing is zeros; what the cache holds
  * behind a request's length is not read into any result.  A value that is no number reaches the rows that see its position and no
  * others; an infinite one is an infinity of its sign in a row's result where its weight is 2^-126 of the row's greatest or more (with one

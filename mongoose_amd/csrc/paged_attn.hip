@@ -577,6 +577,10 @@ __device__ __forceinline__ int power_up(float top, float scale) {
     return top > 0.f && top < INFINITY ? min(15 - __builtin_amdgcn_frexp_expf(top), 118 + __builtin_amdgcn_frexp_expf(scale)) : 0;
 }
 
+// Q8: how far below a row's maximum its reference may lie.  A lane sums up 8 (narrow) or 16 probabilities a unit, in wide tiles of up to 2^2, each times 2^raise, and
+// the sum has to be a number: 2^24 positions are 2^17 narrow units, 2^19 wide ones.
+__device__ __forceinline__ float most_raised(int units) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, units > 1024 ? 100.f : 110.f))); }
+
 // A tile of 16 rows: four waves take a step of KB positions each of every unit, each with its own running maximum, sum and output.
 // Bound by HBM: a lane loads its K and V operands from the pages straight into registers, each where the last step's have gone into
 // their products, the page numbers two steps ahead; nothing is shared between the waves before the end.  8B shape, fp16, 48 requests
@@ -618,13 +622,15 @@ struct NarrowTile {
     float m, l;
     float ref;                     // Q8: probabilities are 2^(x - ref)
     float minus1;                  // Q8: -1, in a register (two_terms)
+    float raise;                   // Q8: rows' references lie up to this below their maxima
+    int careful, spoiled;         // Q8: every step looks for a reference; a weight has passed what fp32 holds
     float4_t o[EPL];
     static constexpr int NP = NARROW * HD / 4 / WG;        // pieces of the result that a thread writes at the end
     PagedShares shares[NP];        // of their rows; asked for at the start
 
     int here, next;                // page numbers of the step at hand and of the one behind it
 
-    __device__ __forceinline__ NarrowTile(const PagedAttention& p_, const PagedTile& t_, int kvh, int u0, int u1) : p(p_), t(t_) {
+    __device__ __forceinline__ NarrowTile(const PagedAttention& p_, const PagedTile& t_, int kvh, int u0, int u1, int careful_) : p(p_), t(t_), careful(careful_), spoiled(0) {
         const int tid = thread_anew();
         lane = tid & 63; l16 = lane & 15; g = lane >> 4;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -644,6 +650,7 @@ struct NarrowTile {
             vOff = (unsigned)(4 * g) * (unsigned)rowBytes + (unsigned)l16 * (VW * 4);
             minus1 = -1.f;
             asm volatile("" : "+v"(minus1));
+            raise = most_raised(u1 - u0);
         }
         here = page_of(u0);
         const float* q = p.q + (size_t)(t.row0 + row.token) * p.ldq + (size_t)row.head * HD;
@@ -943,6 +950,10 @@ struct NarrowTile {
     // Q8: scores to the weights of V's whole numbers, 2^(x - m) times the position's scale.  Both terms of a weight have to fit fp16 whatever
     // the scales are, so a row's weights are held times a power of two, which puts the largest of a step at 2^12: anew
     // where the row's maximum moves, and less where a weight passes 2^15 (rows' references: ref = m - that power's exponent).
+    // A reference never falls, so that what is summed up stays a number: the largest weight so far was 2^11 or more when its reference was
+    // chosen, and smaller ones need no more.  Where a step's scales are all zeros -- rows of zeros are stored so -- there is nothing to go by: the
+    // reference is as low as may be, and the first weight that counts raises it.  Weights past what fp32 holds (scales 2^100 apart) have the
+    // row's units gone through again with a reference looked for in every step, ahead of the weights.
     __device__ __forceinline__ void weigh_q8(float (&x)[NB * 4], float top, float from) {
         constexpr float FIT = 32768.f;
         float f = 1.f, ts = 0.f;
@@ -953,10 +964,12 @@ struct NarrowTile {
             return most;
         };
         auto exponent = [](float most) { return (float)(12 - __builtin_amdgcn_frexp_expf(fminf(most, FLT_MAX))); };
-        if (__any(top > m)) {
+        if (careful || __any(top > m)) {
             const float most = rows_max(most_of([&](int j) { return __builtin_amdgcn_exp2f(x[j] - from) * vs[j / 4][j % 4]; }));
-            const float to = top > m ? from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), 110.f)) : 0.f) : ref;
-            f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to);
+            const float to = fmaxf(m == -INFINITY ? m : ref, from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), raise)) : raise));
+            const float half = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (ref - to));          // (ref may rise by more than 2^126)
+            l = l * half * half;
+            f = half * half;
             ref = to;
             m = top;
         }
@@ -969,15 +982,16 @@ struct NarrowTile {
         float most = most_of([&](int j) { return x[j]; });
         if (__any(most > FIT)) {
             most = rows_max(most);
+            spoiled |= __any(most == INFINITY) ? 1 : 0;
             const float down = most > FIT ? exponent(most) : 0.f, less = __builtin_amdgcn_exp2f(down);
             f *= less;
+            l *= less;
             ts *= less;
             ref -= down;
 #pragma unroll
             for (int j = 0; j < NB * 4; j++) x[j] *= less;
         }
         if (__any(f != 1.f)) {            // (in one place: where a loop changes o in several, the compiler keeps it twice and moves it)
-            l *= f;
 #pragma unroll
             for (int e = 0; e < EPL; e++) o[e] *= f;
         }
@@ -1006,16 +1020,19 @@ struct NarrowTile {
             next = behind;
         }
     }
-    __device__ __forceinline__ void run(int u0, int u1, int kvh, int, float* lds) {
-        units<false>(u0, u1, 0);
+    // The units' results; true: to be gone through again, carefully (Q8, weigh_q8)
+    __device__ __forceinline__ bool run(int u0, int u1, int kvh, int, float* lds) {
         if constexpr (Q8) {
+            units<false>(u0, u1, 0);
+            if (spoiled && !careful) return true;
             const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - m);
             l *= f;
 #pragma unroll
             for (int e = 0; e < EPL; e++) o[e] *= f;
             join(kvh, lds);
-            return;
+            return false;
         }
+        units<false>(u0, u1, 0);
         float odd = 0.f;
 #pragma unroll
         for (int e = 0; e < EPL; e++)
@@ -1047,6 +1064,7 @@ struct NarrowTile {
                 for (int i = 0; i < 4; i++) o[e][i] = with_infinities(o[e][i], plus >> (4 * e + i) & 1, minus >> (4 * e + i) & 1);
         }
         join(kvh, lds);
+        return false;
     }
     // The four waves' results as one, at lds (rows of HD + 4 floats) with maxima and sums behind
     static constexpr int FLOATS = 4 * NARROW * (HD + 4) + 8 * NARROW;
@@ -1184,13 +1202,15 @@ struct WideTile {
     float m, l;
     float ref;                       // Q8: probabilities are 2^(x - ref)
     float minus1;                    // -1, in a register (two_terms)
+    float raise;                     // Q8: as in NarrowTile
+    int careful, spoiled;
     float16_t o[DB];
 
     static __device__ __forceinline__ int swz(int r) { return HALF ? ((r & 3) << 1) | ((r >> 2) & 1) : r & 7; }
 
     int here, next;                  // page numbers of the unit at hand and of the one behind it
 
-    __device__ __forceinline__ WideTile(const PagedAttention& p_, const PagedTile& t_, int kvh, int u0, int u1) : p(p_), t(t_) {
+    __device__ __forceinline__ WideTile(const PagedAttention& p_, const PagedTile& t_, int kvh, int u0, int u1, int careful_) : p(p_), t(t_), careful(careful_), spoiled(0) {
         const int tid = thread_anew();
         lane = tid & 63; n32 = lane & 31; hf = lane >> 5;
         wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -1210,6 +1230,7 @@ struct WideTile {
             const size_t slots = (size_t)p.g.nPages * p.g.pageSize, head = (size_t)kvh * p.g.pageSize * 4;
             Ksc = static_cast<const char*>(p.K) + slots * rowBytes + head;
             Vsc = static_cast<const char*>(p.V) + slots * rowBytes + head;
+            raise = most_raised(u1 - u0);
         }
 #pragma unroll
         for (int i = 0; i < NI; i++) {
@@ -1487,7 +1508,7 @@ struct WideTile {
         return ts;
     }
     // Q8: scores to weights of V's whole numbers, as NarrowTile::weigh_q8; returns the lane's sum of the probabilities (times 2^(m - ref)).  f: what
-    // l and o are multiplied by first (in one place, once: where a loop changes o in several, the compiler keeps it twice and moves it).
+    // o is multiplied by first (in one place, once: where a loop changes o in several, the compiler keeps it twice and moves it).
     __device__ __forceinline__ float weigh_q8(float16_t (&S)[NB], int base, unsigned long long held, bool all, const float4_t (&ks)[4], float4_t (&vs)[4], float& f) {
         constexpr float FIT = 32768.f;
         static_assert(!Q8 || NB == 1, "16 positions a lane");
@@ -1531,7 +1552,7 @@ struct WideTile {
         top = both(top);
         top = top == -INFINITY ? top : top * factor;
         const float mNew = top > m + LAZY || m == -INFINITY ? fmaxf(m, top) : m;
-        if (__any(mNew != m)) {
+        if (careful || __any(mNew != m)) {
             const float from = mNew == -INFINITY ? 0.f : mNew;
             float most = 0.f;
 #pragma unroll
@@ -1539,8 +1560,10 @@ struct WideTile {
 #pragma unroll
                 for (int i = 0; i < 16; i++) most = fmaxf(most, __builtin_amdgcn_exp2f(fmaf(S[b][i], factor, -from)) * vs[i / 4][i % 4]);
             most = both(most);
-            const float to = mNew != m ? from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), 110.f)) : 0.f) : ref;
-            f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - to);
+            const float to = fmaxf(m == -INFINITY ? m : ref, from - (most > 0.f ? fmaxf(-110.f, fminf(exponent(most), raise)) : raise));
+            const float half = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(0.5f * (ref - to));
+            l = l * half * half;
+            f = half * half;
             ref = to;
             m = mNew;
         }
@@ -1556,8 +1579,10 @@ struct WideTile {
             }
         if (__any(most > FIT)) {
             most = both(most);
+            spoiled |= __any(most == INFINITY) ? 1 : 0;
             const float down = most > FIT ? exponent(most) : 0.f, less = __builtin_amdgcn_exp2f(down);
             f *= less;
+            l *= less;
             ts *= less;
             ref -= down;
 #pragma unroll
@@ -1675,7 +1700,6 @@ struct WideTile {
         float f;
         const float ts = weigh_q8(S, base, held, all, ks, vs, f);
         if (__any(f != 1.f)) {
-            l *= f;
 #pragma unroll
             for (int b = 0; b < DB; b++) o[b] *= f;
         }
@@ -1723,9 +1747,15 @@ struct WideTile {
             buf ^= 1;
         }
     }
-    __device__ __forceinline__ void run(int u0, int u1, int, int, float* lds) {
+    __device__ __forceinline__ bool run(int u0, int u1, int, int, float* lds) {
         if constexpr (Q8) {
             units_q8(u0, u1);
+            if (!careful) {
+                unsigned* votes = reinterpret_cast<unsigned*>(lds) + (SCALES + 8 * SCALEB) / 4;          // (behind the scales)
+                if (lane == 0) votes[wave] = spoiled;
+                __syncthreads();
+                if (__builtin_amdgcn_readfirstlane(votes[0] | votes[1] | votes[2] | votes[3])) return true;         // all four waves, or none
+            }
             const float f = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(ref - m);
             l *= f;
 #pragma unroll
@@ -1733,7 +1763,7 @@ struct WideTile {
             float other = l;
             row_swap32(l, other);
             l += other;
-            return;
+            return false;
         }
         units<false>(u0, u1, 0);
         float odd = 0.f;
@@ -1775,6 +1805,7 @@ struct WideTile {
         float other = l;
         row_swap32(l, other);
         l += other;
+        return false;
     }
     // A share lies as its registers do -- a wave's block b, rows of four i / 4, then its 64 lanes -- so that stores and loads are whole lines
     __device__ __forceinline__ void write(int kvh, int w, float* lds) {
@@ -1868,11 +1899,13 @@ __device__ __forceinline__ void attend(const PagedAttention& p, float* lds) {
     const bool ours = p.made->is(p.plan);             // (asked for together with the share)
     PagedTile t = tile_at(&k->tile);
     if (!ours || a >= b) return;
+    int careful = 0;
     for (;;) {
         const int u0 = paged_unit_at(t, a), u1 = paged_unit_at(t, b);
         if (u0 < u1) {
-            Tile<KVT, HD, MOD, SHARED> n(p, t, kvh, u0, u1);
-            n.run(u0, u1, kvh, w, lds);
+            Tile<KVT, HD, MOD, SHARED> n(p, t, kvh, u0, u1, careful);
+            careful = n.run(u0, u1, kvh, w, lds);
+            if (careful) continue;                         // (the same tile once more: not a loop of its own, ahead of which the compiler would move what does not change in it)
             n.write(kvh, w, lds);
         } else if (t.units == 0 && a <= t.cost0 && t.cost0 < b) {
             for (int i = threadIdx.x; i < min(ROWS, t.rows * p.g.group - t.first) * (HD / 4); i += WG) {
