@@ -575,7 +575,7 @@ int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int 
  * pointers); both have the plan's `rows` rows, and out overlaps neither q (other columns of one buffer are fine) nor K and V.  A table entry that is no page hides its positions; a row that sees nothing is zeros; what the cache holds
  * behind a request's length is not read into any result.  A value that is no number reaches the rows that see its position and no
  * others; an infinite one is an infinity of its sign in a row's result where its weight is 2^-126 of the row's greatest or more (with one
- * of the other sign, or a NaN, a NaN).  scale and softcap are 0 or between 1e-30 and 1e30.  MG_E_STATE without
+ * of the other sign, or a NaN, a NaN; of less weight it may be a NaN too).  scale and softcap are 0 or between 1e-30 and 1e30.  MG_E_STATE without
  * a plan. */
 int mg_paged_attention(mg_paged* h, const float* q, int ldq, const void* K, const void* V, const int* table, float* out, int ldo,
                        float scale, float softcap, const float* slopes, void* stream);

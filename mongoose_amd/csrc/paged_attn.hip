@@ -531,8 +531,8 @@ __device__ __forceinline__ int shared_pos(const PagedAttention& p, int row) {
 
 // Values that are no numbers.  Zero times one is no zero, so that one reaches rows that do not see it, and its product with the second
 // term of a weight turns an infinity into a NaN.  A tile whose result has elements that are no numbers therefore goes through its
-// units three times more, with the maxima of the first time: with ones for +infinity and NaN, zeros for all else, and weights of 1 (or 0
-// where they are 0); the same for -infinity and NaN; with zeros for all three.  An element is what the last time gives, plus an
+// units three times more, with the maxima of the first time: with ones for +infinity and NaN, zeros for all else, and weights of 1 where a
+// row sees the position (whatever its weight is: one that fp32 holds as 0 is none); the same for -infinity and NaN; with zeros for all three.  An element is what the last time gives, plus an
 // infinity where the first count is not 0, minus one where the second is not.  Other tiles pay for a look at their result.
 enum { PLUS_INFINITE, MINUS_INFINITE, FINITE };
 // Two weights as elements i and i + 1 of both terms: rounded to fp16, and what that leaves.  The latter in one instruction that takes halves
@@ -933,18 +933,20 @@ struct NarrowTile {
             l += x[j];
         }
         }
-        if (!inner) {
-            bool some = false;
-#pragma unroll
-            for (int j = 0; j < NB * 4; j++) some |= x[j] != 0.f;
-            if (!__any(some)) return;                     // (no row has anything here)
-        }
+        // (no row sees anything here; what one sees counts, whatever its weight, where V is no number)
+        if (!inner && !(__any(mine >= 0) && paged_some_see(span.pos0, span.pos1, base, base + KB, p.window, t.prefix))) return;
         if constexpr (AGAIN) {
 #pragma unroll
-            for (int j = 0; j < NB * 4; j++) {
-                x[j] = pass == FINITE ? x[j] : x[j] > 0.f ? 1.f : 0.f;
+            for (int b = 0; b < NB; b++) {
+                const bool held = page_in(mine, b, g & 2) >= 0;
 #pragma unroll
-                for (int e = 0; e < VW; e++) v[j][e] = stand_in<HALF>(v[j][e], pass);
+                for (int i = 0; i < 4; i++) {
+                    const int key = base + 16 * b + 4 * g + i;
+                    const bool sees = held && !(SHARED && key < t.from) && paged_sees(row.pos, key, t.len, p.window, t.prefix);
+                    if (pass != FINITE) x[4 * b + i] = sees ? 1.f : 0.f;
+#pragma unroll
+                    for (int e = 0; e < VW; e++) v[4 * b + i][e] = stand_in<HALF>(v[4 * b + i][e], pass);
+                }
             }
         }
         const Weights wt = weights(x);
@@ -1624,12 +1626,17 @@ struct WideTile {
             m = mNew;
         }
         l += ts;
-        if (!inner && !__any(ts != 0.f)) return;          // (no row has anything here)
+        // (no row sees anything here, as in NarrowTile)
+        if (!inner && !((held & runs) && paged_some_see(pos0, pos1, base, base + UK, p.window, t.prefix))) return;
         if (AGAIN && pass != FINITE) {
+            const int first = base + 4 * anew(hf);
 #pragma unroll
             for (int b = 0; b < NB; b++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) S[b][i] = S[b][i] > 0.f ? 1.f : 0.f;
+                for (int i = 0; i < 16; i++) {
+                    const int key = first + 32 * b + 8 * (i / 4) + i % 4;
+                    S[b][i] = ((held >> (4 * b + i / 4)) & 1) && !(SHARED && key < t.from) && paged_sees(row.pos, key, t.len, p.window, t.prefix) ? 1.f : 0.f;
+                }
         }
         const Weights w = weights(S);
         const unsigned Vl = v_base(V);

@@ -220,6 +220,11 @@ MG_HD bool paged_sees(int i, int j, int len, int window, int prefix) {
     return (j < len) & (((j <= i) & ((window == 0) | (j > i - window))) | (j < prefix));
 }
 
+// Whether any token at positions first .. last may see any of the positions [begin, end)
+MG_HD bool paged_some_see(int first, int last, int begin, int end, int window, int prefix) {
+    return begin < prefix || (begin <= last && (window == 0 || end > first - window + 1));
+}
+
 // ---------------------------------------------------------------------------
 // The plan of an attention call.  The rows of a request under one KV head (its new tokens x the head group, token by token) are cut
 // into tiles of tileRows, the positions a tile sees into units of unitKeys.  All tiles of a batch, one behind the other, make a line
