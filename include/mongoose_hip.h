@@ -516,6 +516,10 @@ size_t mg_paged_pool_bytes(const mg_paged* h);    /* bytes of a layer's K (or V)
  * (these two may be lens and ringState themselves; otherwise no array overlaps another), rowStart[nReqs + 1] = the first row of every
  * request, slots[rows] = page * pageSize + place of each row and positions[rows] (both -1 behind the last row; a slot is -1 too
  * where the table or the ring hold an entry that is no page), counts[4] = {rows, pages taken, pages given back, 0}.
+ * Pages that requests share (mg_paged_plan_shared) are one request's own: the call takes all of an ended request's pages for its.  A request that
+ * starts behind shared pages -- whole ones -- has them in its row of the table, and lens[r] their positions, ahead of its first step; before
+ * the step that ends it the caller moves its own pages to the front of its row and takes those positions off lens[r], so that only its own
+ * go back.  The one that the shared pages are given back with ends last.
  * A step that does not fit changes no length, no table and no ring: rowStart is 0 throughout, slots and positions -1, counts =
  * {0, 0, 0, why}, why a sum of 1 (more pages needed than free), 2 (more new tokens than `rows`), 4 (a length that is negative or
  * passes maxLen, a newLens below -1), 8 (ringState that fits no ring of nPages). */
@@ -556,7 +560,7 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
  * the first request with rows are the ones that are read).  mg_paged_plan_shared takes the lengths as mg_paged_plan does, without a window or
  * a prefix; the attention calls that follow compute what they would without it -- to rounding --, a group's shared positions once for all
  * its rows.  A shared length is cut to the positions that all of its requests with rows have ahead of their new ones; requests
- * of no group, and groups of one request with rows, share nothing.  mostNew: the most rows that a request of the step has, if the caller knows (0: any
+ * of no group, and groups of one request with rows, share nothing.  Who gives shared pages back: mg_paged_tables.  mostNew: the most rows that a request of the step has, if the caller knows (0: any
  * number; more of them than said cost time, not results).  nGroups <= maxReqs; all arrays are device memory and are copied.
  * mg_paged_share allocates the workspace for it, once, before the first such plan (MG_E_STATE without it): for every KV head a share of a tile
  * (128 rows of headDim + 2 floats) for each of the tiles that groups may have, maxRows * (nHeads / nKVHeads) / 128 + 16 + maxReqs / 2, and for

@@ -1,11 +1,13 @@
 """More of attention behind shared prefixes (HIPPaged.PlanShared): groups whose tiles are many for the workers that there are, so that a worker has
-several of them and leaves a share of each; plans that differ in the most rows that a request has.  Bounds as in test_gpu_paged_shared."""
+several of them and leaves a share of each; plans that differ in the most rows that a request has; requests that come and end.  Bounds as in test_gpu_paged_shared."""
 import copy
 
 import numpy as np
 import pytest
 
 from mongoose_amd import engine as E
+from tests import paged_model as P
+from tests import paged_q8_model as Q
 from tests.test_gpu_paged import _ok, _synced, bufs, rt  # noqa: F401  (fixtures)
 from tests.test_gpu_paged_shared import FORMATS, make, plan
 
@@ -148,3 +150,73 @@ def test_a_plan_of_wide_tiles_that_has_never_run(hip, bufs, rt, fmt):
     _synced()
     c.compare(c.result(), *want)
     c.h.Close()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_requests_behind_one_prefix_come_and_end(hip, bufs, rt, fmt):
+    """Tables, plan, store and attention captured once and replayed.  Request 0 holds the prefix (whole pages); a request that comes behind it has
+    those pages in its row of the table and their length; one that ends gives back its own: they go to the front of its row and its length is theirs.
+    Every page is in one place at any time, and all are free at the end."""
+    heads, kv, hd, page, n, rows, nPages, width, shared = 8, 2, 64, 8, 6, 48, 60, 16, 40
+    maxLen, P0 = page * width, shared // page
+    rng = np.random.default_rng(fmt)
+    ang = np.arange(maxLen)[:, None] * 1e4 ** (-np.arange(hd // 2) * 2.0 / hd)
+    cos, sin = bufs.up(np.cos(ang).astype(np.float32)), bufs.up(np.sin(ang).astype(np.float32))
+    ld = (heads + 2 * kv) * hd
+    h = E.NewHIPPaged(hip, heads, kv, hd, page, nPages, fmt, n, rows, maxLen)
+    assert h is not None and h.TableWidth() == width
+    _ok(h.Share())
+    host = dict(new=np.zeros(n, np.int32), lens=np.zeros(n, np.int32), table=np.full((n, width), -1, np.int32), ring=rng.permutation(nPages).astype(np.int32),
+                state=np.array([7, nPages], np.int32), rowStart=np.zeros(n + 1, np.int32), slots=np.zeros(rows, np.int32), pos=np.zeros(rows, np.int32),
+                counts=np.zeros(4, np.int32), x=np.zeros((rows, ld), np.float32), K=np.zeros(h.PoolBytes(), np.uint8), V=np.zeros(h.PoolBytes(), np.uint8),
+                out=np.zeros((rows, heads * hd), np.float32), groups=np.array([0, n], np.int32), shared=np.array([shared], np.int32))
+    s = {name: bufs.up(a) for name, a in host.items()}
+    x, stream = s["x"].DevicePtr(), rt.stream()
+
+    def step():
+        _ok(h.Tables(s["new"], n, s["lens"], s["lens"], s["table"], s["ring"], s["state"], s["state"], rows, s["rowStart"], s["slots"], s["pos"], s["counts"], stream))
+        _ok(h.PlanShared(s["rowStart"], s["lens"], n, rows, 0, s["groups"], s["shared"], 1, stream))
+        _ok(h.Store(x, x + heads * hd * 4, x + (heads + kv) * hd * 4, ld, ld, ld, x, ld, s["K"], s["V"], s["slots"], s["pos"], rows, cos, sin, maxLen, stream))
+        _ok(h.Attention(x, ld, s["K"], s["V"], s["table"], s["out"], heads * hd, 0.0, 0.0, None, stream))
+
+    graph = rt.capture(stream, step)
+    down = lambda name: bufs.down(s[name], host[name])  # noqa: E731
+    lens = np.zeros(n, np.int64)
+    for t, new in enumerate([[40, 0, 0, 0, 0, 0], [0, 3, 1, 9, 0, 0], [0, 1, 1, 1, 0, 0], [0, 1, -1, 8, 5, 0], [0, 20, 7, 1, 1, 0], [0, -1, 4, -1, 1, 20], [0, 2, 1, 0, -1, 30], [0, 1, -1, 7, 3, -1],
+                             [0, -1, 0, 1, 1, 0], [0, 0, 0, -1, -1, 0], [-1, 0, 0, 0, 0, 0]]):
+        table, at = down("table"), lens.copy()
+        for r in range(1, n):
+            if new[r] > 0 and at[r] == 0:                       # comes
+                table[r, :P0] = table[0, :P0]
+                at[r] = shared
+            elif new[r] < 0:                                    # ends
+                own = -(-at[r] // page) - P0
+                table[r, :own] = table[r, P0:P0 + own].copy()
+                at[r] -= shared
+        q = rng.standard_normal((rows, ld)).astype(np.float32)
+        for name, a in (("table", table), ("lens", at.astype(np.int32)), ("new", np.array(new, np.int32)), ("x", q), ("out", np.full((rows, heads * hd), 7.25, np.float32))):
+            bufs.put(s[name], a)
+        E.KSync()
+        rt.replay(graph, stream)
+        lens = np.where(np.array(new) < 0, 0, at + np.maximum(new, 0))
+        table, counts, state, ring = down("table"), down("counts"), down("state"), down("ring")
+        assert counts[3] == 0 and np.array_equal(down("lens"), lens), (t, counts.tolist())
+        held = [int(table[r, e]) for r in range(n) if lens[r] for e in range(P0 if r else 0, -(-int(lens[r]) // page))]
+        free = [int(ring[(state[0] + i) % nPages]) for i in range(state[1])]
+        assert sorted(held + free) == list(range(nPages)), t
+        for r in range(1, n):
+            assert lens[r] == 0 or np.array_equal(table[r, :P0], table[0, :P0])
+        start = np.concatenate(([0], np.cumsum(np.maximum(new, 0))))
+        pools = []
+        for name in "KV":
+            data = down(name)
+            if fmt == 8:
+                data = Q.values(*Q.from_pool(data, nPages * page, kv, hd, page))
+            else:
+                data = data.view(np.float16 if fmt else np.float32)
+            pools.append(data.reshape(-1, kv * hd))
+        got = down("out")
+        want, bound = P.attention(down("x")[:, :heads * hd], *pools, table, start, lens, page, heads // kv, hd)
+        assert (np.abs(got[:start[-1]] - want) <= bound).all() and (got[start[-1]:] == 7.25).all(), t
+    assert down("state")[1] == nPages
+    h.Close()
