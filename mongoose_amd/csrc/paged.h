@@ -27,6 +27,7 @@ struct PagedLoad {
     const int *table, *rowStart, *lens;
     float *kOut, *vOut;
     int nReqs, rows, ldk, ldv;
+    int row0;                  // a launch's first row
     PagedGeo g;
 };
 hipError_t launch_paged_load(const PagedLoad& p, hipStream_t s);

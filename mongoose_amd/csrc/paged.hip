@@ -299,7 +299,7 @@ template <> __device__ __forceinline__ float4 get4<signed char>(const signed cha
 }
 template <typename KVT>
 __global__ __launch_bounds__(64 * LOAD_ROWS) void paged_load_kernel(PagedLoad p) {
-    const int i = __builtin_amdgcn_readfirstlane(blockIdx.x * LOAD_ROWS + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+    const int i = __builtin_amdgcn_readfirstlane(p.row0 + blockIdx.x * LOAD_ROWS + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
     if (i >= p.rows) return;
     const int r = wave_find(p.rowStart, p.nReqs, i);
     if (r < 0) return;
@@ -337,13 +337,21 @@ __global__ __launch_bounds__(64 * LOAD_ROWS) void paged_load_kernel(PagedLoad p)
             put4(out[w] + e, x);
         }
 }
-hipError_t launch_paged_load(const PagedLoad& p, hipStream_t s) {
-    if (p.rows <= 0 || p.nReqs <= 0) return hipSuccess;
-    const dim3 grid(((unsigned)p.rows + LOAD_ROWS - 1) / LOAD_ROWS), block(64 * LOAD_ROWS);
-    if (p.g.kvFormat == PAGED_Q8) hipLaunchKernelGGL(paged_load_kernel<signed char>, grid, block, 0, s, p);
-    else if (p.g.kvFormat == PAGED_F16) hipLaunchKernelGGL(paged_load_kernel<_Float16>, grid, block, 0, s, p);
-    else hipLaunchKernelGGL(paged_load_kernel<float>, grid, block, 0, s, p);
-    return hipGetLastError();
+hipError_t launch_paged_load(const PagedLoad& p0, hipStream_t s) {
+    if (p0.nReqs <= 0) return hipSuccess;
+    constexpr int MOST = 1 << 24;         // rows of a launch: the runtime counts its threads in 32 bits, and more of them go missing without an error
+    for (long long row0 = 0; row0 < p0.rows; row0 += MOST) {
+        PagedLoad p = p0;
+        p.row0 = (int)row0;
+        const int rows = (int)(p.rows - row0 < MOST ? p.rows - row0 : MOST);
+        const dim3 grid((rows + LOAD_ROWS - 1) / LOAD_ROWS), block(64 * LOAD_ROWS);
+        if (p.g.kvFormat == PAGED_Q8) hipLaunchKernelGGL(paged_load_kernel<signed char>, grid, block, 0, s, p);
+        else if (p.g.kvFormat == PAGED_F16) hipLaunchKernelGGL(paged_load_kernel<_Float16>, grid, block, 0, s, p);
+        else hipLaunchKernelGGL(paged_load_kernel<float>, grid, block, 0, s, p);
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
 }
 
 // The device a handle's memory is on, for the duration of a call
@@ -485,7 +493,7 @@ int mg_paged_load(mg_paged* h, const void* K, const void* V, const int* table, c
     PAGED(h, "mg_paged_load");
     if (const char* why = mg::paged_load_refusal(h->g, K, V, table, rowStart, lens, nReqs, rows, kOut, ldk, vOut, ldv)) return refuse("mg_paged_load", why);
     if (const char* why = mg::paged_load_overlap(h->g, K, V, table, rowStart, lens, nReqs, rows, kOut, ldk, vOut, ldv)) return refuse("mg_paged_load", why);
-    mg::PagedLoad p{K, V, table, rowStart, lens, kOut, vOut, nReqs, rows, ldk, ldv, h->g};
+    mg::PagedLoad p{K, V, table, rowStart, lens, kOut, vOut, nReqs, rows, ldk, ldv, 0, h->g};
     return launched("mg_paged_load", mg::launch_paged_load(p, static_cast<hipStream_t>(stream)));
 }
 int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, int rows, int window, const int* prefixLens, void* stream) {
