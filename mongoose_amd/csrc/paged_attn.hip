@@ -124,7 +124,7 @@ __device__ __forceinline__ int narrow_workers(int n, int units, int kvFormat) {
     return units < 4 ? 1 : kvFormat == PAGED_Q8 ? min(n, max(64, (int)(4.f * sqrtf((float)units)))) : n;
 }
 // One workgroup for the narrow tiles and one for the wide ones.  SHARED: of groups, or of their requests; apart from the plan without, which pays for
-// no question about them (48 requests 6.3 us with them, 5.7 without).
+// no question about them (48 requests 6.3 us with them, 6.0 without).
 template <bool SHARED>
 __device__ __forceinline__ void make_plan(PagedPlan p, bool wide) {
     const int tileRows = wide ? WIDE : NARROW, unitKeys = wide ? wide_keys(p.kvFormat) : narrow_keys(p.kvFormat);
@@ -583,7 +583,9 @@ __device__ __forceinline__ int power_up(float top, float scale) {
 
 // Q8: how far below a row's maximum its reference may lie.  A lane sums up 8 (narrow) or 16 probabilities a unit, in wide tiles of up to 2^2, each times 2^raise, and
 // the sum has to be a number: 2^24 positions are 2^17 narrow units, 2^19 wide ones.
-__device__ __forceinline__ float most_raised(int units) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, units > 1024 ? 100.f : 110.f))); }
+__device__ __forceinline__ float most_raised(int units) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, units > 1024 ? 100.f : 110.f)));       // (in a scalar register)
+}
 
 // A tile of 16 rows: four waves take a step of KB positions each of every unit, each with its own running maximum, sum and output.
 // Bound by HBM: a lane loads its K and V operands from the pages straight into registers, each where the last step's have gone into
@@ -934,7 +936,7 @@ struct NarrowTile {
         }
         }
         // (no row sees anything here; what one sees counts, whatever its weight, where V is no number)
-        if (!inner && !(__any(mine >= 0) && paged_some_see(span.pos0, span.pos1, base, base + KB, p.window, t.prefix))) return;
+        if (!inner && !(__any(mine >= 0) && (!SHARED || base + KB > t.from) && paged_some_see(span.pos0, span.pos1, base, base + KB, p.window, t.prefix))) return;
         if constexpr (AGAIN) {
 #pragma unroll
             for (int b = 0; b < NB; b++) {
