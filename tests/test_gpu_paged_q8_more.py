@@ -19,9 +19,13 @@ def lay(c, sizes, gaps, stretch):
     c.q[:] = 1.0 + 0.1 * c.q
     K *= 0.2
     up = np.log(2.0) / np.sqrt(c.hd)          # (q near ones: a key of k throughout has a score of k sqrt(hd))
+    seen = np.zeros(len(V), bool)             # (rows that requests share: once)
     for r in range(len(c.lens)):
-        at = np.array([c.where(r, j) for j in range(c.lens[r])])
-        s = np.minimum(np.arange(c.lens[r]) // stretch, len(sizes) - 1)
+        j = np.arange(c.lens[r])
+        at = c.table[r][j // c.page].astype(np.int64) * c.page + j % c.page
+        j, at = j[~seen[at]], at[~seen[at]]
+        seen[at] = True
+        s = np.minimum(j // stretch, len(sizes) - 1)
         K[at] += (np.array(gaps)[s] * up)[:, None]
         V[at] *= np.array(sizes)[s][:, None]
     c.set_rows("K", K)
