@@ -564,8 +564,8 @@ int mg_paged_plan(mg_paged* h, const int* rowStart, const int* lens, int nReqs, 
  * number; more of them than said cost time, not results).  nGroups <= maxReqs; all arrays are device memory and are copied.
  * mg_paged_share allocates the workspace for it, once, before the first such plan (MG_E_STATE without it): for every KV head a share of a tile
  * (128 rows of headDim + 2 floats) for each of the tiles that groups may have, maxRows * (nHeads / nKVHeads) / 128 + 16 + maxReqs / 2, and for
- * each of the head's workgroups, 512 / nKVHeads -- 94 MB for 64 requests of 2,048 rows in all, 32 heads on 8 of 128 --, and 128 bytes for each
- * of maxRows * (nHeads / nKVHeads) / 16 + maxReqs tiles.  nGroups and mostNew
+ * each of the head's workgroups, 512 / nKVHeads -- 94 MB for 64 requests of 2,048 rows in all, 32 heads on 8 of 128 --, and 128 + 4 *
+ * nKVHeads bytes for each of maxRows * (nHeads / nKVHeads) / 16 + maxReqs tiles.  nGroups and mostNew
  * are parts of attention's rule on plans: where the plan on the device was made with a mostNew that divides the requests otherwise, a call
  * does nothing. */
 int mg_paged_share(mg_paged* h);
@@ -575,7 +575,8 @@ int mg_paged_plan_shared(mg_paged* h, const int* rowStart, const int* lens, int 
 /* out[row, head] = sum_j softmax_j(s_j) v_j over the positions that the row sees, of KV head `head / (nHeads / nKVHeads)`:
  * s_j = scale * q.k_j (scale 0: 1 / sqrt(headDim)); with softcap > 0 then softcap * tanh(s_j / softcap); with slopes [nHeads]
  * then minus slopes[head] * |i - j|.  Scores, their maxima and sums are fp32; products of an fp32 cache too, those of an fp16 or Q8 cache
- * are of q and the probabilities (times the V rows' scales, of any sizes where the greatest of a row is 2^-100 or more) to 22 bits.  ldq, ldo: floats from one row to the next (multiples of 4, 16-byte aligned
+ * are of q and the probabilities (times the V rows' scales, of any sizes where the greatest of a row is 2^-100 or more) to 22 bits; past elements of
+ * 2^105 in a Q8 cache's K scores may be infinities.  ldq, ldo: floats from one row to the next (multiples of 4, 16-byte aligned
  * pointers); both have the plan's `rows` rows, and out overlaps neither q (other columns of one buffer are fine) nor K and V.  A table entry that is no page hides its positions; a row that sees nothing is zeros; what the cache holds
  * behind a request's length is not read into any result.  A value that is no number reaches the rows that see its position and no
  * others; an infinite one is an infinity of its sign in a row's result where its weight is 2^-126 of the row's greatest or more (with one

@@ -1174,7 +1174,7 @@ struct NarrowTile {
 //     fp16 through the transposing LDS read, fp32 word by word.
 // A row's 16-byte pieces lie in LDS at piece ^ swz(row), so that neither rows of one piece nor (fp16) four rows of two meet in a bank.
 // Q8 caches: as fp16 ones, in units of 32 positions.  Rows come into LDS as they are, two units ahead, and are turned to halves there for all
-// four waves, one ahead, between the scores' matrix instructions.  8B shape, 2,048 tokens over 9,700 positions: 820 us, 880 TFLOP/s with both terms
+// four waves, one ahead, between the scores' matrix instructions.  8B shape, 2,048 tokens over 9,700 positions: 810 us, 890 TFLOP/s with both terms
 // counted.  Bound by the matrix units and, as much, by the vector instructions beside them (270 a unit and wave, 16 + 16 matrix instructions).
 template <typename KVT, int HD, bool MOD, bool SHARED>
 struct WideTile {
